@@ -445,6 +445,162 @@ int pgs_w8a16_decode_span_test_hooks(int spin_limit, int force_giveup);
  */
 int pgs_w8a16_decode_span_trace(void* buffer, size_t bytes);
 
+/*
+ * ---------------------------------------------------------------------------
+ * 4-bit weights with group scales.  No counterpart in the reference, whose one
+ * quantized form is the 8-bit one above; same rules: symmetric, absmax, the
+ * weight stored once in the layout the matmul streams.
+ *
+ * A group is `group` (32, 64 or 128) consecutive columns of a row, the last
+ * one of a row possibly shorter.  Values of a code c (0..15): 0, 0.5, 1, 1.5,
+ * 2, 3, 4, 6 for c % 8 = 0..7, negative for c >= 8 (the E2M1 values gfx950
+ * widens to bf16 in hardware, exactly).
+ *   scale  = bf16( max(max_j |w[r,j]| over the group, 1e-8f) / 6.0f )
+ *   code   = the value nearest to w / scale, a tie to the even code (decided
+ *            by exact products of scale, without a division; a weight that
+ *            rounds to zero has code 0); weight = value * scale
+ * A group holding a NaN gets a NaN scale and codes 0; one holding an infinity
+ * an infinite scale (its finite weights' codes 0).
+ *
+ *   qp   packed codes, pgs_packed4_bytes(n, k): 16-row x 128-column blocks of
+ *        1 KiB, [ceil(n/16)][ceil(k/128)]; inside a block, dword j of the 16
+ *        bytes of lane l (0..63) holds columns 32*j + 8*(l/16) .. +7 of row
+ *        l%16, column 32*j + 8*(l/16) + i in bits 4*i .. 4*i+3
+ *   sp   packed scales, pgs_packed4_scales(n, k, group) bf16 values: per block
+ *        16 * (128/group), [4 row quads][128/group groups][4 rows]
+ * Padding codes and scales are zero.  k must be a multiple of 16.
+ */
+int64_t pgs_packed4_bytes(int64_t n, int64_t k);
+int64_t pgs_packed4_scales(int64_t n, int64_t k, int64_t group);
+
+/* w [n, k] fp32 or bf16, row-major, 16-byte aligned -> qp, sp (padding included). */
+int pgs_quantize4_packed(const void* w, int w_dtype, int64_t n, int64_t k,
+                         int64_t group, void* qp, void* sp, void* stream);
+
+/* out[r,j] = dtype(value * scale): the fp32 product (exact), rounded once. */
+int pgs_dequantize4_packed(const void* qp, const void* sp, int64_t n, int64_t k,
+                           int64_t group, void* out, int out_dtype, void* stream);
+
+/*
+ * y = x . (value * scale)^T (+ bias) for 4-bit weights: x bf16 [m, k] (rows
+ * contiguous, 16-byte aligned), bias bf16 [n] or NULL, y bf16 or fp32 [m, n];
+ * fp32 accumulation.  With residual (bf16 [m, n], else NULL) the output is
+ * residual + the linear's output rounded to y_dtype, as in
+ * pgs_w8a16_linear_residual; y may be the residual buffer.  Made for the few
+ * tokens of a drafting step; above 64 rows the weights are read once per 64.
+ */
+int pgs_w4a16_linear(const void* x, const void* qp, const void* sp,
+                     const void* bias, const void* residual, void* y,
+                     int y_dtype, int64_t m, int64_t n, int64_t k,
+                     int64_t group, void* stream);
+
+/*
+ * ---------------------------------------------------------------------------
+ * The paged cache of keys and values (the reference's engine/paged_attention.py
+ * and engine/block_allocator.py run these on the CPU or as torch calls, one
+ * sequence at a time; here a batch of requests per launch).
+ *
+ * Block tables: int32 [requests, columns], row stride `table_stride`; column c
+ * of request b names the block that holds its tokens c*block_size .. +
+ * block_size - 1.  lens: int32 [requests], tokens cached.  free_blocks: int32
+ * [free_capacity], a stack of the blocks in no table, *free_count of them.
+ * offsets: int32 [requests + 1]: rows offsets[b] .. offsets[b+1] - 1 of a
+ * batch belong to request b; rows behind offsets[requests] to none.
+ * Everything is read on the device: nothing here waits for the host, and every
+ * call can be captured in a HIP graph.
+ */
+
+/*
+ * Extends each request by new_lens[b] tokens (a negative count is 0), in
+ * request order: the blocks it needs are taken from the top of the stack into
+ * its next table columns, lens and free_count are updated.  status[b] = 0 if
+ * request b was served; 1 if it needs blocks and the requests up to it need
+ * more than the stack holds; 2 if its length is negative or its table has too
+ * few columns.  A request that is not served is left as it was.
+ * slots[i], i < rows: the slot (block * block_size + place in the block) of row
+ * i of the batch: token lens[b] (before the call) + n of its request, where n =
+ * index[i], or i - offsets[b] without an index; -1 if n is not in
+ * 0..new_lens[b]-1, the request was not served, or the row belongs to none.
+ */
+int pgs_append_blocks(int32_t* lens, const int32_t* new_lens, int32_t* block_tables,
+                      int64_t table_stride, int64_t columns, const int32_t* free_blocks,
+                      int64_t free_capacity, int32_t* free_count, int64_t block_size,
+                      int64_t requests, const int32_t* offsets, const int32_t* index,
+                      int64_t rows, int64_t* slots, int32_t* status, void* stream);
+
+/*
+ * Shortens each request to keep[b] tokens (0: it is finished; a count above its
+ * length keeps all): blocks no longer needed go back to the stack, their table
+ * columns become -1.  Undoes pgs_append_blocks exactly.  Blocks beyond the
+ * stack's capacity are dropped.
+ */
+int pgs_truncate_blocks(int32_t* lens, const int32_t* keep, int32_t* block_tables,
+                        int64_t table_stride, int64_t columns, int32_t* free_blocks,
+                        int64_t free_capacity, int32_t* free_count, int64_t block_size,
+                        int64_t requests, void* stream);
+
+/* Keys and values of one layer: element strides of [blocks, block_size,
+ * kv_heads, head_dim] (the last dimension contiguous). */
+typedef struct pgs_kv_cache {
+  void* k;
+  void* v;
+  int64_t blocks, block_size, kv_heads, head_dim;
+  int64_t k_block, k_slot, k_head;
+  int64_t v_block, v_slot, v_head;
+} pgs_kv_cache;
+
+/*
+ * Rows i of k and v (bf16 or fp16 [rows, kv_heads, head_dim], element strides
+ * of row and head given) into slot slots[i] of the cache; a slot outside the
+ * cache is left out.  The slots of the rows must differ: of two rows with one
+ * slot, either may stay.
+ */
+int pgs_write_kv(const void* k, int64_t k_row, int64_t k_head, const void* v,
+                 int64_t v_row, int64_t v_head, const pgs_kv_cache* cache,
+                 const int64_t* slots, int64_t rows, void* stream);
+
+/* The arguments of pgs_tree_attention. */
+typedef struct pgs_tree_attention_args {
+  const void* q;               /* [rows, q_heads, head_dim] */
+  const void* k;               /* [rows, kv_heads, head_dim]: the drafted tokens' own */
+  const void* v;
+  void* out;                   /* [rows, q_heads, head_dim] */
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head; /* element strides */
+  const pgs_kv_cache* cache;
+  const int32_t* block_tables; /* [requests, columns] */
+  int64_t table_stride, columns;
+  const int32_t* lens;         /* [requests]: cached tokens */
+  const int32_t* offsets;      /* [requests + 1] */
+  const int32_t* parents;      /* [rows], or NULL: each token's parent is the one before it */
+  int64_t rows, requests, q_heads;
+  int64_t max_tokens;          /* rows per request, at most 64 */
+  int64_t max_context;         /* the longest lens expected: sizes the split, not the result */
+  float scale;
+  int dtype;                   /* PGS_DTYPE_BF16 or PGS_DTYPE_F16, of all tensors */
+} pgs_tree_attention_args;
+
+/*
+ * Attention of drafted tokens over a paged cache.  Token t of request b (row
+ * offsets[b] + t) attends to the request's lens[b] cached tokens, to itself and
+ * to its ancestors among the drafted tokens: parents[row] names a token of the
+ * same request before t (any other value: none), so that the drafted tokens form
+ * trees.  Query heads share key heads in groups of q_heads / kv_heads.
+ *   out = sum_j softmax_j(scale * q . k_j) v_j     (softmax in fp32)
+ * head_dim 64 or 128; block_size a multiple of 16; strides multiples of 8
+ * elements and pointers 16-byte aligned.  Lengths beyond the table's columns
+ * are cut to them; tokens in a block outside the cache are left out; rows of no
+ * request, and a request's rows from max_tokens on, are not written.
+ * workspace: pgs_tree_attention_workspace_bytes() bytes, 256-byte aligned, no
+ * fill needed.
+ */
+int pgs_tree_attention(const pgs_tree_attention_args* args, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of pgs_tree_attention (0: none needed). */
+size_t pgs_tree_attention_workspace_bytes(int64_t rows, int64_t requests, int64_t q_heads,
+                                          int64_t kv_heads, int64_t head_dim,
+                                          int64_t max_tokens, int64_t max_context);
+
 #ifdef __cplusplus
 }
 #endif

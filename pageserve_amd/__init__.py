@@ -5,6 +5,7 @@ computed by hand-written HIP kernels behind a C ABI
 (``include/pageserve_amd.h``).
 """
 
+from .paged import append_blocks, tree_attention, truncate_blocks, write_kv  # noqa: F401
 from .quantization import (  # noqa: F401
     QuantizedWeight,
     W8A16Weight,
@@ -24,5 +25,6 @@ from .quantization import (  # noqa: F401
     save_quantized,
     swiglu,
 )
+from .quantization4 import QuantizedWeight4, linear4  # noqa: F401
 
 __version__ = "0.1.0"

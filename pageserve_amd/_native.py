@@ -70,6 +70,28 @@ class SpanNext(ctypes.Structure):
     ]
 
 
+class KVCache(ctypes.Structure):
+    """``pgs_kv_cache`` of include/pageserve_amd.h."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + [
+        (name, ctypes.c_int64) for name in ("blocks", "block_size", "kv_heads", "head_dim", "k_block", "k_slot",
+                                            "k_head", "v_block", "v_slot", "v_head")]
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    """``pgs_tree_attention_args`` of include/pageserve_amd.h."""
+
+    _fields_ = (
+        [(name, ctypes.c_void_p) for name in ("q", "k", "v", "out")]
+        + [(name, ctypes.c_int64) for name in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "out_row",
+                                               "out_head")]
+        + [("cache", ctypes.POINTER(KVCache)), ("block_tables", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+           ("columns", ctypes.c_int64)]
+        + [(name, ctypes.c_void_p) for name in ("lens", "offsets", "parents")]
+        + [(name, ctypes.c_int64) for name in ("rows", "requests", "q_heads", "max_tokens", "max_context")]
+        + [("scale", ctypes.c_float), ("dtype", ctypes.c_int)])
+
+
 _VP = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
@@ -113,6 +135,17 @@ SIGNATURES = {
     "pgs_w8a16_decode_span_status": (_INT, [_VP, _INT, _VP]),
     "pgs_w8a16_decode_span_test_hooks": (_INT, [_INT, _INT]),
     "pgs_w8a16_decode_span_trace": (_INT, [_VP, _SZ]),
+    "pgs_packed4_bytes": (_I64, [_I64, _I64]),
+    "pgs_packed4_scales": (_I64, [_I64, _I64, _I64]),
+    "pgs_quantize4_packed": (_INT, [_VP, _INT, _I64, _I64, _I64, _VP, _VP, _VP]),
+    "pgs_dequantize4_packed": (_INT, [_VP, _VP, _I64, _I64, _I64, _VP, _INT, _VP]),
+    "pgs_w4a16_linear": (_INT, [_VP, _VP, _VP, _VP, _VP, _VP, _INT, _I64, _I64, _I64, _I64, _VP]),
+    "pgs_append_blocks": (_INT, [_VP, _VP, _VP, _I64, _I64, _VP, _I64, _VP, _I64, _I64, _VP, _VP, _I64, _VP, _VP,
+                                 _VP]),
+    "pgs_truncate_blocks": (_INT, [_VP, _VP, _VP, _I64, _I64, _VP, _I64, _VP, _I64, _I64, _VP]),
+    "pgs_write_kv": (_INT, [_VP, _I64, _I64, _VP, _I64, _I64, ctypes.POINTER(KVCache), _VP, _I64, _VP]),
+    "pgs_tree_attention": (_INT, [ctypes.POINTER(TreeAttentionArgs), _VP, _SZ, _VP]),
+    "pgs_tree_attention_workspace_bytes": (_SZ, [_I64] * 7),
 }
 
 _lock = threading.Lock()

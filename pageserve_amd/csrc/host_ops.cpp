@@ -15,6 +15,8 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <cmath>
 #include <string>
 #include <vector>
 
@@ -227,6 +229,282 @@ at::Tensor swiglu(const at::Tensor& x, const at::Tensor& qg, const at::Tensor& s
   return x.dim() == 2 ? act : act.view(out_shape(x, n));
 }
 
+// ---------------------------------------------------------------------------
+// 4-bit weights (pageserve_amd/quantization4.py)
+// ---------------------------------------------------------------------------
+
+// (codes, scales) of an fp32 or bf16 weight on a GPU, packed
+std::vector<at::Tensor> quantize4(const at::Tensor& w, int64_t group) {
+  const at::Device dev = w.device();
+  at::Tensor w2 = aligned(w, 16);
+  const int64_t n = w2.size(0), k = w2.size(1);
+  at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  at::Tensor qp = at::empty({std::max<int64_t>(pgs_packed4_bytes(n, k), 0)}, w2.options().dtype(at::kByte));
+  at::Tensor sp = at::empty({std::max<int64_t>(pgs_packed4_scales(n, k, group), 0)}, w2.options().dtype(at::kBFloat16));
+  void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+  check_rc(pgs_quantize4_packed(ptr(w2), w2.scalar_type() == at::kFloat ? PGS_DTYPE_F32 : PGS_DTYPE_BF16, n, k, group,
+                                ptr(qp), ptr(sp), st),
+           "quantize4");
+  return {qp, sp};
+}
+
+at::Tensor dequantize4(const at::Tensor& qp, const at::Tensor& sp, int64_t n, int64_t k, int64_t group, int64_t dtype) {
+  const at::Device dev = qp.device();
+  const auto t = dtype == PGS_DTYPE_F32 ? at::kFloat : dtype == PGS_DTYPE_BF16 ? at::kBFloat16 : at::kHalf;
+  at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  at::Tensor out = at::empty({n, k}, qp.options().dtype(t));
+  void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+  check_rc(pgs_dequantize4_packed(ptr(qp), ptr(sp), n, k, group, ptr(out), static_cast<int>(dtype), st), "dequantize4");
+  return out;
+}
+
+at::Tensor linear4(const at::Tensor& x, const at::Tensor& qp, const at::Tensor& sp, const Opt& bias, int64_t n,
+                   int64_t k, int64_t group, bool out_f32, const Opt& residual, const Opt& out) {
+  const at::Device dev = qp.device();
+  const char* what = "linear4";
+  if (x.device() != dev)
+    value_error("linear4: input on " + dev_str(x.device()) + " but weight on " + dev_str(dev));
+  if (x.scalar_type() != at::kBFloat16)
+    type_error("linear4: the W4A16 kernels take bf16 activations, got " + std::string(c10::toString(x.scalar_type())));
+  if (x.dim() < 1 || x.size(-1) != k)
+    value_error("linear4: input has " + std::to_string(x.dim() ? x.size(-1) : 0) + " features, weight expects " +
+                std::to_string(k));
+  int64_t m = 1;
+  for (int64_t i = 0; i + 1 < x.dim(); ++i) m *= x.size(i);
+  at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  at::Tensor x2 = aligned(x.dim() == 2 ? x : x.reshape({m, k}), 16);
+  at::Tensor b = check_bias(bias, n, dev, what), res, y;
+  const auto odt = out_f32 ? at::kFloat : at::kBFloat16;
+  if (out.has_value()) {
+    const at::Tensor& o = *out;
+    if (o.device() != dev || o.scalar_type() != odt || o.numel() != m * n || !o.is_contiguous())
+      value_error("linear4: out must be a contiguous " + std::string(c10::toString(odt)) + " tensor of " +
+                  std::to_string(m * n) + " elements on " + dev_str(dev));
+    y = o.view({m, n});
+  } else {
+    y = at::empty({m, n}, x2.options().dtype(odt));
+  }
+  if (residual.has_value()) {
+    const at::Tensor& r = *residual;
+    if (r.device() != dev || r.scalar_type() != at::kBFloat16 || r.dim() < 1 || r.size(-1) != n || r.numel() != m * n)
+      value_error("linear4: residual must be a bf16 [..., " + std::to_string(n) + "] tensor with " + std::to_string(m) +
+                  " rows on " + dev_str(dev));
+    res = r.reshape({m, n});
+    if (!res.is_contiguous()) res = res.contiguous();
+  }
+  void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+  check_rc(pgs_w4a16_linear(ptr(x2), ptr(qp), ptr(sp), b.defined() ? ptr(b) : nullptr,
+                            res.defined() ? ptr(res) : nullptr, ptr(y), out_f32 ? PGS_DTYPE_F32 : PGS_DTYPE_BF16, m, n, k,
+                            group, st),
+           "w4a16 linear");
+  return x.dim() == 2 ? y : y.view(out_shape(x, n));
+}
+
+// ---------------------------------------------------------------------------
+// the paged cache (pageserve_amd/paged.py)
+// ---------------------------------------------------------------------------
+
+void need_gpu(const at::Tensor& t, const char* what, const char* name) {
+  if (!t.is_cuda()) throw std::runtime_error(std::string(what) + ": " + name + " must be on a ROCm GPU");
+}
+
+// an int32 tensor of `n` elements (any count: -1), contiguous, on dev
+const int32_t* ints(const at::Tensor& t, int64_t n, const at::Device& dev, const char* what, const char* name) {
+  if (t.device() != dev)
+    value_error(std::string(what) + ": " + name + " on " + dev_str(t.device()) + " but the batch is on " + dev_str(dev));
+  if (t.scalar_type() != at::kInt) type_error(std::string(what) + ": " + name + " must be int32");
+  if (!t.is_contiguous() || (n >= 0 && t.numel() != n))
+    value_error(std::string(what) + ": " + name + " must be contiguous" +
+                (n >= 0 ? " with " + std::to_string(n) + " elements" : ""));
+  return static_cast<const int32_t*>(ptr(t));
+}
+int32_t* ints_out(const at::Tensor& t, int64_t n, const at::Device& dev, const char* what, const char* name) {
+  return const_cast<int32_t*>(ints(t, n, dev, what, name));
+}
+
+// block tables: int32 [requests, columns], columns contiguous
+int32_t* table(const at::Tensor& t, int64_t requests, const at::Device& dev, const char* what, int64_t& stride) {
+  if (t.device() != dev)
+    value_error(std::string(what) + ": block_tables on " + dev_str(t.device()) + " but the batch is on " + dev_str(dev));
+  if (t.scalar_type() != at::kInt) type_error(std::string(what) + ": block_tables must be int32");
+  if (t.dim() != 2 || t.size(0) != requests || (t.size(1) > 1 && t.stride(1) != 1) ||
+      (requests > 1 && t.stride(0) < t.size(1)))
+    value_error(std::string(what) + ": block_tables must be [" + std::to_string(requests) +
+                ", columns] with contiguous rows that do not overlap");
+  stride = requests > 1 ? t.stride(0) : t.size(1);
+  return static_cast<int32_t*>(ptr(t));
+}
+
+std::vector<at::Tensor> append_blocks(const at::Tensor& lens, const at::Tensor& new_lens, const at::Tensor& offsets,
+                                      const at::Tensor& block_tables, const at::Tensor& free_blocks,
+                                      const at::Tensor& free_count, int64_t block_size, int64_t rows, const Opt& index) {
+  const char* what = "append_blocks";
+  need_gpu(lens, what, "lens");
+  const at::Device dev = lens.device();
+  const int64_t n = lens.numel();
+  int64_t stride = 0;
+  int32_t* lp = ints_out(lens, n, dev, what, "lens");
+  const int32_t* np = ints(new_lens, n, dev, what, "new_lens");
+  const int32_t* op = ints(offsets, n + 1, dev, what, "offsets");
+  int32_t* tp = table(block_tables, n, dev, what, stride);
+  const int32_t* fp = ints(free_blocks, -1, dev, what, "free_blocks");
+  int32_t* cp = ints_out(free_count, 1, dev, what, "free_count");
+  if (rows < 0) value_error("append_blocks: rows must not be negative");
+  const int32_t* ip = index.has_value() ? ints(*index, rows, dev, what, "index") : nullptr;
+  at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  at::Tensor slots = at::empty({rows}, lens.options().dtype(at::kLong)), status = at::empty({n}, lens.options());
+  void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+  check_rc(pgs_append_blocks(lp, np, tp, stride, block_tables.size(1), fp, free_blocks.numel(), cp, block_size, n, op, ip,
+                             rows, static_cast<int64_t*>(ptr(slots)), static_cast<int32_t*>(ptr(status)), st),
+           what);
+  return {slots, status};
+}
+
+void truncate_blocks(const at::Tensor& lens, const at::Tensor& keep, const at::Tensor& block_tables,
+                     const at::Tensor& free_blocks, const at::Tensor& free_count, int64_t block_size) {
+  const char* what = "truncate_blocks";
+  need_gpu(lens, what, "lens");
+  const at::Device dev = lens.device();
+  const int64_t n = lens.numel();
+  int64_t stride = 0;
+  int32_t* lp = ints_out(lens, n, dev, what, "lens");
+  const int32_t* kp = ints(keep, n, dev, what, "keep");
+  int32_t* tp = table(block_tables, n, dev, what, stride);
+  int32_t* fp = ints_out(free_blocks, -1, dev, what, "free_blocks");
+  int32_t* cp = ints_out(free_count, 1, dev, what, "free_count");
+  at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+  check_rc(pgs_truncate_blocks(lp, kp, tp, stride, block_tables.size(1), fp, free_blocks.numel(), cp, block_size, n, st),
+           what);
+}
+
+int code_of(const at::Tensor& t, const char* what) {
+  if (t.scalar_type() == at::kBFloat16) return PGS_DTYPE_BF16;
+  if (t.scalar_type() == at::kHalf) return PGS_DTYPE_F16;
+  type_error(std::string(what) + ": tensors must be bf16 or fp16, got " + std::string(c10::toString(t.scalar_type())));
+}
+
+// the step of dimension d (0 where it has one index: never multiplied by another)
+int64_t step(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
+// k and v caches [blocks, block_size, kv_heads, head_dim] of one dtype on one device
+pgs_kv_cache check_cache(const at::Tensor& kc, const at::Tensor& vc, const char* what) {
+  for (const at::Tensor* t : {&kc, &vc}) {
+    need_gpu(*t, what, "the cache");
+    if (t->dim() != 4 || (t->size(3) > 1 && t->stride(3) != 1))
+      value_error(std::string(what) + ": k_cache and v_cache must be (blocks, block_size, kv_heads, head_dim) with a "
+                                      "contiguous head_dim");
+  }
+  if (kc.sizes() != vc.sizes() || kc.scalar_type() != vc.scalar_type() || kc.device() != vc.device())
+    value_error(std::string(what) + ": k_cache and v_cache must agree in shape, dtype and device");
+  return pgs_kv_cache{ptr(kc), ptr(vc), kc.size(0), kc.size(1), kc.size(2), kc.size(3), step(kc, 0), step(kc, 1),
+                      step(kc, 2), step(vc, 0), step(vc, 1), step(vc, 2)};
+}
+
+// rows [rows, heads, head_dim] of the cache's dtype, head_dim contiguous
+at::Tensor check_rows(const at::Tensor& t, int64_t rows, int64_t heads, const at::Tensor& kc, const char* what,
+                      const char* name) {
+  if (t.device() != kc.device())
+    value_error(std::string(what) + ": " + name + " on " + dev_str(t.device()) + " but the cache is on " +
+                dev_str(kc.device()));
+  if (t.scalar_type() != kc.scalar_type())
+    type_error(std::string(what) + ": " + name + " must have the cache's dtype");
+  if (t.dim() != 3 || t.size(0) != rows || (heads >= 0 && t.size(1) != heads) || t.size(2) != kc.size(3))
+    value_error(std::string(what) + ": " + name + " must be (" + std::to_string(rows) + ", " +
+                (heads >= 0 ? std::to_string(heads) : std::string("heads")) + ", " + std::to_string(kc.size(3)) + ")");
+  return t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t;
+}
+
+void write_kv(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
+              const at::Tensor& slots) {
+  const char* what = "write_kv";
+  const pgs_kv_cache c = check_cache(k_cache, v_cache, what);
+  code_of(k_cache, what);
+  const int64_t rows = slots.numel();
+  const at::Device dev = k_cache.device();
+  at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  at::Tensor kr = check_rows(k, rows, c.kv_heads, k_cache, what, "k");
+  at::Tensor vr = check_rows(v, rows, c.kv_heads, k_cache, what, "v");
+  if (slots.device() != dev)
+    value_error("write_kv: slots on " + dev_str(slots.device()) + " but the cache is on " + dev_str(dev));
+  if (slots.scalar_type() != at::kLong) type_error("write_kv: slots must be int64");
+  if (!slots.is_contiguous()) value_error("write_kv: slots must be contiguous");
+  void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+  check_rc(pgs_write_kv(ptr(kr), step(kr, 0), step(kr, 1), ptr(vr), step(vr, 0), step(vr, 1), &c,
+                        static_cast<const int64_t*>(ptr(slots)), rows, st),
+           what);
+}
+
+// rows usable by 16-byte accesses as they are, else a contiguous copy
+at::Tensor pieces(const at::Tensor& t) {
+  const bool ok = step(t, 0) % 8 == 0 && step(t, 1) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// whether the memory of contiguous `o` and of `t` can overlap
+bool overlap(const at::Tensor& o, const at::Tensor& t) {
+  if (!o.numel() || !t.numel()) return false;
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  const char *a = static_cast<const char*>(o.data_ptr()), *b = static_cast<const char*>(t.data_ptr());
+  return a < b + (last + 1) * t.element_size() && b < a + o.numel() * o.element_size();
+}
+
+at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache,
+                          const at::Tensor& v_cache, const at::Tensor& block_tables, const at::Tensor& lens,
+                          const at::Tensor& offsets, const Opt& parents, int64_t max_tokens, int64_t max_context,
+                          const c10::optional<double>& scale, const Opt& out) {
+  const char* what = "tree_attention";
+  const pgs_kv_cache c = check_cache(k_cache, v_cache, what);
+  pgs_tree_attention_args a{};
+  a.dtype = code_of(k_cache, what);
+  const at::Device dev = k_cache.device();
+  at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  if (q.dim() != 3) value_error("tree_attention: q must be (rows, q_heads, head_dim)");
+  a.rows = q.size(0);
+  a.q_heads = q.size(1);
+  at::Tensor qr = pieces(check_rows(q, a.rows, -1, k_cache, what, "q"));
+  at::Tensor kr = pieces(check_rows(k, a.rows, c.kv_heads, k_cache, what, "k"));
+  at::Tensor vr = pieces(check_rows(v, a.rows, c.kv_heads, k_cache, what, "v"));
+  a.requests = lens.numel();
+  a.lens = ints(lens, a.requests, dev, what, "lens");
+  a.offsets = ints(offsets, a.requests + 1, dev, what, "offsets");
+  if (parents.has_value()) {
+    a.parents = ints(*parents, a.rows, dev, what, "parents");
+  }
+  a.block_tables = table(block_tables, a.requests, dev, what, a.table_stride);
+  a.columns = block_tables.size(1);
+  at::Tensor o;
+  if (out.has_value()) {
+    o = *out;
+    if (o.device() != dev || o.scalar_type() != k_cache.scalar_type() || o.sizes() != q.sizes() || !o.is_contiguous() ||
+        reinterpret_cast<uintptr_t>(o.data_ptr()) % 16)
+      value_error("tree_attention: out must be a contiguous 16-byte aligned tensor of q's shape, dtype and device");
+    if (overlap(o, kr) || overlap(o, vr) || overlap(o, k_cache) || overlap(o, v_cache))
+      value_error("tree_attention: out must not share memory with k, v or the cache");
+  } else {
+    o = at::empty(q.sizes(), k_cache.options());
+  }
+  a.q = ptr(qr), a.k = ptr(kr), a.v = ptr(vr), a.out = ptr(o);
+  a.q_row = step(qr, 0), a.q_head = step(qr, 1);
+  a.k_row = step(kr, 0), a.k_head = step(kr, 1);
+  a.v_row = step(vr, 0), a.v_head = step(vr, 1);
+  a.out_row = step(o, 0), a.out_head = step(o, 1);
+  a.cache = &c;
+  a.max_tokens = max_tokens;
+  a.max_context = max_context >= 0 ? max_context : a.columns * c.block_size;
+  a.scale = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(c.head_dim)));
+  const size_t need = pgs_tree_attention_workspace_bytes(a.rows, a.requests, a.q_heads, c.kv_heads, c.head_dim,
+                                                         max_tokens, a.max_context);
+  // (a fresh workspace per call, from torch's caching allocator: ordered on this
+  // stream, and inside a capture the graph's own)
+  at::Tensor ws;
+  if (need) ws = at::empty({static_cast<int64_t>(need)}, k_cache.options().dtype(at::kByte));
+  void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+  check_rc(pgs_tree_attention(&a, need ? ws.data_ptr() : nullptr, need, st), what);
+  return o;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
@@ -236,4 +514,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("linear1", &linear1, "one W8A16 projection");
   mod.def("qkv_rope", &qkv_rope, "rms_norm, q|k|v projections and RoPE of q and k");
   mod.def("swiglu", &swiglu, "fused gate/up/silu*up");
+  mod.def("quantize4", &quantize4, "4-bit codes and group scales of a weight, packed");
+  mod.def("dequantize4", &dequantize4, "the dense weight of packed 4-bit codes");
+  mod.def("linear4", &linear4, "one W4A16 projection");
+  mod.def("append_blocks", &append_blocks, "block tables extended, slots of the new rows");
+  mod.def("truncate_blocks", &truncate_blocks, "requests shortened, their blocks given back");
+  mod.def("write_kv", &write_kv, "key and value rows stored at their slots");
+  mod.def("tree_attention", &tree_attention, "attention of drafted tokens over a paged cache");
 }

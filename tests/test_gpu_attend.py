@@ -1,0 +1,321 @@
+"""Tree attention over the paged cache against the oracle in 64 bits.
+
+Tolerance per output.  A score is a sum of D exact products, each addition off by at
+most 2^-23 of the magnitudes, then scaled: off by (D + 4) 2^-23 reach, reach = scale
+max sum |q||k|.  So a weight p = 2^(score - m) is off by a factor of 1 + e, e = (D + 8)
+2^-23 reach + 2^-20 (its own exponent's rounding lies in reach; v_exp_f32 and the
+rescaling by a few more units), and its rounding to the type t by u = half a step of
+t; a p that fp16 rounds to a multiple of 2^-24 may be off by 2^-25 instead, times at most
+`keys` of them against a sum of at least 1.  out = sum p v / sum p with the same rounded
+p above and below: off by (u + e) sum w (|v| + |out|), and a few fp32 additions in each of
+keys / 32 steps, (keys / 32 + 64) 2^-23 of that sum; then the output's own rounding."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import drafting_oracle as D
+from pageserve_amd import tree_attention
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+class Batch:
+    """A batch of requests on the CPU in float64-representable values of a type."""
+
+    def __init__(self, seed, lens, tokens, heads, kv, dim, bs, dtype, parents="tree", pad=0, columns=None):
+        rng = np.random.default_rng(seed)
+        self.heads, self.kv, self.dim, self.bs, self.dtype = heads, kv, dim, bs, dtype
+        self.lens, self.offsets = list(lens), np.concatenate([[0], np.cumsum(tokens)]).astype(int).tolist()
+        rows = self.offsets[-1] + pad
+
+        def values(*shape):
+            return torch.from_numpy(rng.standard_normal(shape)).to(dtype)
+
+        self.q, self.k, self.v = values(rows, heads, dim), values(rows, kv, dim), values(rows, kv, dim)
+        have = [-(-n // bs) for n in lens]
+        blocks = sum(have) + 2
+        self.kc, self.vc = values(blocks, bs, kv, dim), values(blocks, bs, kv, dim)
+        order, at = rng.permutation(blocks).tolist(), 0
+        columns = columns if columns is not None else max(have)
+        self.tables = np.full((len(have), columns), -1, dtype=np.int32)
+        for b, h in enumerate(have):
+            self.tables[b, :h] = order[at:at + h]
+            at += h
+        self.parents = None
+        if parents == "tree":
+            local = np.concatenate([np.arange(t) for t in tokens] + [np.zeros(pad)]).astype(int)
+            self.parents = np.maximum(local - 1 - (rng.random(rows) ** 2 * 5).astype(int), -1)
+        elif parents == "roots":
+            self.parents = np.full(rows, -1)
+
+    def oracle(self, scale=None, max_tokens=64):
+        f = lambda t: t.to(torch.float64).numpy()  # noqa: E731
+        return D.tree_attention(f(self.q), f(self.k), f(self.v), f(self.kc), f(self.vc), self.tables, self.lens,
+                                self.offsets, None if self.parents is None else self.parents.tolist(),
+                                self.dim ** -0.5 if scale is None else scale, max_tokens)
+
+    def args(self, gpu):
+        i = lambda a: torch.as_tensor(np.asarray(a), dtype=torch.int32).to(gpu)  # noqa: E731
+        return [t.to(gpu) for t in (self.q, self.k, self.v, self.kc, self.vc)] + [
+            i(self.tables), i(self.lens), i(self.offsets), None if self.parents is None else i(self.parents)]
+
+    def check(self, got, want, what=""):
+        out, spread, reach = want
+        got = got.to(torch.float64).cpu().numpy()
+        live = ~np.isnan(out)
+        keys = max(list(self.lens) + [0]) + 64
+        u = U[self.dtype]
+        e = (self.dim + 8) * 2.0 ** -23 * reach[..., None] + 2.0 ** -20 + (keys / 32 + 64) * 2.0 ** -23
+        if self.dtype is torch.float16:
+            e = e + keys * 2.0 ** -25
+        tol = (u + e) * spread
+        tol = tol + u * (np.abs(out) + tol) + 2.0 ** -25
+        off = np.where(live, np.abs(got - out) - tol, -1)
+        assert not np.isnan(off).any(), f"{what}: not a number"
+        assert (off <= 0).all(), f"{what}: {off.max():.3g} over the bound at {np.unravel_index(off.argmax(), off.shape)}"
+
+
+HEADS = {"3b": (16, 2, 128), "0.5b": (14, 2, 64), "one": (1, 1, 64), "each": (4, 4, 128), "wide": (24, 1, 128),
+         "odd": (15, 3, 64)}
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("tokens", [1, 2, 5, 16, 31, 64])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_lengths_and_trees(gpu, heads, tokens, dtype):
+    lens = [0, 1, 15, 16, 17, 33, 200]
+    rng = np.random.default_rng(tokens)
+    counts = [tokens] + rng.integers(0, tokens + 1, len(lens) - 2).tolist() + [tokens]
+    b = Batch(tokens, lens, counts, *HEADS[heads], 16, dtype)
+    want = b.oracle()
+    b.check(tree_attention(*b.args(gpu), max_tokens=tokens), want, "max_tokens given")
+    b.check(tree_attention(*b.args(gpu)), want, "defaults")
+    # any expected context gives the same result to rounding: other splits
+    for context in (0, 100, 5000, 10 ** 6):
+        b.check(tree_attention(*b.args(gpu), max_context=context, max_tokens=tokens), want, f"max_context={context}")
+
+
+@pytest.mark.parametrize("lens,tokens,bs", [([1500, 3], [1, 1], 16), ([4000], [7], 48), ([2000, 0, 777], [40, 64, 3], 64),
+                                            ([31, 32, 33, 64, 65], [1, 2, 1, 2, 1], 32), ([2049], [1], 256)])
+@pytest.mark.parametrize("parents", ["tree", "chain", "roots"])
+def test_longer_contexts(gpu, lens, tokens, bs, parents):
+    b = Batch(sum(lens), lens, tokens, 16, 2, 128, bs, torch.bfloat16, parents)
+    b.check(tree_attention(*b.args(gpu), max_tokens=max(tokens), max_context=max(lens)), b.oracle())
+
+
+def test_scales_and_sharp_maxima(gpu):
+    b = Batch(4, [300, 90], [9, 20], 14, 2, 64, 16, torch.bfloat16)
+    for scale in (0.0, -0.3, 1.0, 4.0):
+        b.check(tree_attention(*b.args(gpu), scale=scale), b.oracle(scale), f"scale={scale}")
+    # scores that rise all along, and one key far above the rest, late
+    b.kc *= torch.linspace(0.1, 3, b.kc.shape[0])[:, None, None, None].to(b.dtype)
+    b.k[:, :, :] *= 4
+    b.check(tree_attention(*b.args(gpu)), b.oracle(), "rising")
+
+
+def test_padded_and_cut_batches(gpu):
+    b = Batch(5, [40, 7, 0], [3, 70, 9], 16, 2, 128, 16, torch.float16, pad=6)
+    out = torch.full(b.q.shape, 3.0, dtype=b.dtype, device=gpu)
+    args = b.args(gpu)
+    got = tree_attention(*args, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    want = b.oracle()
+    b.check(got, want)
+    rest = torch.from_numpy(np.isnan(want[0])).to(gpu)  # rows 64.. of the second request, rows of none
+    assert rest[:, 0, 0].nonzero().squeeze(1).tolist() == list(range(67, 73)) + list(range(82, 88)) and (out[rest] == 3).all()
+    out.fill_(3)
+    tree_attention(*args, out=out, max_tokens=4)
+    want = b.oracle(max_tokens=4)
+    b.check(out, want)
+    assert (out[torch.from_numpy(np.isnan(want[0])).to(gpu)] == 3).all()
+    # in place of q
+    q = args[0].clone()
+    tree_attention(q, *args[1:], out=q, max_context=0)
+    b.check(q, b.oracle())
+
+
+def test_absent_blocks_and_lengths_out_of_range(gpu):
+    b = Batch(6, [100, 64, 50], [5, 33, 2], 16, 2, 128, 16, torch.bfloat16)
+    b.tables[0, 2], b.tables[0, 6], b.tables[1, :], b.tables[2, 0] = -1, 2 ** 31 - 1, -5, b.kc.shape[0]
+    b.check(tree_attention(*b.args(gpu)), b.oracle(), "absent blocks")
+    b.lens = [10 ** 9, -4, 2 ** 31 - 1]  # cut to the table's columns; none
+    want = b.oracle()
+    b.check(tree_attention(*b.args(gpu)), want, "lengths")
+    args = b.args(gpu)
+    args[7] = torch.tensor([-3, 10 ** 6, 1, 7], dtype=torch.int32, device=gpu)
+    assert tree_attention(*args).shape == b.q.shape
+    args[8] = torch.full_like(args[8], 2 ** 31 - 1)
+    args[7] = b.args(gpu)[7]
+    b.parents = np.full(b.q.shape[0], -1)
+    b.check(tree_attention(*args), b.oracle(), "parents out of range")
+
+
+def test_what_is_not_seen_does_not_matter(gpu):
+    """Infinities and NaN in the cache behind the length, in blocks of no table and in
+    drafted tokens that a row does not descend from."""
+    for dtype in (torch.bfloat16, torch.float16):
+        b = Batch(7, [37, 0, 20], [6, 40, 34], 16, 2, 128, 16, dtype)
+        used = {int(x) for x in b.tables.ravel() if x >= 0}
+        for c in (b.kc, b.vc):
+            for blk in set(range(c.shape[0])) - used:
+                c[blk] = float("nan")
+            c[int(b.tables[0, 2]), 5:] = float("inf")
+            c[int(b.tables[2, 1]), 4:] = float("nan")
+        b.check(tree_attention(*b.args(gpu)), b.oracle(), "behind the length")
+        # tokens 0 (request 0), 7 and 39 (request 1) are not finite: only they and their descendants show it
+        for row, value in ((0, float("nan")), (13, float("inf")), (45, -float("inf"))):
+            b.v[row, :, 3:70] = value
+        clean = Batch(7, [37, 0, 20], [6, 40, 34], 16, 2, 128, 16, dtype)
+        for c, d in ((b.kc, clean.kc), (b.vc, clean.vc)):
+            d.copy_(c)
+        want = clean.oracle()
+        got = tree_attention(*b.args(gpu)).cpu()
+        for r in range(3):
+            lo, hi = b.offsets[r], b.offsets[r + 1]
+            see = D.ancestors(b.parents[lo:hi].tolist())
+            for t in range(hi - lo):
+                hit = [lo + j for j in see[t] if not torch.isfinite(b.v[lo + j]).all()]
+                touched = torch.zeros(128, dtype=torch.bool)
+                touched[3:70] = bool(hit)
+                assert torch.equal(~torch.isfinite(got[lo + t]), touched.expand(16, 128)), (r, t)
+                if len(hit) == 1:
+                    assert torch.equal(torch.nan_to_num(got[lo + t, 0, 3:5].float(), nan=7.0),
+                                       torch.nan_to_num(b.v[hit[0], 0, 3:5].float(), nan=7.0))
+        got[~torch.isfinite(got)] = 0
+        out = np.where(torch.isfinite(tree_attention(*b.args(gpu))).cpu().numpy(), want[0], 0)
+        clean.check(got, (out, want[1], want[2]), "the rest")
+
+
+def test_layouts_and_copies(gpu):
+    b = Batch(8, [70, 20, 130], [3, 8, 1], 16, 2, 128, 16, torch.bfloat16)
+    args = b.args(gpu)
+    want = tree_attention(*args)
+    b.check(want, b.oracle())
+    # q, k and v as parts of one projection's rows
+    n = b.q.shape[0]
+    wide = torch.cat([t.reshape(n, -1) for t in args[:3]], 1)
+    parts = [p.view(n, -1, 128) for p in wide.split([2048, 256, 256], 1)]
+    assert torch.equal(tree_attention(*parts, *args[3:]), want)
+    # one cache tensor, halves interleaved; heads in front of slots; wide table rows
+    both = torch.stack(args[3:5], 1)
+    assert torch.equal(tree_attention(*args[:3], both[:, 0], both[:, 1], *args[5:]), want)
+    first = [c.transpose(1, 2).contiguous().transpose(1, 2) for c in args[3:5]]
+    assert torch.equal(tree_attention(*args[:3], *first, *args[5:]), want)
+    table = torch.full((3, 50), -9, dtype=torch.int32, device=gpu)
+    table[:, 7:7 + args[5].shape[1]] = args[5]
+    assert torch.equal(tree_attention(*args[:5], table[:, 7:7 + args[5].shape[1]], *args[6:]), want)
+    # a row stride of 1 element more, and a transposed head_dim: copied
+    odd = torch.zeros(n, 2049, dtype=b.dtype, device=gpu)
+    odd[:, 1:] = args[0].view(n, -1)
+    turned = args[1].transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(tree_attention(odd[:, 1:].view(n, 16, 128), turned, *args[2:]), want)
+    # one row of keys for every token
+    k1 = args[1][:1].expand(n, 2, 128)
+    assert torch.equal(tree_attention(args[0], k1, *args[2:]), tree_attention(args[0], k1.contiguous(), *args[2:]))
+    # nothing to do
+    none = [a[:0] for a in args[:3]] + args[3:]
+    none[7], none[8] = torch.zeros(4, dtype=torch.int32, device=gpu), None
+    assert tree_attention(*none).shape == (0, 16, 128)
+
+
+def test_cache_past_four_gigabytes(gpu):
+    b = Batch(9, [100, 37], [4, 1], 8, 4, 128, 64, torch.bfloat16)
+    args = b.args(gpu)
+    big = [torch.empty(70000, 64, 4, 128, dtype=b.dtype, device=gpu) for _ in range(2)]  # 4.6 GB each
+    shift = 70000 - b.kc.shape[0]
+    for c, a in zip(big, args[3:5]):
+        c[shift:] = a
+    got = tree_attention(*args[:3], *big, torch.where(args[5] >= 0, args[5] + shift, -1), *args[6:])
+    assert torch.equal(got, tree_attention(*args))
+
+
+def test_captured_and_replayed_with_other_lengths(gpu):
+    """One graph serves steps whose lengths, trees and tables differ; two graphs on one
+    pool and eager calls between do not disturb it."""
+    steps = [Batch(20 + i, lens, tokens, 16, 2, 128, 16, torch.bfloat16, pad=24 - sum(tokens), columns=128)
+             for i, (lens, tokens) in enumerate([([2000, 100, 5], [8, 8, 8]), ([3, 0, 2048], [1, 0, 12]),
+                                                 ([500, 501, 502], [12, 1, 11])])]
+    big = max(s.kc.shape[0] for s in steps)
+    live = [torch.zeros_like(t) for t in steps[0].args(gpu)]
+    live[3], live[4] = (torch.zeros(big, 16, 2, 128, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+
+    def load(s):
+        for dst, src in zip(live, s.args(gpu)):
+            (dst[:src.shape[0]] if dst.dim() == 4 else dst).copy_(src)
+
+    load(steps[0])
+    pool = torch.cuda.graph_pool_handle()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(tree_attention(*live, max_tokens=12, max_context=2048))
+        graphs.append(g)
+    for turn in range(2):
+        for s in steps:
+            load(s)
+            rows = s.offsets[-1]
+            eager = tree_attention(*live, max_tokens=12, max_context=2048)[:rows].clone()
+            s.check(torch.cat([eager, eager.new_zeros(24 - rows, 16, 128)]), s.oracle())
+            for g, o in zip(graphs, outs):
+                g.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(o[:rows], eager)
+
+
+def test_side_stream(gpu):
+    b = Batch(11, [3000], [4], 16, 2, 128, 16, torch.bfloat16)
+    args = b.args(gpu)
+    want = tree_attention(*args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [tree_attention(*args) for _ in range(3)]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(g, want) for g in got)
+
+
+def test_refusals(gpu):
+    b = Batch(12, [20, 3], [2, 2], 16, 2, 128, 16, torch.bfloat16)
+    good = b.args(gpu)
+
+    def bad(error, match, at=None, value=None, **kw):
+        args = list(good)
+        if at is not None:
+            args[at] = value
+        with pytest.raises(error, match=match):
+            tree_attention(*args, **kw)
+
+    q, k, v, kc, vc, tables, lens, offsets, parents = good
+    bad(RuntimeError, "ROCm GPU", 3, kc.cpu())
+    bad(ValueError, "q on cpu", 0, q.cpu())
+    bad(TypeError, "cache's dtype", 0, q.half())
+    bad(ValueError, "q must be", 0, q[0])
+    bad(ValueError, "k must be", 1, k[:3])
+    bad(ValueError, "multiple of kv_heads", 0, q[:, :15])
+    bad(ValueError, "agree", 4, vc[:1])
+    bad(TypeError, "int32", 6, lens.long())
+    bad(ValueError, "offsets", 7, offsets[:2])
+    bad(ValueError, "parents", 8, parents[:2])
+    bad(ValueError, "block_tables", 5, tables[:1])
+    bad(ValueError, "max_tokens", max_tokens=0)
+    bad(ValueError, "max_tokens", max_tokens=65)
+    bad(ValueError, "scale", scale=float("nan"))
+    bad(ValueError, "out must be", out=torch.empty_like(q)[:2])
+    bad(ValueError, "out must be", out=torch.empty_like(q).float())
+    bad(ValueError, "share memory", at=2, value=q[:, :2], out=q)
+    small = [t[..., :32] for t in good[:5]] + good[5:]
+    with pytest.raises(ValueError, match="head_dim"):
+        tree_attention(*small)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        tree_attention(*good[:3], kc[:, :8].contiguous(), vc[:, :8].contiguous(), *good[5:])
+    shifted = torch.empty(kc.numel() + 1, dtype=kc.dtype, device=gpu)[1:].view(kc.shape)
+    with pytest.raises(ValueError, match="aligned"):
+        tree_attention(*good[:3], shifted, vc, *good[5:])
+    with pytest.raises(ValueError, match="contiguous head_dim"):
+        tree_attention(*good[:3], kc.transpose(1, 3), vc.transpose(1, 3), *good[5:])
