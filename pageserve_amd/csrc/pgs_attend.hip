@@ -31,10 +31,14 @@
 // kernel from fp32 partial outputs in the workspace.
 #include <math.h>
 
+#include <algorithm>
+
 #include "pgs_fp4.h"
 
 namespace pgs {
 namespace {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4;
 constexpr int kMaxTree = 64;
@@ -47,16 +51,35 @@ struct Attend {
   int64_t kc_block, kc_head, vc_block, vc_head;
   uint32_t kc_slot, vc_slot;
   int32_t blocks, bs;
+  uint32_t bs_inv;  // ceil(2^32 / bs)
   const int32_t* tables;
   int64_t tstride;
   int32_t cols;
   const int32_t *lens, *offsets, *parents;
   int32_t rows, requests, q_heads, kv_heads, group;  // group: q_heads / kv_heads
   int32_t max_tokens, row_groups, splits;
-  float c;       // scale * log2(e)
-  float* part;   // [rows * q_heads][splits][D] (splits > 1)
-  float* stat;   // [rows * q_heads][splits][2]: m, l
+  float c;      // scale * log2(e)
+  float* part;  // sums of the parts of rows: [slots][D], slots as Wave::store's caller numbers them
+  float* stat;  // [slots][2]: m, l
 };
+
+// The lane number where it is used: lane-dependent offsets computed from it are not kept
+// in registers across a loop.
+__device__ __forceinline__ int here(int lane) {
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
+// The kernel's argument again, read from its segment at this point: for the parts of a
+// kernel outside its inner loop, whose fields would otherwise all sit in scalar
+// registers throughout (and push vector registers out to memory).
+__device__ __forceinline__ Attend again() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  Attend a;
+  __builtin_memcpy(&a, (const void*)p, sizeof(a));
+  return a;
+}
 
 template <bool F16>
 struct Elem;
@@ -87,11 +110,23 @@ struct Elem<true> {
   static constexpr uint32_t kOnes = 0x3c003c00u, kExp = 0x7c00u;
 };
 
-// the maximum over lanes l, l ^ 16, l ^ 32, l ^ 48
+// the maximum over lanes l, l ^ 16, l ^ 32, l ^ 48 (each swap leaves the two halves
+// of its exchange in two registers)
 __device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  const uint32_t x = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  const uint32_t y = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+
+// A maximum nothing has raised yet: 2^(kLow - m) = 0 for every m of a score.
+constexpr float kLow = -3.0e38f;
+// The reference of the exponents follows the maximum only when a score exceeds it
+// by this (in powers of two): p stays below 2^8, in range for fp16 and as exact in
+// either type as below 1, and the sums are rescaled a few times per row instead of
+// at every step.
+constexpr float kSlack = 8.0f;
 
 // The request of a unit and its sizes, each brought into range: whatever the device
 // arrays hold, no access leaves the tensors.
@@ -111,54 +146,58 @@ __device__ __forceinline__ Request request(const Attend& a, int b) {
   return r;
 }
 
-template <int D, int R, int WR, bool F16>
-__global__ __launch_bounds__(64 * kWaves) void attend_kernel(Attend a) {
+// token / bs without a division: the product's high half is the quotient or one more
+// (bs_inv is too large by less than 1, token below 2^31), which the remainder's sign
+// shows
+__device__ __forceinline__ int block_of(const Attend& a, int token, int& slot) {
+  int q = static_cast<int>(__umulhi(static_cast<uint32_t>(token), a.bs_inv));
+  int r = token - q * a.bs;
+  if (r < 0) --q, r += a.bs;
+  slot = r;
+  return q;
+}
+
+// 16 R rows of a wave and their running sums.
+template <int D, int R, bool F16>
+struct Wave {
   using E = Elem<F16>;
-  constexpr int WK = kWaves / WR;  // key slices
-  constexpr int DC = D / 32;       // 32-dim chunks of a key
-  constexpr int DV = D / 16;       // dims of a value row per lane
-  constexpr int VW = DV / 2;       // their dwords
-  const int lane = threadIdx.x & 63;
-  const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
-  const int li = lane & 15, lg = lane >> 4;
-  const int wr = wave % WR, wk = wave / WR;
+  static constexpr int DC = D / 32;  // 32-dim chunks of a key
+  static constexpr int DV = D / 16;  // dims of a value row per lane
+  static constexpr int VW = DV / 2;  // their dwords
+  int tk[R];                         // token of this lane's row (rows past the last repeat it)
+  u32x4 q[R][DC];
+  f32x4 o[R][DV], l[R];
+  float mx[R];
 
-  // unit: ((request, key head), part, row group); the row groups of one part are
-  // neighbours on one XCD, whose L2 then holds the part's keys
-  int unit = xcd_remap(blockIdx.x, gridDim.x);
-  const int rg = unit % a.row_groups;
-  unit /= a.row_groups;
-  const int part = unit % a.splits;
-  unit /= a.splits;
-  const int kh = unit % a.kv_heads, b = unit / a.kv_heads;
-  const Request rq = request(a, b);
-  const int nrows = rq.tokens * a.group;
-  const int wg_row0 = rg * (16 * R * WR);
-  if (wg_row0 >= nrows) return;
-  const int row0 = wg_row0 + wr * (16 * R);  // of this wave
-
-  // the steps of this part: [t0, t1) of len_tiles + tree_tiles
-  const int tiles = rq.len_tiles + rq.tree_tiles;
-  const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * part / a.splits);
-  const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / a.splits);
-
-  // rows of this lane, one per R: token tk, head hd (rows past the last repeat it)
-  int tk[R];
-  u32x4 qf[R][DC];
+  __device__ __forceinline__ void load(const Attend& a, const Request& rq, int kh, int row0, int nrows, int li, int lg) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = min(row0 + 16 * r + li, nrows - 1);
-    tk[r] = row / a.group;
-    const uint16_t* p = a.q + (rq.row0 + tk[r]) * a.q_row + (kh * a.group + row - tk[r] * a.group) * a.q_head + 8 * lg;
+    for (int r = 0; r < R; ++r) {
+      const int row = min(row0 + 16 * r + li, nrows - 1);
+      tk[r] = row / a.group;
+      const uint16_t* p = a.q + (rq.row0 + tk[r]) * a.q_row + (kh * a.group + row - tk[r] * a.group) * a.q_head + 8 * lg;
 #pragma unroll
-    for (int d = 0; d < DC; ++d) qf[r][d] = ld16(p + 32 * d);
+      for (int d = 0; d < DC; ++d) q[r][d] = ld16(p + 32 * d);
+    }
+    // (they have arrived here: a wait for them inside the loop over the keys would be
+    // a wait for the keys on their way too)
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int d = 0; d < DC; ++d) asm volatile("" : "+v"(q[r][d]));
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mx[r] = kLow;
+      l[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < DV; ++i) o[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
   }
 
-  // ancestors of each row's token as a bit mask over the request's drafted tokens:
-  // lane t starts with bit t and its parent; each step adds the parent's mask and
-  // takes the parent's parent, which doubles the distance covered
-  unsigned long long sees[R];
-  if (t1 > rq.len_tiles) {
+  // see[t] (LDS, the wave's own): which of the request's drafted tokens token t attends
+  // to, itself and its ancestors, as a bit mask.  Lane t starts with bit t and its
+  // parent; each step adds the parent's mask and takes the parent's parent, which
+  // doubles the distance covered.
+  static __device__ __forceinline__ void trees(const Attend& a, const Request& rq, int lane, unsigned long long* see) {
     unsigned long long m = 1ull << lane;
     int par = -1;
     if (lane < rq.tokens) par = a.parents ? a.parents[rq.row0 + lane] : lane - 1;
@@ -171,334 +210,835 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(Attend a) {
         par = pp;
       }
     }
-#pragma unroll
-    for (int r = 0; r < R; ++r) sees[r] = __shfl(m, tk[r]);
+    see[lane] = m;
   }
 
-  f32x4 o[R][DV], l[R];
-  float mx[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    mx[r] = -INFINITY;
-    l[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < DV; ++i) o[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  const int32_t* table = a.tables + b * a.tstride;
-  const u32x4 ones = {E::kOnes, E::kOnes, E::kOnes, E::kOnes};
-
-  for (int t = t0 + wk; t < t1; t += WK) {
-    const bool tree = t >= rq.len_tiles;
-    const int key0 = (tree ? t - rq.len_tiles : t) * 32;
-    const int limit = (tree ? rq.tokens : rq.len);  // keys of this kind
-    // each 16-key half: a uniform base and the last key of it that exists (a key
-    // past the end reads that one instead and is masked)
-    const uint16_t *kb[2], *vb[2];
-    int last[2];
-    bool bad[2];
-    uint32_t ks, vs;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int first = min(key0 + 16 * h, limit - 1);
-      if (tree) {
-        kb[h] = a.k + (rq.row0 + first) * a.k_row + kh * a.k_head;
-        vb[h] = a.v + (rq.row0 + first) * a.v_row + kh * a.v_head;
-        bad[h] = false;
-      } else {
-        const int blk = first / a.bs;
-        const int id = table[blk];
-        bad[h] = id < 0 || id >= a.blocks;
-        const int64_t at = bad[h] ? 0 : id, slot = first - blk * a.bs;
-        kb[h] = a.kc + at * a.kc_block + slot * a.kc_slot + kh * a.kc_head;
-        vb[h] = a.vc + at * a.vc_block + slot * a.vc_slot + kh * a.vc_head;
-      }
-      last[h] = limit - 1 - first;
-    }
-    ks = tree ? static_cast<uint32_t>(a.k_row) : a.kc_slot;
-    vs = tree ? static_cast<uint32_t>(a.v_row) : a.vc_slot;
-
-    u32x4 kf[2][DC];
-    uint32_t vf[8][VW];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint16_t* p = kb[h] + static_cast<uint32_t>(min(li, last[h])) * ks + 8 * lg;
-#pragma unroll
-      for (int d = 0; d < DC; ++d) kf[h][d] = ld16(p + 32 * d);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int h = e >> 2;
-      const uint16_t* p = vb[h] + static_cast<uint32_t>(min(4 * lg + (e & 3), last[h])) * vs + DV * li;
-      if constexpr (VW == 4) {
-        const u32x4 x = ld16(p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vf[e][i] = x[i];
-      } else {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) vf[e][i] = x[i];
-      }
-    }
-
-    // scores: lane's keys key0 + 16 h + 4 lg + i
+  // One step: keys key0 .. key0 + 31 of `limit` (cached, or with tree drafted).
+  // k: A operands of the two 16-key halves; values(v): the lane's eight keys x DV dims.
+  // masked: some key is past the limit, in an absent block (bad) or drafted.
+  // odd: drafted keys whose values are not finite (v holds zeros for them); value(j)
+  // is the row of key key0 + j.
+  template <typename Values, typename Value>
+  __device__ __forceinline__ void step(const Attend& a, const u32x4 (&k)[2][DC], Values values, int key0, int limit,
+                                       bool tree, bool masked, bool bad0, bool bad1, uint32_t odd,
+                                       const unsigned long long* see, int li, int lg, Value value) {
+    // lane's scores: keys key0 + 16 h + 4 lg + i
     f32x4 s[R][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        s[r][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < DC; ++d) s[r][h] = E::mfma(k[h][d], q[r][d], s[r][h]);
+      }
+    uint32_t v[8][VW];
+    values(v);
+    // exponents against the row's reference, and whether a row needs a new one
+    float x[R][8];
+    uint32_t ok[R];
+    bool over = false;
+    if (masked) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const unsigned long long sees = tree ? see[tk[r]] : ~0ull;
+        ok[r] = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = key0 + 16 * (e >> 2) + 4 * lg + (e & 3);
+          const bool in = key < limit && !(e >> 2 ? bad1 : bad0) && (sees >> (key & 63) & 1);
+          ok[r] |= in ? 1u << e : 0;
+          x[r][e] = in ? fmaf(s[r][e >> 2][e & 3], a.c, -mx[r]) : -INFINITY;
+          over = over || x[r][e] > kSlack;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        ok[r] = 0xff;
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[r][e] = fmaf(s[r][e >> 2][e & 3], a.c, -mx[r]);
+          top = fmaxf(top, x[r][e]);
+        }
+        over = over || top > kSlack;
+      }
+    }
+    if (__ballot(over)) {
+      // new references: the largest score of each row so far
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float t = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t = fmaxf(t, ok[r] >> e & 1 ? s[r][e >> 2][e & 3] * a.c : -INFINITY);
+        const float ref = fmaxf(quad_max(t), mx[r]), f = __builtin_amdgcn_exp2f(mx[r] - ref);
+        mx[r] = ref;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[r][i] *= f;
+#pragma unroll
+        for (int d = 0; d < DV; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[r][d][i] *= f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[r][e] = ok[r] >> e & 1 ? fmaf(s[r][e >> 2][e & 3], a.c, -ref) : -INFINITY;
+      }
+    }
+    u32x4 p[R];
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s[r][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < 4; ++i)
+        p[r][i] = E::pack(__builtin_amdgcn_exp2f(x[r][2 * i]), __builtin_amdgcn_exp2f(x[r][2 * i + 1]));
+    const u32x4 ones = {E::kOnes, E::kOnes, E::kOnes, E::kOnes};
 #pragma unroll
-        for (int d = 0; d < DC; ++d) s[r][h] = E::mfma(kf[h][d], qf[r][d], s[r][h]);
+    for (int r = 0; r < R; ++r) l[r] = E::mfma(ones, p[r], l[r]);
+#pragma unroll
+    for (int d = 0; d < DV; ++d) {
+      u32x4 vt;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        vt[e] = __builtin_amdgcn_perm(v[2 * e + 1][d >> 1], v[2 * e][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+      for (int r = 0; r < R; ++r) o[r][d] = E::mfma(vt, p[r], o[r][d]);
+    }
+    for (uint32_t w = odd; w; w &= w - 1) {
+      const int j = __builtin_ctz(w);
+      const uint16_t* row = value(j);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint32_t lo = j & 2 ? p[r][1] : p[r][0], hi = j & 2 ? p[r][3] : p[r][2];
+        const float pj = E::low(__shfl(j & 16 ? hi : lo, 16 * (j >> 2 & 3) + li) >> (16 * (j & 1)));
+        if (!(see[tk[r]] >> ((key0 + j) & 63) & 1)) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int d = 0; d < DV; ++d) o[r][d][i] += pj * E::low(row[(4 * lg + i) * DV + d]);
       }
-    const bool masked = tree || key0 + 32 > limit || bad[0] || bad[1];
+    }
+  }
+
+  // The rows' outputs, or (whole false: other keys of theirs are elsewhere) their
+  // sums: lane's dims (4 lg + i) DV + d.  slot(row, token, head): where to.
+  template <typename Slot>
+  __device__ __forceinline__ void store(const Attend& a, const Request& rq, int kh, int row0, int nrows, int li, int lg,
+                                        bool whole, Slot slot) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = row0 + 16 * r + li;
+      if (row >= nrows) continue;
+      const int head = kh * a.group + row - tk[r] * a.group;
+      const int64_t token = rq.row0 + tk[r];
+      if (whole) {
+        const float inv = l[r][0] == 0.f ? 0.f : 1.f / l[r][0];
+        uint16_t* d = a.out + token * a.out_row + head * a.out_head + 4 * lg * DV;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w[VW];
+#pragma unroll
+          for (int e = 0; e < VW; ++e) w[e] = E::pack(o[r][2 * e][i] * inv, o[r][2 * e + 1][i] * inv);
+          if constexpr (VW == 4) *reinterpret_cast<u32x4*>(d + i * DV) = u32x4{w[0], w[1], w[2], w[3]};
+          else *reinterpret_cast<u32x2*>(d + i * DV) = u32x2{w[0], w[1]};
+        }
+      } else {
+        const int64_t at = slot(row, token, head);
+        float* d = a.part + at * D + 4 * lg * DV;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < DV; e += 4)
+            *reinterpret_cast<f32x4*>(d + i * DV + e) =
+                f32x4{o[r][e][i], o[r][e + 1][i], o[r][e + 2][i], o[r][e + 3][i]};
+        if (lg == 0) {
+          a.stat[2 * at] = mx[r];
+          a.stat[2 * at + 1] = l[r][0];
+        }
+      }
+    }
+  }
+};
+
+// Parts that the keys of a request are cut into, of the `splits` that the grid has:
+// each of WK key slices gets kMinSteps steps at least.
+constexpr int kMinSteps = 4;
+__device__ __forceinline__ int parts_of(const Attend& a, const Request& rq, int wk) {
+  return min(a.splits, max(1, (rq.len_tiles + rq.tree_tiles) / (kMinSteps * wk)));
+}
+
+// Few rows (up to 64 per key head): bound by reading the keys and values once.  A
+// workgroup's four waves are WR row tiles x 4/WR key slices; each wave loads the keys
+// of its steps straight into registers.
+template <int D, int R, int WR, bool F16>
+__global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(Attend a) {
+  using W = Wave<D, R, F16>;
+  using E = Elem<F16>;
+  constexpr int DC = W::DC, DV = W::DV, VW = W::VW;
+  constexpr int WK = kWaves / WR;  // key slices
+  const int lane = threadIdx.x & 63;
+  const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+  const int li = lane & 15, lg = lane >> 4;
+  const int wr = wave % WR, wk = wave / WR;
+  // unit: ((request, key head), part)
+  const int part = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
+  const int kh = unit % a.kv_heads, b = unit / a.kv_heads;
+  const Request rq = request(a, b);
+  const int parts = parts_of(a, rq, WK);
+  const int nrows = rq.tokens * a.group;
+  if (nrows == 0 || part >= parts) return;
+  const int row0 = wr * (16 * R);  // of this wave
+
+  // the steps of this part: [t0, t1) of len_tiles + tree_tiles
+  const int tiles = rq.len_tiles + rq.tree_tiles;
+  const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * part / parts);
+  const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / parts);
+
+  W w;
+  w.load(a, rq, kh, row0, nrows, li, lg);
+  __shared__ unsigned long long lsee[kWaves][kMaxTree];
+  if (t1 > rq.len_tiles) w.trees(a, rq, lane, lsee[wave]);
+
+  const int32_t* table = a.tables + b * a.tstride;
+  // the block ids of a step's two halves, loaded a step ahead of its keys
+  auto ids = [&](int t, int (&id)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int slot;
+      id[h] = t < rq.len_tiles && t < t1 ? table[block_of(a, min(t * 32 + 16 * h, rq.len - 1), slot)] : 0;
+    }
+  };
+  struct Keys {
+    u32x4 k[2][DC];
+    uint32_t v[8][VW];
+    bool bad[2];
+  };
+  auto load = [&](int t, const int (&id)[2], Keys& n) {
+    const bool tree = t >= rq.len_tiles;
+    const int key0 = (tree ? t - rq.len_tiles : t) * 32;
+    const int limit = tree ? rq.tokens : rq.len;
+    // each half: a uniform base and the last key of it that exists (a key past the
+    // end reads that one instead and is masked)
+    const uint32_t ks = tree ? static_cast<uint32_t>(a.k_row) : a.kc_slot;
+    const uint32_t vs = tree ? static_cast<uint32_t>(a.v_row) : a.vc_slot;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int first = min(key0 + 16 * h, limit - 1), last = limit - 1 - first;
+      const uint16_t *kb, *vb;
+      n.bad[h] = false;
+      if (tree) {
+        kb = a.k + (rq.row0 + first) * a.k_row + kh * a.k_head;
+        vb = a.v + (rq.row0 + first) * a.v_row + kh * a.v_head;
+      } else {
+        n.bad[h] = id[h] < 0 || id[h] >= a.blocks;
+        int slot;
+        block_of(a, first, slot);
+        const int64_t at = n.bad[h] ? 0 : id[h];
+        kb = a.kc + at * a.kc_block + static_cast<int64_t>(slot) * a.kc_slot + kh * a.kc_head;
+        vb = a.vc + at * a.vc_block + static_cast<int64_t>(slot) * a.vc_slot + kh * a.vc_head;
+      }
+      const uint16_t* p = kb + static_cast<uint32_t>(min(li, last)) * ks + 8 * lg;
+#pragma unroll
+      for (int d = 0; d < DC; ++d) n.k[h][d] = ld16(p + 32 * d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint16_t* y = vb + static_cast<uint32_t>(min(4 * lg + e, last)) * vs + DV * li;
+        if constexpr (VW == 4) {
+          const u32x4 x = ld16(y);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) n.v[4 * h + e][i] = x[i];
+        } else {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(y);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) n.v[4 * h + e][i] = x[i];
+        }
+      }
+    }
+  };
+
+  int id[2];
+  ids(t0 + wk, id);
+  for (int t = t0 + wk; t < t1; t += WK) {
+    Keys n;
+    load(t, id, n);
+    ids(t + WK, id);
+    const bool tree = t >= rq.len_tiles;
+    const int key0 = (tree ? t - rq.len_tiles : t) * 32;
+    const int limit = tree ? rq.tokens : rq.len;
+    const bool masked = tree || key0 + 32 > limit || n.bad[0] || n.bad[1];
     // values that no row may take must not meet p = 0 as an infinity or NaN: those
     // past the end and of absent blocks become zeros, and a drafted token's that
-    // are not finite are left out of the products (bit of `odd`) and added below
-    // for the rows that see it
+    // are not finite are left out of the products (bit of `odd`) and added for the
+    // rows that see it
     uint32_t odd = 0;
     if (masked) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const bool gone = key0 + 16 * (e >> 2) + 4 * lg + (e & 3) >= limit || bad[e >> 2];
+        const bool gone = key0 + 16 * (e >> 2) + 4 * lg + (e & 3) >= limit || n.bad[e >> 2];
         bool wild = false;
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
-          if (gone) vf[e][i] = 0;
-          wild = wild || (vf[e][i] & E::kExp) == E::kExp || (vf[e][i] & E::kExp << 16) == E::kExp << 16;
+          if (gone) n.v[e][i] = 0;
+          wild = wild || (n.v[e][i] & E::kExp) == E::kExp || (n.v[e][i] & E::kExp << 16) == E::kExp << 16;
         }
-        const unsigned long long w = tree ? __ballot(wild) : 0;
-        if (w) {
+        const unsigned long long m = tree ? __ballot(wild) : 0;
+        if (m) {
 #pragma unroll
           for (int g = 0; g < 4; ++g)
-            if (w >> (16 * g) & 0xffff) odd |= 1u << (16 * (e >> 2) + 4 * g + (e & 3));
-          if (w >> (16 * lg) & 0xffff)
+            if (m >> (16 * g) & 0xffff) odd |= 1u << (16 * (e >> 2) + 4 * g + (e & 3));
+          if (m >> (16 * lg) & 0xffff)
 #pragma unroll
-            for (int i = 0; i < VW; ++i) vf[e][i] = 0;
+            for (int i = 0; i < VW; ++i) n.v[e][i] = 0;
         }
       }
     }
+    auto values = [&](uint32_t(&v)[8][VW]) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (masked) {
+      for (int e = 0; e < 8; ++e)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = key0 + 16 * h + 4 * lg + i;
-            const bool ok = key < limit && !bad[h] && (!tree || ((sees[r] >> (key & 63)) & 1));
-            s[r][h][i] = ok ? s[r][h][i] * a.c : -INFINITY;
-          }
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[r][h][i] *= a.c;
-      }
-      float top = s[r][0][0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[r][i >> 2][i & 3]);
-      top = fmaxf(mx[r], quad_max(top));
-      const float ref = top == -INFINITY ? 0.f : top;  // (nothing seen yet: every p is 0)
-      const float f = __builtin_amdgcn_exp2f(mx[r] - ref);
-      mx[r] = top;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) l[r][i] *= f;
-#pragma unroll
-      for (int d = 0; d < DV; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[r][d][i] *= f;
-      u32x4 p;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p0 = __builtin_amdgcn_exp2f(s[r][i >> 1][2 * (i & 1)] - ref);
-        const float p1 = __builtin_amdgcn_exp2f(s[r][i >> 1][2 * (i & 1) + 1] - ref);
-        p[i] = E::pack(p0, p1);
-      }
-      l[r] = E::mfma(ones, p, l[r]);
-#pragma unroll
-      for (int d = 0; d < DV; ++d) {
-        u32x4 vt;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          vt[e] = __builtin_amdgcn_perm(vf[2 * e + 1][d >> 1], vf[2 * e][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
-        o[r][d] = E::mfma(vt, p, o[r][d]);
-      }
-      for (uint32_t w = odd; w; w &= w - 1) {
-        const int j = __builtin_ctz(w);
-        const uint32_t lo = j & 2 ? p[1] : p[0], hi = j & 2 ? p[3] : p[2];
-        const float pj = E::low(__shfl(j & 16 ? hi : lo, 16 * (j >> 2 & 3) + li) >> (16 * (j & 1)));
-        if (!(sees[r] >> ((key0 + j) & 63) & 1)) continue;
-        const uint16_t* x = (j & 16 ? vb[1] : vb[0]) + static_cast<uint32_t>(j & 15) * vs + 4 * lg * DV;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int d = 0; d < DV; ++d) o[r][d][i] += pj * E::low(x[i * DV + d]);
-      }
-    }
+        for (int i = 0; i < VW; ++i) v[e][i] = n.v[e][i];
+    };
+    w.step(a, n.k, values, key0, limit, tree, masked, n.bad[0], n.bad[1], odd, lsee[wave], li, lg,
+           [&](int j) { return a.v + (rq.row0 + key0 + j) * a.v_row + kh * a.v_head; });
   }
 
-  // join the key slices: slice 0 adds the others' sums, brought to one maximum
+  // join the key slices: slice 0 adds the others' sums, brought to one reference
   if constexpr (WK > 1) {
     __shared__ float lo_[(WK - 1) * WR][R][DV * 4][64];
     __shared__ float ls_[(WK - 1) * WR][R][2][64];
     if (wk > 0) {
-      const int w = (wk - 1) * WR + wr;
+      const int n = (wk - 1) * WR + wr;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        ls_[w][r][0][lane] = mx[r];
-        ls_[w][r][1][lane] = l[r][0];
+        ls_[n][r][0][lane] = w.mx[r];
+        ls_[n][r][1][lane] = w.l[r][0];
 #pragma unroll
         for (int d = 0; d < DV; ++d)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) lo_[w][r][4 * d + i][lane] = o[r][d][i];
+          for (int i = 0; i < 4; ++i) lo_[n][r][4 * d + i][lane] = w.o[r][d][i];
       }
     }
     __syncthreads();
     if (wk > 0) return;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      float top = mx[r];
+      float ref = w.mx[r];
 #pragma unroll
-      for (int s = 0; s < WK - 1; ++s) top = fmaxf(top, ls_[s * WR + wr][r][0][lane]);
-      const float ref = top == -INFINITY ? 0.f : top;
-      const float f = __builtin_amdgcn_exp2f(mx[r] - ref);
-      mx[r] = top;
-      l[r][0] *= f;
+      for (int s = 0; s < WK - 1; ++s) ref = fmaxf(ref, ls_[s * WR + wr][r][0][lane]);
+      const float f = __builtin_amdgcn_exp2f(w.mx[r] - ref);
+      w.mx[r] = ref;
+      w.l[r][0] *= f;
 #pragma unroll
       for (int d = 0; d < DV; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[r][d][i] *= f;
+        for (int i = 0; i < 4; ++i) w.o[r][d][i] *= f;
 #pragma unroll
       for (int s = 0; s < WK - 1; ++s) {
-        const int w = s * WR + wr;
-        const float g = __builtin_amdgcn_exp2f(ls_[w][r][0][lane] - ref);
-        l[r][0] += g * ls_[w][r][1][lane];
+        const int n = s * WR + wr;
+        const float g = __builtin_amdgcn_exp2f(ls_[n][r][0][lane] - ref);
+        w.l[r][0] += g * ls_[n][r][1][lane];
 #pragma unroll
         for (int d = 0; d < DV; ++d)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[r][d][i] += g * lo_[w][r][4 * d + i][lane];
+          for (int i = 0; i < 4; ++i) w.o[r][d][i] += g * lo_[n][r][4 * d + i][lane];
       }
     }
   }
+  w.store(a, rq, kh, row0, nrows, li, lg, parts == 1,
+          [&](int, int64_t token, int head) { return (token * a.q_heads + head) * a.splits + part; });
+}
 
-  // lane: row li, dims (4 lg + i) DV + d
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// The wide kernel's work: the tiles of all (request, key head, row group), in that
+// order, cut into equal shares for the workgroups, whatever the requests' lengths are.
+// A share begins and ends anywhere in a unit; what it has of a unit that is not whole
+// is left as sums in slot 2 g (the share's first unit) or 2 g + 1 (its last).
+constexpr int kShares = 256;    // workgroups: one per CU
+constexpr int kMinShare = 6;    // tiles that a share has at least
+constexpr int kWideWaves = 8, kTile = 64;
+template <int PER>  // rows of a group
+struct Work {
+  static constexpr int NT = 64 * kWideWaves, TK = kTile;
+  Attend a;
+  int64_t* pre;   // LDS [NT]: tiles up to and with request base + i
+  int64_t* wsum;  // LDS [kWideWaves]
+  int base;
+  int64_t carry, total;
+  struct Unit {
+    Request rq;
+    int b, kh, rg, tiles, cached;
+    int64_t begin;  // its first tile's number
+  };
+
+  __device__ __forceinline__ static int tiles_of(const Request& rq) {
+    return (rq.len + TK - 1) / TK + (rq.tokens + TK - 1) / TK;
+  }
+  __device__ __forceinline__ int groups_of(const Request& rq) const { return (rq.tokens * a.group + PER - 1) / PER; }
+
+  // pre for the requests from `first` on; every thread must call it
+  __device__ __forceinline__ void fill(int first, int64_t before) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    base = first;
+    carry = before;
+    int64_t v = 0;
+    if (first + static_cast<int>(threadIdx.x) < a.requests) {
+      const Request rq = request(a, first + threadIdx.x);
+      v = static_cast<int64_t>(tiles_of(rq)) * a.kv_heads * groups_of(rq);
+    }
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = row0 + 16 * r + li;
-    if (row >= nrows) continue;
-    const int head = kh * a.group + row - tk[r] * a.group;
-    const int64_t token = rq.row0 + tk[r];
-    if (a.splits == 1) {
-      const float inv = l[r][0] > 0.f ? 1.f / l[r][0] : l[r][0] == 0.f ? 0.f : NAN;
-      uint16_t* p = a.out + token * a.out_row + head * a.out_head + 4 * lg * DV;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t o = __shfl_up(v, d);
+      if (lane >= d) v += o;
+    }
+    __syncthreads();  // (the last fill's readers are done)
+    if (lane == 63) wsum[wave] = v;
+    __syncthreads();
+    v += carry;
+    for (int i = 0; i < wave; ++i) v += wsum[i];
+    pre[threadIdx.x] = v;
+    __syncthreads();
+  }
+  __device__ __forceinline__ void start() {
+    fill(0, 0);
+    total = pre[NT - 1];
+    for (int f = NT; f < a.requests; f += NT) {
+      fill(f, total);
+      total = pre[NT - 1];
+    }
+    if (base) fill(0, 0);
+  }
+  __device__ __forceinline__ int shares() const {
+    return static_cast<int>(min<int64_t>(kShares, (total + kMinShare - 1) / kMinShare));
+  }
+  __device__ __forceinline__ int64_t begin(int g, int n) const { return g * total / n; }
+
+  __device__ __forceinline__ Unit inside(int b, int64_t local, int64_t first) const {
+    Unit u;
+    u.b = b;
+    u.rq = request(a, b);
+    u.tiles = tiles_of(u.rq);
+    u.cached = (u.rq.len + TK - 1) / TK;
+    const int k = static_cast<int>(local / u.tiles), groups = groups_of(u.rq);
+    u.kh = k / groups;
+    u.rg = k % groups;
+    u.begin = first + static_cast<int64_t>(k) * u.tiles;
+    return u;
+  }
+  // the unit of tile number pos < total, pos not before the last call's
+  __device__ __forceinline__ Unit find(int64_t pos) {
+    while (pos >= pre[NT - 1]) fill(base + NT, pre[NT - 1]);
+    int lo = 0, hi = NT - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= pos) lo = mid + 1;
+      else hi = mid;
+    }
+    const int64_t first = uniform64(lo ? pre[lo - 1] : carry);
+    return inside(base + uniform(lo), pos - first, first);
+  }
+};
+
+// Many rows (more than 64 per key head): bound by the matrix units and the softmax.
+// Eight waves share tiles of 64 keys through LDS, 8/WK row tiles of 32 rows x WK key
+// slices (WK = 2: a wave takes one 32-key half of each tile, and the halves are joined at
+// the end of a unit): a tile's rows go from
+// memory to registers one tile ahead of their use (16 bytes per lane, whole rows per
+// 16 or 8 lanes) and from there to one of two LDS buffers, so that there is one barrier
+// per tile and a load has a tile's arithmetic to arrive.
+//
+// LDS rows are D/8 pieces of 16 bytes.  A wave reads keys as A operands, 16 keys x one
+// piece per access: piece p of key r lies at p ^ (r D / 128), so that the sixteen lanes
+// of an access meet all banks.  Values are read a whole row per 16 lanes and lie plain.
+template <int D, int WK, bool F16>
+__global__ __launch_bounds__(64 * kWideWaves, 2) void attend_wide_kernel(Attend a) {
+  using W = Wave<D, 2, F16>;
+  using E = Elem<F16>;
+  constexpr int DC = W::DC, DV = W::DV, VW = W::VW;
+  constexpr int NW = kWideWaves, TK = kTile;
+  constexpr int PER = 32 * NW / WK;  // rows of a group
+  constexpr int P = D / 8;        // pieces per row
+  constexpr int KI = 64 / P;      // keys of one wave-wide load
+  constexpr int NG = TK / KI;     // loads per tile and matrix
+  constexpr int J = NG / NW;      // of them per wave
+  static_assert(NG % NW == 0 && 16 % KI == 0, "a wave's load lies in one block");
+  __shared__ __attribute__((aligned(16))) uint16_t lkv[2][2][TK * D];
+  auto& lk = lkv[0];
+  auto& lv = lkv[1];
+  __shared__ uint32_t lbad[2][NG];             // the load's block is absent
+  __shared__ unsigned long long lodd[2][NW];  // (drafted tile) keys whose values are not finite
+  const int lane = threadIdx.x & 63;
+  const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+  const int li = lane & 15, lg = lane >> 4;
+  __shared__ unsigned long long lsee[NW][kMaxTree];
+  __shared__ int64_t lpre[64 * NW], lsum[NW];
+  Work<PER> work{again(), lpre, lsum, 0, 0, 0};
+  work.start();
+  const int shares = work.shares(), share = xcd_remap(blockIdx.x, gridDim.x);
+  if (share >= shares) return;
+  const int64_t begin = work.begin(share, shares), end = work.begin(share + 1, shares);
+
+  for (int64_t pos = begin; pos < end;) {
+  work.a = again();
+  const typename Work<PER>::Unit un = work.find(pos);
+  const Request& rq = un.rq;
+  const int nrows = rq.tokens * a.group;
+  const int wr = wave % (NW / WK), wk = wave / (NW / WK);
+  const int row0 = un.rg * PER + wr * 32;  // of this wave
+  const bool active = row0 < nrows;
+  const int kh = un.kh, cached = un.cached;
+
+  // this share's tiles of the unit: cached ones, then the drafted tokens'
+  const int t0 = static_cast<int>(pos - un.begin);
+  const int t1 = static_cast<int>(min<int64_t>(un.tiles, end - un.begin));
+
+  W w;
+  if (active) {
+    const Attend c = again();
+    w.load(c, rq, kh, row0, nrows, li, lg);
+    if (t1 > cached) w.trees(c, rq, lane, lsee[wave]);
+  }
+
+  const int32_t* table = a.tables + un.b * a.tstride;
+  const uint16_t *kc = a.kc + kh * a.kc_head, *vc = a.vc + kh * a.vc_head;
+  int id[J];  // block ids of the next tile to load
+  auto ids = [&](int t) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w[VW];
+    for (int j = 0; j < J; ++j) {
+      int slot;
+      id[j] = t < cached && t < t1 ? table[block_of(a, min(t * TK + (wave * J + j) * KI, rq.len - 1), slot)] : 0;
+    }
+  };
+  u32x4 rk[J], rv[J];  // the tile on its way
+  int bad[J];
+  auto load = [&](int t) {
+    const int ln = here(lane), kin = ln / P, piece = ln % P;
+    const bool tree = t >= cached;
+    const int key0 = (tree ? t - cached : t) * TK, limit = tree ? rq.tokens : rq.len;
+    if (tree) {
+      const Attend c = again();
 #pragma unroll
-        for (int d = 0; d < VW; ++d) w[d] = E::pack(o[r][2 * d][i] * inv, o[r][2 * d + 1][i] * inv);
-        if constexpr (VW == 4) *reinterpret_cast<u32x4*>(p + i * DV) = u32x4{w[0], w[1], w[2], w[3]};
-        else *reinterpret_cast<u32x2*>(p + i * DV) = u32x2{w[0], w[1]};
+      for (int j = 0; j < J; ++j) {
+        const int at = min(key0 + (wave * J + j) * KI + kin, limit - 1);
+        bad[j] = 0;
+        rk[j] = ld16(c.k + (rq.row0 + at) * c.k_row + kh * c.k_head + 8 * piece);
+        rv[j] = ld16(c.v + (rq.row0 + at) * c.v_row + kh * c.v_head + 8 * piece);
       }
     } else {
-      const int64_t at = (token * a.q_heads + head) * a.splits + part;
-      float* p = a.part + at * D + 4 * lg * DV;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int d = 0; d < DV; d += 4)
-          *reinterpret_cast<f32x4*>(p + i * DV + d) = f32x4{o[r][d][i], o[r][d + 1][i], o[r][d + 2][i], o[r][d + 3][i]};
-      if (lg == 0) {
-        a.stat[2 * at] = mx[r];
-        a.stat[2 * at + 1] = l[r][0];
+      for (int j = 0; j < J; ++j) {
+        const int first = min(key0 + (wave * J + j) * KI, limit - 1);
+        const uint32_t at = min(kin, limit - 1 - first);
+        bad[j] = id[j] < 0 || id[j] >= a.blocks;
+        int slot;
+        block_of(a, first, slot);
+        const int64_t blk = bad[j] ? 0 : id[j], at0 = slot;
+        rk[j] = ld16(kc + blk * a.kc_block + at0 * a.kc_slot + at * a.kc_slot + 8 * piece);
+        rv[j] = ld16(vc + blk * a.vc_block + at0 * a.vc_slot + at * a.vc_slot + 8 * piece);
       }
     }
+  };
+  auto park = [&](int t) {
+    const int ln = here(lane), kin = ln / P, piece = ln % P;
+    const int buf = (t - t0) & 1;
+    const bool tree = t >= cached;
+    const int key0 = (tree ? t - cached : t) * TK, limit = tree ? rq.tokens : rq.len;
+    unsigned long long odd = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int g = wave * J + j, key = g * KI + kin;
+      // (as in attend_kernel: no infinity or NaN may meet p = 0)
+      if (bad[j] || key0 + key >= limit) rv[j] = u32x4{0, 0, 0, 0};
+      if (tree) {
+        bool wild = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          wild = wild || (rv[j][i] & E::kExp) == E::kExp || (rv[j][i] & E::kExp << 16) == E::kExp << 16;
+        const unsigned long long m = __ballot(wild), one = (P == 16 ? 0xffffull : 0xffull);
+        if (m) {
+#pragma unroll
+          for (int k = 0; k < KI; ++k)
+            if (m >> (P * k) & one) odd |= 1ull << (g * KI + k);
+          if (m >> (P * kin) & one) rv[j] = u32x4{0, 0, 0, 0};
+        }
+      }
+      *reinterpret_cast<u32x4*>(&lk[buf][(key * P + (piece ^ (key * P / 16 & (P - 1)))) * 8]) = rk[j];
+      *reinterpret_cast<u32x4*>(&lv[buf][(key * P + piece) * 8]) = rv[j];
+      if (lane == 0) lbad[buf][g] = bad[j];
+    }
+    if (tree && lane == 0) lodd[buf][wave] = odd;
+  };
+
+  if (t0 < t1) {
+    ids(t0);
+    load(t0);
+    ids(t0 + 1);
+    park(t0);
+    if (t0 + 1 < t1) load(t0 + 1);
+    ids(t0 + 2);
+    __syncthreads();
+  }
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    if (active) {
+      const int ln = here(lane), li = ln & 15, lg = ln >> 4;
+      const bool tree = t >= cached;
+      const int key0 = (tree ? t - cached : t) * TK, limit = tree ? rq.tokens : rq.len;
+      const unsigned long long bm = __ballot(lane < NG && lbad[buf][lane % NG]);
+      const bool masked = tree || key0 + TK > limit || bm;
+      unsigned long long odd = 0;
+      if (tree)
+#pragma unroll
+        for (int i = 0; i < NW; ++i) odd |= lodd[buf][i];
+#pragma unroll 1
+      for (int h = wk; h < TK / 32; h += WK) {
+        if (key0 + 32 * h >= limit) break;
+        u32x4 k[2][DC];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const int key = 32 * h + 16 * g + li;
+#pragma unroll
+          for (int d = 0; d < DC; ++d)
+            k[g][d] = *reinterpret_cast<const u32x4*>(
+                &lk[buf][(key * P + ((4 * d + lg) ^ (key * P / 16 & (P - 1)))) * 8]);
+        }
+        // (read behind the score products: the registers are the keys' until then)
+        auto values = [&](uint32_t(&v)[8][VW]) {
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint16_t* x = &lv[buf][(32 * h + 16 * (e >> 2) + 4 * lg + (e & 3)) * D + DV * li];
+            if constexpr (VW == 4) {
+              const u32x4 y = *reinterpret_cast<const u32x4*>(x);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) v[e][i] = y[i];
+            } else {
+              const u32x2 y = *reinterpret_cast<const u32x2*>(x);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) v[e][i] = y[i];
+            }
+          }
+        };
+        const uint32_t odd32 = static_cast<uint32_t>(odd >> (32 * h));
+        w.step(a, k, values, key0 + 32 * h, limit, tree, masked, bm >> (32 * h / KI) & 1, bm >> ((32 * h + 16) / KI) & 1, odd32,
+               lsee[wave], li, lg, [&](int j) {
+                 const Attend c = again();
+                 return c.v + (rq.row0 + key0 + 32 * h + j) * c.v_row + kh * c.v_head;
+               });
+      }
+    }
+    if (t + 1 < t1) park(t + 1);
+    if (t + 2 < t1) load(t + 2);
+    ids(t + 3);
+    __syncthreads();
+  }
+  // (WK = 2) the second half's sums are added to the first's, brought to one reference
+  if constexpr (WK == 2) {
+    float* lo = reinterpret_cast<float*>(lkv) + wr * (2 * DV * 4 * 64);
+    static_assert(sizeof(lkv) >= NW / 2 * 2 * DV * 4 * 64 * 4, "a wave's sums fit its part of the tiles");
+    __shared__ float ls[NW / 2][2][2][64];
+    if (active && wk == 1) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        ls[wr][r][0][lane] = w.mx[r];
+        ls[wr][r][1][lane] = w.l[r][0];
+#pragma unroll
+        for (int d = 0; d < DV; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) lo[(r * DV * 4 + 4 * d + i) * 64 + lane] = w.o[r][d][i];
+      }
+    }
+    __syncthreads();
+    if (active && wk == 0) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float m = ls[wr][r][0][lane], ref = fmaxf(w.mx[r], m);
+        const float f = __builtin_amdgcn_exp2f(w.mx[r] - ref), g = __builtin_amdgcn_exp2f(m - ref);
+        w.mx[r] = ref;
+        w.l[r][0] = f * w.l[r][0] + g * ls[wr][r][1][lane];
+#pragma unroll
+        for (int d = 0; d < DV; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w.o[r][d][i] = f * w.o[r][d][i] + g * lo[(r * DV * 4 + 4 * d + i) * 64 + lane];
+      }
+    }
+    __syncthreads();
+  }
+  if (active && wk == 0) {
+    const int64_t slot0 = static_cast<int64_t>(2 * share + (pos != begin)) * PER - un.rg * PER;
+    w.store(again(), rq, kh, row0, nrows, li, lg, t0 == 0 && t1 == un.tiles,
+            [&](int row, int64_t, int) { return slot0 + row; });
+  }
+  pos = un.begin + t1;
   }
 }
 
-// One wave per (request, token, head): the parts' outputs brought to one maximum,
-// added and divided by the joined sum.  Lane l owns D/64 neighbouring dims.
-template <int D, bool F16>
-__global__ __launch_bounds__(256) void join_kernel(Attend a) {
+// A row's output from n parts' sums: brought to one reference, added and divided by the
+// joined sum.  slot(i): where part i is.  Lane l owns D/64 neighbouring dims.
+template <int D, bool F16, typename Slot>
+__device__ __forceinline__ void join_row(const Attend& a, int64_t token, int head, int n, int lane, Slot slot) {
   constexpr int W = D / 64;
-  const int lane = threadIdx.x & 63;
+  float ref = kLow;
+  for (int i = lane; i < n; i += 64) ref = fmaxf(ref, a.stat[2 * slot(i)]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) ref = fmaxf(ref, __shfl_xor(ref, d));
+  float sum = 0.f, o[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) o[i] = 0.f;
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    // lane i: the weight of part i0 + i (0 from the last on)
+    f32x2 st = {kLow, 0.f};
+    if (i0 + lane < n) st = *reinterpret_cast<const f32x2*>(a.stat + 2 * slot(i0 + lane));
+    const float f = i0 + lane < n ? __builtin_amdgcn_exp2f(st[0] - ref) : 0.f;
+    sum += f * st[1];
+    for (int i = i0; i < min(n, i0 + 64); i += 8) {
+      float x[8][W];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float* p = a.part + slot(min(i + e, n - 1)) * D + W * lane;
+        if constexpr (W == 2) {
+          const f32x2 v = *reinterpret_cast<const f32x2*>(p);
+          x[e][0] = v[0], x[e][1] = v[1];
+        } else {
+          x[e][0] = *p;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float g = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i - i0 + e));
+        // (a part read twice has weight 0, and may hold infinities)
+#pragma unroll
+        for (int d = 0; d < W; ++d) o[d] = i + e < n ? fmaf(g, x[e][d], o[d]) : o[d];
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* p = a.out + token * a.out_row + head * a.out_head + W * lane;
+  if constexpr (W == 2) *reinterpret_cast<uint32_t*>(p) = Elem<F16>::pack(o[0] * inv, o[1] * inv);
+  else *p = static_cast<uint16_t>(Elem<F16>::pack(o[0] * inv, 0.f));
+}
+
+// Behind attend_kernel: one wave per (request, token, head).
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void join_kernel(Attend a, int wk) {
   const int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + uniform(static_cast<int>(threadIdx.x >> 6));
   const int head = static_cast<int>(u % a.q_heads);
   const int64_t bt = u / a.q_heads;
   const int b = static_cast<int>(bt / a.max_tokens), t = static_cast<int>(bt % a.max_tokens);
   if (b >= a.requests) return;
   const Request rq = request(a, b);
-  if (t >= rq.tokens) return;
-  const int64_t token = rq.row0 + t;
-  const int64_t at = (token * a.q_heads + head) * a.splits;
-  float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, a.stat[2 * (at + s)]);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-  const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, o[W];
-#pragma unroll
-  for (int i = 0; i < W; ++i) o[i] = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = __builtin_amdgcn_exp2f(a.stat[2 * (at + s)] - ref);
-    sum += f * a.stat[2 * (at + s) + 1];
-    const float* p = a.part + (at + s) * D + W * lane;
-#pragma unroll
-    for (int i = 0; i < W; ++i) o[i] += f * p[i];
-  }
-  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
-  uint16_t* p = a.out + token * a.out_row + head * a.out_head + W * lane;
-  if constexpr (W == 2) {
-    *reinterpret_cast<uint32_t*>(p) = Elem<F16>::pack(o[0] * inv, o[1] * inv);
-  } else {
-    *p = static_cast<uint16_t>(Elem<F16>::pack(o[0] * inv, 0.f));
+  const int parts = parts_of(a, rq, wk);
+  if (t >= rq.tokens || parts == 1) return;
+  const int64_t token = rq.row0 + t, at = (token * a.q_heads + head) * a.splits;
+  join_row<D, F16>(a, token, head, parts, threadIdx.x & 63, [&](int i) { return at + i; });
+}
+
+// Behind attend_wide_kernel: eight waves per kJoinRows rows of a (request, key head, row
+// group) that several shares have parts of.
+constexpr int kJoinRows = 32;
+template <int D, int PER, bool F16>
+__global__ __launch_bounds__(64 * kWideWaves) void join_wide_kernel(Attend a) {
+  constexpr int NW = kWideWaves;
+  __shared__ int64_t lpre[64 * NW], lsum[NW];
+  const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+  int u = blockIdx.x;
+  const int piece = u % (PER / kJoinRows);
+  u /= PER / kJoinRows;
+  const int rg = u % a.row_groups;
+  u /= a.row_groups;
+  const int kh = u % a.kv_heads, b = u / a.kv_heads;
+  const Request rq = request(a, b);
+  const int nrows = rq.tokens * a.group, first = rg * PER + piece * kJoinRows;
+  if (first >= nrows) return;
+  Work<PER> work{a, lpre, lsum, 0, 0, 0};
+  work.start();
+  while (b >= work.base + work.NT) work.fill(work.base + work.NT, lpre[work.NT - 1]);
+  const int64_t before = b > work.base ? lpre[b - work.base - 1] : work.carry;
+  const int tiles = work.tiles_of(rq), n = work.shares();
+  const int64_t s = before + static_cast<int64_t>(kh * work.groups_of(rq) + rg) * tiles, e = s + tiles;
+  // the shares of its first and last tile: the largest g with begin(g) <= tile
+  auto share = [&](int64_t tile) {
+    int g = static_cast<int>(tile * n / work.total);
+    while (g + 1 < n && work.begin(g + 1, n) <= tile) ++g;
+    return g;
+  };
+  const int g0 = share(s), g1 = share(e - 1);
+  if (g0 == g1) return;  // whole: already written
+  for (int row = first + wave; row < min(nrows, first + kJoinRows); row += NW) {
+    const int t = row / a.group;
+    join_row<D, F16>(a, rq.row0 + t, kh * a.group + row - t * a.group, g1 - g0 + 1, threadIdx.x & 63, [&](int i) {
+      const int g = g0 + i;
+      return static_cast<int64_t>(2 * g + (i == 0 && s > work.begin(g, n))) * PER + row - rg * PER;
+    });
   }
 }
 
 // The launch shape, a function of sizes the host knows (never of what the device
 // arrays hold, so that a captured call replays with other lengths).
 struct Plan {
-  int r, wr, row_groups, splits;
+  int wide;  // rows of a group of the wide kernel, or 0
+  int r, wr; // else row tiles per wave, waves per key slice
+  int row_groups, splits;
 };
 Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t max_tokens, int64_t max_context) {
   const int64_t rows = max_tokens * (q_heads / kv_heads);
   Plan p;
+  p.wide = rows <= 64 ? 0 : rows <= 128 ? 128 : 256;
   p.r = rows <= 16 ? 1 : 2;
-  p.wr = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-  p.row_groups = static_cast<int>((rows + 16 * p.r * p.wr - 1) / (16 * p.r * p.wr));
-  const int64_t units = requests * kv_heads * p.row_groups;
-  const int64_t steps = (max_context + 31) / 32 + (max_tokens + 31) / 32;
-  const int64_t most = steps / (4 * (kWaves / p.wr));  // at least four steps for each slice
-  int64_t s = (1024 + units - 1) / units;
-  s = s < most ? s : most;
-  p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
+  p.wr = rows <= 32 ? 1 : 2;
+  p.row_groups = p.wide ? static_cast<int>((rows + p.wide - 1) / p.wide) : 1;
+  p.splits = 1;
+  if (!p.wide) {
+    const int64_t steps = (max_context + 31) / 32 + (max_tokens + 31) / 32;
+    const int64_t most = steps / (kMinSteps * (kWaves / p.wr)), s = (1024 + requests * kv_heads - 1) / (requests * kv_heads);
+    p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({s, most, 256})));
+  }
   return p;
 }
 
+int64_t slots_of(const Plan& p, int64_t rows, int64_t q_heads) {
+  return p.wide ? int64_t{2} * kShares * p.wide : p.splits == 1 ? 0 : rows * q_heads * p.splits;
+}
 size_t workspace_bytes(const Plan& p, int64_t rows, int64_t q_heads, int64_t head_dim) {
-  return p.splits == 1 ? 0 : static_cast<size_t>(rows * q_heads * p.splits) * (head_dim + 2) * 4;
+  return static_cast<size_t>(slots_of(p, rows, q_heads)) * (head_dim + 2) * 4;
 }
 
 bool sizes_ok(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_tokens,
               int64_t max_context) {
   return rows >= 0 && rows <= 0x7fffffff / 64 && requests >= 0 && requests <= 0x100000 && kv_heads >= 1 &&
          q_heads >= kv_heads && q_heads % kv_heads == 0 && q_heads <= 4096 && (head_dim == 64 || head_dim == 128) &&
-         max_tokens >= 1 && max_tokens <= kMaxTree && max_context >= 0 && max_context <= 0x7fffffff;
+         max_tokens >= 1 && max_tokens <= kMaxTree && max_context >= 0 && max_context <= 0x7fffffff &&
+         requests * max_tokens * q_heads <= 0x3fffffff;  // (grids are 32-bit)
+}
+
+template <int D, int WK, bool F16>
+int launch_wide(const Attend& a, hipStream_t st) {
+  constexpr int PER = 32 * kWideWaves / WK;
+  const dim3 blk(64 * kWideWaves);
+  hipLaunchKernelGGL((attend_wide_kernel<D, WK, F16>), dim3(kShares), blk, 0, st, a);
+  if (int rc = check_launch("tree attention kernel")) return rc;
+  const int64_t grid = static_cast<int64_t>(a.requests) * a.kv_heads * a.row_groups * (PER / kJoinRows);
+  hipLaunchKernelGGL((join_wide_kernel<D, PER, F16>), dim3(static_cast<unsigned>(grid)), blk, 0, st, a);
+  return check_launch("tree attention join kernel");
 }
 
 template <int D, bool F16>
 int launch(const Attend& a, const Plan& p, hipStream_t st) {
-  const int64_t grid = static_cast<int64_t>(a.requests) * a.kv_heads * p.row_groups * p.splits;
-  if (grid > 0x7fffffff || static_cast<int64_t>(a.requests) * a.max_tokens * a.q_heads > 0x7fffffff) return fail(PGS_ERR_INVALID_ARGUMENT, "pgs_tree_attention: too many requests");
-  const dim3 g(static_cast<unsigned>(grid)), blk(64 * kWaves);
+  if (p.wide) return p.wide == 256 ? launch_wide<D, 1, F16>(a, st) : launch_wide<D, 2, F16>(a, st);
+  const dim3 g(static_cast<unsigned>(a.requests * a.kv_heads * p.splits)), blk(64 * kWaves);
   if (p.r == 1) hipLaunchKernelGGL((attend_kernel<D, 1, 1, F16>), g, blk, 0, st, a);
   else if (p.wr == 1) hipLaunchKernelGGL((attend_kernel<D, 2, 1, F16>), g, blk, 0, st, a);
-  else if (p.wr == 2) hipLaunchKernelGGL((attend_kernel<D, 2, 2, F16>), g, blk, 0, st, a);
-  else hipLaunchKernelGGL((attend_kernel<D, 2, 4, F16>), g, blk, 0, st, a);
+  else hipLaunchKernelGGL((attend_kernel<D, 2, 2, F16>), g, blk, 0, st, a);
   if (int rc = check_launch("tree attention kernel")) return rc;
   if (p.splits == 1) return PGS_OK;
   const int64_t waves = static_cast<int64_t>(a.requests) * a.max_tokens * a.q_heads;
-  hipLaunchKernelGGL((join_kernel<D, F16>), dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((join_kernel<D, F16>), dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, st, a,
+                     kWaves / p.wr);
   return check_launch("tree attention join kernel");
 }
 
@@ -567,6 +1107,7 @@ extern "C" int pgs_tree_attention(const pgs_tree_attention_args* args, void* wor
   a.kc_block = c.k_block, a.kc_head = c.k_head, a.vc_block = c.v_block, a.vc_head = c.v_head;
   a.kc_slot = static_cast<uint32_t>(c.k_slot), a.vc_slot = static_cast<uint32_t>(c.v_slot);
   a.blocks = static_cast<int32_t>(c.blocks), a.bs = static_cast<int32_t>(c.block_size);
+  a.bs_inv = static_cast<uint32_t>(((uint64_t{1} << 32) + a.bs - 1) / a.bs);
   a.tables = g.block_tables, a.tstride = g.table_stride, a.cols = static_cast<int32_t>(g.columns);
   a.lens = g.lens, a.offsets = g.offsets, a.parents = g.parents;
   a.rows = static_cast<int32_t>(g.rows), a.requests = static_cast<int32_t>(g.requests);
@@ -575,7 +1116,7 @@ extern "C" int pgs_tree_attention(const pgs_tree_attention_args* args, void* wor
   a.max_tokens = static_cast<int32_t>(g.max_tokens), a.row_groups = p.row_groups, a.splits = p.splits;
   a.c = g.scale * 1.44269504088896340736f;
   a.part = static_cast<float*>(workspace);
-  a.stat = a.part + g.rows * g.q_heads * p.splits * c.head_dim;
+  a.stat = a.part + slots_of(p, g.rows, g.q_heads) * c.head_dim;
   if (c.head_dim == 64)
     return g.dtype == PGS_DTYPE_F16 ? launch<64, true>(a, p, st) : launch<64, false>(a, p, st);
   return g.dtype == PGS_DTYPE_F16 ? launch<128, true>(a, p, st) : launch<128, false>(a, p, st);
