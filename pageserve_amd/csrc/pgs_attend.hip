@@ -70,6 +70,21 @@ __device__ __forceinline__ int here(int lane) {
   return lane;
 }
 
+// Four keys x 16 dims per 16 lanes from LDS, transposed: lane i of them gives the address
+// of dims 4 (i % 4) .. +3 of key i / 4 and gets dim i of the four keys.
+template <typename T>
+__device__ __forceinline__ __attribute__((address_space(3))) T* lds(uint32_t address) {
+  return reinterpret_cast<__attribute__((address_space(3))) T*>(address);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t lds_address(T& v) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)&v));
+}
+__device__ __forceinline__ u32x2 read_transposed(uint32_t address) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<s16x4>(address)));
+}
+
 // The kernel's argument again, read from its segment at this point: for the parts of a
 // kernel outside its inner loop, whose fields would otherwise all sit in scalar
 // registers throughout (and push vector registers out to memory).
@@ -157,14 +172,14 @@ __device__ __forceinline__ int block_of(const Attend& a, int token, int& slot) {
   return q;
 }
 
-// 16 R rows of a wave and their running sums.
-template <int D, int R, bool F16>
+// 16 R rows of a wave and their running sums.  The output MFMA d covers the dims
+// (4 lg + i) D/16 + d of its lanes (SPREAD: the direct kernel), or 16 d + 4 lg + i.
+template <int D, int R, bool F16, bool SPREAD>
 struct Wave {
   using E = Elem<F16>;
   static constexpr int DC = D / 32;  // 32-dim chunks of a key
   static constexpr int DV = D / 16;  // dims of a value row per lane
   static constexpr int VW = DV / 2;  // their dwords
-  int tk[R];                         // token of this lane's row (rows past the last repeat it)
   u32x4 q[R][DC];
   f32x4 o[R][DV], l[R];
   float mx[R];
@@ -172,9 +187,8 @@ struct Wave {
   __device__ __forceinline__ void load(const Attend& a, const Request& rq, int kh, int row0, int nrows, int li, int lg) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int row = min(row0 + 16 * r + li, nrows - 1);
-      tk[r] = row / a.group;
-      const uint16_t* p = a.q + (rq.row0 + tk[r]) * a.q_row + (kh * a.group + row - tk[r] * a.group) * a.q_head + 8 * lg;
+      const int row = min(row0 + 16 * r + li, nrows - 1), t = row / a.group;  // (rows past the last repeat it)
+      const uint16_t* p = a.q + (rq.row0 + t) * a.q_row + (kh * a.group + row - t * a.group) * a.q_head + 8 * lg;
 #pragma unroll
       for (int d = 0; d < DC; ++d) q[r][d] = ld16(p + 32 * d);
     }
@@ -214,26 +228,31 @@ struct Wave {
   }
 
   // One step: keys key0 .. key0 + 31 of `limit` (cached, or with tree drafted).
-  // k: A operands of the two 16-key halves; values(v): the lane's eight keys x DV dims.
+  // keys(h, d): A operand of the 16-key half h, 32-dim chunk d; values(d): that of
+  // output MFMA d.  (SPREAD false: both are read here, from LDS, four at a time; left
+  // to itself the compiler reads each just before its use and waits for it alone.)
   // masked: some key is past the limit, in an absent block (bad) or drafted.
   // odd: drafted keys whose values are not finite (v holds zeros for them); value(j)
-  // is the row of key key0 + j.
-  template <typename Values, typename Value>
-  __device__ __forceinline__ void step(const Attend& a, const u32x4 (&k)[2][DC], Values values, int key0, int limit,
-                                       bool tree, bool masked, bool bad0, bool bad1, uint32_t odd,
-                                       const unsigned long long* see, int li, int lg, Value value) {
+  // is the row of key key0 + j.  see(r): which drafted tokens the lane's row r attends to.
+  template <typename Keys, typename Values, typename See, typename Value>
+  __device__ __forceinline__ void step(const Attend& a, Keys keys, Values values, int key0, int limit, bool tree,
+                                       bool masked, bool bad0, bool bad1, uint32_t odd, See see, int li, int lg,
+                                       Value value) {
     // lane's scores: keys key0 + 16 h + 4 lg + i
     f32x4 s[R][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h) {
+      u32x4 k[DC];
+#pragma unroll
+      for (int d = 0; d < DC; ++d) k[d] = keys(h, d);
+      if (!SPREAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         s[r][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int d = 0; d < DC; ++d) s[r][h] = E::mfma(k[h][d], q[r][d], s[r][h]);
+        for (int d = 0; d < DC; ++d) s[r][h] = E::mfma(k[d], q[r][d], s[r][h]);
       }
-    uint32_t v[8][VW];
-    values(v);
+    }
     // exponents against the row's reference, and whether a row needs a new one
     float x[R][8];
     uint32_t ok[R];
@@ -241,7 +260,7 @@ struct Wave {
     if (masked) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const unsigned long long sees = tree ? see[tk[r]] : ~0ull;
+        const unsigned long long sees = tree ? see(r) : ~0ull;
         ok[r] = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -292,15 +311,19 @@ struct Wave {
         p[r][i] = E::pack(__builtin_amdgcn_exp2f(x[r][2 * i]), __builtin_amdgcn_exp2f(x[r][2 * i + 1]));
     const u32x4 ones = {E::kOnes, E::kOnes, E::kOnes, E::kOnes};
 #pragma unroll
-    for (int r = 0; r < R; ++r) l[r] = E::mfma(ones, p[r], l[r]);
+    for (int d0 = 0; d0 < DV; d0 += 4) {
+      u32x4 v[4];
+      if (!SPREAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int d = 0; d < DV; ++d) {
-      u32x4 vt;
+      for (int d = 0; d < 4; ++d) v[d] = values(d0 + d);
+      if (!SPREAD) __builtin_amdgcn_sched_barrier(0);
+      if (d0 == 0)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        vt[e] = __builtin_amdgcn_perm(v[2 * e + 1][d >> 1], v[2 * e][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
+        for (int r = 0; r < R; ++r) l[r] = E::mfma(ones, p[r], l[r]);
 #pragma unroll
-      for (int r = 0; r < R; ++r) o[r][d] = E::mfma(vt, p[r], o[r][d]);
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int r = 0; r < R; ++r) o[r][d0 + d] = E::mfma(v[d], p[r], o[r][d0 + d]);
     }
     for (uint32_t w = odd; w; w &= w - 1) {
       const int j = __builtin_ctz(w);
@@ -309,17 +332,17 @@ struct Wave {
       for (int r = 0; r < R; ++r) {
         const uint32_t lo = j & 2 ? p[r][1] : p[r][0], hi = j & 2 ? p[r][3] : p[r][2];
         const float pj = E::low(__shfl(j & 16 ? hi : lo, 16 * (j >> 2 & 3) + li) >> (16 * (j & 1)));
-        if (!(see[tk[r]] >> ((key0 + j) & 63) & 1)) continue;
+        if (!(see(r) >> ((key0 + j) & 63) & 1)) continue;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int d = 0; d < DV; ++d) o[r][d][i] += pj * E::low(row[(4 * lg + i) * DV + d]);
+          for (int d = 0; d < DV; ++d) o[r][d][i] += pj * E::low(row[SPREAD ? (4 * lg + i) * DV + d : 16 * d + 4 * lg + i]);
       }
     }
   }
 
   // The rows' outputs, or (whole false: other keys of theirs are elsewhere) their
-  // sums: lane's dims (4 lg + i) DV + d.  slot(row, token, head): where to.
+  // sums.  slot(row, token, head): where to.
   template <typename Slot>
   __device__ __forceinline__ void store(const Attend& a, const Request& rq, int kh, int row0, int nrows, int li, int lg,
                                         bool whole, Slot slot) {
@@ -327,28 +350,40 @@ struct Wave {
     for (int r = 0; r < R; ++r) {
       const int row = row0 + 16 * r + li;
       if (row >= nrows) continue;
-      const int head = kh * a.group + row - tk[r] * a.group;
-      const int64_t token = rq.row0 + tk[r];
+      const int t = row / a.group, head = kh * a.group + row - t * a.group;
+      const int64_t token = rq.row0 + t;
       if (whole) {
         const float inv = l[r][0] == 0.f ? 0.f : 1.f / l[r][0];
-        uint16_t* d = a.out + token * a.out_row + head * a.out_head + 4 * lg * DV;
+        uint16_t* d = a.out + token * a.out_row + head * a.out_head + 4 * lg * (SPREAD ? DV : 1);
+        if constexpr (SPREAD) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t w[VW];
+          for (int i = 0; i < 4; ++i) {
+            uint32_t w[VW];
 #pragma unroll
-          for (int e = 0; e < VW; ++e) w[e] = E::pack(o[r][2 * e][i] * inv, o[r][2 * e + 1][i] * inv);
-          if constexpr (VW == 4) *reinterpret_cast<u32x4*>(d + i * DV) = u32x4{w[0], w[1], w[2], w[3]};
-          else *reinterpret_cast<u32x2*>(d + i * DV) = u32x2{w[0], w[1]};
+            for (int e = 0; e < VW; ++e) w[e] = E::pack(o[r][2 * e][i] * inv, o[r][2 * e + 1][i] * inv);
+            if constexpr (VW == 4) *reinterpret_cast<u32x4*>(d + i * DV) = u32x4{w[0], w[1], w[2], w[3]};
+            else *reinterpret_cast<u32x2*>(d + i * DV) = u32x2{w[0], w[1]};
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < DV; ++e)
+            *reinterpret_cast<u32x2*>(d + 16 * e) = u32x2{E::pack(o[r][e][0] * inv, o[r][e][1] * inv),
+                                                          E::pack(o[r][e][2] * inv, o[r][e][3] * inv)};
         }
       } else {
         const int64_t at = slot(row, token, head);
-        float* d = a.part + at * D + 4 * lg * DV;
+        float* d = a.part + at * D + 4 * lg * (SPREAD ? DV : 1);
+        if constexpr (SPREAD) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int e = 0; e < DV; e += 4)
-            *reinterpret_cast<f32x4*>(d + i * DV + e) =
-                f32x4{o[r][e][i], o[r][e + 1][i], o[r][e + 2][i], o[r][e + 3][i]};
+            for (int e = 0; e < DV; e += 4)
+              *reinterpret_cast<f32x4*>(d + i * DV + e) =
+                  f32x4{o[r][e][i], o[r][e + 1][i], o[r][e + 2][i], o[r][e + 3][i]};
+        } else {
+#pragma unroll
+          for (int e = 0; e < DV; ++e) *reinterpret_cast<f32x4*>(d + 16 * e) = o[r][e];
+        }
         if (lg == 0) {
           a.stat[2 * at] = mx[r];
           a.stat[2 * at + 1] = l[r][0];
@@ -370,7 +405,7 @@ __device__ __forceinline__ int parts_of(const Attend& a, const Request& rq, int 
 // of its steps straight into registers.
 template <int D, int R, int WR, bool F16>
 __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(Attend a) {
-  using W = Wave<D, R, F16>;
+  using W = Wave<D, R, F16, true>;
   using E = Elem<F16>;
   constexpr int DC = W::DC, DV = W::DV, VW = W::VW;
   constexpr int WK = kWaves / WR;  // key slices
@@ -395,6 +430,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(Attend a) {
   W w;
   w.load(a, rq, kh, row0, nrows, li, lg);
   __shared__ unsigned long long lsee[kWaves][kMaxTree];
+  int token[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) token[r] = min(row0 + 16 * r + li, nrows - 1) / a.group;
   if (t1 > rq.len_tiles) w.trees(a, rq, lane, lsee[wave]);
 
   const int32_t* table = a.tables + b * a.tstride;
@@ -403,7 +441,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(Attend a) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       int slot;
-      id[h] = t < rq.len_tiles && t < t1 ? table[block_of(a, min(t * 32 + 16 * h, rq.len - 1), slot)] : 0;
+      // (not provably uniform: the value stays in a vector register, unwaited for, until
+      // it is used)
+      if (t < rq.len_tiles && t < t1)
+        id[h] = table[block_of(a, min(t * 32 + 16 * h, rq.len - 1), slot) + (here(lane) >> 6)];
     }
   };
   struct Keys {
@@ -428,10 +469,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(Attend a) {
         kb = a.k + (rq.row0 + first) * a.k_row + kh * a.k_head;
         vb = a.v + (rq.row0 + first) * a.v_row + kh * a.v_head;
       } else {
-        n.bad[h] = id[h] < 0 || id[h] >= a.blocks;
+        const int blk = uniform(id[h]);
+        n.bad[h] = blk < 0 || blk >= a.blocks;
         int slot;
         block_of(a, first, slot);
-        const int64_t at = n.bad[h] ? 0 : id[h];
+        const int64_t at = n.bad[h] ? 0 : blk;
         kb = a.kc + at * a.kc_block + static_cast<int64_t>(slot) * a.kc_slot + kh * a.kc_head;
         vb = a.vc + at * a.vc_block + static_cast<int64_t>(slot) * a.vc_slot + kh * a.vc_head;
       }
@@ -454,7 +496,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(Attend a) {
     }
   };
 
-  int id[2];
+  int id[2] = {0, 0};
   ids(t0 + wk, id);
   for (int t = t0 + wk; t < t1; t += WK) {
     Keys n;
@@ -490,13 +532,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(Attend a) {
         }
       }
     }
-    auto values = [&](uint32_t(&v)[8][VW]) {
+    auto values = [&](int d) {
+      u32x4 vt;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int i = 0; i < VW; ++i) v[e][i] = n.v[e][i];
+      for (int e = 0; e < 4; ++e)
+        vt[e] = __builtin_amdgcn_perm(n.v[2 * e + 1][d >> 1], n.v[2 * e][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
+      return vt;
     };
-    w.step(a, n.k, values, key0, limit, tree, masked, n.bad[0], n.bad[1], odd, lsee[wave], li, lg,
+    w.step(a, [&](int h, int d) { return n.k[h][d]; }, values, key0, limit, tree, masked, n.bad[0], n.bad[1], odd,
+           [&](int r) { return lsee[wave][token[r]]; }, li, lg,
            [&](int j) { return a.v + (rq.row0 + key0 + j) * a.v_row + kh * a.v_head; });
   }
 
@@ -558,10 +602,11 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
 // is left as sums in slot 2 g (the share's first unit) or 2 g + 1 (its last).
 constexpr int kShares = 256;    // workgroups: one per CU
 constexpr int kMinShare = 6;    // tiles that a share has at least
-constexpr int kWideWaves = 8, kTile = 64;
-template <int PER>  // rows of a group
+constexpr int kWideWaves = 16;
+constexpr int tile_keys(int head_dim) { return 8192 / head_dim; }
+template <int PER, int TK>  // rows of a group, keys of a tile
 struct Work {
-  static constexpr int NT = 64 * kWideWaves, TK = kTile;
+  static constexpr int NT = 64 * kWideWaves;
   Attend a;
   int64_t* pre;   // LDS [NT]: tiles up to and with request base + i
   int64_t* wsum;  // LDS [kWideWaves]
@@ -580,12 +625,12 @@ struct Work {
 
   // pre for the requests from `first` on; every thread must call it
   __device__ __forceinline__ void fill(int first, int64_t before) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int thread = here(threadIdx.x), lane = thread & 63, wave = thread >> 6;
     base = first;
     carry = before;
     int64_t v = 0;
-    if (first + static_cast<int>(threadIdx.x) < a.requests) {
-      const Request rq = request(a, first + threadIdx.x);
+    if (first + thread < a.requests) {
+      const Request rq = request(a, first + thread);
       v = static_cast<int64_t>(tiles_of(rq)) * a.kv_heads * groups_of(rq);
     }
 #pragma unroll
@@ -598,30 +643,32 @@ struct Work {
     __syncthreads();
     v += carry;
     for (int i = 0; i < wave; ++i) v += wsum[i];
-    pre[threadIdx.x] = v;
+    pre[thread] = v;
     __syncthreads();
   }
   __device__ __forceinline__ void start() {
+    // (everything but the lane's own sums is the same in all lanes: scalar registers)
     fill(0, 0);
-    total = pre[NT - 1];
+    total = uniform64(pre[NT - 1]);
     for (int f = NT; f < a.requests; f += NT) {
       fill(f, total);
-      total = pre[NT - 1];
+      total = uniform64(pre[NT - 1]);
     }
     if (base) fill(0, 0);
   }
   __device__ __forceinline__ int shares() const {
     return static_cast<int>(min<int64_t>(kShares, (total + kMinShare - 1) / kMinShare));
   }
-  __device__ __forceinline__ int64_t begin(int g, int n) const { return g * total / n; }
+  __device__ __forceinline__ int64_t begin(int g, int n) const { return uniform64(g * total / n); }
 
   __device__ __forceinline__ Unit inside(int b, int64_t local, int64_t first) const {
     Unit u;
+    const Request rq = request(a, b);
     u.b = b;
-    u.rq = request(a, b);
+    u.rq = Request{uniform(rq.row0), uniform(rq.tokens), uniform(rq.len), 0, 0};
     u.tiles = tiles_of(u.rq);
     u.cached = (u.rq.len + TK - 1) / TK;
-    const int k = static_cast<int>(local / u.tiles), groups = groups_of(u.rq);
+    const int k = uniform(static_cast<int>(local / u.tiles)), groups = groups_of(u.rq);
     u.kh = k / groups;
     u.rg = k % groups;
     u.begin = first + static_cast<int64_t>(k) * u.tiles;
@@ -629,7 +676,7 @@ struct Work {
   }
   // the unit of tile number pos < total, pos not before the last call's
   __device__ __forceinline__ Unit find(int64_t pos) {
-    while (pos >= pre[NT - 1]) fill(base + NT, pre[NT - 1]);
+    while (pos >= uniform64(pre[NT - 1])) fill(base + NT, uniform64(pre[NT - 1]));
     int lo = 0, hi = NT - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -642,136 +689,134 @@ struct Work {
 };
 
 // Many rows (more than 64 per key head): bound by the matrix units and the softmax.
-// Eight waves share tiles of 64 keys through LDS, 8/WK row tiles of 32 rows x WK key
-// slices (WK = 2: a wave takes one 32-key half of each tile, and the halves are joined at
-// the end of a unit): a tile's rows go from
-// memory to registers one tile ahead of their use (16 bytes per lane, whole rows per
-// 16 or 8 lanes) and from there to one of two LDS buffers, so that there is one barrier
-// per tile and a load has a tile's arithmetic to arrive.
+// Sixteen waves share tiles of 64 keys (128 at 64 dims) through LDS, 16/WK row tiles of 16
+// rows x WK key slices (WK = 2: a wave takes every second 32-key step of a tile, and the two
+// are joined at the end of a unit).  A tile's rows go from memory to registers one tile
+// ahead of their use, one 16-byte load of keys and one of values per lane, and from there to
+// one of two LDS buffers: one barrier per tile, and a load has a tile's arithmetic to arrive.
+// Four waves per SIMD with 16 rows each hide the chain scores - softmax - output of one
+// another.
 //
 // LDS rows are D/8 pieces of 16 bytes.  A wave reads keys as A operands, 16 keys x one
 // piece per access: piece p of key r lies at p ^ (r D / 128), so that the sixteen lanes
-// of an access meet all banks.  Values are read a whole row per 16 lanes and lie plain.
+// of an access meet all banks.  Values are read transposed, 4 keys x 16 dims per 16 lanes
+// (ds_read_b64_tr_b16: lane n gets dim n of the four keys), a pair of pieces of 16 keys per
+// access: they are exchanged in pairs, p ^ 2 (r D / 128).
 template <int D, int WK, bool F16>
-__global__ __launch_bounds__(64 * kWideWaves, 2) void attend_wide_kernel(Attend a) {
-  using W = Wave<D, 2, F16>;
+__global__ __launch_bounds__(64 * kWideWaves, 4) void attend_wide_kernel(Attend a) {
+  using W = Wave<D, 1, F16, false>;
   using E = Elem<F16>;
-  constexpr int DC = W::DC, DV = W::DV, VW = W::VW;
-  constexpr int NW = kWideWaves, TK = kTile;
-  constexpr int PER = 32 * NW / WK;  // rows of a group
-  constexpr int P = D / 8;        // pieces per row
-  constexpr int KI = 64 / P;      // keys of one wave-wide load
-  constexpr int NG = TK / KI;     // loads per tile and matrix
-  constexpr int J = NG / NW;      // of them per wave
-  static_assert(NG % NW == 0 && 16 % KI == 0, "a wave's load lies in one block");
-  __shared__ __attribute__((aligned(16))) uint16_t lkv[2][2][TK * D];
+  constexpr int DV = W::DV;
+  constexpr int NW = kWideWaves, TK = tile_keys(D);
+  constexpr int PER = 16 * NW / WK;  // rows of a group
+  constexpr int P = D / 8;           // pieces per row
+  constexpr int KI = 64 / P;         // keys of one wave-wide load
+  static_assert(TK == NW * KI && 16 % KI == 0, "one load per wave and tile, inside a block");
+  __shared__ __attribute__((aligned(256))) uint16_t lkv[2][2][TK * D];  // (whole rows aligned: k_at)
   auto& lk = lkv[0];
   auto& lv = lkv[1];
-  __shared__ uint32_t lbad[2][NG];             // the load's block is absent
+  __shared__ uint32_t lbad[2][NW];            // the wave's load was of an absent block
   __shared__ unsigned long long lodd[2][NW];  // (drafted tile) keys whose values are not finite
-  const int lane = threadIdx.x & 63;
-  const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
-  const int li = lane & 15, lg = lane >> 4;
   __shared__ unsigned long long lsee[NW][kMaxTree];
   __shared__ int64_t lpre[64 * NW], lsum[NW];
-  Work<PER> work{again(), lpre, lsum, 0, 0, 0};
+  const int lane = threadIdx.x & 63;
+  const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+  const int wr = wave % (NW / WK), wk = wave / (NW / WK);
+  // LDS byte addresses of this lane's pieces of the first step: key li, piece lg; and
+  // dims 4 (li % 4) .. +3 of key 4 lg + li / 4
+  const int li = lane & 15, lg = lane >> 4, vkey = 4 * lg + (li >> 2);
+  const uint32_t k_at = lds_address(lk) + li * (2 * D) + 16 * (lg ^ (li * P / 16 & (P - 1)));
+  const uint32_t v_at = lds_address(lv) + vkey * (2 * D) + 16 * ((li >> 1 & 1) ^ (2 * (vkey * P / 16) & (P - 1))) + 8 * (li & 1);
+  Work<PER, TK> work{again(), lpre, lsum, 0, 0, 0};
   work.start();
   const int shares = work.shares(), share = xcd_remap(blockIdx.x, gridDim.x);
   if (share >= shares) return;
   const int64_t begin = work.begin(share, shares), end = work.begin(share + 1, shares);
 
   for (int64_t pos = begin; pos < end;) {
-  work.a = again();
-  const typename Work<PER>::Unit un = work.find(pos);
-  const Request& rq = un.rq;
-  const int nrows = rq.tokens * a.group;
-  const int wr = wave % (NW / WK), wk = wave / (NW / WK);
-  const int row0 = un.rg * PER + wr * 32;  // of this wave
-  const bool active = row0 < nrows;
-  const int kh = un.kh, cached = un.cached;
+    work.a = again();
+    const typename Work<PER, TK>::Unit un = work.find(pos);
+    const Request& rq = un.rq;
+    const int nrows = rq.tokens * a.group;
+    const int row0 = un.rg * PER + wr * 16;  // of this wave
+    const bool active = row0 < nrows;
+    const int kh = un.kh, cached = un.cached;
 
-  // this share's tiles of the unit: cached ones, then the drafted tokens'
-  const int t0 = static_cast<int>(pos - un.begin);
-  const int t1 = static_cast<int>(min<int64_t>(un.tiles, end - un.begin));
+    // this share's tiles of the unit: cached ones, then the drafted tokens'
+    const int t0 = static_cast<int>(pos - un.begin);
+    const int t1 = static_cast<int>(min<int64_t>(un.tiles, end - un.begin));
 
-  W w;
-  if (active) {
-    const Attend c = again();
-    w.load(c, rq, kh, row0, nrows, li, lg);
-    if (t1 > cached) w.trees(c, rq, lane, lsee[wave]);
-  }
-
-  const int32_t* table = a.tables + un.b * a.tstride;
-  const uint16_t *kc = a.kc + kh * a.kc_head, *vc = a.vc + kh * a.vc_head;
-  int id[J];  // block ids of the next tile to load
-  auto ids = [&](int t) {
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      int slot;
-      id[j] = t < cached && t < t1 ? table[block_of(a, min(t * TK + (wave * J + j) * KI, rq.len - 1), slot)] : 0;
-    }
-  };
-  u32x4 rk[J], rv[J];  // the tile on its way
-  int bad[J];
-  auto load = [&](int t) {
-    const int ln = here(lane), kin = ln / P, piece = ln % P;
-    const bool tree = t >= cached;
-    const int key0 = (tree ? t - cached : t) * TK, limit = tree ? rq.tokens : rq.len;
-    if (tree) {
+    W w;
+    if (active) {
       const Attend c = again();
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int at = min(key0 + (wave * J + j) * KI + kin, limit - 1);
-        bad[j] = 0;
-        rk[j] = ld16(c.k + (rq.row0 + at) * c.k_row + kh * c.k_head + 8 * piece);
-        rv[j] = ld16(c.v + (rq.row0 + at) * c.v_row + kh * c.v_head + 8 * piece);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int first = min(key0 + (wave * J + j) * KI, limit - 1);
-        const uint32_t at = min(kin, limit - 1 - first);
-        bad[j] = id[j] < 0 || id[j] >= a.blocks;
+      const int ln = here(lane);
+      w.load(c, rq, kh, row0, nrows, ln & 15, ln >> 4);
+      if (t1 > cached) w.trees(c, rq, ln, lsee[wave]);
+    }
+
+    const int32_t* table = a.tables + un.b * a.tstride;
+    const uint16_t *kc = a.kc + kh * a.kc_head, *vc = a.vc + kh * a.vc_head;
+    // The block of the next tile to load, in a vector register until it is used (an index
+    // the compiler cannot prove uniform: it would move a uniform value to a scalar
+    // register at once, and wait there for the tile on its way as well).
+    int id_lane = 0;
+    auto ids = [&](int t) {
+      int slot;
+      if (t < cached && t < t1)
+        id_lane = table[block_of(a, min(t * TK + wave * KI, rq.len - 1), slot) + (here(lane) >> 6)];
+    };
+    u32x4 rk, rv;  // the tile on its way
+    int bad = 0;
+    auto load = [&](int t) {
+      const int ln = here(lane), kin = ln / P, piece = ln % P;
+      if (t >= cached) {
+        const Attend c = again();
+        const int at = min((t - cached) * TK + wave * KI + kin, rq.tokens - 1);
+        bad = 0;
+        rk = ld16(c.k + (rq.row0 + at) * c.k_row + kh * c.k_head + 8 * piece);
+        rv = ld16(c.v + (rq.row0 + at) * c.v_row + kh * c.v_head + 8 * piece);
+      } else {
+        // (a key past the end reads the last one instead and is masked)
+        const int first = min(t * TK + wave * KI, rq.len - 1);
+        const uint32_t at = min(kin, rq.len - 1 - first);
         int slot;
         block_of(a, first, slot);
-        const int64_t blk = bad[j] ? 0 : id[j], at0 = slot;
-        rk[j] = ld16(kc + blk * a.kc_block + at0 * a.kc_slot + at * a.kc_slot + 8 * piece);
-        rv[j] = ld16(vc + blk * a.vc_block + at0 * a.vc_slot + at * a.vc_slot + 8 * piece);
+        const int id = uniform(id_lane);
+        bad = id < 0 || id >= a.blocks;
+        const int64_t blk = bad ? 0 : id, at0 = slot;
+        rk = ld16(kc + blk * a.kc_block + at0 * a.kc_slot + at * a.kc_slot + 8 * piece);
+        rv = ld16(vc + blk * a.vc_block + at0 * a.vc_slot + at * a.vc_slot + 8 * piece);
       }
-    }
-  };
-  auto park = [&](int t) {
-    const int ln = here(lane), kin = ln / P, piece = ln % P;
-    const int buf = (t - t0) & 1;
-    const bool tree = t >= cached;
-    const int key0 = (tree ? t - cached : t) * TK, limit = tree ? rq.tokens : rq.len;
-    unsigned long long odd = 0;
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int g = wave * J + j, key = g * KI + kin;
+    };
+    auto park = [&](int t) {
+      const int ln = here(lane), kin = ln / P, piece = ln % P;
+      const int buf = (t - t0) & 1, key = wave * KI + kin;
+      const bool tree = t >= cached;
+      const int key0 = (tree ? t - cached : t) * TK, limit = tree ? rq.tokens : rq.len;
       // (as in attend_kernel: no infinity or NaN may meet p = 0)
-      if (bad[j] || key0 + key >= limit) rv[j] = u32x4{0, 0, 0, 0};
+      if (bad || key0 + key >= limit) rv = u32x4{0, 0, 0, 0};
       if (tree) {
         bool wild = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          wild = wild || (rv[j][i] & E::kExp) == E::kExp || (rv[j][i] & E::kExp << 16) == E::kExp << 16;
-        const unsigned long long m = __ballot(wild), one = (P == 16 ? 0xffffull : 0xffull);
+          wild = wild || (rv[i] & E::kExp) == E::kExp || (rv[i] & E::kExp << 16) == E::kExp << 16;
+        const unsigned long long m = __ballot(wild), one = P == 16 ? 0xffffull : 0xffull;
+        uint32_t odd = 0;
         if (m) {
 #pragma unroll
           for (int k = 0; k < KI; ++k)
-            if (m >> (P * k) & one) odd |= 1ull << (g * KI + k);
-          if (m >> (P * kin) & one) rv[j] = u32x4{0, 0, 0, 0};
+            if (m >> (P * k) & one) odd |= 1u << k;
+          if (m >> (P * kin) & one) rv = u32x4{0, 0, 0, 0};
         }
+        // (drafted tokens are 64 at most)
+        if (ln == 0) lodd[buf][wave] = static_cast<unsigned long long>(odd) << (wave * KI & 63);
       }
-      *reinterpret_cast<u32x4*>(&lk[buf][(key * P + (piece ^ (key * P / 16 & (P - 1)))) * 8]) = rk[j];
-      *reinterpret_cast<u32x4*>(&lv[buf][(key * P + piece) * 8]) = rv[j];
-      if (lane == 0) lbad[buf][g] = bad[j];
-    }
-    if (tree && lane == 0) lodd[buf][wave] = odd;
-  };
+      const int turn = key * P / 16;
+      *reinterpret_cast<u32x4*>(&lk[buf][(key * P + (piece ^ (turn & (P - 1)))) * 8]) = rk;
+      *reinterpret_cast<u32x4*>(&lv[buf][(key * P + (piece ^ (2 * turn & (P - 1)))) * 8]) = rv;
+      if (ln == 0) lbad[buf][wave] = bad;
+    };
 
-  if (t0 < t1) {
     ids(t0);
     load(t0);
     ids(t0 + 1);
@@ -779,100 +824,79 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void attend_wide_kernel(Attend 
     if (t0 + 1 < t1) load(t0 + 1);
     ids(t0 + 2);
     __syncthreads();
-  }
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    if (active) {
-      const int ln = here(lane), li = ln & 15, lg = ln >> 4;
-      const bool tree = t >= cached;
-      const int key0 = (tree ? t - cached : t) * TK, limit = tree ? rq.tokens : rq.len;
-      const unsigned long long bm = __ballot(lane < NG && lbad[buf][lane % NG]);
-      const bool masked = tree || key0 + TK > limit || bm;
-      unsigned long long odd = 0;
-      if (tree)
+    for (int t = t0; t < t1; ++t) {
+      const int buf = (t - t0) & 1;
+      if (active) {
+        const bool tree = t >= cached;
+        const int key0 = (tree ? t - cached : t) * TK, limit = tree ? rq.tokens : rq.len;
+        const int ln = here(lane);
+        const uint32_t bm = static_cast<uint32_t>(__ballot(ln < NW && lbad[buf][ln % NW]));
+        const bool masked = tree || key0 + TK > limit || bm;
+        unsigned long long odd = 0;
+        if (tree)
 #pragma unroll
-        for (int i = 0; i < NW; ++i) odd |= lodd[buf][i];
+          for (int i = 0; i < NW; ++i) odd |= lodd[buf][i];
 #pragma unroll 1
-      for (int h = wk; h < TK / 32; h += WK) {
-        if (key0 + 32 * h >= limit) break;
-        u32x4 k[2][DC];
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const int key = 32 * h + 16 * g + li;
-#pragma unroll
-          for (int d = 0; d < DC; ++d)
-            k[g][d] = *reinterpret_cast<const u32x4*>(
-                &lk[buf][(key * P + ((4 * d + lg) ^ (key * P / 16 & (P - 1)))) * 8]);
+        for (int h = wk; h < TK / 32; h += WK) {
+          if (key0 + 32 * h >= limit) break;
+          // a piece's exchange is an exclusive or of its row's address with 16 bytes times
+          // the piece, halves of a step and steps are 16 and 32 whole rows apart
+          const uint32_t kat = k_at + (buf * TK + 32 * h) * (2 * D), vat = v_at + (buf * TK + 32 * h) * (2 * D);
+          auto keys = [&](int g, int d) { return *lds<const u32x4>((kat ^ (64 * d)) + 16 * g * (2 * D)); };
+          auto values = [&](int d) {
+            const u32x2 x = read_transposed((vat ^ (32 * d))), y = read_transposed((vat ^ (32 * d)) + 16 * (2 * D));
+            return u32x4{x[0], x[1], y[0], y[1]};
+          };
+          const uint32_t odd32 = h < 2 ? static_cast<uint32_t>(odd >> (32 * h)) : 0;
+          const int ln = here(lane);
+          auto see = [&](int) { return lsee[wave][min(row0 + (ln & 15), nrows - 1) / again().group]; };
+          w.step(a, keys, values, key0 + 32 * h, limit, tree, masked, bm >> (32 * h / KI) & 1,
+                 bm >> ((32 * h + 16) / KI) & 1, odd32, see, ln & 15, ln >> 4, [&](int j) {
+                   const Attend c = again();
+                   return c.v + (rq.row0 + key0 + 32 * h + j) * c.v_row + kh * c.v_head;
+                 });
         }
-        // (read behind the score products: the registers are the keys' until then)
-        auto values = [&](uint32_t(&v)[8][VW]) {
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint16_t* x = &lv[buf][(32 * h + 16 * (e >> 2) + 4 * lg + (e & 3)) * D + DV * li];
-            if constexpr (VW == 4) {
-              const u32x4 y = *reinterpret_cast<const u32x4*>(x);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) v[e][i] = y[i];
-            } else {
-              const u32x2 y = *reinterpret_cast<const u32x2*>(x);
-#pragma unroll
-              for (int i = 0; i < 2; ++i) v[e][i] = y[i];
-            }
-          }
-        };
-        const uint32_t odd32 = static_cast<uint32_t>(odd >> (32 * h));
-        w.step(a, k, values, key0 + 32 * h, limit, tree, masked, bm >> (32 * h / KI) & 1, bm >> ((32 * h + 16) / KI) & 1, odd32,
-               lsee[wave], li, lg, [&](int j) {
-                 const Attend c = again();
-                 return c.v + (rq.row0 + key0 + 32 * h + j) * c.v_row + kh * c.v_head;
-               });
       }
+      if (t + 1 < t1) park(t + 1);
+      if (t + 2 < t1) load(t + 2);
+      ids(t + 3);
+      __syncthreads();
     }
-    if (t + 1 < t1) park(t + 1);
-    if (t + 2 < t1) load(t + 2);
-    ids(t + 3);
-    __syncthreads();
-  }
-  // (WK = 2) the second half's sums are added to the first's, brought to one reference
-  if constexpr (WK == 2) {
-    float* lo = reinterpret_cast<float*>(lkv) + wr * (2 * DV * 4 * 64);
-    static_assert(sizeof(lkv) >= NW / 2 * 2 * DV * 4 * 64 * 4, "a wave's sums fit its part of the tiles");
-    __shared__ float ls[NW / 2][2][2][64];
-    if (active && wk == 1) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        ls[wr][r][0][lane] = w.mx[r];
-        ls[wr][r][1][lane] = w.l[r][0];
+
+    // (WK = 2) the second slice's sums are added to the first's, brought to one reference
+    if constexpr (WK == 2) {
+      float* lo = reinterpret_cast<float*>(lkv) + wr * (DV * 4 * 64);
+      const int ln = here(lane);
+      static_assert(sizeof(lkv) >= NW / 2 * DV * 4 * 64 * 4, "the sums fit the tiles' space");
+      __shared__ float ls[NW / 2][2][64];
+      if (active && wk == 1) {
+        ls[wr][0][ln] = w.mx[0];
+        ls[wr][1][ln] = w.l[0][0];
 #pragma unroll
         for (int d = 0; d < DV; ++d)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) lo[(r * DV * 4 + 4 * d + i) * 64 + lane] = w.o[r][d][i];
+          for (int i = 0; i < 4; ++i) lo[(4 * d + i) * 64 + ln] = w.o[0][d][i];
       }
+      __syncthreads();
+      if (active && wk == 0) {
+        const float m = ls[wr][0][ln], ref = fmaxf(w.mx[0], m);
+        const float f = __builtin_amdgcn_exp2f(w.mx[0] - ref), g = __builtin_amdgcn_exp2f(m - ref);
+        w.mx[0] = ref;
+        w.l[0][0] = f * w.l[0][0] + g * ls[wr][1][ln];
+#pragma unroll
+        for (int d = 0; d < DV; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w.o[0][d][i] = f * w.o[0][d][i] + g * lo[(4 * d + i) * 64 + ln];
+      }
+      __syncthreads();
     }
-    __syncthreads();
     if (active && wk == 0) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float m = ls[wr][r][0][lane], ref = fmaxf(w.mx[r], m);
-        const float f = __builtin_amdgcn_exp2f(w.mx[r] - ref), g = __builtin_amdgcn_exp2f(m - ref);
-        w.mx[r] = ref;
-        w.l[r][0] = f * w.l[r][0] + g * ls[wr][r][1][lane];
-#pragma unroll
-        for (int d = 0; d < DV; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w.o[r][d][i] = f * w.o[r][d][i] + g * lo[(r * DV * 4 + 4 * d + i) * 64 + lane];
-      }
+      const int64_t slot0 = static_cast<int64_t>(2 * share + (pos != begin)) * PER - un.rg * PER;
+      const int ln = here(lane);
+      w.store(again(), rq, kh, row0, nrows, ln & 15, ln >> 4, t0 == 0 && t1 == un.tiles,
+              [&](int row, int64_t, int) { return slot0 + row; });
     }
-    __syncthreads();
-  }
-  if (active && wk == 0) {
-    const int64_t slot0 = static_cast<int64_t>(2 * share + (pos != begin)) * PER - un.rg * PER;
-    w.store(again(), rq, kh, row0, nrows, li, lg, t0 == 0 && t1 == un.tiles,
-            [&](int row, int64_t, int) { return slot0 + row; });
-  }
-  pos = un.begin + t1;
+    pos = un.begin + t1;
   }
 }
 
@@ -938,24 +962,23 @@ __global__ __launch_bounds__(256) void join_kernel(Attend a, int wk) {
   join_row<D, F16>(a, token, head, parts, threadIdx.x & 63, [&](int i) { return at + i; });
 }
 
-// Behind attend_wide_kernel: eight waves per kJoinRows rows of a (request, key head, row
+// Behind attend_wide_kernel: one wave per row of a (request, key head, row
 // group) that several shares have parts of.
-constexpr int kJoinRows = 32;
 template <int D, int PER, bool F16>
 __global__ __launch_bounds__(64 * kWideWaves) void join_wide_kernel(Attend a) {
   constexpr int NW = kWideWaves;
   __shared__ int64_t lpre[64 * NW], lsum[NW];
   const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
   int u = blockIdx.x;
-  const int piece = u % (PER / kJoinRows);
-  u /= PER / kJoinRows;
+  const int piece = u % (PER / NW);
+  u /= PER / NW;
   const int rg = u % a.row_groups;
   u /= a.row_groups;
   const int kh = u % a.kv_heads, b = u / a.kv_heads;
   const Request rq = request(a, b);
-  const int nrows = rq.tokens * a.group, first = rg * PER + piece * kJoinRows;
+  const int nrows = rq.tokens * a.group, first = rg * PER + piece * NW;
   if (first >= nrows) return;
-  Work<PER> work{a, lpre, lsum, 0, 0, 0};
+  Work<PER, tile_keys(D)> work{a, lpre, lsum, 0, 0, 0};
   work.start();
   while (b >= work.base + work.NT) work.fill(work.base + work.NT, lpre[work.NT - 1]);
   const int64_t before = b > work.base ? lpre[b - work.base - 1] : work.carry;
@@ -967,15 +990,16 @@ __global__ __launch_bounds__(64 * kWideWaves) void join_wide_kernel(Attend a) {
     while (g + 1 < n && work.begin(g + 1, n) <= tile) ++g;
     return g;
   };
-  const int g0 = share(s), g1 = share(e - 1);
+  const int g0 = uniform(share(s)), g1 = uniform(share(e - 1));
   if (g0 == g1) return;  // whole: already written
-  for (int row = first + wave; row < min(nrows, first + kJoinRows); row += NW) {
-    const int t = row / a.group;
-    join_row<D, F16>(a, rq.row0 + t, kh * a.group + row - t * a.group, g1 - g0 + 1, threadIdx.x & 63, [&](int i) {
-      const int g = g0 + i;
-      return static_cast<int64_t>(2 * g + (i == 0 && s > work.begin(g, n))) * PER + row - rg * PER;
-    });
-  }
+  const int row = first + wave;
+  if (row >= nrows) return;
+  const bool late = s > work.begin(g0, n);  // (the unit is not the first of its first share)
+  const int t = row / a.group;
+  join_row<D, F16>(a, rq.row0 + t, kh * a.group + row - t * a.group, g1 - g0 + 1, threadIdx.x & 63, [&](int i) {
+    const int g = g0 + i;
+    return static_cast<int64_t>(2 * g + (i == 0 && late)) * PER + row - rg * PER;
+  });
 }
 
 // The launch shape, a function of sizes the host knows (never of what the device
@@ -1018,11 +1042,11 @@ bool sizes_ok(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads,
 
 template <int D, int WK, bool F16>
 int launch_wide(const Attend& a, hipStream_t st) {
-  constexpr int PER = 32 * kWideWaves / WK;
+  constexpr int PER = 16 * kWideWaves / WK;
   const dim3 blk(64 * kWideWaves);
   hipLaunchKernelGGL((attend_wide_kernel<D, WK, F16>), dim3(kShares), blk, 0, st, a);
   if (int rc = check_launch("tree attention kernel")) return rc;
-  const int64_t grid = static_cast<int64_t>(a.requests) * a.kv_heads * a.row_groups * (PER / kJoinRows);
+  const int64_t grid = static_cast<int64_t>(a.requests) * a.kv_heads * a.row_groups * (PER / kWideWaves);
   hipLaunchKernelGGL((join_wide_kernel<D, PER, F16>), dim3(static_cast<unsigned>(grid)), blk, 0, st, a);
   return check_launch("tree attention join kernel");
 }
