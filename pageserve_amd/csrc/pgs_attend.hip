@@ -57,10 +57,11 @@ struct Attend {
   int32_t cols;
   const int32_t *lens, *offsets, *parents;
   int32_t rows, requests, q_heads, kv_heads, group;  // group: q_heads / kv_heads
-  int32_t max_tokens, row_groups, splits;
+  int32_t max_tokens, splits;
   float c;      // scale * log2(e)
   float* part;  // sums of the parts of rows: [slots][D], slots as Wave::store's caller numbers them
   float* stat;  // [slots][2]: m, l
+  int64_t* sums;  // (wide) [requests]: counts of work up to and with each request
 };
 
 // The lane number where it is used: lane-dependent offsets computed from it are not kept
@@ -240,18 +241,28 @@ struct Wave {
                                        Value value) {
     // lane's scores: keys key0 + 16 h + 4 lg + i
     f32x4 s[R][2];
+    u32x4 k[2][DC], v[DV];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      u32x4 k[DC];
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int d = 0; d < DC; ++d) k[d] = keys(h, d);
-      if (!SPREAD) __builtin_amdgcn_sched_barrier(0);
+      for (int d = 0; d < DC; ++d) k[h][d] = keys(h, d);
+    if (!SPREAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        s[r][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int d = 0; d < DC; ++d) s[r][h] = E::mfma(k[d], q[r][d], s[r][h]);
-      }
+      for (int r = 0; r < R; ++r) s[r][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // (the four chains in turn: none waits for its own last product)
+#pragma unroll
+    for (int d = 0; d < DC; ++d)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r][h] = E::mfma(k[h][d], q[r][d], s[r][h]);
+    if constexpr (!SPREAD) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < DV; ++d) v[d] = values(d);
+      __builtin_amdgcn_sched_barrier(0);
     }
     // exponents against the row's reference, and whether a row needs a new one
     float x[R][8];
@@ -311,19 +322,12 @@ struct Wave {
         p[r][i] = E::pack(__builtin_amdgcn_exp2f(x[r][2 * i]), __builtin_amdgcn_exp2f(x[r][2 * i + 1]));
     const u32x4 ones = {E::kOnes, E::kOnes, E::kOnes, E::kOnes};
 #pragma unroll
-    for (int d0 = 0; d0 < DV; d0 += 4) {
-      u32x4 v[4];
-      if (!SPREAD) __builtin_amdgcn_sched_barrier(0);
+    for (int r = 0; r < R; ++r) l[r] = E::mfma(ones, p[r], l[r]);
 #pragma unroll
-      for (int d = 0; d < 4; ++d) v[d] = values(d0 + d);
-      if (!SPREAD) __builtin_amdgcn_sched_barrier(0);
-      if (d0 == 0)
+    for (int d = 0; d < DV; ++d) {
+      if constexpr (SPREAD) v[d] = values(d);
 #pragma unroll
-        for (int r = 0; r < R; ++r) l[r] = E::mfma(ones, p[r], l[r]);
-#pragma unroll
-      for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int r = 0; r < R; ++r) o[r][d0 + d] = E::mfma(v[d], p[r], o[r][d0 + d]);
+      for (int r = 0; r < R; ++r) o[r][d] = E::mfma(v[d], p[r], o[r][d]);
     }
     for (uint32_t w = odd; w; w &= w - 1) {
       const int j = __builtin_ctz(w);
@@ -596,32 +600,54 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
   return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-// The wide kernel's work: the tiles of all (request, key head, row group), in that
-// order, cut into equal shares for the workgroups, whatever the requests' lengths are.
-// A share begins and ends anywhere in a unit; what it has of a unit that is not whole
-// is left as sums in slot 2 g (the share's first unit) or 2 g + 1 (its last).
-constexpr int kShares = 256;    // workgroups: one per CU
-constexpr int kMinShare = 6;    // tiles that a share has at least
-constexpr int kWideWaves = 16;
+// The wide kernel's work: the tiles of all (request, key head, group of kGroup rows), in
+// that order, cut into equal shares for the workgroups, whatever the requests' lengths
+// are.  A group of at most half the rows has two key slices: half the arithmetic per tile,
+// but the same loads.  A tile counts kFull, or kHalf there (`weight`), as measured.  A
+// share has the tiles that begin in it; of a unit that is not whole it leaves sums in slot
+// 2 g (the unit began in an earlier share) or 2 g + 1.
+constexpr int kFull = 5, kHalf = 4;
+constexpr int kShares = 256;          // workgroups: one per CU
+constexpr int kMinShare = 6 * kFull;  // what a share has at least, in these counts
+constexpr int kWideRows = 2;                  // row tiles of 16 per wave
+constexpr int kWideWaves = 16 / kWideRows;
+constexpr int kGroup = 16 * kWideRows * kWideWaves;
 constexpr int tile_keys(int head_dim) { return 8192 / head_dim; }
-template <int PER, int TK>  // rows of a group, keys of a tile
+
+struct Groups {
+  int tiles, n;     // of a request: tiles per group, groups
+  int last;         // weight of the last group (the others': kFull)
+  int64_t per_head; // counts of one key head
+};
+template <int TK>
+__device__ __forceinline__ Groups groups_of(const Attend& a, const Request& rq) {
+  const int rows = rq.tokens * a.group;
+  Groups g;
+  g.tiles = (rq.len + TK - 1) / TK + (rq.tokens + TK - 1) / TK;
+  g.n = (rows + kGroup - 1) / kGroup;
+  g.last = rows - (g.n - 1) * kGroup > kGroup / 2 ? kFull : kHalf;
+  g.per_head = g.n ? static_cast<int64_t>(g.tiles) * (kFull * (g.n - 1) + g.last) : 0;
+  return g;
+}
+__device__ __forceinline__ int shares_of(int64_t total) {
+  return static_cast<int>(min<int64_t>(kShares, (total + kMinShare - 1) / kMinShare));
+}
+// where share g of n begins
+__device__ __forceinline__ int64_t share_begin(int64_t total, int g, int n) { return g * total / n; }
+
+template <int TK>
 struct Work {
   static constexpr int NT = 64 * kWideWaves;
   Attend a;
-  int64_t* pre;   // LDS [NT]: tiles up to and with request base + i
+  int64_t* pre;   // LDS [NT]: counts up to and with request base + i
   int64_t* wsum;  // LDS [kWideWaves]
   int base;
   int64_t carry, total;
   struct Unit {
     Request rq;
-    int b, kh, rg, tiles, cached;
-    int64_t begin;  // its first tile's number
+    int b, kh, rg, tiles, cached, weight;
+    int64_t begin;  // where its first tile's counts begin
   };
-
-  __device__ __forceinline__ static int tiles_of(const Request& rq) {
-    return (rq.len + TK - 1) / TK + (rq.tokens + TK - 1) / TK;
-  }
-  __device__ __forceinline__ int groups_of(const Request& rq) const { return (rq.tokens * a.group + PER - 1) / PER; }
 
   // pre for the requests from `first` on; every thread must call it
   __device__ __forceinline__ void fill(int first, int64_t before) {
@@ -629,10 +655,7 @@ struct Work {
     base = first;
     carry = before;
     int64_t v = 0;
-    if (first + thread < a.requests) {
-      const Request rq = request(a, first + thread);
-      v = static_cast<int64_t>(tiles_of(rq)) * a.kv_heads * groups_of(rq);
-    }
+    if (first + thread < a.requests) v = groups_of<TK>(a, request(a, first + thread)).per_head * a.kv_heads;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int64_t o = __shfl_up(v, d);
@@ -646,35 +669,18 @@ struct Work {
     pre[thread] = v;
     __syncthreads();
   }
-  __device__ __forceinline__ void start() {
-    // (everything but the lane's own sums is the same in all lanes: scalar registers)
-    fill(0, 0);
-    total = uniform64(pre[NT - 1]);
-    for (int f = NT; f < a.requests; f += NT) {
+  // the total; with `keep` the sums of all requests are left there for the join
+  __device__ __forceinline__ void start(int64_t* keep) {
+    const int thread = here(threadIdx.x);
+    total = 0;
+    for (int f = 0; f < a.requests; f += NT) {
       fill(f, total);
+      if (keep && f + thread < a.requests) keep[f + thread] = pre[thread];
       total = uniform64(pre[NT - 1]);
     }
     if (base) fill(0, 0);
   }
-  __device__ __forceinline__ int shares() const {
-    return static_cast<int>(min<int64_t>(kShares, (total + kMinShare - 1) / kMinShare));
-  }
-  __device__ __forceinline__ int64_t begin(int g, int n) const { return uniform64(g * total / n); }
-
-  __device__ __forceinline__ Unit inside(int b, int64_t local, int64_t first) const {
-    Unit u;
-    const Request rq = request(a, b);
-    u.b = b;
-    u.rq = Request{uniform(rq.row0), uniform(rq.tokens), uniform(rq.len), 0, 0};
-    u.tiles = tiles_of(u.rq);
-    u.cached = (u.rq.len + TK - 1) / TK;
-    const int k = uniform(static_cast<int>(local / u.tiles)), groups = groups_of(u.rq);
-    u.kh = k / groups;
-    u.rg = k % groups;
-    u.begin = first + static_cast<int64_t>(k) * u.tiles;
-    return u;
-  }
-  // the unit of tile number pos < total, pos not before the last call's
+  // the unit at pos < total, pos not before the last call's
   __device__ __forceinline__ Unit find(int64_t pos) {
     while (pos >= uniform64(pre[NT - 1])) fill(base + NT, uniform64(pre[NT - 1]));
     int lo = 0, hi = NT - 1;
@@ -683,15 +689,27 @@ struct Work {
       if (pre[mid] <= pos) lo = mid + 1;
       else hi = mid;
     }
+    Unit u;
+    u.b = base + uniform(lo);
+    const Request rq = request(a, u.b);
+    u.rq = Request{uniform(rq.row0), uniform(rq.tokens), uniform(rq.len), 0, 0};
+    const Groups g = groups_of<TK>(a, u.rq);
     const int64_t first = uniform64(lo ? pre[lo - 1] : carry);
-    return inside(base + uniform(lo), pos - first, first);
+    u.kh = uniform(static_cast<int>((pos - first) / g.per_head));
+    const int64_t in = pos - first - u.kh * g.per_head;
+    u.rg = uniform(static_cast<int>(min<int64_t>(in / (static_cast<int64_t>(kFull) * g.tiles), g.n - 1)));
+    u.tiles = g.tiles;
+    u.cached = (u.rq.len + TK - 1) / TK;
+    u.weight = u.rg == g.n - 1 ? g.last : kFull;
+    u.begin = first + u.kh * g.per_head + static_cast<int64_t>(u.rg) * kFull * g.tiles;
+    return u;
   }
 };
 
 // Many rows (more than 64 per key head): bound by the matrix units and the softmax.
-// Sixteen waves share tiles of 64 keys (128 at 64 dims) through LDS, 16/WK row tiles of 16
-// rows x WK key slices (WK = 2: a wave takes every second 32-key step of a tile, and the two
-// are joined at the end of a unit).  A tile's rows go from memory to registers one tile
+// Sixteen waves share tiles of 64 keys (128 at 64 dims) through LDS, 16 row tiles of 16
+// rows, or for a group of at most 128 rows 8 x 2 key slices (a wave then takes every second
+// 32-key step of a tile, and the two are joined at the end of a unit).  A tile's rows go from memory to registers one tile
 // ahead of their use, one 16-byte load of keys and one of values per lane, and from there to
 // one of two LDS buffers: one barrier per tile, and a load has a tile's arithmetic to arrive.
 // Four waves per SIMD with 16 rows each hide the chain scores - softmax - output of one
@@ -702,49 +720,53 @@ struct Work {
 // of an access meet all banks.  Values are read transposed, 4 keys x 16 dims per 16 lanes
 // (ds_read_b64_tr_b16: lane n gets dim n of the four keys), a pair of pieces of 16 keys per
 // access: they are exchanged in pairs, p ^ 2 (r D / 128).
-template <int D, int WK, bool F16>
-__global__ __launch_bounds__(64 * kWideWaves, 4) void attend_wide_kernel(Attend a) {
-  using W = Wave<D, 1, F16, false>;
+template <int D, bool F16>
+__global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_kernel(Attend a) {
+  constexpr int R = kWideRows, J = kWideRows;  // J: loads per wave, tile and matrix
+  using W = Wave<D, R, F16, false>;
   using E = Elem<F16>;
   constexpr int DV = W::DV;
   constexpr int NW = kWideWaves, TK = tile_keys(D);
-  constexpr int PER = 16 * NW / WK;  // rows of a group
   constexpr int P = D / 8;           // pieces per row
   constexpr int KI = 64 / P;         // keys of one wave-wide load
-  static_assert(TK == NW * KI && 16 % KI == 0, "one load per wave and tile, inside a block");
+  static_assert(TK == NW * KI * J && 16 % KI == 0, "a load lies in one block");
   __shared__ __attribute__((aligned(256))) uint16_t lkv[2][2][TK * D];  // (whole rows aligned: k_at)
   auto& lk = lkv[0];
   auto& lv = lkv[1];
-  __shared__ uint32_t lbad[2][NW];            // the wave's load was of an absent block
+  __shared__ uint32_t lbad[2][NW * J];        // the load was of an absent block
   __shared__ unsigned long long lodd[2][NW];  // (drafted tile) keys whose values are not finite
   __shared__ unsigned long long lsee[NW][kMaxTree];
   __shared__ int64_t lpre[64 * NW], lsum[NW];
   const int lane = threadIdx.x & 63;
   const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
-  const int wr = wave % (NW / WK), wk = wave / (NW / WK);
   // LDS byte addresses of this lane's pieces of the first step: key li, piece lg; and
   // dims 4 (li % 4) .. +3 of key 4 lg + li / 4
   const int li = lane & 15, lg = lane >> 4, vkey = 4 * lg + (li >> 2);
   const uint32_t k_at = lds_address(lk) + li * (2 * D) + 16 * (lg ^ (li * P / 16 & (P - 1)));
   const uint32_t v_at = lds_address(lv) + vkey * (2 * D) + 16 * ((li >> 1 & 1) ^ (2 * (vkey * P / 16) & (P - 1))) + 8 * (li & 1);
-  Work<PER, TK> work{again(), lpre, lsum, 0, 0, 0};
-  work.start();
-  const int shares = work.shares(), share = xcd_remap(blockIdx.x, gridDim.x);
+  Work<TK> work{again(), lpre, lsum, 0, 0, 0};
+  work.start(blockIdx.x == 0 ? work.a.sums : nullptr);
+  const int shares = shares_of(work.total), share = xcd_remap(blockIdx.x, gridDim.x);
   if (share >= shares) return;
-  const int64_t begin = work.begin(share, shares), end = work.begin(share + 1, shares);
+  const int64_t begin = uniform64(share_begin(work.total, share, shares));
+  const int64_t end = uniform64(share_begin(work.total, share + 1, shares));
 
   for (int64_t pos = begin; pos < end;) {
     work.a = again();
-    const typename Work<PER, TK>::Unit un = work.find(pos);
+    const typename Work<TK>::Unit un = work.find(pos);
     const Request& rq = un.rq;
     const int nrows = rq.tokens * a.group;
-    const int row0 = un.rg * PER + wr * 16;  // of this wave
+    const int slices = un.weight == kHalf ? 2 : 1;  // of the keys
+    const int wr = slices == 2 ? wave % (NW / 2) : wave, wk = slices == 2 ? wave / (NW / 2) : 0;
+    const int row0 = un.rg * kGroup + wr * (16 * R);  // of this wave
     const bool active = row0 < nrows;
     const int kh = un.kh, cached = un.cached;
 
     // this share's tiles of the unit: cached ones, then the drafted tokens'
-    const int t0 = static_cast<int>(pos - un.begin);
-    const int t1 = static_cast<int>(min<int64_t>(un.tiles, end - un.begin));
+    const int t0 = uniform(static_cast<int>((pos - un.begin + un.weight - 1) / un.weight));
+    const int t1 = uniform(static_cast<int>(min<int64_t>(un.tiles, (end - un.begin + un.weight - 1) / un.weight)));
+    pos = un.begin + static_cast<int64_t>(un.tiles) * un.weight;  // the next unit's
+    if (t0 >= t1) continue;
 
     W w;
     if (active) {
@@ -759,62 +781,75 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void attend_wide_kernel(Attend 
     // The block of the next tile to load, in a vector register until it is used (an index
     // the compiler cannot prove uniform: it would move a uniform value to a scalar
     // register at once, and wait there for the tile on its way as well).
-    int id_lane = 0;
+    int id_lane[J] = {};
     auto ids = [&](int t) {
-      int slot;
-      if (t < cached && t < t1)
-        id_lane = table[block_of(a, min(t * TK + wave * KI, rq.len - 1), slot) + (here(lane) >> 6)];
+      if (t >= cached || t >= t1) return;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        int slot;
+        id_lane[j] = table[block_of(a, min(t * TK + (wave * J + j) * KI, rq.len - 1), slot) + (here(lane) >> 6)];
+      }
     };
-    u32x4 rk, rv;  // the tile on its way
-    int bad = 0;
+    u32x4 rk[J], rv[J];  // the tile on its way
+    int bad[J];
     auto load = [&](int t) {
       const int ln = here(lane), kin = ln / P, piece = ln % P;
       if (t >= cached) {
         const Attend c = again();
-        const int at = min((t - cached) * TK + wave * KI + kin, rq.tokens - 1);
-        bad = 0;
-        rk = ld16(c.k + (rq.row0 + at) * c.k_row + kh * c.k_head + 8 * piece);
-        rv = ld16(c.v + (rq.row0 + at) * c.v_row + kh * c.v_head + 8 * piece);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const int at = min((t - cached) * TK + (wave * J + j) * KI + kin, rq.tokens - 1);
+          bad[j] = 0;
+          rk[j] = ld16(c.k + (rq.row0 + at) * c.k_row + kh * c.k_head + 8 * piece);
+          rv[j] = ld16(c.v + (rq.row0 + at) * c.v_row + kh * c.v_head + 8 * piece);
+        }
       } else {
         // (a key past the end reads the last one instead and is masked)
-        const int first = min(t * TK + wave * KI, rq.len - 1);
-        const uint32_t at = min(kin, rq.len - 1 - first);
-        int slot;
-        block_of(a, first, slot);
-        const int id = uniform(id_lane);
-        bad = id < 0 || id >= a.blocks;
-        const int64_t blk = bad ? 0 : id, at0 = slot;
-        rk = ld16(kc + blk * a.kc_block + at0 * a.kc_slot + at * a.kc_slot + 8 * piece);
-        rv = ld16(vc + blk * a.vc_block + at0 * a.vc_slot + at * a.vc_slot + 8 * piece);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const int first = min(t * TK + (wave * J + j) * KI, rq.len - 1);
+          const uint32_t at = min(kin, rq.len - 1 - first);
+          int slot;
+          block_of(a, first, slot);
+          const int id = uniform(id_lane[j]);
+          bad[j] = id < 0 || id >= a.blocks;
+          const int64_t blk = bad[j] ? 0 : id, at0 = slot;
+          rk[j] = ld16(kc + blk * a.kc_block + at0 * a.kc_slot + at * a.kc_slot + 8 * piece);
+          rv[j] = ld16(vc + blk * a.vc_block + at0 * a.vc_slot + at * a.vc_slot + 8 * piece);
+        }
       }
     };
     auto park = [&](int t) {
       const int ln = here(lane), kin = ln / P, piece = ln % P;
-      const int buf = (t - t0) & 1, key = wave * KI + kin;
+      const int buf = (t - t0) & 1;
       const bool tree = t >= cached;
       const int key0 = (tree ? t - cached : t) * TK, limit = tree ? rq.tokens : rq.len;
-      // (as in attend_kernel: no infinity or NaN may meet p = 0)
-      if (bad || key0 + key >= limit) rv = u32x4{0, 0, 0, 0};
-      if (tree) {
-        bool wild = false;
+      uint32_t odd = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          wild = wild || (rv[i] & E::kExp) == E::kExp || (rv[i] & E::kExp << 16) == E::kExp << 16;
-        const unsigned long long m = __ballot(wild), one = P == 16 ? 0xffffull : 0xffull;
-        uint32_t odd = 0;
-        if (m) {
+      for (int j = 0; j < J; ++j) {
+        const int key = (wave * J + j) * KI + kin;
+        // (as in attend_kernel: no infinity or NaN may meet p = 0)
+        if (bad[j] || key0 + key >= limit) rv[j] = u32x4{0, 0, 0, 0};
+        if (tree) {
+          bool wild = false;
 #pragma unroll
-          for (int k = 0; k < KI; ++k)
-            if (m >> (P * k) & one) odd |= 1u << k;
-          if (m >> (P * kin) & one) rv = u32x4{0, 0, 0, 0};
+          for (int i = 0; i < 4; ++i)
+            wild = wild || (rv[j][i] & E::kExp) == E::kExp || (rv[j][i] & E::kExp << 16) == E::kExp << 16;
+          const unsigned long long m = __ballot(wild), one = P == 16 ? 0xffffull : 0xffull;
+          if (m) {
+#pragma unroll
+            for (int k = 0; k < KI; ++k)
+              if (m >> (P * k) & one) odd |= 1u << (j * KI + k);
+            if (m >> (P * kin) & one) rv[j] = u32x4{0, 0, 0, 0};
+          }
         }
-        // (drafted tokens are 64 at most)
-        if (ln == 0) lodd[buf][wave] = static_cast<unsigned long long>(odd) << (wave * KI & 63);
+        const int turn = key * P / 16;
+        *reinterpret_cast<u32x4*>(&lk[buf][(key * P + (piece ^ (turn & (P - 1)))) * 8]) = rk[j];
+        *reinterpret_cast<u32x4*>(&lv[buf][(key * P + (piece ^ (2 * turn & (P - 1)))) * 8]) = rv[j];
+        if (ln == 0) lbad[buf][wave * J + j] = bad[j];
       }
-      const int turn = key * P / 16;
-      *reinterpret_cast<u32x4*>(&lk[buf][(key * P + (piece ^ (turn & (P - 1)))) * 8]) = rk;
-      *reinterpret_cast<u32x4*>(&lv[buf][(key * P + (piece ^ (2 * turn & (P - 1)))) * 8]) = rv;
-      if (ln == 0) lbad[buf][wave] = bad;
+      // (drafted tokens are 64 at most)
+      if (tree && ln == 0) lodd[buf][wave] = static_cast<unsigned long long>(odd) << (wave * J * KI & 63);
     };
 
     ids(t0);
@@ -830,14 +865,14 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void attend_wide_kernel(Attend 
         const bool tree = t >= cached;
         const int key0 = (tree ? t - cached : t) * TK, limit = tree ? rq.tokens : rq.len;
         const int ln = here(lane);
-        const uint32_t bm = static_cast<uint32_t>(__ballot(ln < NW && lbad[buf][ln % NW]));
+        const uint32_t bm = static_cast<uint32_t>(__ballot(ln < NW * J && lbad[buf][ln % (NW * J)]));
         const bool masked = tree || key0 + TK > limit || bm;
         unsigned long long odd = 0;
         if (tree)
 #pragma unroll
           for (int i = 0; i < NW; ++i) odd |= lodd[buf][i];
 #pragma unroll 1
-        for (int h = wk; h < TK / 32; h += WK) {
+        for (int h = wk; h < TK / 32; h += slices) {
           if (key0 + 32 * h >= limit) break;
           // a piece's exchange is an exclusive or of its row's address with 16 bytes times
           // the piece, halves of a step and steps are 16 and 32 whole rows apart
@@ -849,7 +884,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void attend_wide_kernel(Attend 
           };
           const uint32_t odd32 = h < 2 ? static_cast<uint32_t>(odd >> (32 * h)) : 0;
           const int ln = here(lane);
-          auto see = [&](int) { return lsee[wave][min(row0 + (ln & 15), nrows - 1) / again().group]; };
+          auto see = [&](int r) { return lsee[wave][min(row0 + 16 * r + (ln & 15), nrows - 1) / again().group]; };
           w.step(a, keys, values, key0 + 32 * h, limit, tree, masked, bm >> (32 * h / KI) & 1,
                  bm >> ((32 * h + 16) / KI) & 1, odd32, see, ln & 15, ln >> 4, [&](int j) {
                    const Attend c = again();
@@ -863,40 +898,46 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void attend_wide_kernel(Attend 
       __syncthreads();
     }
 
-    // (WK = 2) the second slice's sums are added to the first's, brought to one reference
-    if constexpr (WK == 2) {
-      float* lo = reinterpret_cast<float*>(lkv) + wr * (DV * 4 * 64);
+    // (two slices) the second's sums are added to the first's, brought to one reference
+    if (slices == 2) {
+      float* lo = reinterpret_cast<float*>(lkv) + wr * (R * DV * 4 * 64);
       const int ln = here(lane);
-      static_assert(sizeof(lkv) >= NW / 2 * DV * 4 * 64 * 4, "the sums fit the tiles' space");
-      __shared__ float ls[NW / 2][2][64];
+      static_assert(sizeof(lkv) >= NW / 2 * R * DV * 4 * 64 * 4, "the sums fit the tiles' space");
+      __shared__ float ls[NW / 2][R][2][64];
       if (active && wk == 1) {
-        ls[wr][0][ln] = w.mx[0];
-        ls[wr][1][ln] = w.l[0][0];
 #pragma unroll
-        for (int d = 0; d < DV; ++d)
+        for (int r = 0; r < R; ++r) {
+          ls[wr][r][0][ln] = w.mx[r];
+          ls[wr][r][1][ln] = w.l[r][0];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) lo[(4 * d + i) * 64 + ln] = w.o[0][d][i];
+          for (int d = 0; d < DV; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lo[(r * DV * 4 + 4 * d + i) * 64 + ln] = w.o[r][d][i];
+        }
       }
       __syncthreads();
       if (active && wk == 0) {
-        const float m = ls[wr][0][ln], ref = fmaxf(w.mx[0], m);
-        const float f = __builtin_amdgcn_exp2f(w.mx[0] - ref), g = __builtin_amdgcn_exp2f(m - ref);
-        w.mx[0] = ref;
-        w.l[0][0] = f * w.l[0][0] + g * ls[wr][1][ln];
 #pragma unroll
-        for (int d = 0; d < DV; ++d)
+        for (int r = 0; r < R; ++r) {
+          const float m = ls[wr][r][0][ln], ref = fmaxf(w.mx[r], m);
+          const float f = __builtin_amdgcn_exp2f(w.mx[r] - ref), g = __builtin_amdgcn_exp2f(m - ref);
+          w.mx[r] = ref;
+          w.l[r][0] = f * w.l[r][0] + g * ls[wr][r][1][ln];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w.o[0][d][i] = f * w.o[0][d][i] + g * lo[(4 * d + i) * 64 + ln];
+          for (int d = 0; d < DV; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w.o[r][d][i] = f * w.o[r][d][i] + g * lo[(r * DV * 4 + 4 * d + i) * 64 + ln];
+        }
       }
       __syncthreads();
     }
     if (active && wk == 0) {
-      const int64_t slot0 = static_cast<int64_t>(2 * share + (pos != begin)) * PER - un.rg * PER;
+      const int64_t slot0 = static_cast<int64_t>(2 * share + (un.begin >= begin) - un.rg) * kGroup;
       const int ln = here(lane);
       w.store(again(), rq, kh, row0, nrows, ln & 15, ln >> 4, t0 == 0 && t1 == un.tiles,
               [&](int row, int64_t, int) { return slot0 + row; });
     }
-    pos = un.begin + t1;
   }
 }
 
@@ -962,60 +1003,47 @@ __global__ __launch_bounds__(256) void join_kernel(Attend a, int wk) {
   join_row<D, F16>(a, token, head, parts, threadIdx.x & 63, [&](int i) { return at + i; });
 }
 
-// Behind attend_wide_kernel: one wave per row of a (request, key head, row
-// group) that several shares have parts of.
-template <int D, int PER, bool F16>
-__global__ __launch_bounds__(64 * kWideWaves) void join_wide_kernel(Attend a) {
-  constexpr int NW = kWideWaves;
-  __shared__ int64_t lpre[64 * NW], lsum[NW];
-  const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
-  int u = blockIdx.x;
-  const int piece = u % (PER / NW);
-  u /= PER / NW;
-  const int rg = u % a.row_groups;
-  u /= a.row_groups;
-  const int kh = u % a.kv_heads, b = u / a.kv_heads;
+// Behind attend_wide_kernel: one wave per row; rows of whole units are already written.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void join_wide_kernel(Attend a) {
+  int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + uniform(static_cast<int>(threadIdx.x >> 6));
+  const int row = static_cast<int>(u % (a.max_tokens * a.group));
+  u /= a.max_tokens * a.group;
+  const int kh = static_cast<int>(u % a.kv_heads), b = static_cast<int>(u / a.kv_heads);
+  if (b >= a.requests) return;
   const Request rq = request(a, b);
-  const int nrows = rq.tokens * a.group, first = rg * PER + piece * NW;
-  if (first >= nrows) return;
-  Work<PER, tile_keys(D)> work{a, lpre, lsum, 0, 0, 0};
-  work.start();
-  while (b >= work.base + work.NT) work.fill(work.base + work.NT, lpre[work.NT - 1]);
-  const int64_t before = b > work.base ? lpre[b - work.base - 1] : work.carry;
-  const int tiles = work.tiles_of(rq), n = work.shares();
-  const int64_t s = before + static_cast<int64_t>(kh * work.groups_of(rq) + rg) * tiles, e = s + tiles;
-  // the shares of its first and last tile: the largest g with begin(g) <= tile
-  auto share = [&](int64_t tile) {
-    int g = static_cast<int>(tile * n / work.total);
-    while (g + 1 < n && work.begin(g + 1, n) <= tile) ++g;
-    return g;
+  if (row >= rq.tokens * a.group) return;
+  const Groups g = groups_of<tile_keys(D)>(a, rq);
+  const int64_t total = a.sums[a.requests - 1];
+  const int n = shares_of(total), rg = row / kGroup;
+  // the unit's first and last tile, and their shares: the largest that begin by then
+  const int64_t s = (b ? a.sums[b - 1] : 0) + kh * g.per_head + static_cast<int64_t>(rg) * kFull * g.tiles;
+  const int64_t e = s + static_cast<int64_t>(g.tiles - 1) * (rg == g.n - 1 ? g.last : kFull);
+  auto share = [&](int64_t at) {
+    int k = static_cast<int>(at * n / total);
+    while (k + 1 < n && share_begin(total, k + 1, n) <= at) ++k;
+    return k;
   };
-  const int g0 = uniform(share(s)), g1 = uniform(share(e - 1));
-  if (g0 == g1) return;  // whole: already written
-  const int row = first + wave;
-  if (row >= nrows) return;
-  const bool late = s > work.begin(g0, n);  // (the unit is not the first of its first share)
+  const int g0 = share(s), g1 = share(e);
+  if (g0 == g1) return;
   const int t = row / a.group;
-  join_row<D, F16>(a, rq.row0 + t, kh * a.group + row - t * a.group, g1 - g0 + 1, threadIdx.x & 63, [&](int i) {
-    const int g = g0 + i;
-    return static_cast<int64_t>(2 * g + (i == 0 && late)) * PER + row - rg * PER;
-  });
+  join_row<D, F16>(a, rq.row0 + t, kh * a.group + row - t * a.group, g1 - g0 + 1, threadIdx.x & 63,
+                   [&](int i) { return static_cast<int64_t>(2 * (g0 + i) + (i == 0) - rg) * kGroup + row; });
 }
 
 // The launch shape, a function of sizes the host knows (never of what the device
 // arrays hold, so that a captured call replays with other lengths).
 struct Plan {
-  int wide;  // rows of a group of the wide kernel, or 0
-  int r, wr; // else row tiles per wave, waves per key slice
-  int row_groups, splits;
+  bool wide;
+  int r, wr;  // else row tiles per wave, waves per key slice
+  int splits;
 };
 Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t max_tokens, int64_t max_context) {
   const int64_t rows = max_tokens * (q_heads / kv_heads);
   Plan p;
-  p.wide = rows <= 64 ? 0 : rows <= 128 ? 128 : 256;
+  p.wide = rows > 64;
   p.r = rows <= 16 ? 1 : 2;
   p.wr = rows <= 32 ? 1 : 2;
-  p.row_groups = p.wide ? static_cast<int>((rows + p.wide - 1) / p.wide) : 1;
   p.splits = 1;
   if (!p.wide) {
     const int64_t steps = (max_context + 31) / 32 + (max_tokens + 31) / 32;
@@ -1026,10 +1054,10 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t max_token
 }
 
 int64_t slots_of(const Plan& p, int64_t rows, int64_t q_heads) {
-  return p.wide ? int64_t{2} * kShares * p.wide : p.splits == 1 ? 0 : rows * q_heads * p.splits;
+  return p.wide ? int64_t{2} * kShares * kGroup : p.splits == 1 ? 0 : rows * q_heads * p.splits;
 }
-size_t workspace_bytes(const Plan& p, int64_t rows, int64_t q_heads, int64_t head_dim) {
-  return static_cast<size_t>(slots_of(p, rows, q_heads)) * (head_dim + 2) * 4;
+size_t workspace_bytes(const Plan& p, int64_t rows, int64_t requests, int64_t q_heads, int64_t head_dim) {
+  return static_cast<size_t>(slots_of(p, rows, q_heads)) * (head_dim + 2) * 4 + (p.wide ? 8 * requests : 0);
 }
 
 bool sizes_ok(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_tokens,
@@ -1040,20 +1068,18 @@ bool sizes_ok(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads,
          requests * max_tokens * q_heads <= 0x3fffffff;  // (grids are 32-bit)
 }
 
-template <int D, int WK, bool F16>
+template <int D, bool F16>
 int launch_wide(const Attend& a, hipStream_t st) {
-  constexpr int PER = 16 * kWideWaves / WK;
-  const dim3 blk(64 * kWideWaves);
-  hipLaunchKernelGGL((attend_wide_kernel<D, WK, F16>), dim3(kShares), blk, 0, st, a);
+  hipLaunchKernelGGL((attend_wide_kernel<D, F16>), dim3(kShares), dim3(64 * kWideWaves), 0, st, a);
   if (int rc = check_launch("tree attention kernel")) return rc;
-  const int64_t grid = static_cast<int64_t>(a.requests) * a.kv_heads * a.row_groups * (PER / kWideWaves);
-  hipLaunchKernelGGL((join_wide_kernel<D, PER, F16>), dim3(static_cast<unsigned>(grid)), blk, 0, st, a);
+  const int64_t rows = static_cast<int64_t>(a.requests) * a.max_tokens * a.q_heads;
+  hipLaunchKernelGGL((join_wide_kernel<D, F16>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, st, a);
   return check_launch("tree attention join kernel");
 }
 
 template <int D, bool F16>
 int launch(const Attend& a, const Plan& p, hipStream_t st) {
-  if (p.wide) return p.wide == 256 ? launch_wide<D, 1, F16>(a, st) : launch_wide<D, 2, F16>(a, st);
+  if (p.wide) return launch_wide<D, F16>(a, st);
   const dim3 g(static_cast<unsigned>(a.requests * a.kv_heads * p.splits)), blk(64 * kWaves);
   if (p.r == 1) hipLaunchKernelGGL((attend_kernel<D, 1, 1, F16>), g, blk, 0, st, a);
   else if (p.wr == 1) hipLaunchKernelGGL((attend_kernel<D, 2, 1, F16>), g, blk, 0, st, a);
@@ -1075,7 +1101,7 @@ extern "C" size_t pgs_tree_attention_workspace_bytes(int64_t rows, int64_t reque
                                                      int64_t head_dim, int64_t max_tokens, int64_t max_context) {
   if (!sizes_ok(rows, requests, q_heads, kv_heads, head_dim, max_tokens, max_context) || rows == 0 || requests == 0)
     return 0;
-  return workspace_bytes(plan(requests, q_heads, kv_heads, max_tokens, max_context), rows, q_heads, head_dim);
+  return workspace_bytes(plan(requests, q_heads, kv_heads, max_tokens, max_context), rows, requests, q_heads, head_dim);
 }
 
 extern "C" int pgs_tree_attention(const pgs_tree_attention_args* args, void* workspace, size_t workspace_bytes_given,
@@ -1114,7 +1140,7 @@ extern "C" int pgs_tree_attention(const pgs_tree_attention_args* args, void* wor
       !aligned(g.block_tables, 4))
     return fail(PGS_ERR_MISALIGNED, "%s: tensors must be 16-byte aligned", fn);
   const Plan p = plan(g.requests, g.q_heads, c.kv_heads, g.max_tokens, g.max_context);
-  const size_t need = workspace_bytes(p, g.rows, g.q_heads, c.head_dim);
+  const size_t need = workspace_bytes(p, g.rows, g.requests, g.q_heads, c.head_dim);
   if (need > 0 && (!workspace || workspace_bytes_given < need || !aligned(workspace, 256)))
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -1137,10 +1163,11 @@ extern "C" int pgs_tree_attention(const pgs_tree_attention_args* args, void* wor
   a.rows = static_cast<int32_t>(g.rows), a.requests = static_cast<int32_t>(g.requests);
   a.q_heads = static_cast<int32_t>(g.q_heads), a.kv_heads = static_cast<int32_t>(c.kv_heads);
   a.group = a.q_heads / a.kv_heads;
-  a.max_tokens = static_cast<int32_t>(g.max_tokens), a.row_groups = p.row_groups, a.splits = p.splits;
+  a.max_tokens = static_cast<int32_t>(g.max_tokens), a.splits = p.splits;
   a.c = g.scale * 1.44269504088896340736f;
   a.part = static_cast<float*>(workspace);
   a.stat = a.part + slots_of(p, g.rows, g.q_heads) * c.head_dim;
+  a.sums = reinterpret_cast<int64_t*>(a.stat + slots_of(p, g.rows, g.q_heads) * 2);
   if (c.head_dim == 64)
     return g.dtype == PGS_DTYPE_F16 ? launch<64, true>(a, p, st) : launch<64, false>(a, p, st);
   return g.dtype == PGS_DTYPE_F16 ? launch<128, true>(a, p, st) : launch<128, false>(a, p, st);
