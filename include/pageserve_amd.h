@@ -488,11 +488,15 @@ int pgs_dequantize4_packed(const void* qp, const void* sp, int64_t n, int64_t k,
  * residual + the linear's output rounded to y_dtype, as in
  * pgs_w8a16_linear_residual; y may be the residual buffer.  Made for the few
  * tokens of a drafting step; above 64 rows the weights are read once per 64.
+ * The workspace holds the partial sums of a K that is split over workgroups
+ * (0 bytes: none is needed, and it may be NULL); it must be 16-byte aligned.
  */
+size_t pgs_w4a16_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int pgs_w4a16_linear(const void* x, const void* qp, const void* sp,
                      const void* bias, const void* residual, void* y,
                      int y_dtype, int64_t m, int64_t n, int64_t k,
-                     int64_t group, void* stream);
+                     int64_t group, void* workspace, size_t workspace_bytes,
+                     void* stream);
 
 /*
  * ---------------------------------------------------------------------------

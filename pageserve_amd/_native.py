@@ -139,7 +139,8 @@ SIGNATURES = {
     "pgs_packed4_scales": (_I64, [_I64, _I64, _I64]),
     "pgs_quantize4_packed": (_INT, [_VP, _INT, _I64, _I64, _I64, _VP, _VP, _VP]),
     "pgs_dequantize4_packed": (_INT, [_VP, _VP, _I64, _I64, _I64, _VP, _INT, _VP]),
-    "pgs_w4a16_linear": (_INT, [_VP, _VP, _VP, _VP, _VP, _VP, _INT, _I64, _I64, _I64, _I64, _VP]),
+    "pgs_w4a16_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "pgs_w4a16_linear": (_INT, [_VP, _VP, _VP, _VP, _VP, _VP, _INT, _I64, _I64, _I64, _I64, _VP, _SZ, _VP]),
     "pgs_append_blocks": (_INT, [_VP, _VP, _VP, _I64, _I64, _VP, _I64, _VP, _I64, _I64, _VP, _VP, _I64, _VP, _VP,
                                  _VP]),
     "pgs_truncate_blocks": (_INT, [_VP, _VP, _VP, _I64, _I64, _VP, _I64, _VP, _I64, _I64, _VP]),

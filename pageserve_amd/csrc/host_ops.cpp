@@ -292,10 +292,13 @@ at::Tensor linear4(const at::Tensor& x, const at::Tensor& qp, const at::Tensor& 
     res = r.reshape({m, n});
     if (!res.is_contiguous()) res = res.contiguous();
   }
+  const size_t need = pgs_w4a16_workspace_bytes(m, n, k);
+  at::Tensor ws;  // (per call, as in tree_attention)
+  if (need) ws = at::empty({static_cast<int64_t>(need)}, x2.options().dtype(at::kByte));
   void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
   check_rc(pgs_w4a16_linear(ptr(x2), ptr(qp), ptr(sp), b.defined() ? ptr(b) : nullptr,
                             res.defined() ? ptr(res) : nullptr, ptr(y), out_f32 ? PGS_DTYPE_F32 : PGS_DTYPE_BF16, m, n, k,
-                            group, st),
+                            group, need ? ws.data_ptr() : nullptr, need, st),
            "w4a16 linear");
   return x.dim() == 2 ? y : y.view(out_shape(x, n));
 }

@@ -3,7 +3,7 @@ against the oracle, ``linear4`` against 64-bit sums.
 
 Tolerance of a sum: the products value * x are exact in fp32 (2 + 8 significant
 bits) and so is a weight's scale; a group's sum has at most ``group`` additions,
-the scaled sums and the waves' parts K / 32 + 32 more, each off by at most 2^-23
+the scaled sums, the waves' parts and the splits of K together K / 32 + 32 more, each off by at most 2^-23
 of the magnitudes added so far (twice a rounding's half step, for adders that cut
 instead of rounding): (group + K / 32 + 32) 2^-23 sum |x| |w|.  The output adds half
 a step of its type, and with a residual the linear's own rounding to that type
@@ -89,7 +89,10 @@ def _check(y, w, x, group, dtype, bias=None, residual=None, what=""):
     (1, 1, 16, 32), (1, 16, 128, 128), (3, 17, 144, 64), (1, 2048, 2048, 128), (5, 1000, 896, 32), (16, 100, 4864, 64),
     (8, 896, 896, 128), (9, 896, 896, 128), (2, 2048, 11008, 32), (17, 48, 272, 32), (32, 896, 4864, 128), (30, 33, 1040, 64),
     (33, 250, 2048, 64), (64, 128, 528, 128), (65, 40, 160, 32), (130, 513, 640, 64), (1, 9000, 256, 64),
-    (24, 40000, 256, 32), (4, 8, 32768, 32)])
+    (24, 40000, 256, 32), (4, 8, 32768, 32),
+    # whole tiles for few tokens, four tiles a workgroup, K split over workgroups
+    (8, 8191, 144, 128), (16, 8209, 272, 32), (31, 8300, 528, 128), (61, 8190, 400, 64),
+    (9, 100, 11008, 64), (16, 2048, 11008, 128), (30, 50, 8208, 32), (60, 896, 4864, 64), (200, 70, 11024, 128)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_linear(gpu, m, n, k, group, dtype):
     qw, w, x = _case(gpu, m, n, k, group)
@@ -133,8 +136,17 @@ def test_tokens_do_not_touch_each_other(gpu):
         assert torch.equal(y[rows], want[rows]) and torch.isnan(y[1]).all() and not torch.isfinite(y[2]).any()
 
 
-def test_streams_and_graph_replays(gpu):
-    qw, w, x = _case(gpu, 5, 512, 2048, 128)
+def test_in_place_residual_of_a_split_sum(gpu):
+    qw, w, x = _case(gpu, 20, 80, 11008, 64)
+    xt, res = bf16_gpu(x, gpu), bf16_gpu(activations(2, 20, 80), gpu)
+    want = linear4(xt, qw, residual=res)
+    linear4(xt, qw, residual=res, out=res)
+    assert torch.equal(res, want)
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 512, 2048), (20, 256, 11008)])
+def test_streams_and_graph_replays(gpu, m, n, k):
+    qw, w, x = _case(gpu, m, n, k, 128)
     xt = bf16_gpu(x, gpu)
     want = linear4(xt, qw)
     side = torch.cuda.Stream()
@@ -148,7 +160,7 @@ def test_streams_and_graph_replays(gpu):
         y = linear4(xt, qw)
         z = QuantizedWeight4(y.float(), 32).dense()
     for seed in range(3):
-        xt.copy_(bf16_gpu(activations(seed, 5, 2048), gpu))
+        xt.copy_(bf16_gpu(activations(seed, m, k), gpu))
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, linear4(xt, qw)) and torch.equal(z, QuantizedWeight4(y.float(), 32).dense())
