@@ -467,7 +467,7 @@ int pgs_w8a16_decode_span_trace(void* buffer, size_t bytes);
  *        bytes of lane l (0..63) holds columns 32*j + 8*(l/16) .. +7 of row
  *        l%16, column 32*j + 8*(l/16) + i in bits 4*i .. 4*i+3
  *   sp   packed scales, pgs_packed4_scales(n, k, group) bf16 values: per block
- *        16 * (128/group), [4 row quads][128/group groups][4 rows]
+ *        [16 rows][128/group groups]
  * Padding codes and scales are zero.  k must be a multiple of 16.
  */
 int64_t pgs_packed4_bytes(int64_t n, int64_t k);

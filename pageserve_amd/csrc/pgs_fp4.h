@@ -3,14 +3,13 @@
 //
 // Layout: 16-row x 128-column blocks of 1 KiB, [ceil(n/16)][ceil(k/128)].  Lane l
 // of a wave owns 16 bytes: dword j holds the eight codes of row l%16, columns
-// 32 j + 8 (l/16) .. +7, i.e. its A operand of the j-th v_mfma_f32_16x16x32_bf16
+// 32 j + 8 (l/16) .. +7, i.e. its B operand of the j-th v_mfma_f32_16x16x32_bf16
 // of the block; a wave's 128-bit loads fetch one contiguous KiB.  Each MFMA spans
 // 32 neighbouring columns, so it lies inside one group for every group size, and
 // the group's scale multiplies its fp32 result instead of the widened codes.
 //
-// Scales: per block 16 * S bf16 (S = 128 / group), [4 row quads][S groups][4
-// rows]: the accumulator lane l holds rows 4 (l/16) .. +3, whose scales of all S
-// groups are then one contiguous piece of 8 S bytes.
+// Scales: per block [16 rows][S groups] bf16 (S = 128 / group): the accumulator lane
+// l holds sums of row l%16, whose scales are one load of 2 S bytes.
 #pragma once
 
 #include "pgs_linear.h"

@@ -8,7 +8,7 @@
 // neither the weights nor the scales are rounded anywhere.
 //
 // Memory bound: every packed KiB is read once, as one 128-bit load per lane that is
-// already the A operand of four MFMAs.  A workgroup owns R 16-row tiles over all of K;
+// already the B operand of four MFMAs.  A workgroup owns R 16-row tiles over its share of K;
 // its NW waves take 128-column chunks round robin, U per batch, a batch's loads issued
 // together, and the waves' partial tiles meet in LDS in a fixed order.
 #include "pgs_fp4.h"
@@ -31,13 +31,21 @@ struct Lin4 {
 constexpr int64_t kMaxRows4 = 0x7ffffff0, kMaxTokens4 = 65535 * 16;
 constexpr int kNowhere = 0x40000000;  // a lane offset past every activation block (at most 64 rows of kMaxK)
 
+// The tokens are the A operand and the weights the B operand: lane l's four sums are of
+// weight row l%16, so it needs the scales of that row only.  (With the weights as A its
+// sums are of four rows: four times the scales to load and widen, 68 us for 62 at
+// 30 x 151936 x 2048 with groups of 32.)
+//
 // FOLD (m <= 8): a workgroup owns eight rows of a tile (half blockIdx.x % 2) and each MFMA
-// takes two chunks: A rows 0-7 are its rows in chunk 2 c, A rows 8-15 the same rows in
-// chunk 2 c + 1, B columns 0-7 the tokens in chunk 2 c and 8-15 in 2 c + 1, so that output
-// (token t, row i) is D[i][t] + D[i + 8][t + 8] (the other two quarters mix chunks and are
-// ignored).  Twice the workgroups for the same bytes and products.
+// takes two chunks: A rows 0-7 are the tokens in chunk 2 c, A rows 8-15 the same tokens in
+// chunk 2 c + 1, B columns 0-7 the weight rows in chunk 2 c and 8-15 in 2 c + 1, so that
+// output (token t, row i) is D[t][i] + D[t + 8][i + 8] (the other two quarters mix chunks
+// and are ignored).  Twice the workgroups for the same bytes and products.
+//
+// (At least two waves per SIMD are asked for: with fewer the products land in accumulation
+// registers, and each has to be copied out to be scaled: 150 us for 106 at 60 x 151936 x 2048.)
 template <int NW, int U, int TM, int R, int S, bool FOLD, bool OUT_F32>
-__global__ __launch_bounds__(64 * NW) void linear4_kernel(Lin4 a) {
+__global__ __launch_bounds__(64 * NW, 2) void linear4_kernel(Lin4 a) {
   static_assert(!FOLD || (TM == 1 && R == 1), "folding serves up to eight tokens");
   constexpr int MT = FOLD ? 8 : 16 * TM;
   const int lane = threadIdx.x & 63;
@@ -63,9 +71,9 @@ __global__ __launch_bounds__(64 * NW) void linear4_kernel(Lin4 a) {
   }
   const __amdgpu_buffer_rsrc_t xres =
       make_rsrc(a.x + static_cast<int64_t>(m0) * a.k, static_cast<int64_t>(rows) * a.k * 2);
-  const int sub = FOLD ? li >> 3 : 0;  // this lane's chunk of the slot, as A row and B column
+  const int sub = FOLD ? li >> 3 : 0;  // this lane's chunk of the slot, as token and as weight row
   const int woff = FOLD ? sub * 1024 + (8 * half + (li & 7) + 16 * kq) * 16 : lane * 16;
-  const int soff = FOLD ? (kq >> 1) * (32 * S) + (2 * half + (kq & 1)) * (8 * S) : kq * (8 * S);
+  const int soff = FOLD ? sub * (32 * S) + (8 * half + (li & 7)) * (2 * S) : li * (2 * S);
   int xoff[TM];
 #pragma unroll
   for (int t = 0; t < TM; ++t)
@@ -79,7 +87,7 @@ __global__ __launch_bounds__(64 * NW) void linear4_kernel(Lin4 a) {
 
   struct Slot {
     u32x4 w[R];
-    uint32_t s[R][2 * S];
+    uint32_t s[R][(S + 1) / 2];
     u32x4 x[4][TM];
   };
   auto load = [&](Slot& b, int slot) {
@@ -88,15 +96,12 @@ __global__ __launch_bounds__(64 * NW) void linear4_kernel(Lin4 a) {
     for (int r = 0; r < R; ++r) {
       b.w[r] = __builtin_amdgcn_raw_buffer_load_b128(wres[r], woff, c * 1024, kLoadNT);
       if constexpr (S == 1) {
-        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(sres[r], soff, c * 32, 0);
-        b.s[r][0] = v[0], b.s[r][1] = v[1];
+        b.s[r][0] = __builtin_amdgcn_raw_buffer_load_b16(sres[r], soff, c * 32, 0);
+      } else if constexpr (S == 2) {
+        b.s[r][0] = __builtin_amdgcn_raw_buffer_load_b32(sres[r], soff, c * 64, 0);
       } else {
-#pragma unroll
-        for (int h = 0; h < S / 2; ++h) {
-          const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(sres[r], soff + 16 * h, c * (32 * S), 0);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) b.s[r][4 * h + i] = v[i];
-        }
+        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(sres[r], soff, c * 128, 0);
+        b.s[r][0] = v[0], b.s[r][1] = v[1];
       }
     }
 #pragma unroll
@@ -117,20 +122,16 @@ __global__ __launch_bounds__(64 * NW) void linear4_kernel(Lin4 a) {
       for (int j = 0; j < 4; ++j) w[j] = fp4x8_to_bf16x8(b.w[r][j]);
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        f32x4 sc;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          sc[2 * i] = __uint_as_float(b.s[r][2 * s + i] << 16);
-          sc[2 * i + 1] = __uint_as_float(b.s[r][2 * s + i] & 0xffff0000u);
-        }
+        const uint32_t v = b.s[r][s / 2];
+        const float sc = __uint_as_float(s & 1 ? v & 0xffff0000u : v << 16);
 #pragma unroll
         for (int t = 0; t < TM; ++t) {
           f32x4 p = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int j = s * (4 / S); j < (s + 1) * (4 / S); ++j)
-            p = mfma16x16x32(w[j], __builtin_bit_cast(bf16x8, b.x[j][t]), p);
+            p = mfma16x16x32(__builtin_bit_cast(bf16x8, b.x[j][t]), w[j], p);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[r][t][i] = fmaf(p[i], sc[i], acc[r][t][i]);
+          for (int i = 0; i < 4; ++i) acc[r][t][i] = fmaf(p[i], sc, acc[r][t][i]);
         }
       }
     }
@@ -147,25 +148,27 @@ __global__ __launch_bounds__(64 * NW) void linear4_kernel(Lin4 a) {
     for (int u = 0; u < U; ++u) mac(b[u]);
   }
 
-  __shared__ f32x4 part[NW][R][TM][64];
+  __shared__ float part[NW][R][TM][4][64];
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int t = 0; t < TM; ++t) part[wave][r][t][lane] = acc[r][t];
+    for (int t = 0; t < TM; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[wave][r][t][i][lane] = acc[r][t][i];
   __syncthreads();
-  const float* pf = reinterpret_cast<const float*>(part);
+  const float* pf = &part[0][0][0][0][0];
   constexpr int PER = FOLD ? 8 : 16 * R;  // weight rows
   for (int o = threadIdx.x; o < rows * PER; o += 64 * NW) {
     const int mm = o / PER, i = o % PER;
     const int n = tile0 * 16 + 8 * half + i;
     if (n >= a.n) continue;
-    // the accumulator lane of D row i % 16, column mm % 16: 16 (i % 16 / 4) + mm % 16, element i % 4
-    const int r = i >> 4, at = ((((i & 15) >> 2) * 16 + (mm & 15)) << 2) + (i & 3);
+    // D row mm % 16, column i % 16: element mm % 4 of lane 16 (mm % 16 / 4) + i % 16
+    const int r = i >> 4, at = (mm & 3) * 64 + ((mm & 15) >> 2) * 16 + (i & 15);
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const float* p = pf + ((w * R + r) * TM + (mm >> 4)) * 256 + at;
-      v += FOLD ? p[0] + p[(32 + 8) * 4] : p[0];
+      v += FOLD ? p[0] + p[32 + 8] : p[0];
     }
     const int64_t e = static_cast<int64_t>(m0 + mm) * a.n + n;
     if (a.part) {
@@ -192,16 +195,17 @@ __global__ __launch_bounds__(256) void linear4_sum_kernel(Lin4 a) {
 // How a call is laid out.  The chip is filled before anything else: a workgroup is one
 // long chain of loads and products, so twice the workgroups is close to half the time
 // until there are one to two per CU.  Measured, microseconds (own/other choice), m x n x k:
-// - up to 8 tokens and fewer than 512 tiles: folded halves of tiles.  5x2048x11008 6.7/8.5
-//   (whole tiles), 1x2048x2048 2.9/3.1.
+// - up to 8 tokens while the halves of the tiles are at most one per CU: folded halves.
+//   5x2048x11008 6.8/8.1 (whole tiles), 1x2048x2048 3.0/3.2; above: 8x4096x4096 5.3 whole,
+//   6.8 folded.
 // - from 128 workgroups of four tiles on: four tiles (the activations are read once per 64
-//   rows).  16x11008x2048 8.0/8.6 (two tiles), 10x151936x2048 35.6/44.8, 30x8192x2048
-//   9.5/10.0 (one tile), 60x8192x2048 16.2/18.4.
-// - else, for a long K, four tiles with K split over workgroups: 16x2048x11008 9.3/13.7,
-//   30x2048x11008 12.5/22.3, 60x2048x11008 17.9/42.4, 60x4096x4096 15.7/18.1 (one tile).
-//   More than 8 splits: 13.0 for 12.5, 19.8 for 17.9.
-// - else one tile: the second launch costs more than it gains.  16x4096x4096 6.7/8.9,
-//   30x4096x4096 10.0/10.7, 60x4096x2048 10.9/12.7, 16x2048x2048 4.5/6.5.
+//   rows).  1x11008x2048 5.1/5.3 (one tile), 16x11008x2048 6.3/8.6, 10x151936x2048
+//   33.8/62.9, 30x8192x2048 8.5/9.6, 60x8192x2048 15.5/18.1.
+// - else, for a long K, four tiles with K split over workgroups: 16x2048x11008 8.6/13.2 (one
+//   tile), 30x2048x11008 11.1/21.9, 60x2048x11008 17.1/41.9, 60x4096x4096 14.9/17.7.  Half
+//   the splits: 10.5 for 8.6, 22.1 for 17.1; twice: 9.6 and 18.9.
+// - else one tile: the second launch costs more than it gains.  16x4096x4096 6.5/8.3,
+//   30x4096x4096 9.8/10.0, 60x4096x2048 10.6/11.9, 16x2048x2048 4.4/6.7.
 struct Plan {
   int tm;      // 16-token tiles of a workgroup
   int wide;    // 16-row tiles of a workgroup: 4, or 1; 0: folded halves
@@ -209,7 +213,7 @@ struct Plan {
 };
 Plan plan(int64_t m, int64_t n, int64_t k) {
   const int64_t tiles = (n + 15) / 16, kb = (k + 127) / 128;
-  if (m <= 8 && tiles < 512) return {1, 0, 1};
+  if (m <= 8 && tiles <= 128) return {1, 0, 1};
   const int tm = m <= 16 ? 1 : m <= 32 ? 2 : 4;
   const int64_t units = (tiles + 3) / 4 * ((m + 16 * tm - 1) / (16 * tm));
   if (units >= 128) return {tm, 4, 1};
@@ -236,8 +240,9 @@ int launch(const Lin4& a, hipStream_t st) {
   return check_launch("linear4 sum kernel");
 }
 
-// (waves, chunks per batch: the batch's loads are all in flight while its registers still
-// leave two waves per SIMD; the next larger ones measured equal or slower)
+// (waves, chunks per batch: with fewer of either, too few loads are in flight at 11008 rows
+// and fewer: 30x11008x2048 8.7 for 9.7 with four waves; more registers do not hold.  Four
+// waves at 64 tokens: eight spill over two waves per SIMD, 101 us for 155 at 60x151936x2048.)
 template <int S, bool OUT_F32>
 int pick(const Plan& p, const Lin4& a, hipStream_t st) {
   if (p.wide == 0) return launch<8, 2, 1, 1, S, true, OUT_F32>(a, st);
@@ -247,7 +252,7 @@ int pick(const Plan& p, const Lin4& a, hipStream_t st) {
     return launch<8, 1, 4, 1, S, false, OUT_F32>(a, st);
   }
   if (p.tm == 1) return launch<8, 1, 1, 4, S, false, OUT_F32>(a, st);
-  if (p.tm == 2) return launch<4, 2, 2, 4, S, false, OUT_F32>(a, st);
+  if (p.tm == 2) return launch<8, 1, 2, 4, S, false, OUT_F32>(a, st);
   return launch<4, 1, 4, 4, S, false, OUT_F32>(a, st);
 }
 

@@ -97,9 +97,9 @@ __global__ __launch_bounds__(kQ4Threads) void quantize4_kernel(const void* __res
   }
   qp[blk * 64 + lane] = make_uint4(out[0], out[1], out[2], out[3]);
   if (lane < 16) {
-    uint16_t* d = sp + blk * (16 * S) + (lane >> 2) * (4 * S) + (lane & 3);
+    uint16_t* d = sp + (blk * 16 + lane) * S;
 #pragma unroll
-    for (int s = 0; s < S; ++s) d[4 * s] = row < n && c0 + s * (128 / S) < k ? sbits[s] : 0;
+    for (int s = 0; s < S; ++s) d[s] = row < n && c0 + s * (128 / S) < k ? sbits[s] : 0;
   }
 }
 
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(kQ4Threads) void dequantize4_kernel(const uint4* __
   const uint32_t d[4] = {v.x, v.y, v.z, v.w};
   float sc[S];
 #pragma unroll
-  for (int s = 0; s < S; ++s) sc[s] = bf16_bits_to_f32(sp[blk * (16 * S) + (r >> 2) * (4 * S) + 4 * s + (r & 3)]);
+  for (int s = 0; s < S; ++s) sc[s] = bf16_bits_to_f32(sp[(blk * 16 + r) * S + s]);
   if (row >= n) return;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {

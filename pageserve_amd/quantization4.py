@@ -57,7 +57,7 @@ def _pack(codes: torch.Tensor, scale: torch.Tensor, group: int) -> tuple[torch.T
     qp = (c[..., 0] | (c[..., 1] << 4)).contiguous().view(-1)
     p = torch.zeros((tn * 16, tk * s), dtype=torch.bfloat16, device=scale.device)
     p[:n, :scale.shape[1]] = scale
-    sp = p.view(tn, 4, 4, tk, s).permute(0, 3, 1, 4, 2).contiguous().view(-1)
+    sp = p.view(tn, 16, tk, s).transpose(1, 2).contiguous().view(-1)
     return qp, sp
 
 
@@ -126,7 +126,7 @@ class QuantizedWeight4:
         n, k = self.shape
         tn, tk = _blocks(n, k)
         s = 128 // self.group
-        p = self.sp.view(tn, tk, 4, s, 4).permute(0, 2, 4, 1, 3).reshape(tn * 16, tk * s)
+        p = self.sp.view(tn, tk, 16, s).transpose(1, 2).reshape(tn * 16, tk * s)
         return p[:n, :-(-k // self.group)].contiguous()
 
     def to(self, device) -> "QuantizedWeight4":

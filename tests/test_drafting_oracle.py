@@ -68,12 +68,12 @@ def test_packed_layout():
     scale = torch.randn(n, -(-k // group)).bfloat16()
     qw = QuantizedWeight4.from_codes(torch.from_numpy(codes), scale, group)
     words = qw.qp.numpy().view(np.uint32).reshape(-1, 64, 4)
-    sp = qw.sp.view(2, 3, 4, 4, 4)
+    sp = qw.sp.view(2, 3, 16, 4)
     for r, c in [(0, 0), (5, 7), (15, 127), (16, 128), (19, 271), (3, 200)]:
         blk, kk = (r // 16) * 3 + c // 128, c % 128
         word = int(words[blk, r % 16 + 16 * (kk % 32 // 8), kk // 32])
         assert word >> (4 * (kk % 8)) & 15 == codes[r, c]
-        assert sp[r // 16, c // 128, r % 16 // 4, kk // 32, r % 4] == scale[r, c // 32]
+        assert sp[r // 16, c // 128, r % 16, kk // 32] == scale[r, c // 32]
     assert not words[5, :, 2:].any() and not (words[3:, 4:16].any())  # columns from 272 on, rows from 20 on
 
 
