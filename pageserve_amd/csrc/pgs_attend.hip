@@ -86,6 +86,17 @@ __device__ __forceinline__ u32x2 read_transposed(uint32_t address) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<s16x4>(address)));
 }
 
+// 16 bytes per lane from memory to LDS (lane l's to `address` + 16 l, wave-uniform) past
+// the registers.  The compiler does not count this load: whoever uses what it brings waits
+// with arrived(n), n: how many such loads issued later may still be on their way.
+__device__ __forceinline__ void load_lds(const uint16_t* p, uint32_t address) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(address), "v"(p) : "m0", "memory");
+}
+template <int N>
+__device__ __forceinline__ void arrived() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 // The kernel's argument again, read from its segment at this point: for the parts of a
 // kernel outside its inner loop, whose fields would otherwise all sit in scalar
 // registers throughout (and push vector registers out to memory).
@@ -612,6 +623,7 @@ constexpr int kMinShare = 6 * kFull;  // what a share has at least, in these cou
 constexpr int kWideRows = 2;                  // row tiles of 16 per wave
 constexpr int kWideWaves = 16 / kWideRows;
 constexpr int kGroup = 16 * kWideRows * kWideWaves;
+constexpr int kBuffers = 3;                   // tiles in LDS: computed, arriving, sent for
 constexpr int tile_keys(int head_dim) { return 8192 / head_dim; }
 
 struct Groups {
@@ -729,12 +741,11 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
   constexpr int NW = kWideWaves, TK = tile_keys(D);
   constexpr int P = D / 8;           // pieces per row
   constexpr int KI = 64 / P;         // keys of one wave-wide load
-  static_assert(TK == NW * KI * J && 16 % KI == 0, "a load lies in one block");
-  __shared__ __attribute__((aligned(256))) uint16_t lkv[2][2][TK * D];  // (whole rows aligned: k_at)
-  auto& lk = lkv[0];
-  auto& lv = lkv[1];
-  __shared__ uint32_t lbad[2][NW * J];        // the load was of an absent block
-  __shared__ unsigned long long lodd[2][NW];  // (drafted tile) keys whose values are not finite
+  constexpr int KW = J * KI;         // keys of a wave's loads
+  static_assert(TK == NW * KW && 16 % KW == 0, "a wave's keys lie in one block");
+  __shared__ __attribute__((aligned(256))) uint16_t lkv[kBuffers][2][TK * D];  // (whole rows aligned: k_at)
+  __shared__ uint32_t lbad[kBuffers][NW];            // the wave's keys are of an absent block
+  __shared__ unsigned long long lodd[kBuffers][NW];  // (drafted tile) keys whose values are not finite
   __shared__ unsigned long long lsee[NW][kMaxTree];
   __shared__ int64_t lpre[64 * NW], lsum[NW];
   const int lane = threadIdx.x & 63;
@@ -742,8 +753,8 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
   // LDS byte addresses of this lane's pieces of the first step: key li, piece lg; and
   // dims 4 (li % 4) .. +3 of key 4 lg + li / 4
   const int li = lane & 15, lg = lane >> 4, vkey = 4 * lg + (li >> 2);
-  const uint32_t k_at = lds_address(lk) + li * (2 * D) + 16 * (lg ^ (li * P / 16 & (P - 1)));
-  const uint32_t v_at = lds_address(lv) + vkey * (2 * D) + 16 * ((li >> 1 & 1) ^ (2 * (vkey * P / 16) & (P - 1))) + 8 * (li & 1);
+  const uint32_t k_at = lds_address(lkv) + li * (2 * D) + 16 * (lg ^ (li * P / 16 & (P - 1)));
+  const uint32_t v_at = lds_address(lkv) + TK * D * 2 + vkey * (2 * D) + 16 * ((li >> 1 & 1) ^ (2 * (vkey * P / 16) & (P - 1))) + 8 * (li & 1);
   Work<TK> work{again(), lpre, lsum, 0, 0, 0};
   work.start(blockIdx.x == 0 ? work.a.sums : nullptr);
   const int shares = shares_of(work.total), share = xcd_remap(blockIdx.x, gridDim.x);
@@ -778,94 +789,103 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
 
     const int32_t* table = a.tables + un.b * a.tstride;
     const uint16_t *kc = a.kc + kh * a.kc_head, *vc = a.vc + kh * a.vc_head;
-    // The block of the next tile to load, in a vector register until it is used (an index
-    // the compiler cannot prove uniform: it would move a uniform value to a scalar
-    // register at once, and wait there for the tile on its way as well).
-    int id_lane[J] = {};
-    auto ids = [&](int t) {
-      if (t >= cached || t >= t1) return;
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        int slot;
-        id_lane[j] = table[block_of(a, min(t * TK + (wave * J + j) * KI, rq.len - 1), slot) + (here(lane) >> 6)];
-      }
-    };
-    u32x4 rk[J], rv[J];  // the tile on its way
-    int bad[J];
-    auto load = [&](int t) {
+    // Lane i: the block of this wave's keys of tile id0 + i.  (Waited for where it is
+    // loaded: a wait for it further on would be one for the keys on their way too.)
+    int id_lane = 0, id0 = t0 - 64;
+    // tile t into buffer `to`; whether its keys are of an absent block
+    auto load = [&](int t, int to) {
       const int ln = here(lane), kin = ln / P, piece = ln % P;
+      const uint32_t at_k = lds_address(lkv) + to * (4 * TK * D) + wave * (1024 * J), at_v = at_k + 2 * TK * D;
+      // (lane l fills piece l % P of its key's row, which is piece ... of the row in memory)
       if (t >= cached) {
         const Attend c = again();
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-          const int at = min((t - cached) * TK + (wave * J + j) * KI + kin, rq.tokens - 1);
-          bad[j] = 0;
-          rk[j] = ld16(c.k + (rq.row0 + at) * c.k_row + kh * c.k_head + 8 * piece);
-          rv[j] = ld16(c.v + (rq.row0 + at) * c.v_row + kh * c.v_head + 8 * piece);
+          const int key = wave * KW + j * KI + kin, turn = key * P / 16;
+          const int64_t at = rq.row0 + min((t - cached) * TK + key, rq.tokens - 1);
+          load_lds(c.k + at * c.k_row + kh * c.k_head + 8 * (piece ^ (turn & (P - 1))), at_k + 1024 * j);
+          load_lds(c.v + at * c.v_row + kh * c.v_head + 8 * (piece ^ (2 * turn & (P - 1))), at_v + 1024 * j);
         }
-      } else {
-        // (a key past the end reads the last one instead and is masked)
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const int first = min(t * TK + (wave * J + j) * KI, rq.len - 1);
-          const uint32_t at = min(kin, rq.len - 1 - first);
-          int slot;
-          block_of(a, first, slot);
-          const int id = uniform(id_lane[j]);
-          bad[j] = id < 0 || id >= a.blocks;
-          const int64_t blk = bad[j] ? 0 : id, at0 = slot;
-          rk[j] = ld16(kc + blk * a.kc_block + at0 * a.kc_slot + at * a.kc_slot + 8 * piece);
-          rv[j] = ld16(vc + blk * a.vc_block + at0 * a.vc_slot + at * a.vc_slot + 8 * piece);
-        }
+        return false;
       }
-    };
-    auto park = [&](int t) {
-      const int ln = here(lane), kin = ln / P, piece = ln % P;
-      const int buf = (t - t0) & 1;
-      const bool tree = t >= cached;
-      const int key0 = (tree ? t - cached : t) * TK, limit = tree ? rq.tokens : rq.len;
-      uint32_t odd = 0;
+      if (t >= id0 + 64) {
+        id0 = t;
+        int slot;
+        const int64_t key = min<int64_t>(static_cast<int64_t>(t + ln) * TK + wave * KW, rq.len - 1);
+        id_lane = table[block_of(a, static_cast<int>(key), slot)];
+        asm volatile("" : "+v"(id_lane));
+      }
+      const int id = __builtin_amdgcn_readlane(id_lane, t - id0);
+      const bool bad = id < 0 || id >= a.blocks;
+      const int64_t blk = bad ? 0 : id;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        const int key = (wave * J + j) * KI + kin;
-        // (as in attend_kernel: no infinity or NaN may meet p = 0)
-        if (bad[j] || key0 + key >= limit) rv[j] = u32x4{0, 0, 0, 0};
-        if (tree) {
-          bool wild = false;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            wild = wild || (rv[j][i] & E::kExp) == E::kExp || (rv[j][i] & E::kExp << 16) == E::kExp << 16;
-          const unsigned long long m = __ballot(wild), one = P == 16 ? 0xffffull : 0xffull;
-          if (m) {
-#pragma unroll
-            for (int k = 0; k < KI; ++k)
-              if (m >> (P * k) & one) odd |= 1u << (j * KI + k);
-            if (m >> (P * kin) & one) rv[j] = u32x4{0, 0, 0, 0};
-          }
-        }
-        const int turn = key * P / 16;
-        *reinterpret_cast<u32x4*>(&lk[buf][(key * P + (piece ^ (turn & (P - 1)))) * 8]) = rk[j];
-        *reinterpret_cast<u32x4*>(&lv[buf][(key * P + (piece ^ (2 * turn & (P - 1)))) * 8]) = rv[j];
-        if (ln == 0) lbad[buf][wave * J + j] = bad[j];
+        // (a key past the end reads the last one instead and is masked)
+        const int first = min(t * TK + wave * KW + j * KI, rq.len - 1);
+        const uint32_t at = min(kin, rq.len - 1 - first);
+        const int turn = (wave * KW + j * KI + kin) * P / 16;
+        int slot;
+        block_of(a, first, slot);
+        const int64_t at0 = slot;
+        load_lds(kc + blk * a.kc_block + at0 * a.kc_slot + at * a.kc_slot + 8 * (piece ^ (turn & (P - 1))), at_k + 1024 * j);
+        load_lds(vc + blk * a.vc_block + at0 * a.vc_slot + at * a.vc_slot + 8 * (piece ^ (2 * turn & (P - 1))),
+                 at_v + 1024 * j);
       }
-      // (drafted tokens are 64 at most)
-      if (tree && ln == 0) lodd[buf][wave] = static_cast<unsigned long long>(odd) << (wave * J * KI & 63);
+      return bad;
+    };
+    // This wave's part of tile t has arrived in buffer `in`: as in attend_kernel, no
+    // infinity or NaN may meet p = 0.
+    auto settle = [&](int t, int in, bool bad) {
+      const bool tree = t >= cached;
+      const int key0 = (tree ? t - cached : t) * TK + wave * KW, limit = tree ? rq.tokens : rq.len;
+      const int ln = here(lane), kin = ln / P;
+      if (tree || bad || key0 + KW > limit) {
+        uint32_t odd = 0;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          u32x4* const at = reinterpret_cast<u32x4*>(&lkv[in][1][(wave * J + j) * 512 + 8 * ln]);
+          const bool gone = bad || key0 + j * KI + kin >= limit;
+          bool wild = false;
+          if (tree && !gone) {
+            const u32x4 v = *at;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              wild = wild || (v[i] & E::kExp) == E::kExp || (v[i] & E::kExp << 16) == E::kExp << 16;
+          }
+          const unsigned long long m = __ballot(wild), one = P == 16 ? 0xffffull : 0xffull;
+#pragma unroll
+          for (int k = 0; k < KI; ++k)
+            if (m >> (P * k) & one) odd |= 1u << (j * KI + k);
+          if (gone || (m >> (P * kin) & one)) *at = u32x4{0, 0, 0, 0};
+        }
+        // (drafted tokens are 64 at most)
+        if (ln == 0) lodd[in][wave] = static_cast<unsigned long long>(odd) << (wave * KW & 63);
+      }
+      if (ln == 0) lbad[in][wave] = bad;
     };
 
-    ids(t0);
-    load(t0);
-    ids(t0 + 1);
-    park(t0);
-    if (t0 + 1 < t1) load(t0 + 1);
-    ids(t0 + 2);
+    // One barrier per tile.  Behind it, tile t is whole in its buffer and the one that held
+    // tile t - 1 is free: tile t + 2 is sent for, t is computed, and each wave waits for its
+    // part of t + 1, whose loads have had two tiles' arithmetic to arrive.
+    bool bad0 = load(t0, 0), bad1 = false;
+    if (t0 + 1 < t1) {
+      bad1 = load(t0 + 1, 1);
+      arrived<2 * J>();
+    } else {
+      arrived<0>();
+    }
+    settle(t0, 0, bad0);
     __syncthreads();
+    int buf = 0;
     for (int t = t0; t < t1; ++t) {
-      const int buf = (t - t0) & 1;
+      const int next = buf == kBuffers - 1 ? 0 : buf + 1;
+      bool bad2 = false;
+      if (t + 2 < t1) bad2 = load(t + 2, next == kBuffers - 1 ? 0 : next + 1);
       if (active) {
         const bool tree = t >= cached;
         const int key0 = (tree ? t - cached : t) * TK, limit = tree ? rq.tokens : rq.len;
         const int ln = here(lane);
-        const uint32_t bm = static_cast<uint32_t>(__ballot(ln < NW * J && lbad[buf][ln % (NW * J)]));
+        const uint32_t bm = static_cast<uint32_t>(__ballot(ln < NW && lbad[buf][ln % NW]));
         const bool masked = tree || key0 + TK > limit || bm;
         unsigned long long odd = 0;
         if (tree)
@@ -876,7 +896,7 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
           if (key0 + 32 * h >= limit) break;
           // a piece's exchange is an exclusive or of its row's address with 16 bytes times
           // the piece, halves of a step and steps are 16 and 32 whole rows apart
-          const uint32_t kat = k_at + (buf * TK + 32 * h) * (2 * D), vat = v_at + (buf * TK + 32 * h) * (2 * D);
+          const uint32_t kat = k_at + buf * (4 * TK * D) + 32 * h * (2 * D), vat = v_at + buf * (4 * TK * D) + 32 * h * (2 * D);
           auto keys = [&](int g, int d) { return *lds<const u32x4>((kat ^ (64 * d)) + 16 * g * (2 * D)); };
           auto values = [&](int d) {
             const u32x2 x = read_transposed((vat ^ (32 * d))), y = read_transposed((vat ^ (32 * d)) + 16 * (2 * D));
@@ -885,16 +905,20 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
           const uint32_t odd32 = h < 2 ? static_cast<uint32_t>(odd >> (32 * h)) : 0;
           const int ln = here(lane);
           auto see = [&](int r) { return lsee[wave][min(row0 + 16 * r + (ln & 15), nrows - 1) / again().group]; };
-          w.step(a, keys, values, key0 + 32 * h, limit, tree, masked, bm >> (32 * h / KI) & 1,
-                 bm >> ((32 * h + 16) / KI) & 1, odd32, see, ln & 15, ln >> 4, [&](int j) {
+          w.step(a, keys, values, key0 + 32 * h, limit, tree, masked, bm >> (32 * h / KW) & 1,
+                 bm >> ((32 * h + 16) / KW) & 1, odd32, see, ln & 15, ln >> 4, [&](int j) {
                    const Attend c = again();
                    return c.v + (rq.row0 + key0 + 32 * h + j) * c.v_row + kh * c.v_head;
                  });
         }
       }
-      if (t + 1 < t1) park(t + 1);
-      if (t + 2 < t1) load(t + 2);
-      ids(t + 3);
+      if (t + 1 < t1) {
+        if (t + 2 < t1) arrived<2 * J>();
+        else arrived<0>();
+        settle(t + 1, next, bad1);
+      }
+      bad1 = bad2;
+      buf = next;
       __syncthreads();
     }
 
