@@ -129,7 +129,7 @@ struct Elem<true> {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
   }
   static __device__ __forceinline__ float low(uint32_t v) {
     return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(v)));
@@ -617,14 +617,14 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
 // but the same loads.  A tile counts kFull, or kHalf there (`weight`), as measured.  A
 // share has the tiles that begin in it; of a unit that is not whole it leaves sums in slot
 // 2 g (the unit began in an earlier share) or 2 g + 1.
-constexpr int kFull = 5, kHalf = 4;
+constexpr int kFull = 10, kHalf = 6, kUnit = 20;
 constexpr int kShares = 256;          // workgroups: one per CU
-constexpr int kMinShare = 6 * kFull;  // what a share has at least, in these counts
+constexpr int kMinShare = 3 * kFull;  // what a share has at least, in these counts
 constexpr int kWideRows = 2;                  // row tiles of 16 per wave
 constexpr int kWideWaves = 16 / kWideRows;
 constexpr int kGroup = 16 * kWideRows * kWideWaves;
-constexpr int kBuffers = 3;                   // tiles in LDS: computed, arriving, sent for
-constexpr int tile_keys(int head_dim) { return 8192 / head_dim; }
+constexpr int kBuffers = 2;                   // tiles in LDS: computed, arriving, sent for
+constexpr int tile_keys(int) { return 128; }
 
 struct Groups {
   int tiles, n;     // of a request: tiles per group, groups
@@ -638,7 +638,7 @@ __device__ __forceinline__ Groups groups_of(const Attend& a, const Request& rq) 
   g.tiles = (rq.len + TK - 1) / TK + (rq.tokens + TK - 1) / TK;
   g.n = (rows + kGroup - 1) / kGroup;
   g.last = rows - (g.n - 1) * kGroup > kGroup / 2 ? kFull : kHalf;
-  g.per_head = g.n ? static_cast<int64_t>(g.tiles) * (kFull * (g.n - 1) + g.last) : 0;
+  g.per_head = g.n ? static_cast<int64_t>(g.tiles) * (kFull * (g.n - 1) + g.last) + kUnit * g.n : 0;
   return g;
 }
 __device__ __forceinline__ int shares_of(int64_t total) {
@@ -709,11 +709,12 @@ struct Work {
     const int64_t first = uniform64(lo ? pre[lo - 1] : carry);
     u.kh = uniform(static_cast<int>((pos - first) / g.per_head));
     const int64_t in = pos - first - u.kh * g.per_head;
-    u.rg = uniform(static_cast<int>(min<int64_t>(in / (static_cast<int64_t>(kFull) * g.tiles), g.n - 1)));
+    const int64_t full = static_cast<int64_t>(kFull) * g.tiles + kUnit;
+    u.rg = uniform(static_cast<int>(min<int64_t>(in / full, g.n - 1)));
     u.tiles = g.tiles;
     u.cached = (u.rq.len + TK - 1) / TK;
     u.weight = u.rg == g.n - 1 ? g.last : kFull;
-    u.begin = first + u.kh * g.per_head + static_cast<int64_t>(u.rg) * kFull * g.tiles;
+    u.begin = first + u.kh * g.per_head + u.rg * full + kUnit;
     return u;
   }
 };
@@ -734,7 +735,7 @@ struct Work {
 // access: they are exchanged in pairs, p ^ 2 (r D / 128).
 template <int D, bool F16>
 __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_kernel(Attend a) {
-  constexpr int R = kWideRows, J = kWideRows;  // J: loads per wave, tile and matrix
+  constexpr int R = kWideRows, J = tile_keys(D) * D / 512 / kWideWaves;  // J: loads per wave, tile and matrix
   using W = Wave<D, R, F16, false>;
   using E = Elem<F16>;
   constexpr int DV = W::DV;
@@ -774,18 +775,10 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
     const int kh = un.kh, cached = un.cached;
 
     // this share's tiles of the unit: cached ones, then the drafted tokens'
-    const int t0 = uniform(static_cast<int>((pos - un.begin + un.weight - 1) / un.weight));
+    const int t0 = uniform(static_cast<int>((max<int64_t>(pos - un.begin, 0) + un.weight - 1) / un.weight));
     const int t1 = uniform(static_cast<int>(min<int64_t>(un.tiles, (end - un.begin + un.weight - 1) / un.weight)));
     pos = un.begin + static_cast<int64_t>(un.tiles) * un.weight;  // the next unit's
     if (t0 >= t1) continue;
-
-    W w;
-    if (active) {
-      const Attend c = again();
-      const int ln = here(lane);
-      w.load(c, rq, kh, row0, nrows, ln & 15, ln >> 4);
-      if (t1 > cached) w.trees(c, rq, ln, lsee[wave]);
-    }
 
     const int32_t* table = a.tables + un.b * a.tstride;
     const uint16_t *kc = a.kc + kh * a.kc_head, *vc = a.vc + kh * a.vc_head;
@@ -818,18 +811,18 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
       const int id = __builtin_amdgcn_readlane(id_lane, t - id0);
       const bool bad = id < 0 || id >= a.blocks;
       const int64_t blk = bad ? 0 : id;
+      // (a key past the end reads the last one instead and is masked)
+      const int first = min(t * TK + wave * KW, rq.len - 1);
+      int slot;
+      block_of(a, first, slot);
+      const int64_t at0 = slot;
+      const uint16_t *kb = kc + blk * a.kc_block + at0 * a.kc_slot, *vb = vc + blk * a.vc_block + at0 * a.vc_slot;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        // (a key past the end reads the last one instead and is masked)
-        const int first = min(t * TK + wave * KW + j * KI, rq.len - 1);
-        const uint32_t at = min(kin, rq.len - 1 - first);
+        const int64_t at = min(j * KI + kin, rq.len - 1 - first);
         const int turn = (wave * KW + j * KI + kin) * P / 16;
-        int slot;
-        block_of(a, first, slot);
-        const int64_t at0 = slot;
-        load_lds(kc + blk * a.kc_block + at0 * a.kc_slot + at * a.kc_slot + 8 * (piece ^ (turn & (P - 1))), at_k + 1024 * j);
-        load_lds(vc + blk * a.vc_block + at0 * a.vc_slot + at * a.vc_slot + 8 * (piece ^ (2 * turn & (P - 1))),
-                 at_v + 1024 * j);
+        load_lds(kb + at * a.kc_slot + 8 * (piece ^ (turn & (P - 1))), at_k + 1024 * j);
+        load_lds(vb + at * a.vc_slot + 8 * (piece ^ (2 * turn & (P - 1))), at_v + 1024 * j);
       }
       return bad;
     };
@@ -868,19 +861,21 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
     // tile t - 1 is free: tile t + 2 is sent for, t is computed, and each wave waits for its
     // part of t + 1, whose loads have had two tiles' arithmetic to arrive.
     bool bad0 = load(t0, 0), bad1 = false;
-    if (t0 + 1 < t1) {
-      bad1 = load(t0 + 1, 1);
-      arrived<2 * J>();
-    } else {
-      arrived<0>();
+    W w;
+    if (active) {
+      const Attend c = again();
+      const int ln = here(lane);
+      w.load(c, rq, kh, row0, nrows, ln & 15, ln >> 4);
+      if (t1 > cached) w.trees(c, rq, ln, lsee[wave]);
     }
+    arrived<0>();
     settle(t0, 0, bad0);
     __syncthreads();
     int buf = 0;
     for (int t = t0; t < t1; ++t) {
       const int next = buf == kBuffers - 1 ? 0 : buf + 1;
       bool bad2 = false;
-      if (t + 2 < t1) bad2 = load(t + 2, next == kBuffers - 1 ? 0 : next + 1);
+      if (t + 1 < t1) bad1 = load(t + 1, next);
       if (active) {
         const bool tree = t >= cached;
         const int key0 = (tree ? t - cached : t) * TK, limit = tree ? rq.tokens : rq.len;
@@ -913,11 +908,9 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
         }
       }
       if (t + 1 < t1) {
-        if (t + 2 < t1) arrived<2 * J>();
-        else arrived<0>();
+        arrived<0>();
         settle(t + 1, next, bad1);
       }
-      bad1 = bad2;
       buf = next;
       __syncthreads();
     }
@@ -965,83 +958,130 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
   }
 }
 
-// A row's output from n parts' sums: brought to one reference, added and divided by the
-// joined sum.  slot(i): where part i is.  Lane l owns D/64 neighbouring dims.
-template <int D, bool F16, typename Slot>
-__device__ __forceinline__ void join_row(const Attend& a, int64_t token, int head, int n, int lane, Slot slot) {
-  constexpr int W = D / 64;
-  float ref = kLow;
-  for (int i = lane; i < n; i += 64) ref = fmaxf(ref, a.stat[2 * slot(i)]);
+// Four rows' outputs from n parts' sums each: brought to one reference, added in order and
+// divided by the joined sum.  Sixteen lanes per row, each with D/16 neighbouring dims;
+// slot(i): where part i of the lane's row is; p: the lane's dims of the output, or null.
+// WAVES: of the workgroup, each taking that share of the parts (all must call it), joined in
+// LDS; or 1.  Bound by memory and, few rows of many parts, by its latency: up to eight
+// parts' loads are on their way together.
+template <int D, bool F16, int WAVES, typename Slot>
+__device__ __forceinline__ void join_rows(const Attend& a, int n, int lane, int wave, uint16_t* p, Slot slot) {
+  constexpr int W = D / 16;
+  const int li = lane & 15;
+  float ref = kLow, sum = 0.f, o[W];
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) ref = fmaxf(ref, __shfl_xor(ref, d));
-  float sum = 0.f, o[W];
+  for (int d = 0; d < W; ++d) o[d] = 0.f;
+  const int end = WAVES == 1 ? n : n * (wave + 1) / WAVES;
+  auto batch = [&](int i0, auto count) {
+    constexpr int U = decltype(count)::value;
+    f32x2 st[U];
+    f32x4 x[U][W / 4];
 #pragma unroll
-  for (int i = 0; i < W; ++i) o[i] = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    // lane i: the weight of part i0 + i (0 from the last on)
-    f32x2 st = {kLow, 0.f};
-    if (i0 + lane < n) st = *reinterpret_cast<const f32x2*>(a.stat + 2 * slot(i0 + lane));
-    const float f = i0 + lane < n ? __builtin_amdgcn_exp2f(st[0] - ref) : 0.f;
-    sum += f * st[1];
-    for (int i = i0; i < min(n, i0 + 64); i += 8) {
-      float x[8][W];
+    for (int e = 0; e < U; ++e) {
+      const int64_t at = slot(min(i0 + e, end - 1));
+      st[e] = *reinterpret_cast<const f32x2*>(a.stat + 2 * at);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float* p = a.part + slot(min(i + e, n - 1)) * D + W * lane;
-        if constexpr (W == 2) {
-          const f32x2 v = *reinterpret_cast<const f32x2*>(p);
-          x[e][0] = v[0], x[e][1] = v[1];
-        } else {
-          x[e][0] = *p;
-        }
-      }
+      for (int d = 0; d < W / 4; ++d) x[e][d] = *reinterpret_cast<const f32x4*>(a.part + at * D + W * li + 4 * d);
+    }
+    float top = ref;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float g = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i - i0 + e));
-        // (a part read twice has weight 0, and may hold infinities)
+    for (int e = 0; e < U; ++e) top = fmaxf(top, st[e][0]);
+    const float f = __builtin_amdgcn_exp2f(ref - top);
+    ref = top;
+    sum *= f;
 #pragma unroll
-        for (int d = 0; d < W; ++d) o[d] = i + e < n ? fmaf(g, x[e][d], o[d]) : o[d];
-      }
+    for (int d = 0; d < W; ++d) o[d] *= f;
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      if (i0 + e >= end) break;  // (a part read again)
+      const float g = __builtin_amdgcn_exp2f(st[e][0] - ref);
+      sum = fmaf(g, st[e][1], sum);
+#pragma unroll
+      for (int d = 0; d < W; ++d) o[d] = fmaf(g, x[e][d / 4][d % 4], o[d]);
+    }
+  };
+  int i = WAVES == 1 ? 0 : n * wave / WAVES;
+  for (; end - i > 4; i += 8) batch(i, Int<8>{});
+  if (end - i > 2) batch(i, Int<4>{});
+  else if (end > i) batch(i, Int<2>{});
+  if constexpr (WAVES > 1) {
+    __shared__ float lref[WAVES][64], lsum[WAVES][64], lo[WAVES][W][64];
+    lref[wave][lane] = ref;
+    lsum[wave][lane] = sum;
+#pragma unroll
+    for (int d = 0; d < W; ++d) lo[wave][d][lane] = o[d];
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) ref = fmaxf(ref, lref[w][lane]);
+    sum = 0.f;
+#pragma unroll
+    for (int d = 0; d < W; ++d) o[d] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float g = __builtin_amdgcn_exp2f(lref[w][lane] - ref);
+      sum = fmaf(g, lsum[w][lane], sum);
+#pragma unroll
+      for (int d = 0; d < W; ++d) o[d] = fmaf(g, lo[w][d][lane], o[d]);
     }
   }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+  if (!p) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint16_t* p = a.out + token * a.out_row + head * a.out_head + W * lane;
-  if constexpr (W == 2) *reinterpret_cast<uint32_t*>(p) = Elem<F16>::pack(o[0] * inv, o[1] * inv);
-  else *p = static_cast<uint16_t>(Elem<F16>::pack(o[0] * inv, 0.f));
+  uint32_t w[W / 2];
+#pragma unroll
+  for (int d = 0; d < W / 2; ++d) w[d] = Elem<F16>::pack(o[2 * d] * inv, o[2 * d + 1] * inv);
+  if constexpr (W == 8) *reinterpret_cast<u32x4*>(p) = u32x4{w[0], w[1], w[2], w[3]};
+  else *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
 }
 
-// Behind attend_kernel: one wave per (request, token, head).
-template <int D, bool F16>
-__global__ __launch_bounds__(256) void join_kernel(Attend a, int wk) {
-  const int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + uniform(static_cast<int>(threadIdx.x >> 6));
-  const int head = static_cast<int>(u % a.q_heads);
-  const int64_t bt = u / a.q_heads;
-  const int b = static_cast<int>(bt / a.max_tokens), t = static_cast<int>(bt % a.max_tokens);
+// Waves that join four rows: sixteen if those have that many parts, else one (and four
+// times four rows a workgroup).  Measured, microseconds sixteen/one: 24 requests x 64 rows x
+// 16 heads of two or three parts 9.5 (one), two requests of 192 rows a key head and 85 parts
+// TODO/25.
+constexpr int kJoinWaves = 16;
+constexpr int join_threads(int waves) { return waves == 1 ? 256 : 64 * waves; }
+// the four rows of a wave
+template <int WAVES>
+__device__ __forceinline__ int64_t join_quad(int wave) {
+  return WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + wave : blockIdx.x;
+}
+
+// Behind attend_kernel: rows are (token, head) of a request.
+template <int D, bool F16, int WAVES>
+__global__ __launch_bounds__(join_threads(WAVES)) void join_kernel(Attend a, int wk) {
+  const int lane = threadIdx.x & 63, li = lane & 15, wave = uniform(static_cast<int>(threadIdx.x >> 6));
+  const int64_t u = join_quad<WAVES>(wave);
+  const int quads = (a.max_tokens * a.q_heads + 3) >> 2;
+  const int b = static_cast<int>(u / quads), first = static_cast<int>(u - static_cast<int64_t>(b) * quads) * 4;
   if (b >= a.requests) return;
   const Request rq = request(a, b);
-  const int parts = parts_of(a, rq, wk);
-  if (t >= rq.tokens || parts == 1) return;
-  const int64_t token = rq.row0 + t, at = (token * a.q_heads + head) * a.splits;
-  join_row<D, F16>(a, token, head, parts, threadIdx.x & 63, [&](int i) { return at + i; });
+  const int parts = parts_of(a, rq, wk), rows = rq.tokens * a.q_heads;
+  if (first >= rows || parts == 1) return;
+  const int row = min(first + (lane >> 4), rows - 1), t = row / a.q_heads;
+  const int64_t at = (static_cast<int64_t>(rq.row0) * a.q_heads + row) * a.splits;
+  uint16_t* p = a.out + (rq.row0 + t) * a.out_row + (row - t * a.q_heads) * a.out_head + D / 16 * li;
+  join_rows<D, F16, WAVES>(a, parts, lane, wave, first + (lane >> 4) < rows ? p : nullptr, [&](int i) { return at + i; });
 }
 
-// Behind attend_wide_kernel: one wave per row; rows of whole units are already written.
-template <int D, bool F16>
-__global__ __launch_bounds__(256) void join_wide_kernel(Attend a) {
-  int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + uniform(static_cast<int>(threadIdx.x >> 6));
-  const int row = static_cast<int>(u % (a.max_tokens * a.group));
-  u /= a.max_tokens * a.group;
+// Behind attend_wide_kernel: rows of a key head; those of whole units are already written.
+template <int D, bool F16, int WAVES>
+__global__ __launch_bounds__(join_threads(WAVES)) void join_wide_kernel(Attend a) {
+  const int lane = threadIdx.x & 63, li = lane & 15, wave = uniform(static_cast<int>(threadIdx.x >> 6));
+  int64_t u = join_quad<WAVES>(wave);
+  const int quads = (a.max_tokens * a.group + 3) >> 2;
+  const int first = static_cast<int>(u % quads) * 4;
+  u /= quads;
   const int kh = static_cast<int>(u % a.kv_heads), b = static_cast<int>(u / a.kv_heads);
   if (b >= a.requests) return;
   const Request rq = request(a, b);
-  if (row >= rq.tokens * a.group) return;
+  const int rows = rq.tokens * a.group;
+  if (first >= rows) return;
   const Groups g = groups_of<tile_keys(D)>(a, rq);
   const int64_t total = a.sums[a.requests - 1];
-  const int n = shares_of(total), rg = row / kGroup;
+  const int n = shares_of(total), rg = first / kGroup;
   // the unit's first and last tile, and their shares: the largest that begin by then
-  const int64_t s = (b ? a.sums[b - 1] : 0) + kh * g.per_head + static_cast<int64_t>(rg) * kFull * g.tiles;
+  const int64_t s = (b ? a.sums[b - 1] : 0) + kh * g.per_head +
+                    rg * (static_cast<int64_t>(kFull) * g.tiles + kUnit) + kUnit;
   const int64_t e = s + static_cast<int64_t>(g.tiles - 1) * (rg == g.n - 1 ? g.last : kFull);
   auto share = [&](int64_t at) {
     int k = static_cast<int>(at * n / total);
@@ -1050,9 +1090,10 @@ __global__ __launch_bounds__(256) void join_wide_kernel(Attend a) {
   };
   const int g0 = share(s), g1 = share(e);
   if (g0 == g1) return;
-  const int t = row / a.group;
-  join_row<D, F16>(a, rq.row0 + t, kh * a.group + row - t * a.group, g1 - g0 + 1, threadIdx.x & 63,
-                   [&](int i) { return static_cast<int64_t>(2 * (g0 + i) + (i == 0) - rg) * kGroup + row; });
+  const int row = min(first + (lane >> 4), rows - 1), t = row / a.group;
+  uint16_t* p = a.out + (rq.row0 + t) * a.out_row + (kh * a.group + row - t * a.group) * a.out_head + D / 16 * li;
+  join_rows<D, F16, WAVES>(a, g1 - g0 + 1, lane, wave, first + (lane >> 4) < rows ? p : nullptr,
+                    [&](int i) { return static_cast<int64_t>(2 * (g0 + i) + (i == 0) - rg) * kGroup + row; });
 }
 
 // The launch shape, a function of sizes the host knows (never of what the device
@@ -1096,8 +1137,14 @@ template <int D, bool F16>
 int launch_wide(const Attend& a, hipStream_t st) {
   hipLaunchKernelGGL((attend_wide_kernel<D, F16>), dim3(kShares), dim3(64 * kWideWaves), 0, st, a);
   if (int rc = check_launch("tree attention kernel")) return rc;
-  const int64_t rows = static_cast<int64_t>(a.requests) * a.max_tokens * a.q_heads;
-  hipLaunchKernelGGL((join_wide_kernel<D, F16>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, st, a);
+  const int64_t quads = static_cast<int64_t>(a.requests) * a.kv_heads * ((a.max_tokens * a.group + 3) / 4);
+  const int64_t units = static_cast<int64_t>(a.requests) * a.kv_heads * ((a.max_tokens * a.group + kGroup - 1) / kGroup);
+  if (kShares / units >= kJoinWaves)
+    hipLaunchKernelGGL((join_wide_kernel<D, F16, kJoinWaves>), dim3(static_cast<unsigned>(quads)),
+                       dim3(join_threads(kJoinWaves)), 0, st, a);
+  else
+    hipLaunchKernelGGL((join_wide_kernel<D, F16, 1>), dim3(static_cast<unsigned>((quads + 3) / 4)), dim3(join_threads(1)),
+                       0, st, a);
   return check_launch("tree attention join kernel");
 }
 
@@ -1110,9 +1157,13 @@ int launch(const Attend& a, const Plan& p, hipStream_t st) {
   else hipLaunchKernelGGL((attend_kernel<D, 2, 2, F16>), g, blk, 0, st, a);
   if (int rc = check_launch("tree attention kernel")) return rc;
   if (p.splits == 1) return PGS_OK;
-  const int64_t waves = static_cast<int64_t>(a.requests) * a.max_tokens * a.q_heads;
-  hipLaunchKernelGGL((join_kernel<D, F16>), dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, st, a,
-                     kWaves / p.wr);
+  const int64_t quads = static_cast<int64_t>(a.requests) * ((a.max_tokens * a.q_heads + 3) / 4);
+  if (p.splits >= kJoinWaves)
+    hipLaunchKernelGGL((join_kernel<D, F16, kJoinWaves>), dim3(static_cast<unsigned>(quads)),
+                       dim3(join_threads(kJoinWaves)), 0, st, a, kWaves / p.wr);
+  else
+    hipLaunchKernelGGL((join_kernel<D, F16, 1>), dim3(static_cast<unsigned>((quads + 3) / 4)), dim3(join_threads(1)), 0,
+                       st, a, kWaves / p.wr);
   return check_launch("tree attention join kernel");
 }
 
