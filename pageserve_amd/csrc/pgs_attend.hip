@@ -40,7 +40,6 @@ namespace {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 4;
 constexpr int kMaxTree = 64;
 
 struct Attend {
@@ -223,10 +222,12 @@ struct Wave {
   // to, itself and its ancestors, as a bit mask.  Lane t starts with bit t and its
   // parent; each step adds the parent's mask and takes the parent's parent, which
   // doubles the distance covered.
-  static __device__ __forceinline__ void trees(const Attend& a, const Request& rq, int lane, unsigned long long* see) {
+  static __device__ __forceinline__ int parent(const Attend& a, const Request& rq, int lane) {
+    if (lane >= rq.tokens) return -1;
+    return a.parents ? a.parents[rq.row0 + lane] : lane - 1;
+  }
+  static __device__ __forceinline__ void trees(int par, int lane, unsigned long long* see) {
     unsigned long long m = 1ull << lane;
-    int par = -1;
-    if (lane < rq.tokens) par = a.parents ? a.parents[rq.row0 + lane] : lane - 1;
     if (par >= lane || par < 0) par = -1;
     while (__ballot(par >= 0)) {
       const unsigned long long pm = __shfl(m, par & 63);
@@ -408,22 +409,22 @@ struct Wave {
   }
 };
 
-// Parts that the keys of a request are cut into, of the `splits` that the grid has:
-// each of WK key slices gets kMinSteps steps at least.
-constexpr int kMinSteps = 4;
-__device__ __forceinline__ int parts_of(const Attend& a, const Request& rq, int wk) {
-  return min(a.splits, max(1, (rq.len_tiles + rq.tree_tiles) / (kMinSteps * wk)));
+// Parts that the keys of a request are cut into, of the `splits` that the grid has: of
+// kMinSteps steps at least, or half of that where two waves share a step.
+constexpr int kMinSteps = 16;
+__device__ __forceinline__ int parts_of(const Attend& a, const Request& rq, int wr) {
+  return min(a.splits, max(1, (rq.len_tiles + rq.tree_tiles) * wr / kMinSteps));
 }
 
 // Few rows (up to 64 per key head): bound by reading the keys and values once.  A
 // workgroup's four waves are WR row tiles x 4/WR key slices; each wave loads the keys
 // of its steps straight into registers.
-template <int D, int R, int WR, bool F16>
-__global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(Attend a) {
+template <int D, int R, int WR, int NW, bool F16>
+__global__ __launch_bounds__(64 * NW, 2) void attend_kernel(Attend a) {
   using W = Wave<D, R, F16, true>;
   using E = Elem<F16>;
   constexpr int DC = W::DC, DV = W::DV, VW = W::VW;
-  constexpr int WK = kWaves / WR;  // key slices
+  constexpr int WK = NW / WR;  // key slices
   const int lane = threadIdx.x & 63;
   const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
   const int li = lane & 15, lg = lane >> 4;
@@ -432,7 +433,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(Attend a) {
   const int part = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
   const int kh = unit % a.kv_heads, b = unit / a.kv_heads;
   const Request rq = request(a, b);
-  const int parts = parts_of(a, rq, WK);
+  const int parts = parts_of(a, rq, WR);
   const int nrows = rq.tokens * a.group;
   if (nrows == 0 || part >= parts) return;
   const int row0 = wr * (16 * R);  // of this wave
@@ -441,14 +442,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(Attend a) {
   const int tiles = rq.len_tiles + rq.tree_tiles;
   const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * part / parts);
   const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / parts);
-
-  W w;
-  w.load(a, rq, kh, row0, nrows, li, lg);
-  __shared__ unsigned long long lsee[kWaves][kMaxTree];
-  int token[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) token[r] = min(row0 + 16 * r + li, nrows - 1) / a.group;
-  if (t1 > rq.len_tiles) w.trees(a, rq, lane, lsee[wave]);
 
   const int32_t* table = a.tables + b * a.tstride;
   // the block ids of a step's two halves, loaded a step ahead of its keys
@@ -511,8 +504,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(Attend a) {
     }
   };
 
+  // (the first block ids, the parents and the rows are on their way together)
   int id[2] = {0, 0};
   ids(t0 + wk, id);
+  const int par = t1 > rq.len_tiles ? W::parent(a, rq, lane) : -1;
+  W w;
+  w.load(a, rq, kh, row0, nrows, li, lg);
+  __shared__ unsigned long long lsee[NW][kMaxTree];
+  int token[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) token[r] = min(row0 + 16 * r + li, nrows - 1) / a.group;
+  if (t1 > rq.len_tiles) w.trees(par, lane, lsee[wave]);
   for (int t = t0 + wk; t < t1; t += WK) {
     Keys n;
     load(t, id, n);
@@ -614,16 +616,18 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
 // The wide kernel's work: the tiles of all (request, key head, group of kGroup rows), in
 // that order, cut into equal shares for the workgroups, whatever the requests' lengths
 // are.  A group of at most half the rows has two key slices: half the arithmetic per tile,
-// but the same loads.  A tile counts kFull, or kHalf there (`weight`), as measured.  A
-// share has the tiles that begin in it; of a unit that is not whole it leaves sums in slot
-// 2 g (the unit began in an earlier share) or 2 g + 1.
+// but the same loads.  A tile counts kFull, or kHalf there (`weight`), and a unit kUnit more
+// for its rows' loads and its sums: fitted to the workgroups' times (4.6, 2.8 and 10 us).  A
+// share has the tiles whose counts begin in it; of a unit that is not whole it leaves sums
+// in slot 2 g (the unit began in an earlier share) or 2 g + 1.
 constexpr int kFull = 10, kHalf = 6, kUnit = 20;
-constexpr int kShares = 256;          // workgroups: one per CU
-constexpr int kMinShare = 3 * kFull;  // what a share has at least, in these counts
-constexpr int kWideRows = 2;                  // row tiles of 16 per wave
+constexpr int kShares = 256;      // workgroups: one per CU
+static_assert(kHalf <= kFull);
+constexpr int kMinShare = kFull;  // counts of a share at least (16 requests of 512 keys: 24 us, 3 kFull 32, 6 kFull 45)
+constexpr int kWideRows = 2;      // row tiles of 16 per wave
 constexpr int kWideWaves = 16 / kWideRows;
 constexpr int kGroup = 16 * kWideRows * kWideWaves;
-constexpr int kBuffers = 2;                   // tiles in LDS: computed, arriving, sent for
+constexpr int kBuffers = 2;  // tiles in LDS: computed, on its way
 constexpr int tile_keys(int) { return 128; }
 
 struct Groups {
@@ -642,7 +646,8 @@ __device__ __forceinline__ Groups groups_of(const Attend& a, const Request& rq) 
   return g;
 }
 __device__ __forceinline__ int shares_of(int64_t total) {
-  return static_cast<int>(min<int64_t>(kShares, (total + kMinShare - 1) / kMinShare));
+  // (not rounded up: a share between a unit's first and last has to have one of its tiles)
+  return static_cast<int>(min<int64_t>(kShares, max<int64_t>(1, total / kMinShare)));
 }
 // where share g of n begins
 __device__ __forceinline__ int64_t share_begin(int64_t total, int g, int n) { return g * total / n; }
@@ -719,20 +724,25 @@ struct Work {
   }
 };
 
-// Many rows (more than 64 per key head): bound by the matrix units and the softmax.
-// Sixteen waves share tiles of 64 keys (128 at 64 dims) through LDS, 16 row tiles of 16
-// rows, or for a group of at most 128 rows 8 x 2 key slices (a wave then takes every second
-// 32-key step of a tile, and the two are joined at the end of a unit).  A tile's rows go from memory to registers one tile
-// ahead of their use, one 16-byte load of keys and one of values per lane, and from there to
-// one of two LDS buffers: one barrier per tile, and a load has a tile's arithmetic to arrive.
-// Four waves per SIMD with 16 rows each hide the chain scores - softmax - output of one
-// another.
+// Many rows: bound by the matrix units and the softmax, and a short group by its loads.
+// Eight waves share tiles of 128 keys through LDS, 8 x 32 rows, or for a group of at most
+// 128 rows 4 x 2 key slices (a wave then takes every second 32-key step of a tile, and the
+// two are joined at the end of a unit).  A tile goes from memory to LDS past the registers,
+// into the buffer that is not computed: one barrier per tile, and a load has a tile's
+// arithmetic to arrive.
 //
 // LDS rows are D/8 pieces of 16 bytes.  A wave reads keys as A operands, 16 keys x one
 // piece per access: piece p of key r lies at p ^ (r D / 128), so that the sixteen lanes
 // of an access meet all banks.  Values are read transposed, 4 keys x 16 dims per 16 lanes
 // (ds_read_b64_tr_b16: lane n gets dim n of the four keys), a pair of pieces of 16 keys per
 // access: they are exchanged in pairs, p ^ 2 (r D / 128).
+//
+// Measured at 24 requests of up to 64 rows x 16 heads of 128 dims: 109 us, a full tile (256
+// rows x 128 keys) 4.6 us, 40% of the matrix units' rate: a step's scores, softmax and
+// output follow one another in a wave, and the second wave of a SIMD covers a part of it.
+// Tiles through registers 133, of 64 keys 121; four waves per SIMD of 16 rows each, or a
+// higher priority for half of the waves: the same; the next step's keys read during the
+// softmax 131 (the barrier then falls into a step and keeps the waves in phase).
 template <int D, bool F16>
 __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_kernel(Attend a) {
   constexpr int R = kWideRows, J = tile_keys(D) * D / 512 / kWideWaves;  // J: loads per wave, tile and matrix
@@ -858,15 +868,16 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
     };
 
     // One barrier per tile.  Behind it, tile t is whole in its buffer and the one that held
-    // tile t - 1 is free: tile t + 2 is sent for, t is computed, and each wave waits for its
-    // part of t + 1, whose loads have had two tiles' arithmetic to arrive.
-    bool bad0 = load(t0, 0), bad1 = false;
+    // tile t - 1 is free: tile t + 1 is sent for, t is computed, and each wave waits for its
+    // part of t + 1.
+    const bool bad0 = load(t0, 0);
     W w;
     if (active) {
       const Attend c = again();
       const int ln = here(lane);
+      const int par = t1 > cached ? w.parent(c, rq, ln) : -1;
       w.load(c, rq, kh, row0, nrows, ln & 15, ln >> 4);
-      if (t1 > cached) w.trees(c, rq, ln, lsee[wave]);
+      if (t1 > cached) w.trees(par, ln, lsee[wave]);
     }
     arrived<0>();
     settle(t0, 0, bad0);
@@ -874,7 +885,7 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
     int buf = 0;
     for (int t = t0; t < t1; ++t) {
       const int next = buf == kBuffers - 1 ? 0 : buf + 1;
-      bool bad2 = false;
+      bool bad1 = false;
       if (t + 1 < t1) bad1 = load(t + 1, next);
       if (active) {
         const bool tree = t >= cached;
@@ -1037,7 +1048,7 @@ __device__ __forceinline__ void join_rows(const Attend& a, int n, int lane, int 
 // Waves that join four rows: sixteen if those have that many parts, else one (and four
 // times four rows a workgroup).  Measured, microseconds sixteen/one: 24 requests x 64 rows x
 // 16 heads of two or three parts 9.5 (one), two requests of 192 rows a key head and 85 parts
-// TODO/25.
+// 7.5/25.
 constexpr int kJoinWaves = 16;
 constexpr int join_threads(int waves) { return waves == 1 ? 256 : 64 * waves; }
 // the four rows of a wave
@@ -1048,14 +1059,14 @@ __device__ __forceinline__ int64_t join_quad(int wave) {
 
 // Behind attend_kernel: rows are (token, head) of a request.
 template <int D, bool F16, int WAVES>
-__global__ __launch_bounds__(join_threads(WAVES)) void join_kernel(Attend a, int wk) {
+__global__ __launch_bounds__(join_threads(WAVES)) void join_kernel(Attend a, int wr) {
   const int lane = threadIdx.x & 63, li = lane & 15, wave = uniform(static_cast<int>(threadIdx.x >> 6));
   const int64_t u = join_quad<WAVES>(wave);
   const int quads = (a.max_tokens * a.q_heads + 3) >> 2;
   const int b = static_cast<int>(u / quads), first = static_cast<int>(u - static_cast<int64_t>(b) * quads) * 4;
   if (b >= a.requests) return;
   const Request rq = request(a, b);
-  const int parts = parts_of(a, rq, wk), rows = rq.tokens * a.q_heads;
+  const int parts = parts_of(a, rq, wr), rows = rq.tokens * a.q_heads;
   if (first >= rows || parts == 1) return;
   const int row = min(first + (lane >> 4), rows - 1), t = row / a.q_heads;
   const int64_t at = (static_cast<int64_t>(rq.row0) * a.q_heads + row) * a.splits;
@@ -1098,23 +1109,35 @@ __global__ __launch_bounds__(join_threads(WAVES)) void join_wide_kernel(Attend a
 
 // The launch shape, a function of sizes the host knows (never of what the device
 // arrays hold, so that a captured call replays with other lengths).
+// Measured, microseconds, 16 query heads on two key heads of 128 dims:
+// - Rows share tiles through LDS (wide) if they are more than 64, or more than 32 and the
+//   cache's part is large; wide/else at 64 rows: 32 requests x 4096 keys 43.7/54.0, but
+//   4 x 16384 33.6/29.3, 64 x 1024 34.8/29.6, 8 x 512 24/16.6 (its shares and joins cost
+//   some 20 whatever the sizes), at 32 rows 32 x 4096 41.5/34.2.
+// - Eight waves a workgroup if there is at most one workgroup per CU; eight/four: 4 requests
+//   x 512 keys 11.1/12.2, 64 x 512 12.6/13.6, 32 x 2048 20.4/21.3, one of 32768 16.8/17.6,
+//   but 64 x 2048 31.0/30.3, 256 x 512 27.6/26.7.  64 dims: 8 x 1024 of 32 rows 12.8/14.1.
+//   Not for more than 16 rows of 128 dims, whose sums from eight waves take too much LDS:
+//   24.2/13.8 at 8 x 512.
 struct Plan {
   bool wide;
-  int r, wr;  // else row tiles per wave, waves per key slice
+  int r, wr;   // else row tiles per wave, waves per key slice
+  int waves;   // of a workgroup
   int splits;
 };
-Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t max_tokens, int64_t max_context) {
-  const int64_t rows = max_tokens * (q_heads / kv_heads);
-  Plan p;
-  p.wide = rows > 64;
+Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_tokens,
+          int64_t max_context) {
+  const int64_t rows = max_tokens * (q_heads / kv_heads), units = requests * kv_heads;
+  Plan p{};
+  p.wide = rows > 64 || (rows > 32 && units * max_context >= (24 << 20) / head_dim);
+  p.splits = 1;
+  if (p.wide) return p;
   p.r = rows <= 16 ? 1 : 2;
   p.wr = rows <= 32 ? 1 : 2;
-  p.splits = 1;
-  if (!p.wide) {
-    const int64_t steps = (max_context + 31) / 32 + (max_tokens + 31) / 32;
-    const int64_t most = steps / (kMinSteps * (kWaves / p.wr)), s = (1024 + requests * kv_heads - 1) / (requests * kv_heads);
-    p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({s, most, 256})));
-  }
+  const int64_t steps = (max_context + 31) / 32 + (max_tokens + 31) / 32;
+  const int64_t most = steps * p.wr / kMinSteps, s = (1024 + units - 1) / units;
+  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({s, most, 256})));
+  p.waves = (p.r == 1 || head_dim == 64) && units * p.splits <= 256 ? 8 : 4;
   return p;
 }
 
@@ -1148,22 +1171,37 @@ int launch_wide(const Attend& a, hipStream_t st) {
   return check_launch("tree attention join kernel");
 }
 
+// (variants that no plan has are not built)
+template <int D, bool F16>
+void launch_direct(const Attend& a, const Plan& p, hipStream_t st) {
+  const dim3 g(static_cast<unsigned>(a.requests * a.kv_heads * p.splits)), blk(64 * p.waves);
+  auto go = [&](auto r, auto wr, auto waves) {
+    hipLaunchKernelGGL((attend_kernel<D, decltype(r)::value, decltype(wr)::value, decltype(waves)::value, F16>), g, blk, 0,
+                       st, a);
+  };
+  if (p.waves == 8 && p.r == 1) return go(Int<1>{}, Int<1>{}, Int<8>{});
+  if constexpr (D == 64) {
+    if (p.waves == 8 && p.wr == 1) return go(Int<2>{}, Int<1>{}, Int<8>{});
+    if (p.waves == 8) return go(Int<2>{}, Int<2>{}, Int<8>{});
+  }
+  if (p.r == 1) go(Int<1>{}, Int<1>{}, Int<4>{});
+  else if (p.wr == 1) go(Int<2>{}, Int<1>{}, Int<4>{});
+  else go(Int<2>{}, Int<2>{}, Int<4>{});
+}
+
 template <int D, bool F16>
 int launch(const Attend& a, const Plan& p, hipStream_t st) {
   if (p.wide) return launch_wide<D, F16>(a, st);
-  const dim3 g(static_cast<unsigned>(a.requests * a.kv_heads * p.splits)), blk(64 * kWaves);
-  if (p.r == 1) hipLaunchKernelGGL((attend_kernel<D, 1, 1, F16>), g, blk, 0, st, a);
-  else if (p.wr == 1) hipLaunchKernelGGL((attend_kernel<D, 2, 1, F16>), g, blk, 0, st, a);
-  else hipLaunchKernelGGL((attend_kernel<D, 2, 2, F16>), g, blk, 0, st, a);
+  launch_direct<D, F16>(a, p, st);
   if (int rc = check_launch("tree attention kernel")) return rc;
   if (p.splits == 1) return PGS_OK;
   const int64_t quads = static_cast<int64_t>(a.requests) * ((a.max_tokens * a.q_heads + 3) / 4);
   if (p.splits >= kJoinWaves)
     hipLaunchKernelGGL((join_kernel<D, F16, kJoinWaves>), dim3(static_cast<unsigned>(quads)),
-                       dim3(join_threads(kJoinWaves)), 0, st, a, kWaves / p.wr);
+                       dim3(join_threads(kJoinWaves)), 0, st, a, p.wr);
   else
     hipLaunchKernelGGL((join_kernel<D, F16, 1>), dim3(static_cast<unsigned>((quads + 3) / 4)), dim3(join_threads(1)), 0,
-                       st, a, kWaves / p.wr);
+                       st, a, p.wr);
   return check_launch("tree attention join kernel");
 }
 
@@ -1176,7 +1214,7 @@ extern "C" size_t pgs_tree_attention_workspace_bytes(int64_t rows, int64_t reque
                                                      int64_t head_dim, int64_t max_tokens, int64_t max_context) {
   if (!sizes_ok(rows, requests, q_heads, kv_heads, head_dim, max_tokens, max_context) || rows == 0 || requests == 0)
     return 0;
-  return workspace_bytes(plan(requests, q_heads, kv_heads, max_tokens, max_context), rows, requests, q_heads, head_dim);
+  return workspace_bytes(plan(requests, q_heads, kv_heads, head_dim, max_tokens, max_context), rows, requests, q_heads, head_dim);
 }
 
 extern "C" int pgs_tree_attention(const pgs_tree_attention_args* args, void* workspace, size_t workspace_bytes_given,
@@ -1214,7 +1252,7 @@ extern "C" int pgs_tree_attention(const pgs_tree_attention_args* args, void* wor
       !aligned(c.v, 16) || !aligned(g.lens, 4) || !aligned(g.offsets, 4) || !aligned(g.parents, 4) ||
       !aligned(g.block_tables, 4))
     return fail(PGS_ERR_MISALIGNED, "%s: tensors must be 16-byte aligned", fn);
-  const Plan p = plan(g.requests, g.q_heads, c.kv_heads, g.max_tokens, g.max_context);
+  const Plan p = plan(g.requests, g.q_heads, c.kv_heads, c.head_dim, g.max_tokens, g.max_context);
   const size_t need = workspace_bytes(p, g.rows, g.requests, g.q_heads, c.head_dim);
   if (need > 0 && (!workspace || workspace_bytes_given < need || !aligned(workspace, 256)))
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
