@@ -268,6 +268,37 @@ def test_captured_and_replayed_with_other_lengths(gpu):
                 assert torch.equal(o[:rows], eager)
 
 
+@pytest.mark.parametrize("heads,tokens,context", [
+    # rows of many parts (9000 keys), joined by sixteen waves; 12 rows and 3, 24, 64 and 128
+    ("one", [1], None), ("3b", [1], None), ("each", [3], None), ("3b", [3], None), ("3b", [8], None), ("3b", [16], None),
+    # the same call sized for a longer context: 33 to 64 rows through LDS, parts that stay empty
+    ("3b", [5], 1 << 20), ("0.5b", [9], 1 << 20), ("3b", [2], 1 << 20), ("one", [64], 1 << 20), ("0.5b", [5], 1 << 20)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_parts(gpu, heads, tokens, context, dtype):
+    b = Batch(30, [9000], tokens, *HEADS[heads], 16, dtype)
+    b.check(tree_attention(*b.args(gpu), max_tokens=tokens[0], max_context=context), b.oracle())
+    b = Batch(31, [40, 9000, 0, 700], [tokens[0], 1, tokens[0], 0], *HEADS[heads], 32, dtype)
+    b.check(tree_attention(*b.args(gpu), max_tokens=tokens[0], max_context=context), b.oracle())
+
+
+@pytest.mark.parametrize("requests,tokens,heads", [(1, 1, "0.5b"), (40, 4, "0.5b"), (300, 1, "one"), (2, 9, "0.5b"),
+                                                   (3, 16, "3b"), (150, 40, "one"), (40, 17, "3b")])
+def test_many_small_requests(gpu, requests, tokens, heads):
+    """Grids on both sides of one workgroup per CU; units of less than a share and of several."""
+    rng = np.random.default_rng(requests)
+    b = Batch(32, rng.integers(0, 300, requests).tolist(), rng.integers(0, tokens + 1, requests).tolist(),
+              *HEADS[heads], 16, torch.bfloat16)
+    b.check(tree_attention(*b.args(gpu), max_tokens=tokens), b.oracle())
+
+
+@pytest.mark.parametrize("lens,tokens", [([300], [7]), ([5000, 20], [64, 5])])
+def test_in_place(gpu, lens, tokens):
+    b = Batch(33, lens, tokens, 16, 2, 128, 16, torch.bfloat16)
+    args = b.args(gpu)
+    want = tree_attention(*args)
+    assert tree_attention(*args, out=args[0]) is not None and torch.equal(args[0], want)
+
+
 def test_side_stream(gpu):
     b = Batch(11, [3000], [4], 16, 2, 128, 16, torch.bfloat16)
     args = b.args(gpu)
