@@ -590,8 +590,8 @@ typedef struct pgs_tree_attention_args {
  * same request before t (any other value: none), so that the drafted tokens form
  * trees.  Query heads share key heads in groups of q_heads / kv_heads.
  *   out = sum_j softmax_j(scale * q . k_j) v_j     (softmax in fp32)
- * head_dim 64 or 128; block_size a multiple of 16; strides multiples of 8
- * elements and pointers 16-byte aligned.  Lengths beyond the table's columns
+ * head_dim 64 or 128; block_size a multiple of 16, columns * block_size at most
+ * 2^31 - 65536; strides multiples of 8 elements and pointers 16-byte aligned.  Lengths beyond the table's columns
  * are cut to them; tokens in a block outside the cache are left out; rows of no
  * request, and a request's rows from max_tokens on, are not written.
  * workspace: pgs_tree_attention_workspace_bytes() bytes, 256-byte aligned, no

@@ -258,6 +258,15 @@ at::Tensor dequantize4(const at::Tensor& qp, const at::Tensor& sp, int64_t n, in
   return out;
 }
 
+// whether the memory of contiguous `o` and of `t` can overlap
+bool overlap(const at::Tensor& o, const at::Tensor& t) {
+  if (!o.numel() || !t.numel()) return false;
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  const char *a = static_cast<const char*>(o.data_ptr()), *b = static_cast<const char*>(t.data_ptr());
+  return a < b + (last + 1) * t.element_size() && b < a + o.numel() * o.element_size();
+}
+
 at::Tensor linear4(const at::Tensor& x, const at::Tensor& qp, const at::Tensor& sp, const Opt& bias, int64_t n,
                    int64_t k, int64_t group, bool out_f32, const Opt& residual, const Opt& out) {
   const at::Device dev = qp.device();
@@ -280,6 +289,7 @@ at::Tensor linear4(const at::Tensor& x, const at::Tensor& qp, const at::Tensor& 
     if (o.device() != dev || o.scalar_type() != odt || o.numel() != m * n || !o.is_contiguous())
       value_error("linear4: out must be a contiguous " + std::string(c10::toString(odt)) + " tensor of " +
                   std::to_string(m * n) + " elements on " + dev_str(dev));
+    if (overlap(o, x2)) value_error("linear4: out must not share memory with the input");
     y = o.view({m, n});
   } else {
     y = at::empty({m, n}, x2.options().dtype(odt));
@@ -291,6 +301,8 @@ at::Tensor linear4(const at::Tensor& x, const at::Tensor& qp, const at::Tensor& 
                   " rows on " + dev_str(dev));
     res = r.reshape({m, n});
     if (!res.is_contiguous()) res = res.contiguous();
+    if (overlap(y, res) && (y.data_ptr() != res.data_ptr() || out_f32))
+      value_error("linear4: out may be the residual itself, but not share memory with a part of it");
   }
   const size_t need = pgs_w4a16_workspace_bytes(m, n, k);
   at::Tensor ws;  // (per call, as in tree_attention)
@@ -444,15 +456,6 @@ at::Tensor pieces(const at::Tensor& t) {
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
-// whether the memory of contiguous `o` and of `t` can overlap
-bool overlap(const at::Tensor& o, const at::Tensor& t) {
-  if (!o.numel() || !t.numel()) return false;
-  int64_t last = 0;
-  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-  const char *a = static_cast<const char*>(o.data_ptr()), *b = static_cast<const char*>(t.data_ptr());
-  return a < b + (last + 1) * t.element_size() && b < a + o.numel() * o.element_size();
-}
-
 at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache,
                           const at::Tensor& v_cache, const at::Tensor& block_tables, const at::Tensor& lens,
                           const at::Tensor& offsets, const Opt& parents, int64_t max_tokens, int64_t max_context,
@@ -483,6 +486,8 @@ at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& k, const at::Te
     if (o.device() != dev || o.scalar_type() != k_cache.scalar_type() || o.sizes() != q.sizes() || !o.is_contiguous() ||
         reinterpret_cast<uintptr_t>(o.data_ptr()) % 16)
       value_error("tree_attention: out must be a contiguous 16-byte aligned tensor of q's shape, dtype and device");
+    if (overlap(o, qr) && (o.data_ptr() != qr.data_ptr() || !qr.is_contiguous()))
+      value_error("tree_attention: out may be q itself, but not share memory with a part of it");
     if (overlap(o, kr) || overlap(o, vr) || overlap(o, k_cache) || overlap(o, v_cache))
       value_error("tree_attention: out must not share memory with k, v or the cache");
   } else {

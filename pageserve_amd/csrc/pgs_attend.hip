@@ -1234,7 +1234,8 @@ extern "C" int pgs_tree_attention(const pgs_tree_attention_args* args, void* wor
   if (c.blocks < 1 || c.blocks > 0x7fffffff || c.block_size < 16 || c.block_size > 0x10000 || c.block_size % 16 != 0)
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: the cache needs blocks of a multiple of 16 tokens (block_size=%lld)", fn,
                 (long long)c.block_size);
-  if (g.columns < 0 || g.table_stride < g.columns || g.columns * c.block_size > 0x7fffffff)
+  // (a tile behind the last token still has a 32-bit number)
+  if (g.columns < 0 || g.table_stride < g.columns || g.columns > 0x7fff0000 / c.block_size)
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: bad block table", fn);
   const int64_t strides[] = {g.q_row, g.q_head, g.k_row, g.k_head, g.v_row, g.v_head, g.out_row, g.out_head,
                              c.k_block, c.k_slot, c.k_head, c.v_block, c.v_slot, c.v_head};

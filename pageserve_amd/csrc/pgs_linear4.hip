@@ -29,7 +29,7 @@ struct Lin4 {
 };
 
 constexpr int64_t kMaxRows4 = 0x7ffffff0, kMaxTokens4 = 65535 * 16;
-constexpr int kNowhere = 0x40000000;  // a lane offset past every activation block (at most 64 rows of kMaxK)
+constexpr int kNowhere = 0x40000000;  // a lane offset past every resource (the largest: 64 rows of kMaxK activations)
 
 // The tokens are the A operand and the weights the B operand: lane l's four sums are of
 // weight row l%16, so it needs the scales of that row only.  (With the weights as A its
@@ -60,17 +60,19 @@ __global__ __launch_bounds__(64 * NW, 2) void linear4_kernel(Lin4 a) {
   const int m0 = blockIdx.y * MT;
   const int rows = min(a.m - m0, MT);
 
-  // (one resource per tile: a chunk past K, or a tile past N, reads zeros)
+  // One resource per tile (a tile past N: the last one again, its sums are not stored).  What
+  // lies past K reads zeros by a lane offset past every resource; the scalar offset added
+  // to it never passes the resource's end, so the check holds however it counts that.
   __amdgpu_buffer_rsrc_t wres[R], sres[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int64_t t = tile0 + r;
-    const bool live = t < tiles;
-    wres[r] = make_rsrc(a.qp + (live ? t : 0) * kb * 1024, live ? static_cast<int64_t>(kb) * 1024 : 0);
-    sres[r] = make_rsrc(a.sp + (live ? t : 0) * kb * (16 * S), live ? static_cast<int64_t>(kb) * (32 * S) : 0);
+    const int64_t t = min(tile0 + r, tiles - 1);
+    wres[r] = make_rsrc(a.qp + t * kb * 1024, static_cast<int64_t>(kb) * 1024);
+    sres[r] = make_rsrc(a.sp + t * kb * (16 * S), static_cast<int64_t>(kb) * (32 * S));
   }
+  // (up to the last chunk's end of the last row)
   const __amdgpu_buffer_rsrc_t xres =
-      make_rsrc(a.x + static_cast<int64_t>(m0) * a.k, static_cast<int64_t>(rows) * a.k * 2);
+      make_rsrc(a.x + static_cast<int64_t>(m0) * a.k, (static_cast<int64_t>(rows - 1) * a.k + 128 * kb) * 2);
   const int sub = FOLD ? li >> 3 : 0;  // this lane's chunk of the slot, as token and as weight row
   const int woff = FOLD ? sub * 1024 + (8 * half + (li & 7) + 16 * kq) * 16 : lane * 16;
   const int soff = FOLD ? sub * (32 * S) + (8 * half + (li & 7)) * (2 * S) : li * (2 * S);
@@ -91,16 +93,18 @@ __global__ __launch_bounds__(64 * NW, 2) void linear4_kernel(Lin4 a) {
     u32x4 x[4][TM];
   };
   auto load = [&](Slot& b, int slot) {
-    const int c = FOLD ? 2 * slot : slot;
+    const int c0 = FOLD ? 2 * slot : slot, c = min(c0, kb - 1);
+    const bool live = c0 + sub < kb;
+    const int wo = live ? woff : kNowhere, so = live ? soff : kNowhere;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      b.w[r] = __builtin_amdgcn_raw_buffer_load_b128(wres[r], woff, c * 1024, kLoadNT);
+      b.w[r] = __builtin_amdgcn_raw_buffer_load_b128(wres[r], wo, c * 1024, kLoadNT);
       if constexpr (S == 1) {
-        b.s[r][0] = __builtin_amdgcn_raw_buffer_load_b16(sres[r], soff, c * 32, 0);
+        b.s[r][0] = __builtin_amdgcn_raw_buffer_load_b16(sres[r], so, c * 32, 0);
       } else if constexpr (S == 2) {
-        b.s[r][0] = __builtin_amdgcn_raw_buffer_load_b32(sres[r], soff, c * 64, 0);
+        b.s[r][0] = __builtin_amdgcn_raw_buffer_load_b32(sres[r], so, c * 64, 0);
       } else {
-        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(sres[r], soff, c * 128, 0);
+        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(sres[r], so, c * 128, 0);
         b.s[r][0] = v[0], b.s[r][1] = v[1];
       }
     }
@@ -108,7 +112,7 @@ __global__ __launch_bounds__(64 * NW, 2) void linear4_kernel(Lin4 a) {
     for (int j = 0; j < 4; ++j) {
       // (columns from K on: zeros, not the next row's values, which may be
       // infinite and would not vanish against the zero codes there)
-      const bool in = (c + sub) * 128 + 32 * j + 8 * kq < a.k;
+      const bool in = (c0 + sub) * 128 + 32 * j + 8 * kq < a.k;
 #pragma unroll
       for (int t = 0; t < TM; ++t)
         b.x[j][t] = __builtin_amdgcn_raw_buffer_load_b128(xres, in ? xoff[t] : kNowhere, c * 256 + 64 * j, 0);

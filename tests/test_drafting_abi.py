@@ -60,7 +60,8 @@ CASES = [
     (_write, {"head_dim": 0}), (_write, {"k_slot": -1}),
     (_attend, {"dtype": 0}), (_attend, {"max_tokens": 65}), (_attend, {"max_tokens": 0}), (_attend, {"q_heads": 15}),
     (_attend, {"rows": -1}), (_attend, {"q": None}), (_attend, {"q": 264}), (_attend, {"q_row": 2047}),
-    (_attend, {"scale": float("nan")}), (_attend, {"table_stride": 3}), (_attend, {"columns": 1 << 40}),
+    (_attend, {"scale": float("nan")}), (_attend, {"table_stride": 3}), (_attend, {"columns": 1 << 40, "table_stride": 1 << 40}),
+    (_attend, {"columns": (1 << 27) - 1, "table_stride": 1 << 27}), (_attend, {"columns": 1 << 62, "table_stride": 1 << 62}),
     (_attend, {"lens": 258}), (_attend, {"workspace": None}), (_attend, {"given": 8}),
     (_attend, {"workspace": ctypes.c_void_p(128)}),
     (_attend, {"cache": {"head_dim": 96}}), (_attend, {"cache": {"block_size": 24}}), (_attend, {"cache": {"k": 0}}),

@@ -350,3 +350,5 @@ def test_refusals(gpu):
         tree_attention(*good[:3], shifted, vc, *good[5:])
     with pytest.raises(ValueError, match="contiguous head_dim"):
         tree_attention(*good[:3], kc.transpose(1, 3), vc.transpose(1, 3), *good[5:])
+    room = torch.zeros(5, 16, 128, dtype=torch.bfloat16, device=gpu)
+    bad(ValueError, "a part of it", 0, room[:4], out=room[1:])

@@ -183,3 +183,11 @@ def test_refusals(gpu):
         linear4(xt, qw, residual=torch.zeros(3, 32, dtype=torch.bfloat16, device=gpu))
     with pytest.raises(ValueError, match="out must"):
         linear4(xt, qw, out=torch.zeros(2, 32, device=gpu))
+    room = torch.zeros(5 * 64, dtype=torch.bfloat16, device=gpu)
+    with pytest.raises(ValueError, match="share memory with the input"):
+        linear4(room[:128].view(2, 64), qw, out=room[120:184].view(2, 32))
+    with pytest.raises(ValueError, match="residual itself"):
+        linear4(xt, qw, residual=room[:64].view(2, 32), out=room[8:72].view(2, 32))
+    with pytest.raises(ValueError, match="residual itself"):
+        linear4(xt, qw, residual=room[:64].view(2, 32), out=room[:128].view(torch.float32).view(2, 32),
+                out_dtype=torch.float32)
