@@ -26,9 +26,9 @@
 // registers.  block_size is a multiple of 16, so a 16-key half lies in one block: its
 // address is wave-uniform.
 //
-// Work: (request, key head, row group, part of the keys).  A workgroup's four waves
-// are WR row tiles x 4/WR key slices, joined in LDS; parts are joined by a second
-// kernel from fp32 partial outputs in the workspace.
+// Work: (request, key head, row group, part of the keys).  A workgroup's waves are
+// row tiles x key slices, joined in LDS; parts are joined by a second kernel from
+// fp32 partial outputs in the workspace.
 #include <math.h>
 
 #include <algorithm>
@@ -416,9 +416,12 @@ __device__ __forceinline__ int parts_of(const Attend& a, const Request& rq, int 
   return min(a.splits, max(1, (rq.len_tiles + rq.tree_tiles) * wr / kMinSteps));
 }
 
-// Few rows (up to 64 per key head): bound by reading the keys and values once.  A
-// workgroup's four waves are WR row tiles x 4/WR key slices; each wave loads the keys
-// of its steps straight into registers.
+// Few rows (up to 64 per key head): bound by reading the keys and values once, and for
+// short contexts by the chain of loads (lengths, block numbers, keys).  A workgroup's NW
+// waves are WR row tiles x NW/WR key slices; each wave loads the keys of its steps straight
+// into registers.  Measured, 16 heads on two key heads of 128 dims: one token of 256
+// requests of 512 keys 26.6 us (5.0 TB/s of keys and values), of 64 of 2048 29.2 (4.6), of
+// one of 32768 with the join 17.5 (1.9); 4 tokens of 64 of 2048 32.4 (4.2).
 template <int D, int R, int WR, int NW, bool F16>
 __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(Attend a) {
   using W = Wave<D, R, F16, true>;

@@ -11,6 +11,11 @@
 // already the B operand of four MFMAs.  A workgroup owns R 16-row tiles over its share of K;
 // its NW waves take 128-column chunks round robin, U per batch, a batch's loads issued
 // together, and the waves' partial tiles meet in LDS in a fixed order.
+//
+// Measured (weights not in any cache): 1 x 151936 x 2048, groups of 128, 30 us, 5.3 TB/s of
+// codes and scales; 30 tokens, groups of 32, 61 us: each wave loads the tokens' values for
+// its four tiles, twice the bytes of their codes, from L2, and scales eight products a tile.
+// 1 x 11008 x 2048 5.1 us, 5 x 2048 x 11008 6.7 us: a launch and the first loads' latency.
 #include "pgs_fp4.h"
 
 namespace pgs {
