@@ -743,9 +743,9 @@ struct Work {
 // Measured at 24 requests of up to 64 rows x 16 heads of 128 dims: 109 us, a full tile (256
 // rows x 128 keys) 4.6 us, 40% of the matrix units' rate: a step's scores, softmax and
 // output follow one another in a wave, and the second wave of a SIMD covers a part of it.
-// Tiles through registers 133, of 64 keys 121; four waves per SIMD of 16 rows each, or a
-// higher priority for half of the waves: the same; the next step's keys read during the
-// softmax 131 (the barrier then falls into a step and keeps the waves in phase).
+// Tiles through registers 133, of 64 keys 121.  The same: four waves per SIMD of 16 rows
+// each, a higher priority for half of the waves, half of them starting a tile later (116),
+// the next step's keys read during the softmax (and 131 for 123 across the barrier).
 template <int D, bool F16>
 __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_kernel(Attend a) {
   constexpr int R = kWideRows, J = tile_keys(D) * D / 512 / kWideWaves;  // J: loads per wave, tile and matrix

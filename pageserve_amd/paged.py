@@ -58,7 +58,7 @@ def append_blocks(lens: torch.Tensor, new_lens: torch.Tensor, offsets: torch.Ten
     the batch is its request's ``n``-th new token, ``n = index[i]``, or ``i -
     offsets[b]`` without an index; its slot is -1 where ``n`` is not in
     ``0 .. new_lens[b] - 1``, the request was not served or the row belongs to
-    none.
+    none.  Rows of a request with the same index get the same slot.
 
     All tensors int32 and on one GPU: ``lens`` and ``new_lens`` [requests],
     ``offsets`` [requests + 1], ``block_tables`` [requests, columns],
@@ -85,8 +85,8 @@ def write_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     slots of the caches (the reference's write_kv, engine/paged_attention.py:62-79,
     for a whole batch).  A row whose slot (int64) is outside the cache, as -1 is,
     is left out.  No two rows may have the same slot (:func:`append_blocks` gives
-    none twice): of two that do, pieces of either may stay.  bf16 or fp16, the
-    rows in any strides whose last is 1."""
+    none twice, unless ``index`` names a token twice): of two that do, pieces of
+    either may stay.  bf16 or fp16, the rows in any strides whose last is 1."""
     _native.load_host().write_kv(k, v, k_cache, v_cache, slots)
 
 
