@@ -86,11 +86,12 @@ class QuantizedWeight4:
             raise TypeError("weight must be a torch.Tensor")
         _check_shape(weight.shape, group)
         self.dtype, self.shape, self.group = weight.dtype, torch.Size(weight.shape), group
+        weight = weight.detach()
         if not weight.is_cuda:
             self.qp, self.sp = _pack(*_cpu_quantize4(weight, group), group)
             return
         w = weight if weight.dtype in (torch.float32, torch.bfloat16) else weight.float()
-        self.qp, self.sp = _native.load_host().quantize4(w.detach(), group)
+        self.qp, self.sp = _native.load_host().quantize4(w, group)
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scale: torch.Tensor, group: int,
@@ -106,7 +107,7 @@ class QuantizedWeight4:
             raise ValueError(f"scale must be [{n}, {-(-k // group)}] on {codes.device}")
         obj = cls.__new__(cls)
         obj.dtype, obj.shape, obj.group = dtype, torch.Size(codes.shape), group
-        obj.qp, obj.sp = _pack(codes & 15, scale, group)
+        obj.qp, obj.sp = _pack(codes & 15, scale.detach(), group)
         return obj
 
     @property

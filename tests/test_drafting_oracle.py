@@ -61,6 +61,15 @@ def test_not_finite_groups():
     assert not codes[0, :32].any() and codes[1, 32:].astype(bool).sum() == 1
 
 
+def test_a_parameter_leaves_no_graph():
+    w = torch.nn.Parameter(torch.from_numpy(_weights(1, 20, 64)))
+    qw = QuantizedWeight4(w, 32)
+    again = QuantizedWeight4.from_codes(qw.codes, qw.scale.clone().requires_grad_(), 32, torch.float32)
+    for t in (qw.qp, qw.sp, qw.scale, qw.dense(), again.sp, again.dense()):
+        assert not t.requires_grad
+    assert torch.equal(qw.dense(), again.dense())
+
+
 def test_packed_layout():
     """Column 32 j + 8 g + i of row r of a block: bits 4 i of dword j of lane r + 16 g."""
     n, k, group = 20, 272, 32
