@@ -311,6 +311,23 @@ def test_side_stream(gpu):
     assert all(torch.equal(g, want) for g in got)
 
 
+@pytest.mark.parametrize("tokens", [1, 20])
+def test_two_streams_at_once(gpu, tokens):
+    """Split calls on two streams with nothing between them: each its own workspace."""
+    args = [Batch(40 + s, [5000, 700], [tokens, 1], 16, 2, 128, 16, torch.bfloat16).args(gpu) for s in range(2)]
+    want = [tree_attention(*a, max_tokens=tokens)[:tokens + 1] for a in args]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(tree_attention(*args[i], max_tokens=tokens))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+
+
 def test_refusals(gpu):
     b = Batch(12, [20, 3], [2, 2], 16, 2, 128, 16, torch.bfloat16)
     good = b.args(gpu)

@@ -122,6 +122,33 @@ def test_out_in_place_shapes_and_views(gpu):
     assert linear4(xt[:, :64], empty).shape == (6, 0) and empty.dense().shape == (0, 64)
 
 
+def test_no_columns(gpu):
+    qw = QuantizedWeight4(torch.zeros(20, 0, device=gpu), 64)
+    x, bias = torch.zeros(3, 0, dtype=torch.bfloat16, device=gpu), torch.arange(20, device=gpu).bfloat16()
+    assert qw.dense().shape == (20, 0) and qw.scale.shape == (20, 0) and qw.codes.shape == (20, 0)
+    assert not linear4(x, qw).any()
+    res = torch.ones(3, 20, dtype=torch.bfloat16, device=gpu)
+    assert torch.equal(linear4(x, qw, bias, residual=res), (bias + 1).expand(3, 20))
+    assert linear4(x[0], qw).shape == (20,)
+
+
+def test_two_streams_at_once(gpu):
+    """Calls that need a workspace, on two streams with nothing between them: each its own."""
+    qw, _, x = _case(gpu, 20, 512, 11008, 64)
+    xs = [bf16_gpu(activations(s, 20, 11008), gpu) for s in range(2)]
+    want = [linear4(t, qw) for t in xs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(linear4(xs[i], qw))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+
+
 def test_tokens_do_not_touch_each_other(gpu):
     """K ends inside a block: the next row's first values (not finite here) are not read as
     this row's, and a token's infinity stays its own."""
