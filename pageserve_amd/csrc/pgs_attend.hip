@@ -1048,11 +1048,14 @@ __device__ __forceinline__ void join_rows(const Attend& a, int n, int lane, int 
   else *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
 }
 
-// Waves that join four rows: sixteen if those have that many parts, else one (and four
-// times four rows a workgroup).  Measured, microseconds sixteen/one: 24 requests x 64 rows x
-// 16 heads of two or three parts 9.5 (one), two requests of 192 rows a key head and 85 parts
-// 7.5/25.
+// Waves that join four rows: sixteen if those have eight parts and there are few of them, so
+// that the parts' latency counts, else one (and four times four rows a workgroup).  Measured,
+// the whole call in microseconds, sixteen/one, 16 heads on two key heads of 128 dims: one
+// token of 32768 keys 17.0/32.0, of 4096 (8 parts) 14.4/15.8, of 2048 (4) 14.1/13.9; 64
+// requests of 4 tokens and 4096 keys (8 parts, 1024 fours) 63.2/61.6; two requests of 64
+// tokens and 4096 keys (32 parts, 512 fours) 38.2/39.5, four of 2048 (16, 1024) 44.6/36.4.
 constexpr int kJoinWaves = 16;
+inline bool join_by_many(int64_t parts, int64_t fours) { return parts >= 8 && fours <= 512; }
 constexpr int join_threads(int waves) { return waves == 1 ? 256 : 64 * waves; }
 // the four rows of a wave
 template <int WAVES>
@@ -1165,7 +1168,7 @@ int launch_wide(const Attend& a, hipStream_t st) {
   if (int rc = check_launch("tree attention kernel")) return rc;
   const int64_t quads = static_cast<int64_t>(a.requests) * a.kv_heads * ((a.max_tokens * a.group + 3) / 4);
   const int64_t units = static_cast<int64_t>(a.requests) * a.kv_heads * ((a.max_tokens * a.group + kGroup - 1) / kGroup);
-  if (kShares / units >= kJoinWaves)
+  if (join_by_many(kShares / units, quads))
     hipLaunchKernelGGL((join_wide_kernel<D, F16, kJoinWaves>), dim3(static_cast<unsigned>(quads)),
                        dim3(join_threads(kJoinWaves)), 0, st, a);
   else
@@ -1199,7 +1202,7 @@ int launch(const Attend& a, const Plan& p, hipStream_t st) {
   if (int rc = check_launch("tree attention kernel")) return rc;
   if (p.splits == 1) return PGS_OK;
   const int64_t quads = static_cast<int64_t>(a.requests) * ((a.max_tokens * a.q_heads + 3) / 4);
-  if (p.splits >= kJoinWaves)
+  if (join_by_many(p.splits, quads))
     hipLaunchKernelGGL((join_kernel<D, F16, kJoinWaves>), dim3(static_cast<unsigned>(quads)),
                        dim3(join_threads(kJoinWaves)), 0, st, a, p.wr);
   else
