@@ -56,7 +56,7 @@ struct Attend {
   int32_t cols;
   const int32_t *lens, *offsets, *parents;
   int32_t rows, requests, q_heads, kv_heads, group;  // group: q_heads / kv_heads
-  int32_t max_tokens, splits;
+  int32_t max_tokens, splits, min_steps;
   float c;      // scale * log2(e)
   float* part;  // sums of the parts of rows: [slots][D], slots as Wave::store's caller numbers them
   float* stat;  // [slots][2]: m, l
@@ -409,11 +409,13 @@ struct Wave {
   }
 };
 
-// Parts that the keys of a request are cut into, of the `splits` that the grid has: of
-// kMinSteps steps at least, or half of that where two waves share a step.
-constexpr int kMinSteps = 16;
+// Parts that the keys of a request are cut into, of the `splits` that the grid has, by its
+// 32-key steps (twice those where two waves share a step): none below kWholeSteps, else of
+// min_steps at least.
+constexpr int kWholeSteps = 32, kCoarseSteps = 16, kFineSteps = 8;
 __device__ __forceinline__ int parts_of(const Attend& a, const Request& rq, int wr) {
-  return min(a.splits, max(1, (rq.len_tiles + rq.tree_tiles) * wr / kMinSteps));
+  const int steps = (rq.len_tiles + rq.tree_tiles) * wr;
+  return steps < kWholeSteps ? 1 : min(a.splits, steps / a.min_steps);
 }
 
 // Few rows (up to 64 per key head): bound by reading the keys and values once, and for
@@ -1125,11 +1127,15 @@ __global__ __launch_bounds__(join_threads(WAVES)) void join_wide_kernel(Attend a
 //   but 64 x 2048 31.0/30.3, 256 x 512 27.6/26.7.  64 dims: 8 x 1024 of 32 rows 12.8/14.1.
 //   Not for more than 16 rows of 128 dims, whose sums from eight waves take too much LDS:
 //   24.2/13.8 at 8 x 512.
+// - Parts of eight steps while parts of sixteen would leave half of the CUs idle; eight/sixteen:
+//   one request of 1024 keys 12.3/13.3, of 8192 13.1/14.6, 8 x 1024 12.6/13.8, but 128 x 512
+//   20.4/16.9, 8 x 4000 of 64 rows 24.7/22.3; of four 12.0, 13.2, 12.2, 24.4 and 33.9.  Below 32
+//   steps the join costs more than two parts gain: 512 keys 11.6/10.8.
 struct Plan {
   bool wide;
   int r, wr;   // else row tiles per wave, waves per key slice
   int waves;   // of a workgroup
-  int splits;
+  int splits, min_steps;  // of the keys, as parts_of takes them
 };
 Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_tokens,
           int64_t max_context) {
@@ -1140,9 +1146,10 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
   if (p.wide) return p;
   p.r = rows <= 16 ? 1 : 2;
   p.wr = rows <= 32 ? 1 : 2;
-  const int64_t steps = (max_context + 31) / 32 + (max_tokens + 31) / 32;
-  const int64_t most = steps * p.wr / kMinSteps, s = (1024 + units - 1) / units;
-  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({s, most, 256})));
+  const int64_t steps = ((max_context + 31) / 32 + (max_tokens + 31) / 32) * p.wr;
+  p.min_steps = units * (steps / kCoarseSteps) <= 128 ? kFineSteps : kCoarseSteps;
+  if (steps >= kWholeSteps)
+    p.splits = static_cast<int>(std::min<int64_t>({(1024 + units - 1) / units, steps / p.min_steps, 256}));
   p.waves = (p.r == 1 || head_dim == 64) && units * p.splits <= 256 ? 8 : 4;
   return p;
 }
@@ -1283,7 +1290,7 @@ extern "C" int pgs_tree_attention(const pgs_tree_attention_args* args, void* wor
   a.rows = static_cast<int32_t>(g.rows), a.requests = static_cast<int32_t>(g.requests);
   a.q_heads = static_cast<int32_t>(g.q_heads), a.kv_heads = static_cast<int32_t>(c.kv_heads);
   a.group = a.q_heads / a.kv_heads;
-  a.max_tokens = static_cast<int32_t>(g.max_tokens), a.splits = p.splits;
+  a.max_tokens = static_cast<int32_t>(g.max_tokens), a.splits = p.splits, a.min_steps = p.min_steps;
   a.c = g.scale * 1.44269504088896340736f;
   a.part = static_cast<float*>(workspace);
   a.stat = a.part + slots_of(p, g.rows, g.q_heads) * c.head_dim;
