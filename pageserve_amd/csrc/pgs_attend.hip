@@ -423,7 +423,7 @@ __device__ __forceinline__ int parts_of(const Attend& a, const Request& rq, int 
 // waves are WR row tiles x NW/WR key slices; each wave loads the keys of its steps straight
 // into registers.  Measured, 16 heads on two key heads of 128 dims: one token of 256
 // requests of 512 keys 26.6 us (5.0 TB/s of keys and values), of 64 of 2048 29.2 (4.6), of
-// one of 32768 with the join 17.5 (1.9); 4 tokens of 64 of 2048 32.4 (4.2).
+// one of 32768 with the join 16.6 (2.0); 4 tokens of 64 of 2048 32.4 (4.2).
 template <int D, int R, int WR, int NW, bool F16>
 __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(Attend a) {
   using W = Wave<D, R, F16, true>;
