@@ -770,7 +770,8 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
   // dims 4 (li % 4) .. +3 of key 4 lg + li / 4
   const int li = lane & 15, lg = lane >> 4, vkey = 4 * lg + (li >> 2);
   const uint32_t k_at = lds_address(lkv) + li * (2 * D) + 16 * (lg ^ (li * P / 16 & (P - 1)));
-  const uint32_t v_at = lds_address(lkv) + TK * D * 2 + vkey * (2 * D) + 16 * ((li >> 1 & 1) ^ (2 * (vkey * P / 16) & (P - 1))) + 8 * (li & 1);
+  const uint32_t v_at = lds_address(lkv) + TK * D * 2 + vkey * (2 * D) +
+                        16 * ((li >> 1 & 1) ^ (2 * (vkey * P / 16) & (P - 1))) + 8 * (li & 1);
   Work<TK> work{again(), lpre, lsum, 0, 0, 0};
   work.start(blockIdx.x == 0 ? work.a.sums : nullptr);
   const int shares = shares_of(work.total), share = xcd_remap(blockIdx.x, gridDim.x);
@@ -804,7 +805,7 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
     auto load = [&](int t, int to) {
       const int ln = here(lane), kin = ln / P, piece = ln % P;
       const uint32_t at_k = lds_address(lkv) + to * (4 * TK * D) + wave * (1024 * J), at_v = at_k + 2 * TK * D;
-      // (lane l fills piece l % P of its key's row, which is piece ... of the row in memory)
+      // (lane l fills piece l % P of its key's row in LDS: the exchange picks what it reads)
       if (t >= cached) {
         const Attend c = again();
 #pragma unroll
@@ -907,7 +908,8 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
           if (key0 + 32 * h >= limit) break;
           // a piece's exchange is an exclusive or of its row's address with 16 bytes times
           // the piece, halves of a step and steps are 16 and 32 whole rows apart
-          const uint32_t kat = k_at + buf * (4 * TK * D) + 32 * h * (2 * D), vat = v_at + buf * (4 * TK * D) + 32 * h * (2 * D);
+          const uint32_t kat = k_at + buf * (4 * TK * D) + 32 * h * (2 * D);
+          const uint32_t vat = v_at + buf * (4 * TK * D) + 32 * h * (2 * D);
           auto keys = [&](int g, int d) { return *lds<const u32x4>((kat ^ (64 * d)) + 16 * g * (2 * D)); };
           auto values = [&](int d) {
             const u32x2 x = read_transposed((vat ^ (32 * d))), y = read_transposed((vat ^ (32 * d)) + 16 * (2 * D));
@@ -1227,7 +1229,8 @@ extern "C" size_t pgs_tree_attention_workspace_bytes(int64_t rows, int64_t reque
                                                      int64_t head_dim, int64_t max_tokens, int64_t max_context) {
   if (!sizes_ok(rows, requests, q_heads, kv_heads, head_dim, max_tokens, max_context) || rows == 0 || requests == 0)
     return 0;
-  return workspace_bytes(plan(requests, q_heads, kv_heads, head_dim, max_tokens, max_context), rows, requests, q_heads, head_dim);
+  const Plan p = plan(requests, q_heads, kv_heads, head_dim, max_tokens, max_context);
+  return workspace_bytes(p, rows, requests, q_heads, head_dim);
 }
 
 extern "C" int pgs_tree_attention(const pgs_tree_attention_args* args, void* workspace, size_t workspace_bytes_given,
