@@ -96,18 +96,20 @@ class QuantizedWeight4:
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scale: torch.Tensor, group: int,
                    dtype: torch.dtype = torch.bfloat16) -> "QuantizedWeight4":
-        """A weight from row-major codes (uint8 [out_features, in_features], 0..15:
-        the value's index, plus 8 for a negative one) and scales (bf16
-        [out_features, ceil(in_features / group)])."""
-        if codes.dtype != torch.uint8 or scale.dtype != torch.bfloat16:
-            raise TypeError("codes must be uint8 and scale bf16")
+        """A weight from row-major codes (any integer type, [out_features, in_features],
+        0..15: the value's index, plus 8 for a negative one; of others the low four bits
+        count) and scales (bf16 [out_features, ceil(in_features / group)])."""
+        if codes.is_floating_point() or codes.is_complex() or codes.dtype is torch.bool:
+            raise TypeError(f"codes must be of an integer type, got {codes.dtype}")
+        if scale.dtype != torch.bfloat16:
+            raise TypeError(f"scale must be bf16, got {scale.dtype}")
         _check_shape(codes.shape, group)
         n, k = codes.shape
         if tuple(scale.shape) != (n, -(-k // group)) or scale.device != codes.device:
             raise ValueError(f"scale must be [{n}, {-(-k // group)}] on {codes.device}")
         obj = cls.__new__(cls)
         obj.dtype, obj.shape, obj.group = dtype, torch.Size(codes.shape), group
-        obj.qp, obj.sp = _pack(codes & 15, scale.detach(), group)
+        obj.qp, obj.sp = _pack(codes.to(torch.uint8) & 15, scale.detach(), group)
         return obj
 
     @property

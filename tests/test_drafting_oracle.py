@@ -70,6 +70,24 @@ def test_a_parameter_leaves_no_graph():
     assert torch.equal(qw.dense(), again.dense())
 
 
+@pytest.mark.parametrize("dtype", [torch.int8, torch.int16, torch.int32, torch.int64])
+def test_codes_of_any_integer_type(dtype):
+    """Torch's own arithmetic on masks and bytes yields int64: the same weight."""
+    gen = torch.Generator().manual_seed(7)
+    codes = torch.randint(0, 16, (20, 144), generator=gen, dtype=torch.uint8)
+    scale = torch.rand(20, 5, generator=gen).bfloat16()
+    want = QuantizedWeight4.from_codes(codes, scale, 32)
+    got = QuantizedWeight4.from_codes(codes.to(dtype), scale, 32)
+    assert torch.equal(got.qp, want.qp) and torch.equal(got.codes, codes)
+    low = QuantizedWeight4.from_codes(codes.to(dtype) - 16, scale, 32)  # the low four bits count
+    assert torch.equal(low.qp, want.qp)
+    for bad in (codes.float(), codes.bool(), codes.to(torch.complex64)):
+        with pytest.raises(TypeError, match="integer type"):
+            QuantizedWeight4.from_codes(bad, scale, 32)
+    with pytest.raises(TypeError, match="bf16"):
+        QuantizedWeight4.from_codes(codes, scale.float(), 32)
+
+
 def test_packed_layout():
     """Column 32 j + 8 g + i of row r of a block: bits 4 i of dword j of lane r + 16 g."""
     n, k, group = 20, 272, 32
