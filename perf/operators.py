@@ -241,8 +241,7 @@ def prepare(case, seed):
         # the weight in the layout that the program keeps it in
         from pageserve_amd import QuantizedWeight4
 
-        state["weight"] = QuantizedWeight4.from_codes(state["codes"].to(torch.uint8), state["scale"], case["group"],
-                                                      torch.bfloat16)
+        state["weight"] = QuantizedWeight4.from_codes(state["codes"], state["scale"], case["group"], torch.bfloat16)
     return state
 
 
