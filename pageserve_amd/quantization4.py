@@ -63,14 +63,14 @@ def _pack(codes: torch.Tensor, scale: torch.Tensor, group: int) -> tuple[torch.T
 
 def _cpu_quantize4(weight: torch.Tensor, group: int) -> tuple[torch.Tensor, torch.Tensor]:
     n, k = weight.shape
-    w = torch.nn.functional.pad(weight.float(), (0, -k % group)).view(n, -1, group)
+    w = torch.nn.functional.pad(weight.float(), (0, -k % group)).view(n, -(-k // group), group)
     a = w.abs()
     scale = (a.amax(2, keepdim=True).clamp(min=1e-8) / 6.0).to(torch.bfloat16) if k else a.new_zeros(n, 0, 1).bfloat16()
     s = scale.float()
     code = ((a > 0.25 * s).to(torch.uint8) + (a >= 0.75 * s) + (a > 1.25 * s) + (a >= 1.75 * s) + (a > 2.5 * s)
             + (a >= 3.5 * s) + (a > 5.0 * s))
     code = code + 8 * ((w < 0) & (code > 0)).to(torch.uint8)
-    return code.reshape(n, -1)[:, :k], scale.squeeze(2)
+    return code.flatten(1)[:, :k], scale.squeeze(2)
 
 
 class QuantizedWeight4:

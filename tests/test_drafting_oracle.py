@@ -51,6 +51,13 @@ def test_cpu_weight_matches_the_oracle(n, k, group, dtype):
     assert qw.storage_bytes == blocks * (1024 + 32 * (128 // group))
 
 
+@pytest.mark.parametrize("n,k", [(0, 64), (5, 0), (0, 0)])
+def test_cpu_weight_without_rows_or_columns(n, k):
+    qw = QuantizedWeight4(torch.zeros(n, k), 32)
+    assert qw.codes.shape == qw.dense().shape == (n, k) and qw.scale.shape == (n, k // 32) and qw.storage_bytes == 0
+    assert QuantizedWeight4.from_codes(qw.codes, qw.scale, 32).dense().shape == (n, k)
+
+
 def test_not_finite_groups():
     w = _weights(5, 2, 64)
     w[0, 3], w[1, 40] = np.nan, np.inf
