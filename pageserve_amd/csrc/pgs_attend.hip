@@ -146,13 +146,24 @@ __device__ __forceinline__ float quad_max(float v) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// A maximum nothing has raised yet: 2^(kLow - m) = 0 for every m of a score.
-constexpr float kLow = -3.0e38f;
+// A maximum nothing has raised yet: the lowest value that is finite.
+constexpr float kLow = -3.402823466e38f;
 // The reference of the exponents follows the maximum only when a score exceeds it
 // by this (in powers of two): p stays below 2^8, in range for fp16 and as exact in
 // either type as below 1, and the sums are rescaled a few times per row instead of
 // at every step.
 constexpr float kSlack = 8.0f;
+// A reference is a rounded product c s, and fma(s, c, -reference) sees that rounding: up to
+// half a step of the reference, which the largest weight is off by (as a power of two; all
+// weights of the row are alike).  Beyond kFar that is more than 1/2 and in the end out of any
+// range, so there the product is rounded before the reference is taken off, as it was for
+// the reference: the largest weight is 2^0.
+constexpr float kFar = 8388608.0f;
+__device__ __forceinline__ float exponent(float s, float c, float reference, bool far) {
+#pragma clang fp contract(off)
+  const float t = s * c;
+  return far ? t - reference : fmaf(s, c, -reference);
+}
 
 // The request of a unit and its sizes, each brought into range: whatever the device
 // arrays hold, no access leaves the tensors.
@@ -194,6 +205,7 @@ struct Wave {
   u32x4 q[R][DC];
   f32x4 o[R][DV], l[R];
   float mx[R];
+  bool far;  // some row's reference is beyond kFar (the same in all lanes)
 
   __device__ __forceinline__ void load(const Attend& a, const Request& rq, int kh, int row0, int nrows, int li, int lg) {
 #pragma unroll
@@ -209,6 +221,7 @@ struct Wave {
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int d = 0; d < DC; ++d) asm volatile("" : "+v"(q[r][d]));
+    far = false;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       mx[r] = kLow;
@@ -280,7 +293,7 @@ struct Wave {
     float x[R][8];
     uint32_t ok[R];
     bool over = false;
-    if (masked) {
+    if (masked || far) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const unsigned long long sees = tree ? see(r) : ~0ull;
@@ -290,7 +303,7 @@ struct Wave {
           const int key = key0 + 16 * (e >> 2) + 4 * lg + (e & 3);
           const bool in = key < limit && !(e >> 2 ? bad1 : bad0) && (sees >> (key & 63) & 1);
           ok[r] |= in ? 1u << e : 0;
-          x[r][e] = in ? fmaf(s[r][e >> 2][e & 3], a.c, -mx[r]) : -INFINITY;
+          x[r][e] = in ? exponent(s[r][e >> 2][e & 3], a.c, mx[r], far) : -INFINITY;
           over = over || x[r][e] > kSlack;
         }
       }
@@ -309,6 +322,7 @@ struct Wave {
     }
     if (__ballot(over)) {
       // new references: the largest score of each row so far
+      bool beyond = false;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         float t = -INFINITY;
@@ -316,15 +330,19 @@ struct Wave {
         for (int e = 0; e < 8; ++e) t = fmaxf(t, ok[r] >> e & 1 ? s[r][e >> 2][e & 3] * a.c : -INFINITY);
         const float ref = fmaxf(quad_max(t), mx[r]), f = __builtin_amdgcn_exp2f(mx[r] - ref);
         mx[r] = ref;
+        beyond = beyond || fabsf(ref) > kFar;
 #pragma unroll
         for (int i = 0; i < 4; ++i) l[r][i] *= f;
 #pragma unroll
         for (int d = 0; d < DV; ++d)
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[r][d][i] *= f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[r][e] = ok[r] >> e & 1 ? fmaf(s[r][e >> 2][e & 3], a.c, -ref) : -INFINITY;
       }
+      far = __ballot(beyond);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[r][e] = ok[r] >> e & 1 ? exponent(s[r][e >> 2][e & 3], a.c, mx[r], far) : -INFINITY;
     }
     u32x4 p[R];
 #pragma unroll

@@ -118,6 +118,70 @@ def test_scales_and_sharp_maxima(gpu):
     b.check(tree_attention(*b.args(gpu)), b.oracle(), "rising")
 
 
+# kernels: few rows in one part and in many, 33 rows and more through LDS, one key slice and two
+LARGE = [("0.5b", [300, 0], [1, 1], 1), ("3b", [5000], [1], 1), ("3b", [700, 40], [4, 3], 4), ("0.5b", [200], [9], 9),
+         ("odd", [130, 260], [40, 64], 64), ("wide", [1000], [12], 12), ("3b", [257], [32], 32)]
+
+
+@pytest.mark.parametrize("heads,lens,tokens,most", LARGE)
+@pytest.mark.parametrize("dtype,powers", [(torch.float16, (3, 10, 12, 13)), (torch.bfloat16, (3, 10, 13, 30, 58))])
+def test_large_scores_of_one_key(gpu, heads, lens, tokens, most, dtype, powers):
+    """One key far above the rest, whose values are the answer, with nothing to round: a
+    weight of 1 (to a factor near 1 that the sum has too) against zeros.  Scores of both
+    signs from 2^6 or so to the type's largest, the key cached, first, last or among the others, or
+    the token's own; a key that is there twice takes the mean, off by its rounding."""
+    h, kv, dim = HEADS[heads]
+    b = Batch(50, lens, tokens, h, kv, dim, 16, dtype, parents="roots")
+    rng = np.random.default_rng(9)
+    base = (torch.from_numpy(rng.uniform(0.5, 0.9, (kv, dim))) * torch.from_numpy(rng.choice([-1, 1], (kv, dim)))).to(dtype)
+    b.k.zero_(), b.kc.zero_()
+    rows = b.offsets[-1]
+    for power in powers:
+        # (a quarter of a power less for each further head: the scores differ and stay in range)
+        size = [2.0 ** (power - i % 3) for i in range(h)]
+        for sign in (1, -1):
+            q = torch.stack([base[i // (h // kv)] * size[i] for i in range(h)])
+            b.q[:] = q
+            top = base * 2.0 ** power
+            # sign 1: the key among zeros; -1: all others at twice the negative score
+            rest = torch.zeros_like(top) if sign > 0 else -2 * top
+            b.k[:], b.kc[:] = rest, rest
+            want = torch.empty(rows, kv, dim, dtype=dtype)
+            for r, n in enumerate(lens):
+                lo, hi = b.offsets[r], b.offsets[r + 1]
+                places = [0, n - 1, n // 2, n // 3] if n else []
+                for t in range(lo, hi):
+                    # the key in the cache (one place for the request), or the token itself
+                    own = not places or r % 2
+                    if own:
+                        b.k[t] = sign * top
+                        want[t] = b.v[t]
+                if places and not r % 2:
+                    at = places[(power + sign) % 4]
+                    slot = int(b.tables[r, at // 16]), at % 16
+                    b.kc[slot] = sign * top
+                    want[lo:hi] = b.vc[slot]
+            full = want.repeat_interleave(h // kv, 1)
+            args = b.args(gpu)
+            for kw in (dict(max_tokens=most), dict(max_tokens=most, max_context=1 << 20), dict()):
+                got = tree_attention(*args, **kw).cpu()
+                assert torch.equal(got, full), (power, sign, kw, (got.float() - full.float()).abs().max())
+            # negative scale: the same scores from turned queries
+            args[0] = -args[0]
+            assert torch.equal(tree_attention(*args, max_tokens=most, scale=-(dim ** -0.5)).cpu(), full), (power, sign)
+            if lens[0] > 32 and sign > 0:
+                at = 20
+                slot = int(b.tables[0, at // 16]), at % 16
+                once = b.kc[slot].clone()
+                b.kc[slot] = top
+                if not torch.equal(once, top):
+                    hi = b.offsets[1]
+                    mean = (want[:hi].double() + b.vc[slot].double()) / 2
+                    got = tree_attention(*b.args(gpu), max_tokens=most)[:hi].cpu().double()
+                    mean = mean.repeat_interleave(h // kv, 1)
+                    assert ((got - mean).abs() <= U[dtype] * mean.abs() + 2.0 ** -22).all(), (power, "twice")
+
+
 def test_padded_and_cut_batches(gpu):
     b = Batch(5, [40, 7, 0], [3, 70, 9], 16, 2, 128, 16, torch.float16, pad=6)
     out = torch.full(b.q.shape, 3.0, dtype=b.dtype, device=gpu)
