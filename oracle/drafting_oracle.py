@@ -90,7 +90,7 @@ def truncate(lens, keep, tables, free, count, bs):
         have = min(-(-max(lens[b], 0) // bs), len(tables[b]))
         lens[b] = min(max(keep[b], 0), max(lens[b], 0))
         left = min(-(-lens[b] // bs), have)
-        back += tables[b][left:have]
+        back += [block for block in tables[b][left:have] if block >= 0]
         tables[b][left:have] = [-1] * (have - left)
     for e, block in enumerate(back):
         at = count + len(back) - 1 - e

@@ -161,8 +161,9 @@ __global__ __launch_bounds__(kRowThreads) void slots_kernel(Tables t, const int3
   rw.slots[i] = slot;
 }
 
-// Shortens requests: entry e (in request order, then column order) of the blocks
-// given back goes to free[count + total - 1 - e], the place append took it from.
+// Shortens requests.  Of the table entries given up (in request order, then column order)
+// those that name a block go to the stack, the last one first, so that append's lie where
+// it took them from; an entry below 0 names none and is not counted.
 __global__ __launch_bounds__(kScanThreads) void truncate_kernel(Tables t, const int32_t* __restrict__ keep) {
   extern __shared__ int32_t lds[];
   int32_t* start = lds;
@@ -186,14 +187,20 @@ __global__ __launch_bounds__(kScanThreads) void truncate_kernel(Tables t, const 
   }
   __syncthreads();
   const int64_t total = carry;
-  for (int64_t e = threadIdx.x; e < total; e += kScanThreads) {
-    const int b = upper_bound(start, t.requests, static_cast<int32_t>(min<int64_t>(e, 0x7fffffff))) - 1;
-    int32_t* p = t.tables + b * t.stride + left[b] + (e - start[b]);
-    const int64_t at = c0 + total - 1 - e;
-    if (at < t.cap) t.free[at] = *p;
-    *p = -1;
+  carry = c0;
+  for (int64_t f = 0; f < total; f += kScanThreads) {
+    const int64_t e = total - 1 - f - threadIdx.x;
+    int32_t id = -1;
+    if (e >= 0) {
+      const int b = upper_bound(start, t.requests, static_cast<int32_t>(min<int64_t>(e, 0x7fffffff))) - 1;
+      int32_t* p = t.tables + b * t.stride + left[b] + (e - start[b]);
+      id = *p;
+      *p = -1;
+    }
+    const int64_t upto = block_scan(id >= 0, carry, wsum);  // blocks on the stack with this one
+    if (id >= 0 && upto <= t.cap) t.free[upto - 1] = id;
   }
-  if (threadIdx.x == 0) *t.count = static_cast<int32_t>(min<int64_t>(c0 + total, t.cap));
+  if (threadIdx.x == 0) *t.count = static_cast<int32_t>(min<int64_t>(carry, t.cap));
 }
 
 struct WriteArgs {

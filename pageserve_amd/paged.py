@@ -73,9 +73,9 @@ def truncate_blocks(lens: torch.Tensor, keep: torch.Tensor, block_tables: torch.
                     free_count: torch.Tensor, block_size: int) -> None:
     """Shortens request ``b`` to ``keep[b]`` tokens, in place: 0 for one that is
     finished, any count from its length on to leave it.  The blocks it no longer
-    needs go back to the stack and their table columns become -1.  Undoes
-    :func:`append_blocks` exactly.  Tensors as there, ``keep`` int32
-    [requests]."""
+    needs go back to the stack and their table columns become -1; a negative
+    column (an absent block) gives nothing back.  Undoes :func:`append_blocks`
+    exactly.  Tensors as there, ``keep`` int32 [requests]."""
     _native.load_host().truncate_blocks(lens, keep, block_tables, free_blocks, free_count, block_size)
 
 

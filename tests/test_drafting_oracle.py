@@ -126,5 +126,14 @@ def test_append_and_truncate_by_hand():
     assert status == [0, 1, 0] and lens == [12, 4, 3] and count == 0 and slots == [16, -1, 10]
 
 
+def test_a_hole_in_a_table_is_not_given_back():
+    lens, tables, free = [40, 20], [[3, -1, 5], [-1, 7, -1]], [9, 0, 0, 0, 0]
+    count = D.truncate(lens, [0, 3], tables, free, 1, 16)
+    assert count == 4 and free[:4] == [9, 7, 5, 3]
+    assert lens == [0, 3] and tables == [[-1, -1, -1], [-1, -1, -1]]
+    slots, status, count = D.append(lens, [40, 0], [0, 40, 40], tables, free, count, 16, 40)
+    assert status == [0, 0] and count == 1 and tables[0] == [3, 5, 7] and min(slots) >= 0
+
+
 def test_ancestors():
     assert D.ancestors([-1, 0, 0, 1, 5, 9]) == [{0}, {0, 1}, {0, 2}, {0, 1, 3}, {4}, {5}]

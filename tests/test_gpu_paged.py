@@ -94,6 +94,34 @@ def test_append_then_truncate(gpu, requests, tokens, bs, indexed):
     assert s.count == len(s.free) and sorted(s.free) == list(range(len(s.free)))
 
 
+@pytest.mark.parametrize("requests,columns", [(1, 5), (3, 3), (40, 30), (700, 7)])
+def test_holes_are_not_given_back(gpu, requests, columns):
+    """Absent blocks below the length: the stack gets the others, in order, and nothing
+    that append hands out afterwards is absent."""
+    rng = np.random.default_rng(columns)
+    lens = rng.integers(0, 4 * columns + 1, requests).tolist()
+    lens[0] = 4 * columns
+    s = _State(gpu, lens, columns, 4, spare=3, seed=requests)
+    holes = 0
+    for b, n in enumerate(lens):
+        for c in range(-(-n // 4)):
+            if rng.random() < 0.4 or (b, c) == (0, 1):
+                s.tables[b][c], holes = -1 - c, holes + 1
+    s.t.copy_(_i32(s.tables, gpu))
+    s.truncate([n // 2 for n in lens])
+    s.truncate([0] * requests)
+    assert s.count == len(s.free) - holes and min(s.free[:s.count]) >= 0
+    new = [min(4 * columns, 4 * s.count)] + [0] * (requests - 1)
+    slots, status, _ = s.append(new, _offsets(new), new[0])
+    assert status == [0] * requests and min(slots) >= 0 and len(set(slots)) == new[0]
+    # a stack that is too short keeps what was on it and drops the last that come
+    s = _State(gpu, [8, 9], 3, 4, spare=0)
+    s.free, s.f = s.free[:2], s.f[:2].contiguous()
+    s.tables[0][0] = -1
+    s.t.copy_(_i32(s.tables, gpu))
+    s.truncate([0, 0])
+
+
 def test_too_few_blocks_columns_and_odd_lengths(gpu):
     for spare in range(0, 9):
         s = _State(gpu, [4, 15, 16, 0, 31, 40], 4, 16, spare=spare, seed=spare)
