@@ -579,7 +579,7 @@ typedef struct pgs_tree_attention_args {
   const int32_t* offsets;      /* [requests + 1] */
   const int32_t* parents;      /* [rows], or NULL: each token's parent is the one before it */
   int64_t rows, requests, q_heads;
-  int64_t max_tokens;          /* rows per request, at most 64 */
+  int64_t max_tokens;          /* rows per request, at most 64; the kernels are chosen by it */
   int64_t max_context;         /* the longest lens expected: sizes the split, not the result */
   float scale;
   int dtype;                   /* PGS_DTYPE_BF16 or PGS_DTYPE_F16, of all tensors */

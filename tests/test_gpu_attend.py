@@ -363,6 +363,22 @@ def test_in_place(gpu, lens, tokens):
     assert tree_attention(*args, out=args[0]) is not None and torch.equal(args[0], want)
 
 
+@pytest.mark.parametrize("lens,tokens", [([40], [1]), ([900, 30], [1, 1]), ([60], [7])])
+def test_default_bound_is_planned_as_the_rows(gpu, lens, tokens):
+    """Without max_tokens: the same kernel, so the same bits, and no workspace for 64 tokens
+    a request (68 MB) beside the output and what the few rows need."""
+    b = Batch(34, lens, tokens, 16, 2, 128, 16, torch.bfloat16)
+    args, rows = b.args(gpu), sum(tokens)
+    want = tree_attention(*args, max_tokens=rows)
+    b.check(want, b.oracle())
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = tree_attention(*args)
+    assert torch.cuda.max_memory_allocated() - before < 4 << 20
+    assert torch.equal(got, want)
+
+
 def test_side_stream(gpu):
     b = Batch(11, [3000], [4], 16, 2, 128, 16, torch.bfloat16)
     args = b.args(gpu)
