@@ -33,7 +33,7 @@
 
 #include <algorithm>
 
-#include "pgs_fp4.h"
+#include "pgs_linear.h"
 
 namespace pgs {
 namespace {

@@ -9,6 +9,12 @@
 
 namespace pgs {
 
+// a number as a type, for generic lambdas
+template <int V>
+struct Int {
+  static constexpr int value = V;
+};
+
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));

@@ -16,11 +16,6 @@
 
 namespace pgs {
 
-template <int V>
-struct Int {
-  static constexpr int value = V;
-};
-
 __host__ __device__ inline int64_t fp4_kblocks(int64_t k) { return (k + 127) / 128; }
 __host__ __device__ inline int64_t fp4_blocks(int64_t n, int64_t k) { return ((n + 15) / 16) * fp4_kblocks(k); }
 

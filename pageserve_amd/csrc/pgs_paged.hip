@@ -186,21 +186,53 @@ __global__ __launch_bounds__(kScanThreads) void truncate_kernel(Tables t, const 
     if (b < t.requests) start[b] = static_cast<int32_t>(min<int64_t>(upto - give, 0x7fffffff));
   }
   __syncthreads();
+  // Entries from the last on, U per thread and turn: a wave's are 64 U neighbours, counted by
+  // ballots; the waves' counts are in one of two arrays in turn, so that one barrier will do.
+  __shared__ int32_t found[2][kScanThreads / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t total = carry;
-  carry = c0;
-  for (int64_t f = 0; f < total; f += kScanThreads) {
-    const int64_t e = total - 1 - f - threadIdx.x;
-    int32_t id = -1;
-    if (e >= 0) {
+  int64_t on = c0;  // blocks on the stack
+  int turn = 0;
+  auto give_back = [&](int64_t f, auto per) {
+    constexpr int U = decltype(per)::value;
+    int32_t* p[U];
+    int32_t id[U];
+    int at[U], mine = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t e = total - 1 - f - ((wave * U + u) * 64 + lane);
+      p[u] = nullptr;
+      if (e < 0) continue;
       const int b = upper_bound(start, t.requests, static_cast<int32_t>(min<int64_t>(e, 0x7fffffff))) - 1;
-      int32_t* p = t.tables + b * t.stride + left[b] + (e - start[b]);
-      id = *p;
-      *p = -1;
+      p[u] = t.tables + b * t.stride + left[b] + (e - start[b]);
     }
-    const int64_t upto = block_scan(id >= 0, carry, wsum);  // blocks on the stack with this one
-    if (id >= 0 && upto <= t.cap) t.free[upto - 1] = id;
-  }
-  if (threadIdx.x == 0) *t.count = static_cast<int32_t>(min<int64_t>(carry, t.cap));
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = p[u] ? *p[u] : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned long long m = __ballot(id[u] >= 0);
+      at[u] = mine + __popcll(m & ((1ull << lane) - 1));
+      mine += __popcll(m);
+    }
+    if (lane == 0) found[turn][wave] = mine;
+    __syncthreads();
+    int64_t to = on;
+#pragma unroll
+    for (int w = 0; w < kScanThreads / 64; ++w) {
+      if (w < wave) to += found[turn][w];
+      on += found[turn][w];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (p[u]) *p[u] = -1;
+      if (id[u] >= 0 && to + at[u] < t.cap) t.free[to + at[u]] = id[u];
+    }
+    turn ^= 1;
+  };
+  int64_t f = 0;
+  for (; total - f > kScanThreads; f += 4 * kScanThreads) give_back(f, Int<4>{});
+  if (f < total) give_back(f, Int<1>{});
+  if (threadIdx.x == 0) *t.count = static_cast<int32_t>(min<int64_t>(on, t.cap));
 }
 
 struct WriteArgs {
