@@ -525,6 +525,8 @@ int pgs_w4a16_linear(const void* x, const void* qp, const void* sp,
  * i of the batch: token lens[b] (before the call) + n of its request, where n =
  * index[i], or i - offsets[b] without an index; -1 if n is not in
  * 0..new_lens[b]-1, the request was not served, or the row belongs to none.
+ * No array that is written (here and in pgs_truncate_blocks) may share memory
+ * with another.
  */
 int pgs_append_blocks(int32_t* lens, const int32_t* new_lens, int32_t* block_tables,
                       int64_t table_stride, int64_t columns, const int32_t* free_blocks,

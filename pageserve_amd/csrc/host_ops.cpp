@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <string>
 #include <vector>
 
@@ -350,6 +351,32 @@ int32_t* table(const at::Tensor& t, int64_t requests, const at::Device& dev, con
   return static_cast<int32_t*>(ptr(t));
 }
 
+// Whether two int32 arrays share an element: rows of `cols` contiguous elements, `stride` apart.
+struct Ints {
+  const char* name;
+  const int32_t* p;
+  int64_t rows, cols, stride;
+};
+bool share(const Ints& a, const Ints& b) {
+  if (b.rows > 1) return a.rows > 1 ? share(a, {b.name, b.p, 1, (b.rows - 1) * b.stride + b.cols, 0}) : share(b, a);
+  if (!a.rows || !a.cols || !b.rows || !b.cols) return false;
+  // b is [d, d + cols) in elements from a's first (everything here is 4-byte aligned)
+  const int64_t d = (reinterpret_cast<intptr_t>(b.p) - reinterpret_cast<intptr_t>(a.p)) / 4, end = d + b.cols;
+  if (a.rows == 1) return d < a.cols && end > 0;
+  const int64_t r = d < 0 ? 0 : std::min(d / a.stride, a.rows - 1);  // the last row that begins by d
+  return (d < r * a.stride + a.cols && end > r * a.stride) || (r + 1 < a.rows && end > (r + 1) * a.stride);
+}
+// `written` share no element with one another nor with `read`
+void check_apart(const char* what, std::initializer_list<Ints> written, std::initializer_list<Ints> read) {
+  for (const Ints* w = written.begin(); w != written.end(); ++w) {
+    for (const Ints* o = w + 1; o != written.end(); ++o)
+      if (share(*w, *o)) value_error(std::string(what) + ": " + w->name + " and " + o->name + " must not share memory");
+    for (const Ints& r : read)
+      if (share(*w, r)) value_error(std::string(what) + ": " + w->name + " and " + r.name + " must not share memory");
+  }
+}
+constexpr int64_t kMaxRequests = 4096;  // (more are refused by the kernels' entry, first)
+
 std::vector<at::Tensor> append_blocks(const at::Tensor& lens, const at::Tensor& new_lens, const at::Tensor& offsets,
                                       const at::Tensor& block_tables, const at::Tensor& free_blocks,
                                       const at::Tensor& free_count, int64_t block_size, int64_t rows, const Opt& index) {
@@ -366,6 +393,11 @@ std::vector<at::Tensor> append_blocks(const at::Tensor& lens, const at::Tensor& 
   int32_t* cp = ints_out(free_count, 1, dev, what, "free_count");
   if (rows < 0) value_error("append_blocks: rows must not be negative");
   const int32_t* ip = index.has_value() ? ints(*index, rows, dev, what, "index") : nullptr;
+  if (n <= kMaxRequests)
+    check_apart(what,
+                {{"lens", lp, 1, n, 0}, {"block_tables", tp, n, block_tables.size(1), stride}, {"free_count", cp, 1, 1, 0}},
+                {{"new_lens", np, 1, n, 0}, {"offsets", op, 1, n + 1, 0}, {"free_blocks", fp, 1, free_blocks.numel(), 0},
+                 {"index", ip, 1, ip ? rows : 0, 0}});
   at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
   at::Tensor slots = at::empty({rows}, lens.options().dtype(at::kLong)), status = at::empty({n}, lens.options());
   void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
@@ -387,6 +419,11 @@ void truncate_blocks(const at::Tensor& lens, const at::Tensor& keep, const at::T
   int32_t* tp = table(block_tables, n, dev, what, stride);
   int32_t* fp = ints_out(free_blocks, -1, dev, what, "free_blocks");
   int32_t* cp = ints_out(free_count, 1, dev, what, "free_count");
+  if (n <= kMaxRequests)  // (keep may be lens itself: nothing to shorten)
+    check_apart(what,
+                {{"lens", lp, 1, n, 0}, {"block_tables", tp, n, block_tables.size(1), stride},
+                 {"free_blocks", fp, 1, free_blocks.numel(), 0}, {"free_count", cp, 1, 1, 0}},
+                {{"keep", kp, 1, kp == lp ? 0 : n, 0}});
   at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
   void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
   check_rc(pgs_truncate_blocks(lp, kp, tp, stride, block_tables.size(1), fp, free_blocks.numel(), cp, block_size, n, st),

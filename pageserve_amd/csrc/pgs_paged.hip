@@ -129,8 +129,10 @@ __global__ __launch_bounds__(kScanThreads) void append_kernel(Tables t, const in
         const int64_t n = rw.index ? rw.index[i] : i - first;
         if (i >= first && n >= 0 && n < max(add[b], 0)) {
           const int64_t pos = old[b] + n;
-          const int blk = static_cast<int>(pos / t.bs), have = static_cast<int>((static_cast<int64_t>(old[b]) + t.bs - 1) / t.bs);
-          const int32_t id = blk < have ? t.tables[b * t.stride + blk] : t.free[c0 - 1 - (start[b] + blk - have)];
+          const int64_t blk = pos / t.bs, have = (static_cast<int64_t>(old[b]) + t.bs - 1) / t.bs;
+          // (new_lens is read again here: whatever it holds by now, no entry that was not taken)
+          const int64_t e = start[b] + blk - have;
+          const int32_t id = blk < have ? t.tables[b * t.stride + blk] : e < used ? t.free[c0 - 1 - e] : -1;
           if (id >= 0) slot = static_cast<int64_t>(id) * t.bs + pos % t.bs;
         }
       }
@@ -154,7 +156,7 @@ __global__ __launch_bounds__(kRowThreads) void slots_kernel(Tables t, const int3
     const int64_t n = rw.index ? rw.index[i] : i - first, more = max(add[b], 0);
     if (i >= first && n >= 0 && n < more) {
       const int64_t pos = t.lens[b] - more + n;
-      const int32_t id = t.tables[b * t.stride + pos / t.bs];
+      const int32_t id = pos >= 0 ? t.tables[b * t.stride + pos / t.bs] : -1;  // (as in append_kernel)
       if (id >= 0) slot = static_cast<int64_t>(id) * t.bs + pos % t.bs;
     }
   }

@@ -63,7 +63,8 @@ def append_blocks(lens: torch.Tensor, new_lens: torch.Tensor, offsets: torch.Ten
     All tensors int32 and on one GPU: ``lens`` and ``new_lens`` [requests],
     ``offsets`` [requests + 1], ``block_tables`` [requests, columns],
     ``free_blocks`` [any], ``free_count`` [1], ``index`` [rows].  At most 4096
-    requests per call."""
+    requests per call.  Those that are changed may be parts of one buffer, but
+    share no element with one another nor with those that are read."""
     slots, status = _native.load_host().append_blocks(lens, new_lens, offsets, block_tables, free_blocks, free_count,
                                                       block_size, rows, index)
     return slots, status

@@ -155,6 +155,36 @@ def test_wrong_offsets_stay_inside(gpu):
     assert slots.numel() == 6 and ((slots >= -1) & (slots < 16)).all()
 
 
+def test_arrays_that_share_memory_are_refused(gpu):
+    """What a call writes shares no element with its other arrays; parts of one buffer,
+    between a table's rows too, are fine."""
+    buf = torch.zeros(200, dtype=torch.int32, device=gpu)
+    table = buf[100:148].view(4, 12)[:, :5]  # rows of 5, 12 apart
+    good = dict(lens=buf[:4], new_lens=buf[4:8], offsets=buf[8:13], block_tables=table, free_blocks=buf[20:40],
+                free_count=buf[40:41], block_size=16, rows=3, index=buf[41:44])
+    append_blocks(**good)
+    append_blocks(**{**good, "lens": buf[105:109], "new_lens": buf[117:121], "free_blocks": buf[129:136]})
+    for kw in (dict(new_lens=buf[:4]), dict(new_lens=buf[3:7]), dict(offsets=buf[2:7]), dict(index=buf[3:6]),
+               dict(free_blocks=buf[:4]), dict(free_count=buf[1:2]), dict(lens=buf[100:104]), dict(lens=buf[97:101]),
+               dict(lens=buf[109:113]), dict(new_lens=buf[116:120]), dict(offsets=buf[136:141]),
+               dict(offsets=buf[140:145]), dict(free_blocks=buf[90:190]), dict(free_blocks=buf[105:125]),
+               dict(index=buf[40:43])):
+        with pytest.raises(ValueError, match="share memory"):
+            append_blocks(**{**good, **kw})
+    keep = dict(lens=buf[:4], keep=buf[4:8], block_tables=table, free_blocks=buf[20:40], free_count=buf[40:41], block_size=16)
+    truncate_blocks(**keep)
+    truncate_blocks(**{**keep, "keep": buf[:4]})
+    for kw in (dict(keep=buf[1:5]), dict(keep=buf[101:105]), dict(free_blocks=buf[:20]), dict(free_blocks=buf[40:50]),
+               dict(free_count=buf[112:113]), dict(lens=buf[20:24]), dict(keep=buf[38:42])):
+        with pytest.raises(ValueError, match="share memory"):
+            truncate_blocks(**{**keep, **kw})
+    # tables of one row and of one column
+    one = dict(good, lens=buf[:1], new_lens=buf[1:2], offsets=buf[2:4], block_tables=buf[4:9].view(1, 5))
+    append_blocks(**one)
+    with pytest.raises(ValueError, match="share memory"):
+        append_blocks(**{**one, "index": buf[8:11]})
+
+
 def test_append_replayed_with_other_lengths(gpu):
     s = _State(gpu, [3, 20, 0], 8, 4, spare=18)
     new, offsets = _i32([0, 0, 0], gpu), _i32([0, 0, 0, 0], gpu)
