@@ -561,7 +561,8 @@ typedef struct pgs_kv_cache {
  * Rows i of k and v (bf16 or fp16 [rows, kv_heads, head_dim], element strides
  * of row and head given) into slot slots[i] of the cache; a slot outside the
  * cache is left out.  The slots of the rows must differ: of two rows with one
- * slot, either may stay.
+ * slot, either may stay.  The rows must not lie in the cache, nor two of its
+ * elements in one place.
  */
 int pgs_write_kv(const void* k, int64_t k_row, int64_t k_head, const void* v,
                  int64_t v_row, int64_t v_head, const pgs_kv_cache* cache,

@@ -16,6 +16,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <initializer_list>
 #include <string>
@@ -259,13 +260,17 @@ at::Tensor dequantize4(const at::Tensor& qp, const at::Tensor& sp, int64_t n, in
   return out;
 }
 
-// whether the memory of contiguous `o` and of `t` can overlap
-bool overlap(const at::Tensor& o, const at::Tensor& t) {
-  if (!o.numel() || !t.numel()) return false;
+// bytes from a tensor's first element to the end of its last
+int64_t extent(const at::Tensor& t) {
   int64_t last = 0;
   for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  return (last + 1) * t.element_size();
+}
+// whether the memory of `o` and of `t` can overlap
+bool overlap(const at::Tensor& o, const at::Tensor& t) {
+  if (!o.numel() || !t.numel()) return false;
   const char *a = static_cast<const char*>(o.data_ptr()), *b = static_cast<const char*>(t.data_ptr());
-  return a < b + (last + 1) * t.element_size() && b < a + o.numel() * o.element_size();
+  return a < b + extent(t) && b < a + extent(o);
 }
 
 at::Tensor linear4(const at::Tensor& x, const at::Tensor& qp, const at::Tensor& sp, const Opt& bias, int64_t n,
@@ -467,6 +472,20 @@ at::Tensor check_rows(const at::Tensor& t, int64_t rows, int64_t heads, const at
   return t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t;
 }
 
+// every element of a cache that is written has a place of its own: each step is past all
+// that the smaller ones span
+void check_places(const at::Tensor& c, const char* what, const char* name) {
+  std::array<int64_t, 4> order{0, 1, 2, 3};
+  std::sort(order.begin(), order.end(), [&](int64_t a, int64_t b) { return c.stride(a) < c.stride(b); });
+  int64_t span = 1;
+  for (int64_t d : order) {
+    if (c.size(d) < 2) continue;
+    if (c.stride(d) < span)
+      value_error(std::string(what) + ": " + name + " must not overlap itself (strides of its dimensions)");
+    span += (c.size(d) - 1) * c.stride(d);
+  }
+}
+
 void write_kv(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
               const at::Tensor& slots) {
   const char* what = "write_kv";
@@ -477,6 +496,11 @@ void write_kv(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cach
   at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
   at::Tensor kr = check_rows(k, rows, c.kv_heads, k_cache, what, "k");
   at::Tensor vr = check_rows(v, rows, c.kv_heads, k_cache, what, "v");
+  check_places(k_cache, what, "k_cache");
+  check_places(v_cache, what, "v_cache");
+  // rows of the cache itself (moved to other slots) are read before any is written
+  if (overlap(kr, k_cache) || overlap(kr, v_cache)) kr = kr.clone();
+  if (overlap(vr, k_cache) || overlap(vr, v_cache)) vr = vr.clone();
   if (slots.device() != dev)
     value_error("write_kv: slots on " + dev_str(slots.device()) + " but the cache is on " + dev_str(dev));
   if (slots.scalar_type() != at::kLong) type_error("write_kv: slots must be int64");

@@ -87,7 +87,10 @@ def write_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     for a whole batch).  A row whose slot (int64) is outside the cache, as -1 is,
     is left out.  No two rows may have the same slot (:func:`append_blocks` gives
     none twice, unless ``index`` names a token twice): of two that do, pieces of
-    either may stay.  bf16 or fp16, the rows in any strides whose last is 1."""
+    either may stay.  Rows that are views of the caches themselves are copied
+    first, so rows can be moved to other slots, also of one another.  bf16 or fp16,
+    the rows in any strides whose last is 1; no two elements of a cache may share a
+    place (an expanded one is refused)."""
     _native.load_host().write_kv(k, v, k_cache, v_cache, slots)
 
 

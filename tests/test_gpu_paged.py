@@ -243,6 +243,43 @@ def test_write_kv(gpu, rows, heads, dim, bs, dtype):
     assert torch.equal(c.cpu(), want)
 
 
+@pytest.mark.parametrize("dim", [64, 20])  # 16-byte pieces, single elements
+def test_rows_moved_within_the_cache(gpu, dim):
+    base = torch.randn(2, 300, 16, 2, dim, generator=torch.Generator().manual_seed(dim)).bfloat16()
+    slots = torch.randperm(4800, generator=torch.Generator().manual_seed(1))
+    slots[::7] = -1
+    shift = torch.arange(1, 4801)  # every row to its neighbour's place, the last one out
+    for s in (slots, shift):
+        c = base.to(gpu)
+        rows = c.flatten(1, 2)
+        write_kv(rows[0], rows[1], c[0], c[1], s.to(gpu))
+        want = base.clone()
+        _reference_write(base[0].flatten(0, 1), base[1].flatten(0, 1), want[0], want[1], s)
+        assert torch.equal(c.cpu(), want)
+    # keys from the value cache and values from the key cache
+    c = base.to(gpu)
+    rows = c.flatten(1, 2)
+    write_kv(rows[1, :40], rows[0, 8:48], c[0], c[1], shift[:40].to(gpu))
+    want = base.clone()
+    _reference_write(base[1].flatten(0, 1)[:40], base[0].flatten(0, 1)[8:48], want[0], want[1], shift[:40])
+    assert torch.equal(c.cpu(), want)
+
+
+def test_caches_that_overlap_themselves_are_refused(gpu):
+    c = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16, device=gpu)
+    k, s = torch.ones(3, 2, 64, dtype=torch.bfloat16, device=gpu), torch.arange(3, device=gpu)
+    for bad in (c[:1].expand(4, 16, 2, 64), c[:, :1].expand(4, 16, 2, 64), c[:, :, :1].expand(4, 16, 2, 64),
+                c.view(-1).as_strided((4, 16, 2, 64), (1024, 128, 64, 1))):
+        for pair in ((bad, c), (c, bad)):
+            with pytest.raises(ValueError, match="overlap itself"):
+                write_kv(k, k, *pair, s)
+    assert not c.any()
+    # one block, one slot, one head: a step of any size
+    one = c[:1, :1, :1].expand(1, 1, 1, 64)
+    write_kv(k[:1, :1], k[:1, :1], one, one, s[:1])
+    assert c.sum() == 64
+
+
 def test_write_past_four_gigabytes(gpu):
     c = torch.empty(40000, 64, 8, 128, dtype=torch.bfloat16, device=gpu)  # 5.2 GB
     k = torch.randn(3, 8, 128, device=gpu).bfloat16()
