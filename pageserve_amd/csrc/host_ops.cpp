@@ -296,6 +296,8 @@ at::Tensor linear4(const at::Tensor& x, const at::Tensor& qp, const at::Tensor& 
       value_error("linear4: out must be a contiguous " + std::string(c10::toString(odt)) + " tensor of " +
                   std::to_string(m * n) + " elements on " + dev_str(dev));
     if (overlap(o, x2)) value_error("linear4: out must not share memory with the input");
+    if ((b.defined() && overlap(o, b)) || overlap(o, qp) || overlap(o, sp))
+      value_error("linear4: out must not share memory with the weight or the bias");
     y = o.view({m, n});
   } else {
     y = at::empty({m, n}, x2.options().dtype(odt));

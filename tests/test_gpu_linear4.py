@@ -218,3 +218,17 @@ def test_refusals(gpu):
     with pytest.raises(ValueError, match="residual itself"):
         linear4(xt, qw, residual=room[:64].view(2, 32), out=room[:128].view(torch.float32).view(2, 32),
                 out_dtype=torch.float32)
+
+
+def test_out_in_the_weight_or_the_bias_is_refused(gpu):
+    qw, _, x = _case(gpu, 1, 64, 64, 32)
+    xt = bf16_gpu(x, gpu)
+    room = torch.zeros(200, dtype=torch.bfloat16, device=gpu)
+    codes = qw.qp.clone()
+    for kw in (dict(bias=room[:64], out=room[32:96].view(1, 64)), dict(out=qw.qp.view(torch.bfloat16)[64:128].view(1, 64)),
+               dict(out=qw.sp[8:72].view(1, 64)), dict(out=qw.sp[:128].view(torch.float32).view(1, 64), out_dtype=torch.float32)):
+        with pytest.raises(ValueError, match="weight or the bias"):
+            linear4(xt, qw, **kw)
+    assert torch.equal(qw.qp, codes)
+    y = linear4(xt, qw, bias=room[:64], out=room[64:128].view(1, 64))
+    assert torch.equal(y, linear4(xt, qw))
