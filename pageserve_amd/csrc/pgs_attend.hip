@@ -118,6 +118,8 @@ struct Elem<false> {
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
   static __device__ __forceinline__ float low(uint32_t v) { return __uint_as_float(v << 16); }
   static constexpr uint32_t kOnes = 0x3f803f80u, kExp = 0x7f80u;  // 1.0 twice; the exponent's bits
+  // A reference is this much (in powers of two) below the maximum that it is taken from.
+  static constexpr float kHead = 0.f;
 };
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -134,6 +136,10 @@ struct Elem<true> {
     return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(v)));
   }
   static constexpr uint32_t kOnes = 0x3c003c00u, kExp = 0x7c00u;
+  // fp16 has no steps finer than 2^-24: of a key far above n others, weights of 2^-25 of its
+  // own were lost, n 2^-25 of the sum.  With the largest at 2^7 to 2^15 (kSlack; the type ends at 2^16)
+  // that is n 2^-32.
+  static constexpr float kHead = 7.f;
 };
 
 // the maximum over lanes l, l ^ 16, l ^ 32, l ^ 48 (each swap leaves the two halves
@@ -149,9 +155,8 @@ __device__ __forceinline__ float quad_max(float v) {
 // A maximum nothing has raised yet: the lowest value that is finite.
 constexpr float kLow = -3.402823466e38f;
 // The reference of the exponents follows the maximum only when a score exceeds it
-// by this (in powers of two): p stays below 2^8, in range for fp16 and as exact in
-// either type as below 1, and the sums are rescaled a few times per row instead of
-// at every step.
+// by this (in powers of two) and Elem::kHead: p stays below 2^8 times 2^kHead, as exact as
+// below 1, and the sums are rescaled a few times per row instead of at every step.
 constexpr float kSlack = 8.0f;
 // A reference is a rounded product c s, and fma(s, c, -reference) sees that rounding: up to
 // half a step of the reference, which the largest weight is off by (as a power of two; all
@@ -304,7 +309,7 @@ struct Wave {
           const bool in = key < limit && !(e >> 2 ? bad1 : bad0) && (sees >> (key & 63) & 1);
           ok[r] |= in ? 1u << e : 0;
           x[r][e] = in ? exponent(s[r][e >> 2][e & 3], a.c, mx[r], far) : -INFINITY;
-          over = over || x[r][e] > kSlack;
+          over = over || x[r][e] > kSlack + E::kHead;
         }
       }
     } else {
@@ -317,7 +322,7 @@ struct Wave {
           x[r][e] = fmaf(s[r][e >> 2][e & 3], a.c, -mx[r]);
           top = fmaxf(top, x[r][e]);
         }
-        over = over || top > kSlack;
+        over = over || top > kSlack + E::kHead;
       }
     }
     if (__ballot(over)) {
@@ -328,7 +333,8 @@ struct Wave {
         float t = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 8; ++e) t = fmaxf(t, ok[r] >> e & 1 ? s[r][e >> 2][e & 3] * a.c : -INFINITY);
-        const float ref = fmaxf(quad_max(t), mx[r]), f = __builtin_amdgcn_exp2f(mx[r] - ref);
+        t = quad_max(t);
+        const float ref = fmaxf(fabsf(t) > kFar ? t : t - E::kHead, mx[r]), f = __builtin_amdgcn_exp2f(mx[r] - ref);
         mx[r] = ref;
         beyond = beyond || fabsf(ref) > kFar;
 #pragma unroll

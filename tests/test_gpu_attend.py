@@ -182,6 +182,38 @@ def test_large_scores_of_one_key(gpu, heads, lens, tokens, most, dtype, powers):
                     assert ((got - mean).abs() <= U[dtype] * mean.abs() + 2.0 ** -22).all(), (power, "twice")
 
 
+@pytest.mark.parametrize("heads,requests,tokens", [("one", 1100, 1), ("one", 300, 33), ("3b", 140, 8)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_small_weights_beside_a_large_one(gpu, heads, requests, tokens, dtype):
+    """A first key at score 0 whose values are 0, 16383 more at 2^-x of its weight with
+    values 1: out = n 2^-x / (1 + n 2^-x).  Weights are rounded by half a step of the type, u,
+    fp16's no finer than 2^-32 of the largest; sums, exponents and the reciprocal by 2^-12 at most
+    (16384 / 32 steps of 2^-23, and scores of at most 2^5 off by (D + 8) 2^-23 of that)."""
+    h, kv, dim = HEADS[heads]
+    n, bs = 16384, 64
+    i = dict(dtype=torch.int32, device=gpu)
+    tables = torch.arange(n // bs, **i).expand(requests, -1).contiguous()  # all read the same blocks
+    rows = requests * tokens
+    q = torch.zeros(rows, h, dim, dtype=dtype, device=gpu)
+    q[..., 0] = 1
+    kc, vc = (torch.zeros(n // bs, bs, kv, dim, dtype=dtype, device=gpu) for _ in range(2))
+    k, v = (torch.zeros(rows, kv, dim, dtype=dtype, device=gpu) for _ in range(2))
+    vc[:] = 1
+    vc[0, 0] = 0
+    offsets, lens = torch.arange(0, rows + 1, tokens, **i), torch.full((requests,), n, **i)
+    k[..., 0] = -60000.0  # (the drafted tokens: nothing)
+    for x in (20.5, 25.5, 27.25):
+        kc[..., 0] = -x
+        kc[0, 0, :, 0] = 0
+        out = tree_attention(q, k, v, kc, vc, tables, lens, offsets, max_tokens=tokens, max_context=n,
+                             scale=float(np.log(2.0)))
+        w = (n - 1) * 2.0 ** -x
+        want = w / (1 + w)
+        tol = want * (U[dtype] + 2.0 ** -12) + (n * 2.0 ** -32 if dtype is torch.float16 else 0)
+        tol += U[dtype] * (want + tol) + 2.0 ** -25
+        assert ((out.double() - want).abs() <= tol).all(), (x, want, out.double().min().item(), out.double().max().item())
+
+
 def test_padded_and_cut_batches(gpu):
     b = Batch(5, [40, 7, 0], [3, 70, 9], 16, 2, 128, 16, torch.float16, pad=6)
     out = torch.full(b.q.shape, 3.0, dtype=b.dtype, device=gpu)
