@@ -287,6 +287,41 @@ def test_what_is_not_seen_does_not_matter(gpu):
         clean.check(got, (out, want[1], want[2]), "the rest")
 
 
+@pytest.mark.parametrize("heads,tokens", [
+    # few rows in one tile, in two of a wave, in two waves; two tiles of drafted tokens; through LDS
+    ("0.5b", [2, 2, 1]), ("0.5b", [4, 4, 3]), ("0.5b", [9, 6, 7]), ("one", [6, 40, 34]), ("0.5b", [6, 40, 34]),
+    ("3b", [2, 2, 1]), ("3b", [4, 3, 4]), ("3b", [8, 6, 7]), ("each", [6, 40, 34]), ("wide", [6, 40, 34])])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_what_is_not_seen_does_not_matter_to_any_kernel(gpu, heads, tokens, dtype):
+    h, kv, dim = HEADS[heads]
+    lens, last = [37, 0, 20], dim - 9
+    b, clean = (Batch(17, lens, tokens, h, kv, dim, 16, dtype) for _ in range(2))
+    used = {int(x) for x in b.tables.ravel() if x >= 0}
+    for c in (b.kc, b.vc):
+        for blk in set(range(c.shape[0])) - used:
+            c[blk] = float("nan")
+        c[int(b.tables[0, 2]), 5:] = float("inf")
+        c[int(b.tables[2, 1]), 4:] = float("nan")
+    for row, value in ((0, float("nan")), (b.offsets[1] + 1, float("inf")), (b.offsets[2] - 1, -float("inf"))):
+        b.v[row, :, 3:last] = value
+    want = clean.oracle()
+    got = tree_attention(*b.args(gpu), max_tokens=max(tokens)).cpu()
+    for r in range(3):
+        lo, hi = b.offsets[r], b.offsets[r + 1]
+        see = D.ancestors(b.parents[lo:hi].tolist())
+        for t in range(hi - lo):
+            hit = [lo + j for j in see[t] if not torch.isfinite(b.v[lo + j]).all()]
+            touched = torch.zeros(dim, dtype=torch.bool)
+            touched[3:last] = bool(hit)
+            assert torch.equal(~torch.isfinite(got[lo + t]), touched.expand(h, dim)), (r, t)
+            if len(hit) == 1:
+                assert torch.equal(torch.nan_to_num(got[lo + t, 0, 3:last].float(), nan=7.0),
+                                   torch.nan_to_num(b.v[hit[0], 0, 3:last].float(), nan=7.0))
+    rest = torch.isfinite(got)
+    clean.check(torch.where(rest, got, 0), (np.where(rest.numpy(), want[0], 0), *want[1:]), "the rest")
+
+
+
 def test_layouts_and_copies(gpu):
     b = Batch(8, [70, 20, 130], [3, 8, 1], 16, 2, 128, 16, torch.bfloat16)
     args = b.args(gpu)
@@ -328,6 +363,22 @@ def test_cache_past_four_gigabytes(gpu):
         c[shift:] = a
     got = tree_attention(*args[:3], *big, torch.where(args[5] >= 0, args[5] + shift, -1), *args[6:])
     assert torch.equal(got, tree_attention(*args))
+
+
+@pytest.mark.parametrize("heads,tokens", [("each", [1, 1]), ("3b", [4, 1]), ("0.5b", [9, 2]), ("3b", [40, 3])])
+def test_cache_past_four_gigabytes_in_every_kernel(gpu, heads, tokens):
+    h, kv, dim = HEADS[heads]
+    b = Batch(19, [100, 37], tokens, h, kv, dim, 64, torch.bfloat16)
+    args = b.args(gpu)
+    blocks = (5 << 30) // (64 * kv * dim * 2)
+    big = [torch.empty(blocks, 64, kv, dim, dtype=b.dtype, device=gpu) for _ in range(2)]  # 5 GiB each
+    shift = blocks - b.kc.shape[0]
+    for c, a in zip(big, args[3:5]):
+        c[shift:] = a
+    got = tree_attention(*args[:3], *big, torch.where(args[5] >= 0, args[5] + shift, -1), *args[6:], max_tokens=max(tokens))
+    assert torch.equal(got, tree_attention(*args, max_tokens=max(tokens)))
+    b.check(got, b.oracle())
+
 
 
 def test_captured_and_replayed_with_other_lengths(gpu):
@@ -385,6 +436,27 @@ def test_many_small_requests(gpu, requests, tokens, heads):
     b = Batch(32, rng.integers(0, 300, requests).tolist(), rng.integers(0, tokens + 1, requests).tolist(),
               *HEADS[heads], 16, torch.bfloat16)
     b.check(tree_attention(*b.args(gpu), max_tokens=tokens), b.oracle())
+
+
+@pytest.mark.parametrize("requests,every,heads,long", [(600, 5, "one", (550,)), (1100, 9, "odd", (0, 700, 1060)),
+                                                      (1100, 30, "wide", (511, 1024))])
+def test_many_requests_through_lds(gpu, requests, every, heads, long):
+    """More requests than the prefix sums take at a time (512), most of them without tokens, some
+    of 40 and long ones on both sides of the bounds: their units are cut into shares and joined."""
+    rng = np.random.default_rng(requests + every)
+    tokens = np.where(np.arange(requests) % every == 3, rng.integers(0, 41, requests), 0)
+    lens = rng.integers(0, 120, requests)
+    lens[rng.random(requests) < 0.1] = 0
+    for r in long:
+        tokens[r], lens[r] = 37, 5000
+    b = Batch(60, lens.tolist(), tokens.tolist(), *HEADS[heads], 16, torch.bfloat16)
+    want = b.oracle()
+    args = b.args(gpu)
+    got = tree_attention(*args, max_tokens=40, max_context=5000)
+    b.check(got, want)
+    for _ in range(2):
+        assert torch.equal(tree_attention(*args, max_tokens=40, max_context=5000), got)
+
 
 
 @pytest.mark.parametrize("lens,tokens", [([300], [7]), ([5000, 20], [64, 5])])
