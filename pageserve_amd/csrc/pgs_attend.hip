@@ -21,10 +21,11 @@
 //                   D/16 piece in its registers; MFMA i covers the dims
 //                   (l%16) D/16 + i.
 //
-// The row sums come from one more MFMA per step with ones as A, i.e. they add the
-// rounded p that the output uses.  Keys and values go from memory straight to
-// registers.  block_size is a multiple of 16, so a 16-key half lies in one block: its
-// address is wave-uniform.
+// P is rounded to the tensors' type for that product (in two terms it would take twice the
+// MFMAs, which bound the kernel for many rows), and the row sums, one more MFMA per step with
+// ones as A, add the rounded p that the output uses: a weight is off by half a step of the
+// type at most, the output by 1.3 to 1.4 times what it is with P in fp32.  block_size is a
+// multiple of 16, so a 16-key half lies in one block: its address is wave-uniform.
 //
 // Work: (request, key head, row group, part of the keys).  A workgroup's waves are
 // row tiles x key slices, joined in LDS; parts are joined by a second kernel from
@@ -70,8 +71,7 @@ __device__ __forceinline__ int here(int lane) {
   return lane;
 }
 
-// Four keys x 16 dims per 16 lanes from LDS, transposed: lane i of them gives the address
-// of dims 4 (i % 4) .. +3 of key i / 4 and gets dim i of the four keys.
+// LDS by its byte address
 template <typename T>
 __device__ __forceinline__ __attribute__((address_space(3))) T* lds(uint32_t address) {
   return reinterpret_cast<__attribute__((address_space(3))) T*>(address);
@@ -80,6 +80,8 @@ template <typename T>
 __device__ __forceinline__ uint32_t lds_address(T& v) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)&v));
 }
+// Four keys x 16 dims per 16 lanes from LDS, transposed: lane i of them gives the address
+// of dims 4 (i % 4) .. +3 of key i / 4 and gets dim i of the four keys.
 __device__ __forceinline__ u32x2 read_transposed(uint32_t address) {
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<s16x4>(address)));
@@ -649,6 +651,7 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
 // for its rows' loads and its sums: fitted to the workgroups' times (4.6, 2.8 and 10 us).  A
 // share has the tiles whose counts begin in it; of a unit that is not whole it leaves sums
 // in slot 2 g (the unit began in an earlier share) or 2 g + 1.
+// (all at 128 dims; 64 dims use the same.)
 constexpr int kFull = 10, kHalf = 6, kUnit = 20;
 constexpr int kShares = 256;      // workgroups: one per CU
 static_assert(kHalf <= kFull);
@@ -657,18 +660,17 @@ constexpr int kWideRows = 2;      // row tiles of 16 per wave
 constexpr int kWideWaves = 16 / kWideRows;
 constexpr int kGroup = 16 * kWideRows * kWideWaves;
 constexpr int kBuffers = 2;  // tiles in LDS: computed, on its way
-constexpr int tile_keys(int) { return 128; }
+constexpr int kTile = 128;   // keys of a tile
 
 struct Groups {
   int tiles, n;     // of a request: tiles per group, groups
   int last;         // weight of the last group (the others': kFull)
   int64_t per_head; // counts of one key head
 };
-template <int TK>
 __device__ __forceinline__ Groups groups_of(const Attend& a, const Request& rq) {
   const int rows = rq.tokens * a.group;
   Groups g;
-  g.tiles = (rq.len + TK - 1) / TK + (rq.tokens + TK - 1) / TK;
+  g.tiles = (rq.len + kTile - 1) / kTile + (rq.tokens + kTile - 1) / kTile;
   g.n = (rows + kGroup - 1) / kGroup;
   g.last = rows - (g.n - 1) * kGroup > kGroup / 2 ? kFull : kHalf;
   g.per_head = g.n ? static_cast<int64_t>(g.tiles) * (kFull * (g.n - 1) + g.last) + kUnit * g.n : 0;
@@ -681,7 +683,6 @@ __device__ __forceinline__ int shares_of(int64_t total) {
 // where share g of n begins
 __device__ __forceinline__ int64_t share_begin(int64_t total, int g, int n) { return g * total / n; }
 
-template <int TK>
 struct Work {
   static constexpr int NT = 64 * kWideWaves;
   Attend a;
@@ -701,7 +702,7 @@ struct Work {
     base = first;
     carry = before;
     int64_t v = 0;
-    if (first + thread < a.requests) v = groups_of<TK>(a, request(a, first + thread)).per_head * a.kv_heads;
+    if (first + thread < a.requests) v = groups_of(a, request(a, first + thread)).per_head * a.kv_heads;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int64_t o = __shfl_up(v, d);
@@ -739,14 +740,14 @@ struct Work {
     u.b = base + uniform(lo);
     const Request rq = request(a, u.b);
     u.rq = Request{uniform(rq.row0), uniform(rq.tokens), uniform(rq.len), 0, 0};
-    const Groups g = groups_of<TK>(a, u.rq);
+    const Groups g = groups_of(a, u.rq);
     const int64_t first = uniform64(lo ? pre[lo - 1] : carry);
     u.kh = uniform(static_cast<int>((pos - first) / g.per_head));
     const int64_t in = pos - first - u.kh * g.per_head;
     const int64_t full = static_cast<int64_t>(kFull) * g.tiles + kUnit;
     u.rg = uniform(static_cast<int>(min<int64_t>(in / full, g.n - 1)));
     u.tiles = g.tiles;
-    u.cached = (u.rq.len + TK - 1) / TK;
+    u.cached = (u.rq.len + kTile - 1) / kTile;
     u.weight = u.rg == g.n - 1 ? g.last : kFull;
     u.begin = first + u.kh * g.per_head + u.rg * full + kUnit;
     return u;
@@ -774,11 +775,11 @@ struct Work {
 // the next step's keys read during the softmax (and 131 for 123 across the barrier).
 template <int D, bool F16>
 __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_kernel(Attend a) {
-  constexpr int R = kWideRows, J = tile_keys(D) * D / 512 / kWideWaves;  // J: loads per wave, tile and matrix
+  constexpr int R = kWideRows, J = kTile * D / 512 / kWideWaves;  // J: loads per wave, tile and matrix
   using W = Wave<D, R, F16, false>;
   using E = Elem<F16>;
   constexpr int DV = W::DV;
-  constexpr int NW = kWideWaves, TK = tile_keys(D);
+  constexpr int NW = kWideWaves, TK = kTile;
   constexpr int P = D / 8;           // pieces per row
   constexpr int KI = 64 / P;         // keys of one wave-wide load
   constexpr int KW = J * KI;         // keys of a wave's loads
@@ -796,7 +797,7 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
   const uint32_t k_at = lds_address(lkv) + li * (2 * D) + 16 * (lg ^ (li * P / 16 & (P - 1)));
   const uint32_t v_at = lds_address(lkv) + TK * D * 2 + vkey * (2 * D) +
                         16 * ((li >> 1 & 1) ^ (2 * (vkey * P / 16) & (P - 1))) + 8 * (li & 1);
-  Work<TK> work{again(), lpre, lsum, 0, 0, 0};
+  Work work{again(), lpre, lsum, 0, 0, 0};
   work.start(blockIdx.x == 0 ? work.a.sums : nullptr);
   const int shares = shares_of(work.total), share = xcd_remap(blockIdx.x, gridDim.x);
   if (share >= shares) return;
@@ -805,7 +806,7 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
 
   for (int64_t pos = begin; pos < end;) {
     work.a = again();
-    const typename Work<TK>::Unit un = work.find(pos);
+    const Work::Unit un = work.find(pos);
     const Request& rq = un.rq;
     const int nrows = rq.tokens * a.group;
     const int slices = un.weight == kHalf ? 2 : 1;  // of the keys
@@ -1121,7 +1122,7 @@ __global__ __launch_bounds__(join_threads(WAVES)) void join_wide_kernel(Attend a
   const Request rq = request(a, b);
   const int rows = rq.tokens * a.group;
   if (first >= rows) return;
-  const Groups g = groups_of<tile_keys(D)>(a, rq);
+  const Groups g = groups_of(a, rq);
   const int64_t total = a.sums[a.requests - 1];
   const int n = shares_of(total), rg = first / kGroup;
   // the unit's first and last tile, and their shares: the largest that begin by then
