@@ -524,7 +524,8 @@ int pgs_w4a16_linear(const void* x, const void* qp, const void* sp,
  * slots[i], i < rows: the slot (block * block_size + place in the block) of row
  * i of the batch: token lens[b] (before the call) + n of its request, where n =
  * index[i], or i - offsets[b] without an index; -1 if n is not in
- * 0..new_lens[b]-1, the request was not served, or the row belongs to none.
+ * 0..new_lens[b]-1, the request was not served, the row belongs to none, or the
+ * table's column for it (an older one) holds a negative number.
  * No array that is written (here and in pgs_truncate_blocks) may share memory
  * with another.
  */
@@ -536,7 +537,7 @@ int pgs_append_blocks(int32_t* lens, const int32_t* new_lens, int32_t* block_tab
 
 /*
  * Shortens each request to keep[b] tokens (0: it is finished; a count above its
- * length keeps all): blocks no longer needed go back to the stack, their table
+ * length keeps all; a negative length becomes 0): blocks no longer needed go back to the stack, their table
  * columns become -1.  Undoes pgs_append_blocks exactly.  A column that holds a
  * negative number names no block and gives none back; other numbers are not
  * checked (nothing here says how many blocks there are).  Blocks beyond the
@@ -596,9 +597,10 @@ typedef struct pgs_tree_attention_args {
  * trees.  Query heads share key heads in groups of q_heads / kv_heads.
  *   out = sum_j softmax_j(scale * q . k_j) v_j     (softmax in fp32)
  * head_dim 64 or 128; block_size a multiple of 16, columns * block_size at most
- * 2^31 - 65536; strides multiples of 8 elements and pointers 16-byte aligned.  Lengths beyond the table's columns
- * are cut to them; tokens in a block outside the cache are left out; rows of no
- * request, and a request's rows from max_tokens on, are not written.
+ * 2^31 - 65536; strides multiples of 8 elements and pointers 16-byte aligned.
+ * Lengths beyond the table's columns are cut to them; tokens in a block outside
+ * the cache are left out; rows of no request, and a request's rows from max_tokens
+ * on, are not written.
  * workspace: pgs_tree_attention_workspace_bytes() bytes, 256-byte aligned, no
  * fill needed.
  */

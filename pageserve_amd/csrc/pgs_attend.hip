@@ -445,11 +445,12 @@ __device__ __forceinline__ int parts_of(const Attend& a, const Request& rq, int 
 }
 
 // Few rows (up to 64 per key head): bound by reading the keys and values once, and for
-// short contexts by the chain of loads (lengths, block numbers, keys).  A workgroup's NW
-// waves are WR row tiles x NW/WR key slices; each wave loads the keys of its steps straight
-// into registers.  Measured, 16 heads on two key heads of 128 dims: one token of 256
-// requests of 512 keys 26.6 us (5.0 TB/s of keys and values), of 64 of 2048 29.2 (4.6), of
-// one of 32768 with the join 16.6 (2.0); 4 tokens of 64 of 2048 32.4 (4.2).
+// short contexts by the chain of loads (lengths, block numbers, and a round of keys per step:
+// only the next step's block numbers are loaded ahead).  A workgroup's NW waves are WR row
+// tiles x NW/WR key slices; each wave loads the keys of its steps straight into registers.
+// Measured in a replayed graph, 16 heads on two key heads of 128 dims: one token of 256
+// requests of 512 keys 26.2 us (5.1 TB/s of keys and values), of 64 of 2048 29.1 (4.6), of
+// one of 32768 with the join 17.9 (1.9); 4 tokens of 64 of 2048 32.0 (4.2).
 template <int D, int R, int WR, int NW, bool F16>
 __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(Attend a) {
   using W = Wave<D, R, F16, true>;
@@ -767,8 +768,8 @@ struct Work {
 // (ds_read_b64_tr_b16: lane n gets dim n of the four keys), a pair of pieces of 16 keys per
 // access: they are exchanged in pairs, p ^ 2 (r D / 128).
 //
-// Measured at 24 requests of up to 64 rows x 16 heads of 128 dims: 109 us, a full tile (256
-// rows x 128 keys) 4.6 us, 40% of the matrix units' rate: a step's scores, softmax and
+// Measured at 24 requests of up to 64 rows x 16 heads of 128 dims: 105 us with the join
+// (106 to 114 and 9 in a trace of few calls), a full tile (256 rows x 128 keys) 4.6 us, 40% of the matrix units' rate: a step's scores, softmax and
 // output follow one another in a wave, and the second wave of a SIMD covers a part of it.
 // Tiles through registers 133, of 64 keys 121.  The same: four waves per SIMD of 16 rows
 // each, a higher priority for half of the waves, half of them starting a tile later (116),

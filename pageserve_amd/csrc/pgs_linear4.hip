@@ -12,10 +12,13 @@
 // its NW waves take 128-column chunks round robin, U per batch, a batch's loads issued
 // together, and the waves' partial tiles meet in LDS in a fixed order.
 //
-// Measured (weights not in any cache): 1 x 151936 x 2048, groups of 128, 30 us, 5.3 TB/s of
-// codes and scales; 30 tokens, groups of 32, 61 us: each wave loads the tokens' values for
-// its four tiles, twice the bytes of their codes, from L2, and scales eight products a tile.
-// 1 x 11008 x 2048 5.1 us, 5 x 2048 x 11008 6.7 us: a launch and the first loads' latency.
+// Measured in a replayed graph, weights in no cache: 1 x 151936 x 2048, groups of 128, 29 us,
+// 5.5 TB/s of codes and scales; 30 tokens, groups of 32, 59 us: each wave loads the tokens'
+// values for its four tiles, twice the bytes of their codes, from L2, and scales eight products
+// a tile; 60 tokens 110 us, groups of 128 98: four times the bytes of the codes.  Nothing is on
+// its way while a batch is multiplied: 1 x 11008 x 2048 5.1 us, a launch and two rounds of loads
+// (16 chunks on eight waves); 5 x 2048 x 11008 6.6 us, three rounds (43 pairs of chunks,
+// sixteen a round).
 #include "pgs_fp4.h"
 
 namespace pgs {
@@ -39,7 +42,7 @@ constexpr int kNowhere = 0x40000000;  // a lane offset past every resource (the 
 // The tokens are the A operand and the weights the B operand: lane l's four sums are of
 // weight row l%16, so it needs the scales of that row only.  (With the weights as A its
 // sums are of four rows: four times the scales to load and widen, 68 us for 62 at
-// 30 x 151936 x 2048 with groups of 32.)
+// 30 x 151936 x 2048 with groups of 32, when this was changed.)
 //
 // FOLD (m <= 8): a workgroup owns eight rows of a tile (half blockIdx.x % 2) and each MFMA
 // takes two chunks: A rows 0-7 are the tokens in chunk 2 c, A rows 8-15 the same tokens in
@@ -250,8 +253,9 @@ int launch(const Lin4& a, hipStream_t st) {
 }
 
 // (waves, chunks per batch: with fewer of either, too few loads are in flight at 11008 rows
-// and fewer: 30x11008x2048 8.7 for 9.7 with four waves; more registers do not hold.  Four
-// waves at 64 tokens: eight spill over two waves per SIMD, 101 us for 155 at 60x151936x2048.)
+// and fewer: 30x11008x2048 8.7 for 9.7 with four waves.  Registers, of 256: 66 with 16 tokens
+// and four tiles, where a second chunk would fit, up to 237 with 64.  Four waves there: eight
+// spill over two waves per SIMD, 101 us for 155 at 60x151936x2048.)
 template <int S, bool OUT_F32>
 int pick(const Plan& p, const Lin4& a, hipStream_t st) {
   if (p.wide == 0) return launch<8, 2, 1, 1, S, true, OUT_F32>(a, st);

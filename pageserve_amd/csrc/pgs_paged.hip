@@ -165,7 +165,8 @@ __global__ __launch_bounds__(kRowThreads) void slots_kernel(Tables t, const int3
 
 // Shortens requests.  Of the table entries given up (in request order, then column order)
 // those that name a block go to the stack, the last one first, so that append's lie where
-// it took them from; an entry below 0 names none and is not counted.
+// it took them from; an entry below 0 names none and is not counted.  Bound by latency:
+// append and truncate together 9.9 us for 64 requests of 16 blocks each, 19 for 1000 of 4, 79 of 32.
 __global__ __launch_bounds__(kScanThreads) void truncate_kernel(Tables t, const int32_t* __restrict__ keep) {
   extern __shared__ int32_t lds[];
   int32_t* start = lds;
@@ -318,7 +319,7 @@ extern "C" int pgs_append_blocks(int32_t* lens, const int32_t* new_lens, int32_t
   const Rows r{offsets, index, rows, slots};
   const size_t ints = 4 * static_cast<size_t>(requests);
   // One launch while the one workgroup is through the rows sooner than a second launch
-  // starts.  Measured with truncate_kernel behind it, microseconds one/two: 64 requests of
+  // starts.  Measured with a truncate behind each, microseconds one/two: 64 requests of
   // 256 rows in all 7.4/8.4, 2048 11.7/12.7, 4096 14.4/12.9, 16384 31.2/13.0.
   if (rows <= 2048) {
     hipLaunchKernelGGL(append_kernel<true>, dim3(1), dim3(kScanThreads), 3 * ints, st, t, new_lens, r, status);

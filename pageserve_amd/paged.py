@@ -57,8 +57,9 @@ def append_blocks(lens: torch.Tensor, new_lens: torch.Tensor, offsets: torch.Ten
     place in the block``, i.e. indexes ``k_cache.flatten(0, 1)``.  Row ``i`` of
     the batch is its request's ``n``-th new token, ``n = index[i]``, or ``i -
     offsets[b]`` without an index; its slot is -1 where ``n`` is not in
-    ``0 .. new_lens[b] - 1``, the request was not served or the row belongs to
-    none.  Rows of a request with the same index get the same slot.
+    ``0 .. new_lens[b] - 1``, the request was not served, the row belongs to
+    none or its block was absent (negative) in the table already.  Rows of a
+    request with the same index get the same slot.
 
     All tensors int32 and on one GPU: ``lens`` and ``new_lens`` [requests],
     ``offsets`` [requests + 1], ``block_tables`` [requests, columns],
@@ -73,7 +74,8 @@ def append_blocks(lens: torch.Tensor, new_lens: torch.Tensor, offsets: torch.Ten
 def truncate_blocks(lens: torch.Tensor, keep: torch.Tensor, block_tables: torch.Tensor, free_blocks: torch.Tensor,
                     free_count: torch.Tensor, block_size: int) -> None:
     """Shortens request ``b`` to ``keep[b]`` tokens, in place: 0 for one that is
-    finished, any count from its length on to leave it.  The blocks it no longer
+    finished, any count from its length on to leave it (a negative length becomes
+    0).  The blocks it no longer
     needs go back to the stack and their table columns become -1; a negative
     column (an absent block) gives nothing back.  Undoes :func:`append_blocks`
     exactly.  Tensors as there, ``keep`` int32 [requests]."""
@@ -113,9 +115,10 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     (rows, kv_heads, head_dim), q_heads a multiple of kv_heads; bf16 or fp16, as
     the caches; head_dim 64 or 128; the caches' block_size a multiple of 16.
     ``max_tokens`` bounds the rows of a request (1..64; a request's rows beyond it
-    are not computed), ``max_context`` its cached tokens: it sizes the split of
-    long contexts over the GPU, never the result (default: what the tables can
-    hold).  ``scale``: of q . k, head_dim ** -0.5 by default.
+    are not computed).  The kernels are chosen by it, or by the number of rows if
+    that is less: plain decoding of a batch gives 1.  ``max_context`` bounds its
+    cached tokens: it sizes the split of long contexts over the GPU, never the
+    result (default: what the tables can hold).  ``scale``: of q . k, head_dim ** -0.5 by default.
 
     Returns (rows, q_heads, head_dim), or writes to ``out`` (contiguous; it may be
     q itself).  Rows that belong to no request are not written: in a new tensor
