@@ -537,11 +537,11 @@ int pgs_append_blocks(int32_t* lens, const int32_t* new_lens, int32_t* block_tab
 
 /*
  * Shortens each request to keep[b] tokens (0: it is finished; a count above its
- * length keeps all; a negative length becomes 0): blocks no longer needed go back to the stack, their table
- * columns become -1.  Undoes pgs_append_blocks exactly.  A column that holds a
- * negative number names no block and gives none back; other numbers are not
- * checked (nothing here says how many blocks there are).  Blocks beyond the
- * stack's capacity are dropped.
+ * length keeps all; a negative length becomes 0): blocks no longer needed go back
+ * to the stack, their table columns become -1.  Undoes pgs_append_blocks exactly.
+ * A column that holds a negative number names no block and gives none back; other
+ * numbers are not checked (nothing here says how many blocks there are).  Blocks
+ * beyond the stack's capacity are dropped.
  */
 int pgs_truncate_blocks(int32_t* lens, const int32_t* keep, int32_t* block_tables,
                         int64_t table_stride, int64_t columns, int32_t* free_blocks,

@@ -138,8 +138,8 @@ struct Elem<true> {
     return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(v)));
   }
   static constexpr uint32_t kOnes = 0x3c003c00u, kExp = 0x7c00u;
-  // fp16 has no steps finer than 2^-24: of a key far above n others, weights of 2^-25 of its
-  // own were lost, n 2^-25 of the sum.  With the largest at 2^7 to 2^15 (kSlack; the type ends at 2^16)
+  // fp16 has no steps finer than 2^-24: beside a weight of 1, n others of up to 2^-25 would be
+  // lost, n 2^-25 of the sum.  With the largest at 2^7 to 2^15 (kSlack; the type ends at 2^16)
   // that is n 2^-32.
   static constexpr float kHead = 7.f;
 };
@@ -768,12 +768,13 @@ struct Work {
 // (ds_read_b64_tr_b16: lane n gets dim n of the four keys), a pair of pieces of 16 keys per
 // access: they are exchanged in pairs, p ^ 2 (r D / 128).
 //
-// Measured at 24 requests of up to 64 rows x 16 heads of 128 dims: 105 us with the join
-// (106 to 114 and 9 in a trace of few calls), a full tile (256 rows x 128 keys) 4.6 us, 40% of the matrix units' rate: a step's scores, softmax and
-// output follow one another in a wave, and the second wave of a SIMD covers a part of it.
-// Tiles through registers 133, of 64 keys 121.  The same: four waves per SIMD of 16 rows
-// each, a higher priority for half of the waves, half of them starting a tile later (116),
-// the next step's keys read during the softmax (and 131 for 123 across the barrier).
+// Measured at 24 requests of up to 64 rows x 16 heads of 128 dims: 105 us with the join (106 to
+// 114 and 9 in a trace of few calls), a full tile (256 rows x 128 keys) 4.6 us, 40% of the
+// matrix units' rate: a step's scores, softmax and output follow one another in a wave, and the
+// second wave of a SIMD covers a part of it.  Tiles through registers 133, of 64 keys 121.  The
+// same: four waves per SIMD of 16 rows each, a higher priority for half of the waves, half of
+// them starting a tile later (116), the next step's keys read during the softmax (and 131 for
+// 123 across the barrier).
 template <int D, bool F16>
 __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_kernel(Attend a) {
   constexpr int R = kWideRows, J = kTile * D / 512 / kWideWaves;  // J: loads per wave, tile and matrix
