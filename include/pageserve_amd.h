@@ -612,6 +612,147 @@ size_t pgs_tree_attention_workspace_bytes(int64_t rows, int64_t requests, int64_
                                           int64_t kv_heads, int64_t head_dim,
                                           int64_t max_tokens, int64_t max_context);
 
+/*
+ * ---------------------------------------------------------------------------
+ * Long texts in a bounded cache.  No counterpart in the reference, whose
+ * attention reads every cached token of a sequence in its own type
+ * (engine/paged_attention.py:16-50).
+ *
+ * Row t of a request of n rows and len cached tokens, the rows' own among them,
+ * stands at p = len - n + t and sees token j if
+ *   j <= p  and  (j > p - window  or  j < sinks)
+ * A window past every text (2^31 - 1) sees them all.
+ */
+
+/* A layer's keys and values in 4 bits, heads in front of slots, contiguous:
+ *   k, v              uint8 [blocks, kv_heads, block_size, head_dim / 2]
+ *   k_scale, v_scale  bf16 [blocks, kv_heads, block_size, head_dim / 32]
+ * Per 32 dims of a token and head one scale, max(absmax, 1e-8) / 6 cut to its
+ * first 6 significant bits, and a code per dim (the values and the rounding are
+ * those of the 4-bit weights above), so that value * scale is a bf16 number.  A
+ * group that holds an infinity or a NaN gets it as its scale, and its finite
+ * numbers codes 0.
+ * With C = head_dim / 32: byte 4 (C a + c) + i of a key's row (a, i < 4, c < C)
+ * holds dims 32 c + 8 a + 2 i (low half) and the next one.  Of 16 tokens' values,
+ * token 4 a + b has its dims m, 16 + m, 32 + m, ... (m < 16) in the C bytes from
+ * byte C (4 (16 a + m) + b) of the sixteen on, low halves first. */
+typedef struct pgs_kv_cache4 {
+  void* k;
+  void* k_scale;
+  void* v;
+  void* v_scale;
+  int64_t blocks, block_size, kv_heads, head_dim;
+} pgs_kv_cache4;
+
+/*
+ * Rows i of k and v (bf16 or fp16 [rows, kv_heads, head_dim], element strides of
+ * row and head given) in 4 bits into slot slots[i] of the cache; a slot outside
+ * the cache is left out.  The slots of the rows must differ (of two rows with one
+ * slot, pieces of either may stay).  head_dim 64 or 128, block_size a multiple
+ * of 16, the cache 16-byte aligned.
+ */
+int pgs_write_kv4(const void* k, int64_t k_row, int64_t k_head, const void* v,
+                  int64_t v_row, int64_t v_head, int dtype,
+                  const pgs_kv_cache4* cache, const int64_t* slots, int64_t rows,
+                  void* stream);
+
+/* The rows at slots[i] back: k, v [rows, kv_heads, head_dim] (bf16, fp16 or
+ * fp32, contiguous, 16-byte aligned); zeros for a slot outside the cache. */
+int pgs_read_kv4(const pgs_kv_cache4* cache, const int64_t* slots, int64_t rows,
+                 void* k, void* v, int dtype, void* stream);
+
+/* The arguments of pgs_window_attention. */
+typedef struct pgs_window_attention_args {
+  const void* q;               /* [rows, q_heads, head_dim] */
+  void* out;                   /* [rows, q_heads, head_dim] */
+  float* lse;                  /* [rows, q_heads], or NULL */
+  int64_t q_row, q_head, out_row, out_head; /* element strides */
+  const pgs_kv_cache* cache;   /* of the rows' dtype, or NULL: cache4 */
+  const pgs_kv_cache4* cache4;
+  const int32_t* block_tables; /* [requests, columns] */
+  int64_t table_stride, columns;
+  const int32_t* lens;         /* [requests]: cached tokens, the rows' own among them */
+  const int32_t* offsets;      /* [requests + 1] */
+  int64_t rows, requests, q_heads;
+  int64_t max_tokens;          /* rows per request; the kernels are chosen by it */
+  int64_t max_context;         /* the longest lens expected: sizes the split, not the result */
+  int64_t window, sinks;
+  float scale;
+  int dtype;                   /* PGS_DTYPE_BF16 or PGS_DTYPE_F16, of q and out */
+} pgs_window_attention_args;
+
+/*
+ * out = sum_j softmax_j(scale * q . k_j) v_j and lse = ln sum_j e^(scale q . k_j)
+ * over the tokens that a row sees (softmax in fp32); a row that sees none gets
+ * zeros and -inf.  Query heads share key heads in groups of q_heads / kv_heads.
+ * head_dim 64 or 128; block_size a multiple of 16, columns * block_size at most
+ * 2^31 - 65536; strides multiples of 8 elements and pointers 16-byte aligned.
+ * Lengths beyond the table's columns are cut to them; tokens in a block outside
+ * the cache are left out; rows of no request, and a request's rows from max_tokens
+ * on, are not written.  With fp16 rows, 4-bit keys and values beyond fp16's range
+ * may count as infinite.
+ * workspace: pgs_window_attention_workspace_bytes() bytes, 256-byte aligned, no
+ * fill needed.
+ */
+int pgs_window_attention(const pgs_window_attention_args* args, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of pgs_window_attention (0: none needed). */
+size_t pgs_window_attention_workspace_bytes(int64_t rows, int64_t requests, int64_t q_heads,
+                                            int64_t kv_heads, int64_t head_dim,
+                                            int64_t max_tokens, int64_t max_context,
+                                            int64_t window, int64_t sinks);
+
+/* The arguments of pgs_accumulate_weights; those with a name of
+ * pgs_window_attention_args mean the same. */
+typedef struct pgs_accumulate_weights_args {
+  const void* q;
+  int64_t q_row, q_head;
+  const pgs_kv_cache* cache;   /* (its values are not read and may be NULL) */
+  const pgs_kv_cache4* cache4;
+  const int32_t* block_tables;
+  int64_t table_stride, columns;
+  const int32_t* lens;
+  const int32_t* offsets;
+  const float* lse;            /* [rows, q_heads], as pgs_window_attention gave it */
+  const int32_t* new_lens;     /* [requests], or NULL: as many last tokens of a request start from 0 */
+  float* weights;              /* [blocks, block_size] */
+  int64_t rows, requests, q_heads, max_tokens, max_context, window, sinks;
+  float scale;
+  int dtype;
+} pgs_accumulate_weights_args;
+
+/*
+ * Adds to weights[slot of token j] the attention weights of the rows and query
+ * heads that see j: sum of e^(scale q . k_j - lse).  Sums are fp32, in a fixed
+ * order.  Tokens in a block outside the cache are left out.
+ */
+int pgs_accumulate_weights(const pgs_accumulate_weights_args* args, void* stream);
+
+/*
+ * Cuts each request of more than budget[b] tokens to budget[b] (below 0: 0): the
+ * first `sinks`, the last `recent` and, of those between, the ones of largest
+ * weight stay (of equal ones the first; a NaN is the largest, a token in a block
+ * outside the cache the smallest), in their order, moved together to the front.
+ * sinks come before recent where the budget does not hold both.  kept[b]: the
+ * tokens that stay; lens and the tables are left as they are (pgs_truncate_blocks
+ * with kept shortens them).  weights [blocks, block_size] and the rows of every
+ * cache (of one layer each: `count` in 16 bits, `count4` in 4, each kind of one
+ * size) move alike; what lies behind the kept tokens is left as it is, and so is
+ * a place whose token, or which itself, is in a block outside the cache.  A
+ * request of more than max_context tokens is left as it is.  No block may be in
+ * two requests' tables, no two caches may share an element, and no array that is
+ * written may share memory with another.
+ * workspace: pgs_evict_tokens_workspace_bytes() bytes, no fill needed.
+ */
+int pgs_evict_tokens(float* weights, const int32_t* lens, const int32_t* budget,
+                     const int32_t* block_tables, int64_t table_stride, int64_t columns,
+                     int64_t blocks, int64_t block_size, int64_t requests, int64_t sinks,
+                     int64_t recent, int64_t max_context, const pgs_kv_cache* caches,
+                     int64_t count, const pgs_kv_cache4* caches4, int64_t count4,
+                     int32_t* kept, void* workspace, size_t workspace_bytes, void* stream);
+size_t pgs_evict_tokens_workspace_bytes(int64_t requests, int64_t max_context);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,6 +5,7 @@ computed by hand-written HIP kernels behind a C ABI
 (``include/pageserve_amd.h``).
 """
 
+from .cache4 import KVCache4, read_kv4, write_kv4  # noqa: F401
 from .paged import append_blocks, tree_attention, truncate_blocks, write_kv  # noqa: F401
 from .quantization import (  # noqa: F401
     QuantizedWeight,
@@ -26,5 +27,6 @@ from .quantization import (  # noqa: F401
     swiglu,
 )
 from .quantization4 import QuantizedWeight4, linear4  # noqa: F401
+from .window import accumulate_weights, evict_tokens, window_attention, window_attention4  # noqa: F401
 
 __version__ = "0.1.0"

@@ -23,7 +23,7 @@ DTYPE_BF16 = 1
 DTYPE_F16 = 2
 OK = 0
 MAX_GROUP = 4
-ABI_VERSION = 10
+ABI_VERSION = 11
 ERR_TIMEOUT = 5
 
 
@@ -92,6 +92,40 @@ class TreeAttentionArgs(ctypes.Structure):
         + [("scale", ctypes.c_float), ("dtype", ctypes.c_int)])
 
 
+class KVCache4(ctypes.Structure):
+    """``pgs_kv_cache4`` of include/pageserve_amd.h."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("k", "k_scale", "v", "v_scale")] + [
+        (name, ctypes.c_int64) for name in ("blocks", "block_size", "kv_heads", "head_dim")]
+
+
+class WindowAttentionArgs(ctypes.Structure):
+    """``pgs_window_attention_args`` of include/pageserve_amd.h."""
+
+    _fields_ = (
+        [(name, ctypes.c_void_p) for name in ("q", "out", "lse")]
+        + [(name, ctypes.c_int64) for name in ("q_row", "q_head", "out_row", "out_head")]
+        + [("cache", ctypes.POINTER(KVCache)), ("cache4", ctypes.POINTER(KVCache4)), ("block_tables", ctypes.c_void_p),
+           ("table_stride", ctypes.c_int64), ("columns", ctypes.c_int64)]
+        + [(name, ctypes.c_void_p) for name in ("lens", "offsets")]
+        + [(name, ctypes.c_int64) for name in ("rows", "requests", "q_heads", "max_tokens", "max_context", "window",
+                                               "sinks")]
+        + [("scale", ctypes.c_float), ("dtype", ctypes.c_int)])
+
+
+class AccumulateWeightsArgs(ctypes.Structure):
+    """``pgs_accumulate_weights_args`` of include/pageserve_amd.h."""
+
+    _fields_ = (
+        [("q", ctypes.c_void_p), ("q_row", ctypes.c_int64), ("q_head", ctypes.c_int64),
+         ("cache", ctypes.POINTER(KVCache)), ("cache4", ctypes.POINTER(KVCache4)), ("block_tables", ctypes.c_void_p),
+         ("table_stride", ctypes.c_int64), ("columns", ctypes.c_int64)]
+        + [(name, ctypes.c_void_p) for name in ("lens", "offsets", "lse", "new_lens", "weights")]
+        + [(name, ctypes.c_int64) for name in ("rows", "requests", "q_heads", "max_tokens", "max_context", "window",
+                                               "sinks")]
+        + [("scale", ctypes.c_float), ("dtype", ctypes.c_int)])
+
+
 _VP = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
@@ -147,6 +181,14 @@ SIGNATURES = {
     "pgs_write_kv": (_INT, [_VP, _I64, _I64, _VP, _I64, _I64, ctypes.POINTER(KVCache), _VP, _I64, _VP]),
     "pgs_tree_attention": (_INT, [ctypes.POINTER(TreeAttentionArgs), _VP, _SZ, _VP]),
     "pgs_tree_attention_workspace_bytes": (_SZ, [_I64] * 7),
+    "pgs_write_kv4": (_INT, [_VP, _I64, _I64, _VP, _I64, _I64, _INT, ctypes.POINTER(KVCache4), _VP, _I64, _VP]),
+    "pgs_read_kv4": (_INT, [ctypes.POINTER(KVCache4), _VP, _I64, _VP, _VP, _INT, _VP]),
+    "pgs_window_attention": (_INT, [ctypes.POINTER(WindowAttentionArgs), _VP, _SZ, _VP]),
+    "pgs_window_attention_workspace_bytes": (_SZ, [_I64] * 9),
+    "pgs_accumulate_weights": (_INT, [ctypes.POINTER(AccumulateWeightsArgs), _VP]),
+    "pgs_evict_tokens": (_INT, [_VP] * 4 + [_I64] * 8 + [ctypes.POINTER(KVCache), _I64, ctypes.POINTER(KVCache4), _I64,
+                                                         _VP, _VP, _SZ, _VP]),
+    "pgs_evict_tokens_workspace_bytes": (_SZ, [_I64, _I64]),
 }
 
 _lock = threading.Lock()

@@ -580,6 +580,262 @@ at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& k, const at::Te
   return o;
 }
 
+// ---------------------------------------------------------------------------
+// long texts in a bounded cache (pageserve_amd/window.py, pageserve_amd/cache4.py)
+// ---------------------------------------------------------------------------
+
+// codes and scales of a 4-bit cache: uint8 [blocks, kv_heads, block_size, head_dim / 2], bf16 [.., head_dim / 32]
+pgs_kv_cache4 check_cache4(const at::Tensor& k, const at::Tensor& ks, const at::Tensor& v, const at::Tensor& vs,
+                           const char* what) {
+  for (const at::Tensor* t : {&k, &ks, &v, &vs}) {
+    need_gpu(*t, what, "the cache");
+    if (t->dim() != 4 || !t->is_contiguous() || t->device() != k.device())
+      value_error(std::string(what) + ": the cache's parts must be contiguous and on one device");
+  }
+  if (k.scalar_type() != at::kByte || v.scalar_type() != at::kByte || ks.scalar_type() != at::kBFloat16 ||
+      vs.scalar_type() != at::kBFloat16)
+    type_error(std::string(what) + ": the cache's codes must be uint8 and its scales bf16");
+  if (k.sizes() != v.sizes() || ks.sizes() != vs.sizes() || ks.size(0) != k.size(0) || ks.size(1) != k.size(1) ||
+      ks.size(2) != k.size(2) || ks.size(3) * 16 != k.size(3))
+    value_error(std::string(what) + ": the cache's parts must agree in shape");
+  return pgs_kv_cache4{ptr(k), ptr(ks), ptr(v), ptr(vs), k.size(0), k.size(2), k.size(1), 2 * k.size(3)};
+}
+
+// rows [rows, heads, dim] in bf16 or fp16 on dev, usable by 16-byte accesses
+at::Tensor rows_of(const at::Tensor& t, int64_t rows, int64_t heads, int64_t dim, const at::Device& dev, const char* what,
+                   const char* name) {
+  if (t.device() != dev)
+    value_error(std::string(what) + ": " + name + " on " + dev_str(t.device()) + " but the cache is on " + dev_str(dev));
+  code_of(t, what);
+  if (t.dim() != 3 || (rows >= 0 && t.size(0) != rows) || (heads >= 0 && t.size(1) != heads) || t.size(2) != dim)
+    value_error(std::string(what) + ": " + name + " must be (" + (rows >= 0 ? std::to_string(rows) : std::string("rows")) +
+                ", " + (heads >= 0 ? std::to_string(heads) : std::string("heads")) + ", " + std::to_string(dim) + ")");
+  return pieces(t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t);
+}
+
+const int64_t* slots_of(const at::Tensor& slots, const at::Device& dev, const char* what) {
+  if (slots.device() != dev)
+    value_error(std::string(what) + ": slots on " + dev_str(slots.device()) + " but the cache is on " + dev_str(dev));
+  if (slots.scalar_type() != at::kLong) type_error(std::string(what) + ": slots must be int64");
+  if (!slots.is_contiguous()) value_error(std::string(what) + ": slots must be contiguous");
+  return static_cast<const int64_t*>(ptr(slots));
+}
+
+void write_kv4(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ck, const at::Tensor& cks, const at::Tensor& cv,
+               const at::Tensor& cvs, const at::Tensor& slots) {
+  const char* what = "write_kv4";
+  const pgs_kv_cache4 c = check_cache4(ck, cks, cv, cvs, what);
+  const int64_t rows = slots.numel();
+  const at::Device dev = ck.device();
+  at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  const at::Tensor kr = rows_of(k, rows, c.kv_heads, c.head_dim, dev, what, "k");
+  const at::Tensor vr = rows_of(v, rows, c.kv_heads, c.head_dim, dev, what, "v");
+  if (kr.scalar_type() != vr.scalar_type()) type_error("write_kv4: k and v must have one dtype");
+  const int64_t* sp = slots_of(slots, dev, what);
+  for (const at::Tensor* w : {&ck, &cks, &cv, &cvs})
+    if (overlap(kr, *w) || overlap(vr, *w) || overlap(slots, *w))
+      value_error("write_kv4: k, v and slots must not share memory with the cache");
+  void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+  check_rc(pgs_write_kv4(ptr(kr), step(kr, 0), step(kr, 1), ptr(vr), step(vr, 0), step(vr, 1), code_of(kr, what), &c, sp, rows, st),
+           what);
+}
+
+std::vector<at::Tensor> read_kv4(const at::Tensor& ck, const at::Tensor& cks, const at::Tensor& cv, const at::Tensor& cvs,
+                                 const at::Tensor& slots, int64_t dtype) {
+  const char* what = "read_kv4";
+  const pgs_kv_cache4 c = check_cache4(ck, cks, cv, cvs, what);
+  const at::Device dev = ck.device();
+  at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  const int64_t* sp = slots_of(slots, dev, what);
+  const auto type = dtype == PGS_DTYPE_F32 ? at::kFloat : dtype == PGS_DTYPE_F16 ? at::kHalf : at::kBFloat16;
+  at::Tensor k = at::empty({slots.numel(), c.kv_heads, c.head_dim}, ck.options().dtype(type)), v = at::empty_like(k);
+  void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+  check_rc(pgs_read_kv4(&c, sp, slots.numel(), ptr(k), ptr(v), static_cast<int>(dtype), st), what);
+  return {k, v};
+}
+
+constexpr int64_t kEverything = 0x7fffffff;
+
+// cache: k_cache and v_cache, or the four parts of a 4-bit one
+std::vector<at::Tensor> window_attention(const at::Tensor& q, const std::vector<at::Tensor>& cache,
+                                         const at::Tensor& block_tables, const at::Tensor& lens, const at::Tensor& offsets,
+                                         const c10::optional<int64_t>& window, int64_t sinks,
+                                         const c10::optional<int64_t>& max_tokens, const c10::optional<int64_t>& max_context,
+                                         const c10::optional<double>& scale, bool want_lse, const Opt& out) {
+  const bool four = cache.size() == 4;
+  const char* what = four ? "window_attention4" : "window_attention";
+  pgs_window_attention_args a{};
+  pgs_kv_cache c{};
+  pgs_kv_cache4 c4{};
+  if (four) {
+    c4 = check_cache4(cache[0], cache[1], cache[2], cache[3], what);
+    a.cache4 = &c4;
+  } else {
+    c = check_cache(cache[0], cache[1], what);
+    a.cache = &c;
+  }
+  const int64_t dim = four ? c4.head_dim : c.head_dim, size = four ? c4.block_size : c.block_size;
+  const int64_t kv_heads = four ? c4.kv_heads : c.kv_heads;
+  const at::Device dev = cache[0].device();
+  at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  const at::Tensor qr = rows_of(q, -1, -1, dim, dev, what, "q");
+  if (!four && qr.scalar_type() != cache[0].scalar_type()) type_error("window_attention: q must have the cache's dtype");
+  a.dtype = code_of(qr, what);
+  a.rows = q.size(0), a.q_heads = q.size(1);
+  a.requests = lens.numel();
+  a.lens = ints(lens, a.requests, dev, what, "lens");
+  a.offsets = ints(offsets, a.requests + 1, dev, what, "offsets");
+  a.block_tables = table(block_tables, a.requests, dev, what, a.table_stride);
+  a.columns = block_tables.size(1);
+  at::Tensor o, lse;
+  if (out.has_value()) {
+    o = *out;
+    if (o.device() != dev || o.scalar_type() != q.scalar_type() || o.sizes() != q.sizes() || !o.is_contiguous() ||
+        reinterpret_cast<uintptr_t>(o.data_ptr()) % 16)
+      value_error(std::string(what) + ": out must be a contiguous 16-byte aligned tensor of q's shape, dtype and device");
+    if (overlap(o, qr) && (o.data_ptr() != qr.data_ptr() || !qr.is_contiguous()))
+      value_error(std::string(what) + ": out may be q itself, but not share memory with a part of it");
+    for (const at::Tensor& t : cache)
+      if (overlap(o, t)) value_error(std::string(what) + ": out must not share memory with the cache");
+    for (const at::Tensor* t : {&lens, &offsets, &block_tables})
+      if (overlap(o, *t)) value_error(std::string(what) + ": out must not share memory with lens, offsets or block_tables");
+  } else {
+    o = at::empty(q.sizes(), qr.options());
+  }
+  if (want_lse) lse = at::empty({a.rows, a.q_heads}, qr.options().dtype(at::kFloat));
+  a.q = ptr(qr), a.out = ptr(o);
+  a.lse = want_lse ? static_cast<float*>(ptr(lse)) : nullptr;
+  a.q_row = step(qr, 0), a.q_head = step(qr, 1), a.out_row = step(o, 0), a.out_head = step(o, 1);
+  a.max_tokens = max_tokens.has_value() ? *max_tokens : std::max<int64_t>(a.rows, 1);
+  a.max_context = max_context.has_value() ? std::max<int64_t>(*max_context, 0) : a.columns * size;
+  a.window = window.has_value() ? *window : kEverything;
+  a.sinks = sinks;
+  a.scale = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(dim)));
+  const size_t need = pgs_window_attention_workspace_bytes(a.rows, a.requests, a.q_heads, kv_heads, dim, a.max_tokens,
+                                                           a.max_context, a.window, a.sinks);
+  at::Tensor ws;  // (per call, as in tree_attention)
+  if (need) ws = at::empty({static_cast<int64_t>(need)}, qr.options().dtype(at::kByte));
+  void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+  check_rc(pgs_window_attention(&a, need ? ws.data_ptr() : nullptr, need, st), what);
+  if (want_lse) return {o, lse};
+  return {o};
+}
+
+// sums per slot: fp32 [blocks, block_size], contiguous
+float* sums_of(const at::Tensor& w, int64_t blocks, int64_t size, const at::Device& dev, const char* what) {
+  if (w.device() != dev)
+    value_error(std::string(what) + ": weights on " + dev_str(w.device()) + " but the cache is on " + dev_str(dev));
+  if (w.scalar_type() != at::kFloat) type_error(std::string(what) + ": weights must be fp32");
+  if (w.dim() != 2 || !w.is_contiguous() || (blocks >= 0 && (w.size(0) != blocks || w.size(1) != size)))
+    value_error(std::string(what) + ": weights must be contiguous (blocks, block_size), one for each of the cache's slots");
+  return static_cast<float*>(ptr(w));
+}
+
+// cache: k_cache, or the four parts of a 4-bit one
+void accumulate_weights(const at::Tensor& q, const std::vector<at::Tensor>& cache, const at::Tensor& block_tables,
+                        const at::Tensor& lens, const at::Tensor& offsets, const at::Tensor& lse, const at::Tensor& weights,
+                        const Opt& new_lens, const c10::optional<int64_t>& window, int64_t sinks,
+                        const c10::optional<int64_t>& max_tokens, const c10::optional<int64_t>& max_context,
+                        const c10::optional<double>& scale) {
+  const char* what = "accumulate_weights";
+  const bool four = cache.size() == 4;
+  pgs_accumulate_weights_args a{};
+  pgs_kv_cache c{};
+  pgs_kv_cache4 c4{};
+  if (four) {
+    c4 = check_cache4(cache[0], cache[1], cache[2], cache[3], what);
+    a.cache4 = &c4;
+  } else {
+    c = check_cache(cache[0], cache[0], what);
+    a.cache = &c;
+  }
+  const int64_t dim = four ? c4.head_dim : c.head_dim, size = four ? c4.block_size : c.block_size;
+  const int64_t blocks = four ? c4.blocks : c.blocks;
+  const at::Device dev = cache[0].device();
+  at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  const at::Tensor qr = rows_of(q, -1, -1, dim, dev, what, "q");
+  if (!four && qr.scalar_type() != cache[0].scalar_type()) type_error("accumulate_weights: q must have the cache's dtype");
+  a.dtype = code_of(qr, what);
+  a.q = ptr(qr), a.q_row = step(qr, 0), a.q_head = step(qr, 1);
+  a.rows = q.size(0), a.q_heads = q.size(1);
+  a.requests = lens.numel();
+  a.lens = ints(lens, a.requests, dev, what, "lens");
+  a.offsets = ints(offsets, a.requests + 1, dev, what, "offsets");
+  if (new_lens.has_value()) a.new_lens = ints(*new_lens, a.requests, dev, what, "new_lens");
+  a.block_tables = table(block_tables, a.requests, dev, what, a.table_stride);
+  a.columns = block_tables.size(1);
+  if (lse.device() != dev || lse.scalar_type() != at::kFloat || !lse.is_contiguous() || lse.dim() != 2 ||
+      lse.size(0) != a.rows || lse.size(1) != a.q_heads)
+    value_error("accumulate_weights: lse must be contiguous fp32 (rows, q_heads) on the cache's device, as window_attention "
+                "returns it");
+  a.lse = static_cast<const float*>(ptr(lse));
+  a.weights = sums_of(weights, blocks, size, dev, what);
+  for (const at::Tensor& t : cache)
+    if (overlap(weights, t)) value_error("accumulate_weights: weights must not share memory with the cache");
+  for (const at::Tensor* t : {&qr, &lse, &lens, &offsets, &block_tables})
+    if (overlap(weights, *t)) value_error("accumulate_weights: weights must not share memory with what is read");
+  if (new_lens.has_value() && overlap(weights, *new_lens))
+    value_error("accumulate_weights: weights must not share memory with what is read");
+  a.max_tokens = max_tokens.has_value() ? *max_tokens : std::max<int64_t>(a.rows, 1);
+  a.max_context = max_context.has_value() ? std::max<int64_t>(*max_context, 0) : a.columns * size;
+  a.window = window.has_value() ? *window : kEverything;
+  a.sinks = sinks;
+  a.scale = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(dim)));
+  void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+  check_rc(pgs_accumulate_weights(&a, st), what);
+}
+
+at::Tensor evict_tokens(const at::Tensor& weights, const at::Tensor& lens, const at::Tensor& budget,
+                        const at::Tensor& block_tables, const std::vector<std::vector<at::Tensor>>& caches, int64_t sinks,
+                        int64_t recent, const c10::optional<int64_t>& max_context) {
+  const char* what = "evict_tokens";
+  need_gpu(lens, what, "lens");
+  const at::Device dev = lens.device();
+  at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  const int64_t n = lens.numel();
+  const int32_t* lp = ints(lens, n, dev, what, "lens");
+  const int32_t* bp = ints(budget, n, dev, what, "budget");
+  int64_t stride = 0;
+  const int32_t* tp = table(block_tables, n, dev, what, stride);
+  float* wp = sums_of(weights, -1, -1, dev, what);
+  const int64_t blocks = weights.size(0), size = weights.size(1);
+  std::vector<pgs_kv_cache> c;
+  std::vector<pgs_kv_cache4> c4;
+  std::vector<const void*> at_;
+  for (const std::vector<at::Tensor>& t : caches) {
+    if (t.size() == 4) {
+      c4.push_back(check_cache4(t[0], t[1], t[2], t[3], what));
+    } else {
+      c.push_back(check_cache(t[0], t[1], what));
+      code_of(t[0], what);
+      check_places(t[0], what, "k_cache");
+      check_places(t[1], what, "v_cache");
+    }
+    for (const at::Tensor& x : t) {
+      if (x.device() != dev) value_error("evict_tokens: the caches must be on the device of lens");
+      if (x.numel()) at_.push_back(x.data_ptr());
+      if (overlap(x, weights) || overlap(x, lens) || overlap(x, budget) || overlap(x, block_tables))
+        value_error("evict_tokens: a cache must not share memory with weights, lens, budget or block_tables");
+    }
+  }
+  std::sort(at_.begin(), at_.end());
+  if (std::adjacent_find(at_.begin(), at_.end()) != at_.end()) value_error("evict_tokens: a cache is given twice");
+  for (const at::Tensor* t : {&lens, &budget, &block_tables})
+    if (overlap(weights, *t)) value_error("evict_tokens: weights must not share memory with lens, budget or block_tables");
+  const int64_t columns = block_tables.size(1);
+  const int64_t most = std::min(max_context.has_value() ? std::max<int64_t>(*max_context, 0) : kEverything, columns * size);
+  at::Tensor kept = at::empty({n}, lens.options());
+  const size_t need = pgs_evict_tokens_workspace_bytes(n, most);
+  at::Tensor ws;  // (per call, as in tree_attention)
+  if (need) ws = at::empty({static_cast<int64_t>(need)}, lens.options().dtype(at::kByte));
+  void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+  check_rc(pgs_evict_tokens(wp, lp, bp, tp, stride, columns, blocks, size, n, sinks, recent, most, c.data(),
+                            static_cast<int64_t>(c.size()), c4.data(), static_cast<int64_t>(c4.size()),
+                            static_cast<int32_t*>(ptr(kept)), need ? ws.data_ptr() : nullptr, need, st),
+           what);
+  return kept;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
@@ -596,4 +852,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("truncate_blocks", &truncate_blocks, "requests shortened, their blocks given back");
   mod.def("write_kv", &write_kv, "key and value rows stored at their slots");
   mod.def("tree_attention", &tree_attention, "attention of drafted tokens over a paged cache");
+  mod.def("write_kv4", &write_kv4, "key and value rows stored in 4 bits at their slots");
+  mod.def("read_kv4", &read_kv4, "rows of a 4-bit cache");
+  mod.def("window_attention", &window_attention, "attention over a sliding window with sinks");
+  mod.def("accumulate_weights", &accumulate_weights, "attention weights added up per cached token");
+  mod.def("evict_tokens", &evict_tokens, "requests cut to their tokens of largest weight");
 }

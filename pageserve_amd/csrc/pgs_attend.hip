@@ -34,12 +34,10 @@
 
 #include <algorithm>
 
-#include "pgs_linear.h"
+#include "pgs_attend.h"
 
 namespace pgs {
 namespace {
-
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kMaxTree = 64;
 
@@ -64,114 +62,6 @@ struct Attend {
   int64_t* sums;  // (wide) [requests]: counts of work up to and with each request
 };
 
-// The lane number where it is used: lane-dependent offsets computed from it are not kept
-// in registers across a loop.
-__device__ __forceinline__ int here(int lane) {
-  asm volatile("" : "+v"(lane));
-  return lane;
-}
-
-// LDS by its byte address
-template <typename T>
-__device__ __forceinline__ __attribute__((address_space(3))) T* lds(uint32_t address) {
-  return reinterpret_cast<__attribute__((address_space(3))) T*>(address);
-}
-template <typename T>
-__device__ __forceinline__ uint32_t lds_address(T& v) {
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)&v));
-}
-// Four keys x 16 dims per 16 lanes from LDS, transposed: lane i of them gives the address
-// of dims 4 (i % 4) .. +3 of key i / 4 and gets dim i of the four keys.
-__device__ __forceinline__ u32x2 read_transposed(uint32_t address) {
-  typedef short s16x4 __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds<s16x4>(address)));
-}
-
-// 16 bytes per lane from memory to LDS (lane l's to `address` + 16 l, wave-uniform) past
-// the registers.  The compiler does not count this load: whoever uses what it brings waits
-// with arrived(n), n: how many such loads issued later may still be on their way.
-__device__ __forceinline__ void load_lds(const uint16_t* p, uint32_t address) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(address), "v"(p) : "m0", "memory");
-}
-template <int N>
-__device__ __forceinline__ void arrived() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
-// The kernel's argument again, read from its segment at this point: for the parts of a
-// kernel outside its inner loop, whose fields would otherwise all sit in scalar
-// registers throughout (and push vector registers out to memory).
-__device__ __forceinline__ Attend again() {
-  auto p = __builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(p));
-  Attend a;
-  __builtin_memcpy(&a, (const void*)p, sizeof(a));
-  return a;
-}
-
-template <bool F16>
-struct Elem;
-template <>
-struct Elem<false> {
-  typedef bf16x8 x8;
-  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return mfma16x16x32(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c);
-  }
-  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
-  static __device__ __forceinline__ float low(uint32_t v) { return __uint_as_float(v << 16); }
-  static constexpr uint32_t kOnes = 0x3f803f80u, kExp = 0x7f80u;  // 1.0 twice; the exponent's bits
-  // A reference is this much (in powers of two) below the maximum that it is taken from.
-  static constexpr float kHead = 0.f;
-};
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-template <>
-struct Elem<true> {
-  typedef f16x8 x8;
-  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
-  }
-  static __device__ __forceinline__ float low(uint32_t v) {
-    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(v)));
-  }
-  static constexpr uint32_t kOnes = 0x3c003c00u, kExp = 0x7c00u;
-  // fp16 has no steps finer than 2^-24: beside a weight of 1, n others of up to 2^-25 would be
-  // lost, n 2^-25 of the sum.  With the largest at 2^7 to 2^15 (kSlack; the type ends at 2^16)
-  // that is n 2^-32.
-  static constexpr float kHead = 7.f;
-};
-
-// the maximum over lanes l, l ^ 16, l ^ 32, l ^ 48 (each swap leaves the two halves
-// of its exchange in two registers)
-__device__ __forceinline__ float quad_max(float v) {
-  const uint32_t x = __float_as_uint(v);
-  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  const uint32_t y = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
-  const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
-// A maximum nothing has raised yet: the lowest value that is finite.
-constexpr float kLow = -3.402823466e38f;
-// The reference of the exponents follows the maximum only when a score exceeds it
-// by this (in powers of two) and Elem::kHead: p stays below 2^8 times 2^kHead, as exact as
-// below 1, and the sums are rescaled a few times per row instead of at every step.
-constexpr float kSlack = 8.0f;
-// A reference is a rounded product c s, and fma(s, c, -reference) sees that rounding: up to
-// half a step of the reference, which the largest weight is off by (as a power of two; all
-// weights of the row are alike).  Beyond kFar that is more than 1/2 and in the end out of any
-// range, so there the product is rounded before the reference is taken off, as it was for
-// the reference: the largest weight is 2^0.
-constexpr float kFar = 8388608.0f;
-__device__ __forceinline__ float exponent(float s, float c, float reference, bool far) {
-#pragma clang fp contract(off)
-  const float t = s * c;
-  return far ? t - reference : fmaf(s, c, -reference);
-}
-
 // The request of a unit and its sizes, each brought into range: whatever the device
 // arrays hold, no access leaves the tensors.
 struct Request {
@@ -188,17 +78,6 @@ __device__ __forceinline__ Request request(const Attend& a, int b) {
   r.len_tiles = (r.len + 31) >> 5;
   r.tree_tiles = (r.tokens + 31) >> 5;
   return r;
-}
-
-// token / bs without a division: the product's high half is the quotient or one more
-// (bs_inv is too large by less than 1, token below 2^31), which the remainder's sign
-// shows
-__device__ __forceinline__ int block_of(const Attend& a, int token, int& slot) {
-  int q = static_cast<int>(__umulhi(static_cast<uint32_t>(token), a.bs_inv));
-  int r = token - q * a.bs;
-  if (r < 0) --q, r += a.bs;
-  slot = r;
-  return q;
 }
 
 // 16 R rows of a wave and their running sums.  The output MFMA d covers the dims
@@ -639,12 +518,6 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(Attend a) {
           [&](int, int64_t token, int head) { return (token * a.q_heads + head) * a.splits + part; });
 }
 
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
-  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-}
-
 // The wide kernel's work: the tiles of all (request, key head, group of kGroup rows), in
 // that order, cut into equal shares for the workgroups, whatever the requests' lengths
 // are.  A group of at most half the rows has two key slices: half the arithmetic per tile,
@@ -799,7 +672,7 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
   const uint32_t k_at = lds_address(lkv) + li * (2 * D) + 16 * (lg ^ (li * P / 16 & (P - 1)));
   const uint32_t v_at = lds_address(lkv) + TK * D * 2 + vkey * (2 * D) +
                         16 * ((li >> 1 & 1) ^ (2 * (vkey * P / 16) & (P - 1))) + 8 * (li & 1);
-  Work work{again(), lpre, lsum, 0, 0, 0};
+  Work work{again<Attend>(), lpre, lsum, 0, 0, 0};
   work.start(blockIdx.x == 0 ? work.a.sums : nullptr);
   const int shares = shares_of(work.total), share = xcd_remap(blockIdx.x, gridDim.x);
   if (share >= shares) return;
@@ -807,7 +680,7 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
   const int64_t end = uniform64(share_begin(work.total, share + 1, shares));
 
   for (int64_t pos = begin; pos < end;) {
-    work.a = again();
+    work.a = again<Attend>();
     const Work::Unit un = work.find(pos);
     const Request& rq = un.rq;
     const int nrows = rq.tokens * a.group;
@@ -834,7 +707,7 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
       const uint32_t at_k = lds_address(lkv) + to * (4 * TK * D) + wave * (1024 * J), at_v = at_k + 2 * TK * D;
       // (lane l fills piece l % P of its key's row in LDS: the exchange picks what it reads)
       if (t >= cached) {
-        const Attend c = again();
+        const Attend c = again<Attend>();
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           const int key = wave * KW + j * KI + kin, turn = key * P / 16;
@@ -906,7 +779,7 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
     const bool bad0 = load(t0, 0);
     W w;
     if (active) {
-      const Attend c = again();
+      const Attend c = again<Attend>();
       const int ln = here(lane);
       const int par = t1 > cached ? w.parent(c, rq, ln) : -1;
       w.load(c, rq, kh, row0, nrows, ln & 15, ln >> 4);
@@ -944,10 +817,10 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
           };
           const uint32_t odd32 = h < 2 ? static_cast<uint32_t>(odd >> (32 * h)) : 0;
           const int ln = here(lane);
-          auto see = [&](int r) { return lsee[wave][min(row0 + 16 * r + (ln & 15), nrows - 1) / again().group]; };
+          auto see = [&](int r) { return lsee[wave][min(row0 + 16 * r + (ln & 15), nrows - 1) / again<Attend>().group]; };
           w.step(a, keys, values, key0 + 32 * h, limit, tree, masked, bm >> (32 * h / KW) & 1,
                  bm >> ((32 * h + 16) / KW) & 1, odd32, see, ln & 15, ln >> 4, [&](int j) {
-                   const Attend c = again();
+                   const Attend c = again<Attend>();
                    return c.v + (rq.row0 + key0 + 32 * h + j) * c.v_row + kh * c.v_head;
                  });
         }
@@ -997,86 +870,10 @@ __global__ __launch_bounds__(64 * kWideWaves, kWideWaves / 4) void attend_wide_k
     if (active && wk == 0) {
       const int64_t slot0 = static_cast<int64_t>(2 * share + (un.begin >= begin) - un.rg) * kGroup;
       const int ln = here(lane);
-      w.store(again(), rq, kh, row0, nrows, ln & 15, ln >> 4, t0 == 0 && t1 == un.tiles,
+      w.store(again<Attend>(), rq, kh, row0, nrows, ln & 15, ln >> 4, t0 == 0 && t1 == un.tiles,
               [&](int row, int64_t, int) { return slot0 + row; });
     }
   }
-}
-
-// Four rows' outputs from n parts' sums each: brought to one reference, added in order and
-// divided by the joined sum.  Sixteen lanes per row, each with D/16 neighbouring dims;
-// slot(i): where part i of the lane's row is; p: the lane's dims of the output, or null.
-// WAVES: of the workgroup, each taking that share of the parts (all must call it), joined in
-// LDS; or 1.  Bound by memory and, few rows of many parts, by its latency: up to eight
-// parts' loads are on their way together.
-template <int D, bool F16, int WAVES, typename Slot>
-__device__ __forceinline__ void join_rows(const Attend& a, int n, int lane, int wave, uint16_t* p, Slot slot) {
-  constexpr int W = D / 16;
-  const int li = lane & 15;
-  float ref = kLow, sum = 0.f, o[W];
-#pragma unroll
-  for (int d = 0; d < W; ++d) o[d] = 0.f;
-  const int end = WAVES == 1 ? n : n * (wave + 1) / WAVES;
-  auto batch = [&](int i0, auto count) {
-    constexpr int U = decltype(count)::value;
-    f32x2 st[U];
-    f32x4 x[U][W / 4];
-#pragma unroll
-    for (int e = 0; e < U; ++e) {
-      const int64_t at = slot(min(i0 + e, end - 1));
-      st[e] = *reinterpret_cast<const f32x2*>(a.stat + 2 * at);
-#pragma unroll
-      for (int d = 0; d < W / 4; ++d) x[e][d] = *reinterpret_cast<const f32x4*>(a.part + at * D + W * li + 4 * d);
-    }
-    float top = ref;
-#pragma unroll
-    for (int e = 0; e < U; ++e) top = fmaxf(top, st[e][0]);
-    const float f = __builtin_amdgcn_exp2f(ref - top);
-    ref = top;
-    sum *= f;
-#pragma unroll
-    for (int d = 0; d < W; ++d) o[d] *= f;
-#pragma unroll
-    for (int e = 0; e < U; ++e) {
-      if (i0 + e >= end) break;  // (a part read again)
-      const float g = __builtin_amdgcn_exp2f(st[e][0] - ref);
-      sum = fmaf(g, st[e][1], sum);
-#pragma unroll
-      for (int d = 0; d < W; ++d) o[d] = fmaf(g, x[e][d / 4][d % 4], o[d]);
-    }
-  };
-  int i = WAVES == 1 ? 0 : n * wave / WAVES;
-  for (; end - i > 4; i += 8) batch(i, Int<8>{});
-  if (end - i > 2) batch(i, Int<4>{});
-  else if (end > i) batch(i, Int<2>{});
-  if constexpr (WAVES > 1) {
-    __shared__ float lref[WAVES][64], lsum[WAVES][64], lo[WAVES][W][64];
-    lref[wave][lane] = ref;
-    lsum[wave][lane] = sum;
-#pragma unroll
-    for (int d = 0; d < W; ++d) lo[wave][d][lane] = o[d];
-    __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) ref = fmaxf(ref, lref[w][lane]);
-    sum = 0.f;
-#pragma unroll
-    for (int d = 0; d < W; ++d) o[d] = 0.f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float g = __builtin_amdgcn_exp2f(lref[w][lane] - ref);
-      sum = fmaf(g, lsum[w][lane], sum);
-#pragma unroll
-      for (int d = 0; d < W; ++d) o[d] = fmaf(g, lo[w][d][lane], o[d]);
-    }
-  }
-  if (!p) return;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint32_t w[W / 2];
-#pragma unroll
-  for (int d = 0; d < W / 2; ++d) w[d] = Elem<F16>::pack(o[2 * d] * inv, o[2 * d + 1] * inv);
-  if constexpr (W == 8) *reinterpret_cast<u32x4*>(p) = u32x4{w[0], w[1], w[2], w[3]};
-  else *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
 }
 
 // Waves that join four rows: sixteen if those have eight parts and there are few of them, so
@@ -1108,7 +905,8 @@ __global__ __launch_bounds__(join_threads(WAVES)) void join_kernel(Attend a, int
   const int row = min(first + (lane >> 4), rows - 1), t = row / a.q_heads;
   const int64_t at = (static_cast<int64_t>(rq.row0) * a.q_heads + row) * a.splits;
   uint16_t* p = a.out + (rq.row0 + t) * a.out_row + (row - t * a.q_heads) * a.out_head + D / 16 * li;
-  join_rows<D, F16, WAVES>(a, parts, lane, wave, first + (lane >> 4) < rows ? p : nullptr, [&](int i) { return at + i; });
+  join_rows<D, F16, WAVES, 2>(a.part, a.stat, parts, lane, wave, first + (lane >> 4) < rows ? p : nullptr, nullptr,
+                              [&](int i) { return at + i; });
 }
 
 // Behind attend_wide_kernel: rows of a key head; those of whole units are already written.
@@ -1140,8 +938,8 @@ __global__ __launch_bounds__(join_threads(WAVES)) void join_wide_kernel(Attend a
   if (g0 == g1) return;
   const int row = min(first + (lane >> 4), rows - 1), t = row / a.group;
   uint16_t* p = a.out + (rq.row0 + t) * a.out_row + (kh * a.group + row - t * a.group) * a.out_head + D / 16 * li;
-  join_rows<D, F16, WAVES>(a, g1 - g0 + 1, lane, wave, first + (lane >> 4) < rows ? p : nullptr,
-                    [&](int i) { return static_cast<int64_t>(2 * (g0 + i) + (i == 0) - rg) * kGroup + row; });
+  join_rows<D, F16, WAVES, 2>(a.part, a.stat, g1 - g0 + 1, lane, wave, first + (lane >> 4) < rows ? p : nullptr, nullptr,
+                              [&](int i) { return static_cast<int64_t>(2 * (g0 + i) + (i == 0) - rg) * kGroup + row; });
 }
 
 // The launch shape, a function of sizes the host knows (never of what the device

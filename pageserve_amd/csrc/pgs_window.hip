@@ -1,0 +1,631 @@
+// Attention of a request's newest rows over the cached tokens of a sliding window and the
+// first few (sinks), the paged cache in 16 or in 4 bits (gfx950; pgs_window.h).  For row
+// (t, h) over the tokens j that it sees:
+//
+//   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(c s_j - m),  s_j = q . k_j,  c = scale log2(e)
+//   lse = ln sum_j e^(scale s_j) = (m + log2 sum_j p_j) ln 2
+//
+// in one pass with a running maximum m and sums.  Rows and keys lie as in the attention of
+// drafted tokens (pgs_attend.hip): S^T = K Q^T and O^T = V^T P^T by v_mfma_f32_16x16x32, the
+// tokens x query heads of one key head as columns, so that a row's scores, maximum, sums and
+// output stay in the lanes l%16 = row.
+#include <algorithm>
+
+#include "pgs_window.h"
+
+namespace pgs {
+namespace {
+
+// 16 R rows of a wave and their running sums.  The output MFMA d covers the dims
+// (4 lg + i) D/16 + d of its lanes (SPREAD: values straight from 16-bit rows), or 16 d + 4 lg + i.
+template <int D, int R, bool F16, bool SPREAD>
+struct Rows {
+  using E = Elem<F16>;
+  static constexpr int DC = D / 32, DV = D / 16;
+  u32x4 q[R][DC];
+  f32x4 o[R][DV], l[R];  // (l: every element the same)
+  float exact[R], mx[R];  // the lane's own part of the weights' sum before they are rounded; the reference
+  int pos[R], low[R];     // where the row stands; pos - window
+  bool far;               // some row's reference is beyond kFar (the same in all lanes)
+
+  __device__ __forceinline__ void load(const Window& a, const Ragged& rq, int kh, int row0, int nrows, int li, int lg) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = min(row0 + 16 * r + li, nrows - 1), t = row / a.group;  // (rows past the last repeat it)
+      const uint16_t* p = a.q + (rq.row0 + t) * a.q_row + (kh * a.group + row - t * a.group) * a.q_head + 8 * lg;
+#pragma unroll
+      for (int d = 0; d < DC; ++d) q[r][d] = ld16(p + 32 * d);
+      pos[r] = rq.first + t;
+      low[r] = low_of(pos[r], a.window);
+    }
+    // (they have arrived here: a wait for them inside the loop over the keys would be
+    // a wait for the keys on their way too)
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int d = 0; d < DC; ++d) asm volatile("" : "+v"(q[r][d]));
+    far = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mx[r] = kLow;
+      exact[r] = 0.f;
+      l[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < DV; ++i) o[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  // Weights of a step: s[r][h] the scores of keys key0 + 16 h + 4 lg + i, x[r][4 h + i] the
+  // weights' exponents against the rows' references, which are raised first where a score
+  // needs it.  masked: some row may not see some key, or a half's block is absent (bad).
+  __device__ __forceinline__ void weights(const Window& a, const f32x4 (&s)[R][2], float (&x)[R][8], uint32_t (&ok)[R],
+                                          int key0, bool masked, bool bad0, bool bad1, int lg) {
+    bool over = false;
+    if (masked || far) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        ok[r] = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = key0 + 16 * (e >> 2) + 4 * lg + (e & 3);
+          const bool in = visible(key, pos[r], low[r], a.sinks) && !(e >> 2 ? bad1 : bad0);
+          ok[r] |= in ? 1u << e : 0;
+          x[r][e] = in ? exponent(s[r][e >> 2][e & 3], a.c, mx[r], far) : -INFINITY;
+          over = over || x[r][e] > kSlack + E::kHead;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        ok[r] = 0xff;
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[r][e] = fmaf(s[r][e >> 2][e & 3], a.c, -mx[r]);
+          top = fmaxf(top, x[r][e]);
+        }
+        over = over || top > kSlack + E::kHead;
+      }
+    }
+    if (__ballot(over)) {
+      // new references: the largest score of each row so far
+      bool beyond = false;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float t = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t = fmaxf(t, ok[r] >> e & 1 ? s[r][e >> 2][e & 3] * a.c : -INFINITY);
+        t = quad_max(t);
+        const float ref = fmaxf(fabsf(t) > kFar ? t : t - E::kHead, mx[r]), f = __builtin_amdgcn_exp2f(mx[r] - ref);
+        mx[r] = ref;
+        beyond = beyond || fabsf(ref) > kFar;
+        exact[r] *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[r][i] *= f;
+#pragma unroll
+        for (int d = 0; d < DV; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[r][d][i] *= f;
+      }
+      far = __ballot(beyond);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[r][e] = ok[r] >> e & 1 ? exponent(s[r][e >> 2][e & 3], a.c, mx[r], far) : -INFINITY;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[r][e] = __builtin_amdgcn_exp2f(x[r][e]);
+  }
+
+  // The step's part of the sums and outputs, the weights rounded to the rows' type; the row
+  // sum that divides adds the rounded ones, the logarithm's (want) those before.  values(d):
+  // A operand of output MFMA d.  odd: keys whose values are not finite (values() holds
+  // zeros for them); value(j) is the row of key key0 + j.
+  template <typename Values, typename Value>
+  __device__ __forceinline__ void add(const Window& a, const float (&x)[R][8], Values values, int key0, uint32_t odd,
+                                      bool want, int li, int lg, Value value) {
+    u32x4 p[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[r][i] = E::pack(x[r][2 * i], x[r][2 * i + 1]);
+    if (want)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        exact[r] += ((x[r][0] + x[r][1]) + (x[r][2] + x[r][3])) + ((x[r][4] + x[r][5]) + (x[r][6] + x[r][7]));
+    const u32x4 ones = {E::kOnes, E::kOnes, E::kOnes, E::kOnes};
+#pragma unroll
+    for (int r = 0; r < R; ++r) l[r] = E::mfma(ones, p[r], l[r]);
+#pragma unroll
+    for (int d = 0; d < DV; ++d) {
+      const u32x4 v = values(d);
+#pragma unroll
+      for (int r = 0; r < R; ++r) o[r][d] = E::mfma(v, p[r], o[r][d]);
+    }
+    for (uint32_t w = odd; w; w &= w - 1) {
+      const int j = __builtin_ctz(w);
+      const auto row = value(j);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint32_t lo = j & 2 ? p[r][1] : p[r][0], hi = j & 2 ? p[r][3] : p[r][2];
+        const float pj = E::low(__shfl(j & 16 ? hi : lo, 16 * (j >> 2 & 3) + li) >> (16 * (j & 1)));
+        if (!visible(key0 + j, pos[r], low[r], a.sinks)) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int d = 0; d < DV; ++d) o[r][d][i] += pj * row(SPREAD ? (4 * lg + i) * DV + d : 16 * d + 4 * lg + i);
+      }
+    }
+  }
+
+  // The same from 4-bit values, whose scales multiply the weights in front of the rounding:
+  // one operand per 32 dims.  It is bf16 whatever the rows are (a weight times a scale may
+  // leave fp16's range; the codes are exact in both), in two terms where they are fp16, whose
+  // finer rounding the output shall have.  A token that is not seen has weight 0 whatever its
+  // scale holds.
+  __device__ __forceinline__ void add4(const float (&x)[R][8], const uint32_t (&ok)[R], const Values4<D>& n, bool masked) {
+    static_assert(!SPREAD, "the codes' order");
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      exact[r] += ((x[r][0] + x[r][1]) + (x[r][2] + x[r][3])) + ((x[r][4] + x[r][5]) + (x[r][6] + x[r][7]));
+    group4<0>(x, ok, n, masked);
+    group4<1>(x, ok, n, masked);
+    if constexpr (DC == 4) {
+      group4<2>(x, ok, n, masked);
+      group4<3>(x, ok, n, masked);
+    }
+  }
+  template <int G>
+  __device__ __forceinline__ void group4(const float (&x)[R][8], const uint32_t (&ok)[R], const Values4<D>& n, bool masked) {
+    // codes of dims 32 G + li and 16 further, pairs of keys
+    u32x4 v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t k0, k1;
+        if constexpr (DC == 4) k0 = widen2<G>(n.v[h][2 * i]), k1 = widen2<G>(n.v[h][2 * i + 1]);
+        else k0 = widen2<G>(n.v[h][i]), k1 = widen2<G + 2>(n.v[h][i]);
+        v[0][2 * h + i] = __builtin_amdgcn_perm(k1, k0, 0x05040100u);
+        v[1][2 * h + i] = __builtin_amdgcn_perm(k1, k0, 0x07060302u);
+      }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      u32x4 p, rest;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float y[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int e = 2 * i + j;
+          y[j] = x[r][e] * n.scale(e >> 2, e & 3, G);
+          if (masked) y[j] = ok[r] >> e & 1 ? y[j] : 0.f;
+        }
+        p[i] = pack_bf16x2(y[0], y[1]);
+        if constexpr (F16) rest[i] = pack_bf16x2(y[0] - low_bf16(p[i]), y[1] - high_bf16(p[i]));
+      }
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        o[r][2 * G + d] = Elem<false>::mfma(v[d], p, o[r][2 * G + d]);
+        if constexpr (F16) o[r][2 * G + d] = Elem<false>::mfma(v[d], rest, o[r][2 * G + d]);
+      }
+    }
+  }
+
+  // The rows' outputs, or (whole false: other keys of theirs are elsewhere) their
+  // sums.  slot(row, token, head): where to.
+  template <typename Slot>
+  __device__ __forceinline__ void store(const Window& a, const Ragged& rq, int kh, int row0, int nrows, int li, int lg,
+                                        bool whole, Slot slot) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = row0 + 16 * r + li;
+      if (row >= nrows) continue;
+      const int t = row / a.group, head = kh * a.group + row - t * a.group;
+      const int64_t token = rq.row0 + t;
+      if (whole) {
+        const float inv = l[r][0] == 0.f ? 0.f : 1.f / l[r][0];
+        uint16_t* d = a.out + token * a.out_row + head * a.out_head + 4 * lg * (SPREAD ? DV : 1);
+        if constexpr (SPREAD) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t w[DC];
+#pragma unroll
+            for (int e = 0; e < DC; ++e) w[e] = E::pack(o[r][2 * e][i] * inv, o[r][2 * e + 1][i] * inv);
+            if constexpr (DC == 4) *reinterpret_cast<u32x4*>(d + i * DV) = u32x4{w[0], w[1], w[2], w[3]};
+            else *reinterpret_cast<u32x2*>(d + i * DV) = u32x2{w[0], w[1]};
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < DV; ++e)
+            *reinterpret_cast<u32x2*>(d + 16 * e) = u32x2{E::pack(o[r][e][0] * inv, o[r][e][1] * inv),
+                                                          E::pack(o[r][e][2] * inv, o[r][e][3] * inv)};
+        }
+        if (a.lse && lg == 0) a.lse[token * a.q_heads + head] = log_sum(mx[r], exact[r]);
+      } else {
+        const int64_t at = slot(row, token, head);
+        float* d = a.part + at * D + 4 * lg * (SPREAD ? DV : 1);
+        if constexpr (SPREAD) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < DV; e += 4)
+              *reinterpret_cast<f32x4*>(d + i * DV + e) =
+                  f32x4{o[r][e][i], o[r][e + 1][i], o[r][e + 2][i], o[r][e + 3][i]};
+        } else {
+#pragma unroll
+          for (int e = 0; e < DV; ++e) *reinterpret_cast<f32x4*>(d + 16 * e) = o[r][e];
+        }
+        if (lg == 0) *reinterpret_cast<f32x4*>(a.stat + 4 * at) = f32x4{mx[r], l[r][0], exact[r], 0.f};
+      }
+    }
+  }
+};
+
+// Parts that the keys of a row group are cut into, of the `splits` that the grid has, by its
+// steps of 32 keys (twice those where two waves share a step): none below kWholeSteps, else
+// of min_steps at least.
+constexpr int kWholeSteps = 32, kCoarseSteps = 16, kFineSteps = 8;
+__device__ __forceinline__ int parts_of(const Window& a, int tiles, int wr) {
+  const int steps = tiles * wr;
+  return steps < kWholeSteps ? 1 : max(min(a.splits, steps / a.min_steps), 1);
+}
+// what the rows [first, first + RG) of a request's `nrows` see
+template <int RG>
+__device__ __forceinline__ Span group_span(const Window& a, const Ragged& rq, int first, int nrows) {
+  return span_of<5>(a, rq.first + first / a.group, rq.first + (min(first + RG, nrows) - 1) / a.group);
+}
+
+// Rows straight from memory: a workgroup's NW waves are WR row tiles of 16 R x NW/WR key
+// slices; each wave loads the keys and values of its steps into registers.
+template <int D, int R, int WR, int NW, bool F16, bool FP4>
+__global__ __launch_bounds__(64 * NW, 2) void window_kernel(Window a) {
+  using W = Rows<D, R, F16, !FP4>;
+  using E = Elem<F16>;
+  constexpr int DC = W::DC, DV = W::DV;
+  constexpr int WK = NW / WR;      // key slices
+  constexpr int RG = 16 * R * WR;  // rows of a workgroup
+  const int lane = threadIdx.x & 63;
+  const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+  const int li = lane & 15, lg = lane >> 4;
+  const int wr = wave % WR, wk = wave / WR;
+  // unit: (request, row group, key head), part
+  const int part = blockIdx.x % a.splits;
+  int unit = blockIdx.x / a.splits;
+  const int kh = unit % a.kv_heads;
+  unit /= a.kv_heads;
+  const int rg = unit % a.groups, b = unit / a.groups;
+  const Ragged rq = ragged(a, b);
+  const int nrows = rq.tokens * a.group;
+  if (rg * RG >= nrows) return;
+  const Span span = group_span<RG>(a, rq, rg * RG, nrows);
+  const int parts = parts_of(a, span.tiles, FP4 ? (WR + 1) / 2 : WR);
+  if (part >= parts) return;
+  const int pmin = rq.first + rg * RG / a.group, pmax = rq.first + (min(rg * RG + RG, nrows) - 1) / a.group;
+  const int row0 = rg * RG + wr * (16 * R);  // of this wave
+  const int t0 = static_cast<int>(static_cast<int64_t>(span.tiles) * part / parts);
+  const int t1 = static_cast<int>(static_cast<int64_t>(span.tiles) * (part + 1) / parts);
+  const int32_t* table = a.tables + b * a.tstride;
+
+  // the block ids of a step's two halves, loaded a step ahead of its keys (a half behind the
+  // last key reads the other one's block instead, and is masked)
+  auto first_of = [&](int key0, int h) { return key0 + (key0 + 16 * h <= pmax ? 16 * h : 0); };
+  auto ids = [&](int t, int (&id)[2]) {
+    if (t >= t1) return;
+    const int key0 = span.tile(t) * 32;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int slot;
+      // (not provably uniform: the value stays in a vector register, unwaited for, until
+      // it is used)
+      id[h] = table[block_of(a, first_of(key0, h), slot) + (here(lane) >> 6)];
+    }
+  };
+  int id[2] = {0, 0};
+  ids(t0 + wk, id);
+  W w;
+  w.load(a, rq, kh, min(row0, nrows - 1), nrows, li, lg);
+  const bool want = a.lse != nullptr;
+  for (int t = t0 + wk; t < t1; t += WK) {
+    const int key0 = span.tile(t) * 32;
+    bool bad[2];
+    int64_t blk[2];
+    int slot[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = uniform(id[h]);
+      bad[h] = i < 0 || i >= a.blocks;
+      blk[h] = bad[h] ? 0 : i;
+      block_of(a, first_of(key0, h), slot[h]);
+    }
+    const bool masked = bad[0] || bad[1] || !all_visible(a, key0, key0 + 31, pmin, pmax);
+    f32x4 s[R][2];
+    float x[R][8];
+    uint32_t ok[R];
+    if constexpr (FP4) {
+      Keys4<D> k;
+      Values4<D> v;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t row = row_of(a, blk[h], slot[h], kh);
+        load_keys4<D>(a, row, li, lg, k.k[h], k.s[h]);
+        load_values4<D>(a, row, li, lg, v.v[h], v.s[h]);
+      }
+      ids(t + WK, id);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r][h] = scores<D, F16>(k, h, w.q[r]);
+      w.weights(a, s, x, ok, key0, masked, bad[0], bad[1], lg);
+      w.add4(x, ok, v, masked);
+    } else {
+      Keys16<D> k;
+      Values16<D> v;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        load_keys<D>(a, blk[h], slot[h], kh, li, lg, k.k[h]);
+        load_values<D>(a, blk[h], slot[h], kh, li, lg, v.v + 4 * h);
+      }
+      ids(t + WK, id);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r][h] = scores<D, F16>(k, h, w.q[r]);
+      // No value that a row does not see may meet its weight 0 as an infinity or NaN: those
+      // of a masked step that are not finite are left out of the products (bit of `odd`) and
+      // added for the rows that see them.
+      uint32_t odd = 0;
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool gone = key0 + 16 * (e >> 2) + 4 * lg + (e & 3) > pmax || bad[e >> 2];
+          bool wild = false;
+#pragma unroll
+          for (int i = 0; i < DC; ++i) {
+            if (gone) v.v[e][i] = 0;
+            wild = wild || (v.v[e][i] & E::kExp) == E::kExp || (v.v[e][i] & E::kExp << 16) == E::kExp << 16;
+          }
+          const unsigned long long m = __ballot(wild);
+          if (m) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              if (m >> (16 * g) & 0xffff) odd |= 1u << (16 * (e >> 2) + 4 * g + (e & 3));
+            if (m >> (16 * lg) & 0xffff)
+#pragma unroll
+              for (int i = 0; i < DC; ++i) v.v[e][i] = 0;
+          }
+        }
+      }
+      w.weights(a, s, x, ok, key0, masked, bad[0], bad[1], lg);
+      auto values = [&](int d) {
+        u32x4 vt;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          vt[e] = __builtin_amdgcn_perm(v.v[2 * e + 1][d >> 1], v.v[2 * e][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
+        return vt;
+      };
+      w.add(a, x, values, key0, odd, want, li, lg, [&](int j) {
+        const int h = j >> 4;
+        const uint16_t* p = static_cast<const uint16_t*>(a.vc) + blk[h] * a.vc_block +
+                            static_cast<int64_t>(slot[h] + (j & 15)) * a.vc_slot + kh * a.vc_head;
+        return [p](int i) { return E::low(p[i]); };
+      });
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    w.exact[r] = quad_sum(w.exact[r]);
+    if constexpr (FP4) w.l[r][0] = w.exact[r];  // (4-bit: the weights are rounded once per scale group)
+  }
+
+  // join the key slices: slice 0 adds the others' sums, brought to one reference
+  if constexpr (WK > 1) {
+    __shared__ float lo_[(WK - 1) * WR][R][DV * 4][64];
+    __shared__ float ls_[(WK - 1) * WR][R][3][64];
+    if (wk > 0) {
+      const int n = (wk - 1) * WR + wr;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        ls_[n][r][0][lane] = w.mx[r];
+        ls_[n][r][1][lane] = w.l[r][0];
+        ls_[n][r][2][lane] = w.exact[r];
+#pragma unroll
+        for (int d = 0; d < DV; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) lo_[n][r][4 * d + i][lane] = w.o[r][d][i];
+      }
+    }
+    __syncthreads();
+    if (wk > 0) return;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float ref = w.mx[r];
+#pragma unroll
+      for (int s = 0; s < WK - 1; ++s) ref = fmaxf(ref, ls_[s * WR + wr][r][0][lane]);
+      const float f = __builtin_amdgcn_exp2f(w.mx[r] - ref);
+      w.mx[r] = ref;
+      w.l[r][0] *= f;
+      w.exact[r] *= f;
+#pragma unroll
+      for (int d = 0; d < DV; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.o[r][d][i] *= f;
+#pragma unroll
+      for (int s = 0; s < WK - 1; ++s) {
+        const int n = s * WR + wr;
+        const float g = __builtin_amdgcn_exp2f(ls_[n][r][0][lane] - ref);
+        w.l[r][0] += g * ls_[n][r][1][lane];
+        w.exact[r] += g * ls_[n][r][2][lane];
+#pragma unroll
+        for (int d = 0; d < DV; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w.o[r][d][i] += g * lo_[n][r][4 * d + i][lane];
+      }
+    }
+  }
+  w.store(a, rq, kh, row0, nrows, li, lg, parts == 1,
+          [&](int, int64_t token, int head) { return (token * a.q_heads + head) * a.splits + part; });
+}
+
+// Waves that join four rows: sixteen if those have eight parts and there are few of them, so
+// that the parts' latency counts, else one (and four times four rows a workgroup).
+constexpr int kJoinWaves = 16;
+inline bool join_by_many(int64_t parts, int64_t fours) { return parts >= 8 && fours <= 512; }
+constexpr int join_threads(int waves) { return waves == 1 ? 256 : 64 * waves; }
+
+// Behind window_kernel: four rows of a key head, of one row group.
+template <int D, bool F16, int WAVES, int RG>
+__global__ __launch_bounds__(join_threads(WAVES)) void window_join_kernel(Window a, int wr) {
+  const int lane = threadIdx.x & 63, li = lane & 15, wave = uniform(static_cast<int>(threadIdx.x >> 6));
+  int64_t u = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + wave : blockIdx.x;
+  const int quads = (a.max_tokens * a.group + 3) >> 2;
+  const int first = static_cast<int>(u % quads) * 4;
+  u /= quads;
+  const int kh = static_cast<int>(u % a.kv_heads), b = static_cast<int>(u / a.kv_heads);
+  if (b >= a.requests) return;
+  const Ragged rq = ragged(a, b);
+  const int rows = rq.tokens * a.group;
+  if (first >= rows) return;
+  const int parts = parts_of(a, group_span<RG>(a, rq, first / RG * RG, rows).tiles, wr);
+  if (parts == 1) return;
+  const int row = min(first + (lane >> 4), rows - 1), t = row / a.group, head = kh * a.group + row - t * a.group;
+  const int64_t of = static_cast<int64_t>(rq.row0 + t) * a.q_heads + head, at = of * a.splits;
+  uint16_t* p = a.out + (rq.row0 + t) * a.out_row + head * a.out_head + D / 16 * li;
+  join_rows<D, F16, WAVES, 4>(a.part, a.stat, parts, lane, wave, first + (lane >> 4) < rows ? p : nullptr,
+                              a.lse ? a.lse + of : nullptr, [&](int i) { return at + i; });
+}
+
+// The launch shape, a function of sizes the host knows (never of what the device
+// arrays hold, so that a captured call replays with other lengths).
+struct Plan {
+  int r, wr;  // row tiles per wave, waves per key slice (4-bit: one tile per wave, r times the waves)
+  int groups, splits, min_steps;
+};
+Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t max_tokens, int64_t max_context, int64_t window,
+          int64_t sinks) {
+  const int64_t rows = max_tokens * (q_heads / kv_heads);
+  Plan p{};
+  p.r = rows <= 16 ? 1 : 2;
+  p.wr = rows <= 32 ? 1 : 2;
+  p.groups = static_cast<int>((rows + 63) / 64);
+  const int64_t units = requests * kv_heads * p.groups;
+  const int64_t tokens = std::min<int64_t>(max_tokens, 64);  // of a row group
+  // (the most tokens that a row group sees)
+  const int64_t seen = window + std::min(sinks, max_context) + tokens >= max_context ? max_context : window + sinks + tokens;
+  const int64_t steps = (seen + 31) / 32 * p.wr;
+  p.min_steps = units * (steps / kCoarseSteps) <= 128 ? kFineSteps : kCoarseSteps;
+  p.splits = 1;
+  if (steps >= kWholeSteps)
+    p.splits = static_cast<int>(
+        std::max<int64_t>(1, std::min<int64_t>({(1024 + units - 1) / units, steps / p.min_steps, 256})));
+  return p;
+}
+int64_t slots_of(const Plan& p, int64_t rows, int64_t q_heads) { return p.splits == 1 ? 0 : rows * q_heads * p.splits; }
+size_t workspace_bytes(const Plan& p, int64_t rows, int64_t q_heads, int64_t head_dim) {
+  return static_cast<size_t>(slots_of(p, rows, q_heads)) * (head_dim + 4) * 4;
+}
+
+bool sizes_ok(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_tokens,
+              int64_t max_context, int64_t window, int64_t sinks) {
+  if (!(rows >= 0 && rows <= 0x7fffffff / 64 && requests >= 0 && requests <= 0x100000 && kv_heads >= 1 &&
+        q_heads >= kv_heads && q_heads % kv_heads == 0 && q_heads <= 4096 && (head_dim == 64 || head_dim == 128) &&
+        max_tokens >= 1 && max_tokens <= 0x7fffffff / 64 && max_context >= 0 && max_context <= 0x7fffffff && window >= 1 &&
+        window <= 0x7fffffff && sinks >= 0 && sinks <= 0x7fffffff))
+    return false;
+  const int64_t most = std::min(max_tokens, std::max<int64_t>(rows, 1)) * q_heads;  // rows x heads of a request
+  return most <= 0x3fffffff && requests * (most + 64 * kv_heads) <= int64_t{0x3fffffff};  // (grids are 32-bit)
+}
+
+template <int D, bool F16, bool FP4>
+int launch(const Window& a, const Plan& p, hipStream_t st) {
+  const dim3 g(static_cast<unsigned>(static_cast<int64_t>(a.requests) * a.kv_heads * p.groups * p.splits));
+  constexpr int R = FP4 ? 1 : 2;
+  if (p.r == 1) hipLaunchKernelGGL((window_kernel<D, 1, 1, 4, F16, FP4>), g, dim3(256), 0, st, a);
+  else if (p.wr == 1) hipLaunchKernelGGL((window_kernel<D, R, 2 / R, 4, F16, FP4>), g, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((window_kernel<D, R, 4 / R, 4, F16, FP4>), g, dim3(256), 0, st, a);
+  if (int rc = check_launch("window attention kernel")) return rc;
+  if (p.splits == 1) return PGS_OK;
+  const int64_t quads = static_cast<int64_t>(a.requests) * a.kv_heads * ((a.max_tokens * a.group + 3) / 4);
+  auto join = [&](auto waves, auto rg) {
+    constexpr int W = decltype(waves)::value;
+    hipLaunchKernelGGL((window_join_kernel<D, F16, W, decltype(rg)::value>),
+                       dim3(static_cast<unsigned>(W == 1 ? (quads + 3) / 4 : quads)), dim3(join_threads(W)), 0, st, a, p.wr);
+  };
+  auto by = [&](auto waves) {
+    if (p.r == 1) join(waves, Int<16>{});
+    else if (p.wr == 1) join(waves, Int<32>{});
+    else join(waves, Int<64>{});
+  };
+  if (join_by_many(p.splits, quads)) by(Int<kJoinWaves>{});
+  else by(Int<1>{});
+  return check_launch("window attention join kernel");
+}
+
+}  // namespace
+}  // namespace pgs
+
+using namespace pgs;
+
+extern "C" size_t pgs_window_attention_workspace_bytes(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads,
+                                                       int64_t head_dim, int64_t max_tokens, int64_t max_context,
+                                                       int64_t window, int64_t sinks) {
+  if (!sizes_ok(rows, requests, q_heads, kv_heads, head_dim, max_tokens, max_context, window, sinks) || rows == 0 ||
+      requests == 0)
+    return 0;
+  const Plan p = plan(requests, q_heads, kv_heads, std::min(max_tokens, rows), max_context, window, sinks);
+  return workspace_bytes(p, rows, q_heads, head_dim);
+}
+
+extern "C" int pgs_window_attention(const pgs_window_attention_args* args, void* workspace, size_t workspace_bytes_given,
+                                    void* stream) {
+  const char* fn = "pgs_window_attention";
+  if (!args) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: null arguments", fn);
+  const pgs_window_attention_args& g = *args;
+  if (g.dtype != PGS_DTYPE_BF16 && g.dtype != PGS_DTYPE_F16)
+    return fail(PGS_ERR_INVALID_ARGUMENT, "%s: dtype %d must be bf16 or fp16", fn, g.dtype);
+  Window a{};
+  if (int rc = take_cache(fn, a, g.cache, g.cache4, true, g.block_tables, g.table_stride, g.columns)) return rc;
+  const int64_t dim = g.cache ? g.cache->head_dim : g.cache4->head_dim;
+  if (!sizes_ok(g.rows, g.requests, g.q_heads, a.kv_heads, dim, g.max_tokens, g.max_context, g.window, g.sinks))
+    return fail(PGS_ERR_INVALID_ARGUMENT,
+                "%s: rows=%lld requests=%lld q_heads=%lld kv_heads=%d max_tokens=%lld window=%lld sinks=%lld: q_heads is a "
+                "multiple of kv_heads, max_tokens and window 1 at least, sinks 0 at least",
+                fn, (long long)g.rows, (long long)g.requests, (long long)g.q_heads, a.kv_heads, (long long)g.max_tokens,
+                (long long)g.window, (long long)g.sinks);
+  for (int64_t s : {g.q_row, g.q_head, g.out_row, g.out_head})
+    if (s < 0 || s % 8 != 0) return fail(PGS_ERR_MISALIGNED, "%s: strides must be multiples of 8 elements", fn);
+  if (!(g.scale == g.scale)) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: scale is NaN", fn);
+  if (g.rows == 0 || g.requests == 0) return PGS_OK;
+  if (!g.q || !g.out || !g.lens || !g.offsets) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
+  if (!aligned(g.q, 16) || !aligned(g.out, 16) || !aligned(g.lse, 4) || !aligned(g.lens, 4) || !aligned(g.offsets, 4))
+    return fail(PGS_ERR_MISALIGNED, "%s: misaligned", fn);
+  const int64_t most = std::min(g.max_tokens, g.rows);  // (no request has more rows than the batch)
+  const Plan p = plan(g.requests, g.q_heads, a.kv_heads, most, g.max_context, g.window, g.sinks);
+  const size_t need = workspace_bytes(p, g.rows, g.q_heads, dim);
+  if (need > 0 && (!workspace || workspace_bytes_given < need || !aligned(workspace, 256)))
+    return fail(PGS_ERR_INVALID_ARGUMENT, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (int rc = require_device(fn, st)) return rc;
+  a.q = static_cast<const uint16_t*>(g.q);
+  a.out = static_cast<uint16_t*>(g.out);
+  a.lse = g.lse;
+  a.q_row = g.q_row, a.q_head = g.q_head, a.out_row = g.out_row, a.out_head = g.out_head;
+  a.lens = g.lens, a.offsets = g.offsets;
+  a.rows = static_cast<int32_t>(g.rows), a.requests = static_cast<int32_t>(g.requests);
+  a.q_heads = static_cast<int32_t>(g.q_heads), a.group = a.q_heads / a.kv_heads;
+  a.max_tokens = static_cast<int32_t>(most);
+  a.window = static_cast<int32_t>(g.window), a.sinks = static_cast<int32_t>(g.sinks);
+  a.groups = p.groups, a.splits = p.splits, a.min_steps = p.min_steps;
+  a.c = g.scale * 1.44269504088896340736f;
+  a.part = static_cast<float*>(workspace);
+  a.stat = a.part + slots_of(p, g.rows, g.q_heads) * dim;
+  auto go = [&](auto d, auto f16) {
+    constexpr int D = decltype(d)::value;
+    constexpr bool F = decltype(f16)::value;
+    return g.cache ? launch<D, F, false>(a, p, st) : launch<D, F, true>(a, p, st);
+  };
+  if (dim == 64) return g.dtype == PGS_DTYPE_F16 ? go(Int<64>{}, Int<1>{}) : go(Int<64>{}, Int<0>{});
+  return g.dtype == PGS_DTYPE_F16 ? go(Int<128>{}, Int<1>{}) : go(Int<128>{}, Int<0>{});
+}
