@@ -712,7 +712,7 @@ std::vector<at::Tensor> window_attention(const at::Tensor& q, const std::vector<
   a.sinks = sinks;
   a.scale = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(dim)));
   const size_t need = pgs_window_attention_workspace_bytes(a.rows, a.requests, a.q_heads, kv_heads, dim, a.max_tokens,
-                                                           a.max_context, a.window, a.sinks);
+                                                           a.max_context, a.window, a.sinks, four);
   at::Tensor ws;  // (per call, as in tree_attention)
   if (need) ws = at::empty({static_cast<int64_t>(need)}, qr.options().dtype(at::kByte));
   void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();

@@ -47,6 +47,7 @@ struct Window {
   float c;      // scale * log2(e)
   float* part;  // sums of the parts of rows: [slots][D]
   float* stat;  // [slots][4]: reference, sum, sum of the weights before their rounding, -
+  int64_t* sums;  // (wide) [requests]: counts of work up to and with each request
 };
 
 // The request of a unit and its sizes, each brought into range: whatever the device

@@ -497,16 +497,409 @@ __global__ __launch_bounds__(join_threads(WAVES)) void window_join_kernel(Window
                               a.lse ? a.lse + of : nullptr, [&](int i) { return at + i; });
 }
 
+// ---------------------------------------------------------------------------
+// many rows
+// ---------------------------------------------------------------------------
+
+// The wide kernel's work: the tiles of all units, (request, key head, group of RG rows), in
+// that order, cut into equal shares for the workgroups, whatever the requests' rows and lengths
+// are.  What a group costs is counted in keys times `group`, so that it grows by RG from one
+// to the next until the window holds it, and sums over groups need no loop: group g of a
+// request costs min(base + RG (g + 1), cap) + unit (unit alone while that is below 0).  A share takes of each unit the part of
+// its tiles that its part of the counts covers; of a unit that is not whole it leaves sums
+// in slot 2 share (the unit began in an earlier share) or 2 share + 1.
+constexpr int kTile = 128;    // keys of a tile
+constexpr int kShares = 256;  // workgroups: one per CU
+constexpr int kUnit = 2 * kTile;  // what a unit costs besides its tiles, in keys
+
+struct Groups {
+  int n;            // of a request
+  int none, rising;  // those before `none` see nothing; those before `rising` cost less than cap
+  int64_t base, cap, unit;
+  // counts of the first m groups
+  template <int RG>
+  __device__ __forceinline__ int64_t upto(int m) const {
+    const int64_t lo = min(m, none), hi = min(m, rising);
+    return m * unit + (hi - lo) * base + RG * ((hi * (hi + 1) - lo * (lo + 1)) / 2) + (m - hi) * cap;
+  }
+};
+template <int RG>
+__device__ __forceinline__ Groups groups_of(const Window& a, const Ragged& rq) {
+  Groups g;
+  g.n = (rq.tokens * a.group + RG - 1) / RG;
+  g.base = static_cast<int64_t>(rq.first) * a.group;
+  // (the most that a group sees: its windows and the sinks)
+  g.cap = min<int64_t>(static_cast<int64_t>(a.window) + min(a.sinks, rq.len), rq.len) * a.group + RG;
+  g.none = static_cast<int>(min<int64_t>(max<int64_t>(-g.base, 0) / RG, g.n));
+  g.rising = static_cast<int>(min<int64_t>(max<int64_t>((g.cap - g.base) / RG, g.none), g.n));
+  g.unit = static_cast<int64_t>(kUnit) * a.group;
+  return g;
+}
+// A unit of T tiles costs at most T (3 kTile + 1) group + 2 RG counts, so that a share inside of it
+// has one of its tiles at least.
+__device__ __forceinline__ int shares_of(const Window& a, int64_t total) {
+  return static_cast<int>(min<int64_t>(kShares, max<int64_t>(1, total / (4 * (kTile * a.group + 128)))));
+}
+__device__ __forceinline__ int64_t share_begin(int64_t total, int g, int n) {
+  // (total * g may pass 64 bits only where total passes 2^54)
+  return total / n * g + total % n * g / n;
+}
+
+template <int RG, int NT>
+struct Work {
+  Window a;
+  int64_t* pre;   // LDS [NT]: counts up to and with request base + i
+  int64_t* wsum;  // LDS [NT / 64]
+  int base;
+  int64_t carry, total;
+  struct Unit {
+    Ragged rq;
+    int b, kh, rg;
+    int64_t begin, cost;  // where its counts begin, how many they are
+  };
+  // pre for the requests from `first` on; every thread must call it
+  __device__ __forceinline__ void fill(int first, int64_t before) {
+    const int thread = here(threadIdx.x), lane = thread & 63, wave = thread >> 6;
+    base = first;
+    carry = before;
+    int64_t v = 0;
+    if (first + thread < a.requests) {
+      const Groups g = groups_of<RG>(a, ragged(a, first + thread));
+      v = g.template upto<RG>(g.n) * a.kv_heads;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t o = __shfl_up(v, d);
+      if (lane >= d) v += o;
+    }
+    __syncthreads();  // (the last fill's readers are done)
+    if (lane == 63) wsum[wave] = v;
+    __syncthreads();
+    v += carry;
+    for (int i = 0; i < wave; ++i) v += wsum[i];
+    pre[thread] = v;
+    __syncthreads();
+  }
+  // the total; with `keep` the sums of all requests are left there for the join
+  __device__ __forceinline__ void start(int64_t* keep) {
+    const int thread = here(threadIdx.x);
+    total = 0;
+    for (int f = 0; f < a.requests; f += NT) {
+      fill(f, total);
+      if (keep && f + thread < a.requests) keep[f + thread] = pre[thread];
+      total = uniform64(pre[NT - 1]);
+    }
+    if (base) fill(0, 0);
+  }
+  // the unit at pos < total, pos not before the last call's
+  __device__ __forceinline__ Unit find(int64_t pos) {
+    while (pos >= uniform64(pre[NT - 1])) fill(base + NT, uniform64(pre[NT - 1]));
+    int lo = 0, hi = NT - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= pos) lo = mid + 1;
+      else hi = mid;
+    }
+    Unit u;
+    u.b = base + uniform(lo);
+    const Ragged rq = ragged(a, u.b);
+    u.rq = Ragged{uniform(rq.row0), uniform(rq.tokens), uniform(rq.len), uniform(rq.first)};
+    const Groups g = groups_of<RG>(a, u.rq);
+    const int64_t first = uniform64(lo ? pre[lo - 1] : carry), per = g.template upto<RG>(g.n);
+    u.kh = uniform(static_cast<int>((pos - first) / per));
+    const int64_t head = first + u.kh * per;
+    // the last group that begins by pos
+    int at = 0, end = g.n - 1;
+    while (at < end) {
+      const int mid = (at + end + 1) >> 1;
+      if (head + g.template upto<RG>(mid) <= pos) at = mid;
+      else end = mid - 1;
+    }
+    u.rg = uniform(at);
+    u.begin = head + g.template upto<RG>(u.rg);
+    u.cost = g.template upto<RG>(u.rg + 1) - g.template upto<RG>(u.rg);
+    return u;
+  }
+};
+// the first of a unit's `tiles` that lies behind `counts` of its cost
+__device__ __forceinline__ int tile_at(int64_t counts, int64_t cost, int tiles) {
+  return counts <= 0 ? 0 : counts >= cost ? tiles : static_cast<int>(counts * tiles / cost);
+}
+
+// NW waves of 16 R rows share tiles of 128 keys through LDS.  A tile goes from memory to LDS
+// past the registers, into the buffer that is not computed: one barrier per tile, and a load
+// has a tile's arithmetic to arrive.
+//
+// LDS rows are D/8 pieces of 16 bytes.  A wave reads keys as A operands, 16 keys x one
+// piece per access: piece p of key r lies at p ^ (r D / 128), so that the sixteen lanes
+// of an access meet all banks.  Values are read transposed, 4 keys x 16 dims per 16 lanes
+// (ds_read_b64_tr_b16: lane n gets dim n of the four keys), a pair of pieces of 16 keys per
+// access: they are exchanged in pairs, p ^ 2 (r D / 128).
+template <int D, int R, int NW, bool F16>
+__global__ __launch_bounds__(64 * NW, 1) void window_wide_kernel(Window a0) {
+  using W = Rows<D, R, F16, false>;
+  using E = Elem<F16>;
+  constexpr int TK = kTile, RG = 16 * R * NW;
+  constexpr int P = D / 8;            // pieces per row
+  constexpr int KI = 64 / P;          // keys of one wave-wide load
+  constexpr int KW = TK / NW;         // keys of a wave's loads
+  constexpr int J = KW / KI;          // loads per wave, tile and matrix
+  constexpr int H = KW / 16;          // halves of steps in them, each in one block
+  static_assert(KW % 16 == 0 && 16 % KI == 0);
+  __shared__ __attribute__((aligned(256))) uint16_t lkv[2][2][TK * D];  // (whole rows aligned: k_at)
+  __shared__ uint32_t lbad[2][TK / 16], lodd[2][TK / 16];  // of sixteen keys: absent; those whose values are not finite
+  __shared__ int64_t lpre[64 * NW], lsum[NW];
+  const int lane = threadIdx.x & 63;
+  const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+  // LDS byte addresses of this lane's pieces of the first step: key li, piece lg; and
+  // dims 4 (li % 4) .. +3 of key 4 lg + li / 4
+  const int li = lane & 15, lg = lane >> 4, vkey = 4 * lg + (li >> 2);
+  const uint32_t k_at = lds_address(lkv) + li * (2 * D) + 16 * (lg ^ (li * P / 16 & (P - 1)));
+  const uint32_t v_at = lds_address(lkv) + TK * D * 2 + vkey * (2 * D) +
+                        16 * ((li >> 1 & 1) ^ (2 * (vkey * P / 16) & (P - 1))) + 8 * (li & 1);
+  Work<RG, 64 * NW> work{again<Window>(), lpre, lsum, 0, 0, 0};
+  work.start(blockIdx.x == 0 ? work.a.sums : nullptr);
+  const int shares = shares_of(work.a, work.total), share = xcd_remap(blockIdx.x, gridDim.x);
+  if (share >= shares) return;
+  const int64_t begin = uniform64(share_begin(work.total, share, shares));
+  const int64_t end = uniform64(share_begin(work.total, share + 1, shares));
+
+  for (int64_t pos = begin; pos < end;) {
+    work.a = again<Window>();
+    const auto un = work.find(pos);
+    const Window& a = a0;
+    const Ragged& rq = un.rq;
+    const int nrows = rq.tokens * a.group, first_row = un.rg * RG;
+    const int pmin = rq.first + first_row / a.group, pmax = rq.first + (min(first_row + RG, nrows) - 1) / a.group;
+    const Span span = span_of<7>(a, pmin, pmax);
+    // this share's tiles of the unit
+    const int t0 = uniform(tile_at(pos - un.begin, un.cost, span.tiles));
+    const int t1 = uniform(tile_at(end - un.begin, un.cost, span.tiles));
+    pos = un.begin + un.cost;  // the next unit's
+    const bool whole = t0 == 0 && t1 == span.tiles;
+    if (t0 >= t1 && !(span.tiles == 0 && un.begin >= begin)) continue;
+    const int row0 = first_row + wave * (16 * R);  // of this wave
+    const bool active = row0 < nrows;
+    const int kh = un.kh;
+    // what this wave's rows are at
+    const int wmin = rq.first + min(row0, nrows - 1) / a.group, wmax = rq.first + (min(row0 + 16 * R, nrows) - 1) / a.group;
+
+    const int32_t* table = a.tables + un.b * a.tstride;
+    const uint16_t *kc = static_cast<const uint16_t*>(a.kc) + kh * a.kc_head;
+    const uint16_t *vc = static_cast<const uint16_t*>(a.vc) + kh * a.vc_head;
+    // Lane i: the blocks of this wave's keys of tile number id0 + i.  (Waited for where they are
+    // loaded: a wait for them further on would be one for the keys on their way too.)
+    int id_lane[H], id0 = -64;
+    // this share's i-th tile into buffer `to`; bit h: its half h of this wave's is absent
+    auto load = [&](int i, int to) {
+      const int ln = here(lane), kin = ln / P, piece = ln % P;
+      const uint32_t at_k = lds_address(lkv) + to * (4 * TK * D) + wave * (KW * 2 * D), at_v = at_k + 2 * TK * D;
+      const int t = span.tile(i);
+      if (t >= id0 + 64 || t < id0) {
+        id0 = t;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          int slot;
+          const int64_t key = min<int64_t>(static_cast<int64_t>(t + ln) * TK + wave * KW + 16 * h, pmax & ~15);
+          id_lane[h] = table[block_of(a, static_cast<int>(key), slot)];
+        }
+#pragma unroll
+        for (int h = 0; h < H; ++h) asm volatile("" : "+v"(id_lane[h]));
+      }
+      uint32_t bad = 0;
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        // (sixteen keys past the last one are the sixteen with the last one instead, and masked)
+        const int id = __builtin_amdgcn_readlane(id_lane[h], t - id0);
+        if (id < 0 || id >= a.blocks) bad |= 1u << h;
+        const int64_t blk = id < 0 || id >= a.blocks ? 0 : id;
+        int slot;
+        block_of(a, min(t * TK + wave * KW + 16 * h, pmax & ~15), slot);
+        const int64_t at0 = slot;
+        const uint16_t *kb = kc + blk * a.kc_block + at0 * a.kc_slot, *vb = vc + blk * a.vc_block + at0 * a.vc_slot;
+        // (lane l fills piece l % P of its key's row in LDS: the exchange picks what it reads)
+#pragma unroll
+        for (int j = 0; j < 16 / KI; ++j) {
+          const uint32_t at = j * KI + kin;
+          const int turn = (wave * KW + 16 * h + j * KI + kin) * P / 16;
+          load_lds(kb + at * a.kc_slot + 8 * (piece ^ (turn & (P - 1))), at_k + 1024 * (h * (16 / KI) + j));
+          load_lds(vb + at * a.vc_slot + 8 * (piece ^ (2 * turn & (P - 1))), at_v + 1024 * (h * (16 / KI) + j));
+        }
+      }
+      return bad;
+    };
+    // This wave's part of the i-th tile has arrived in buffer `in`: as in window_kernel, no
+    // infinity or NaN may meet a weight of 0.
+    auto settle = [&](int i, int in, uint32_t bad) {
+      const int ln = here(lane), kin = ln / P;
+      const int key0 = span.tile(i) * TK + wave * KW;
+      uint32_t odd[H] = {};
+      if (bad || !all_visible(a, key0, key0 + KW - 1, pmin, pmax)) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const int h = j * KI / 16;
+          u32x4* const at = reinterpret_cast<u32x4*>(&lkv[in][1][(wave * J + j) * 512 + 8 * ln]);
+          const bool gone = (bad >> h & 1) || key0 + j * KI + kin > pmax;
+          const u32x4 v = *at;
+          bool wild = false;
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            wild = wild || (v[x] & E::kExp) == E::kExp || (v[x] & E::kExp << 16) == E::kExp << 16;
+          const unsigned long long m = __ballot(wild && !gone), one = P == 16 ? 0xffffull : 0xffull;
+#pragma unroll
+          for (int k = 0; k < KI; ++k)
+            if (m >> (P * k) & one) odd[h] |= 1u << (j * KI % 16 + k);
+          if (gone || (m >> (P * kin) & one)) *at = u32x4{0, 0, 0, 0};
+        }
+      }
+      if (ln == 0) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) lbad[in][wave * H + h] = bad >> h & 1, lodd[in][wave * H + h] = odd[h];
+      }
+    };
+
+    // One barrier per tile.  Behind it, tile i is whole in its buffer and the one that held
+    // tile i - 1 is free: tile i + 1 is sent for, i is computed, and each wave waits for its
+    // part of i + 1.
+    uint32_t bad = t0 < t1 ? load(t0, 0) : 0;
+    W w;
+    if (active) {
+      const int ln = here(lane);
+      w.load(again<Window>(), rq, kh, row0, nrows, ln & 15, ln >> 4);
+    }
+    const bool want = a.lse != nullptr;
+    arrived<0>();
+    if (t0 < t1) settle(t0, 0, bad);
+    __syncthreads();
+    int buf = 0;
+    for (int i = t0; i < t1; ++i) {
+      if (i + 1 < t1) bad = load(i + 1, buf ^ 1);
+      if (active) {
+        const int tile0 = span.tile(i) * TK;
+        const int ln = here(lane);
+        const uint32_t bm = static_cast<uint32_t>(__ballot(ln < TK / 16 && lbad[buf][ln % (TK / 16)]));
+#pragma unroll 1
+        for (int h = 0; h < TK / 32; ++h) {
+          const int key0 = tile0 + 32 * h;
+          // (no row of this wave sees any of them)
+          if (key0 > wmax) break;
+          if (key0 + 31 <= low_of(wmin, a.window) && key0 >= a.sinks) continue;
+          const bool bad0 = bm >> (2 * h) & 1, bad1 = bm >> (2 * h + 1) & 1;
+          const bool masked = bad0 || bad1 || !all_visible(a, key0, key0 + 31, wmin, wmax);
+          // a piece's exchange is an exclusive or of its row's address with 16 bytes times
+          // the piece, halves of a step and steps are 16 and 32 whole rows apart
+          const uint32_t kat = k_at + buf * (4 * TK * D) + 32 * h * (2 * D);
+          const uint32_t vat = v_at + buf * (4 * TK * D) + 32 * h * (2 * D);
+          const int lg_ = here(lane) >> 4;
+          Keys16<D> k;
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) k.k[g][d] = *lds<const u32x4>((kat ^ (64 * d)) + 16 * g * (2 * D));
+          f32x4 s[R][2];
+          float x[R][8];
+          uint32_t ok[R];
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int r = 0; r < R; ++r) s[r][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+              for (int r = 0; r < R; ++r) s[r][g] = E::mfma(k.k[g][d], w.q[r][d], s[r][g]);
+          w.weights(a, s, x, ok, key0, masked, bad0, bad1, lg_);
+          auto values = [&](int d) {
+            const u32x2 y = read_transposed((vat ^ (32 * d))), z = read_transposed((vat ^ (32 * d)) + 16 * (2 * D));
+            return u32x4{y[0], y[1], z[0], z[1]};
+          };
+          uint32_t odd = 0;
+          if (masked) odd = lodd[buf][2 * h] | lodd[buf][2 * h + 1] << 16;
+          const int ln = here(lane);
+          w.add(a, x, values, key0, uniform(static_cast<int>(odd)), want, ln & 15, ln >> 4, [&](int j) {
+            int slot;
+            const int id = table[block_of(a, key0 + j, slot)];
+            const uint16_t* p = vc + static_cast<int64_t>(id) * a.vc_block + static_cast<int64_t>(slot) * a.vc_slot;
+            return [p](int e) { return E::low(p[e]); };
+          });
+        }
+      }
+      if (i + 1 < t1) {
+        arrived<0>();
+        settle(i + 1, buf ^ 1, bad);
+      }
+      buf ^= 1;
+      __syncthreads();
+    }
+    if (active) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) w.exact[r] = quad_sum(w.exact[r]);
+      const int64_t slot0 = static_cast<int64_t>(2 * share + (un.begin >= begin)) * RG - first_row;
+      const int ln = here(lane);
+      w.store(again<Window>(), rq, kh, row0, nrows, ln & 15, ln >> 4, whole, [&](int row, int64_t, int) { return slot0 + row; });
+    }
+  }
+}
+
+// Behind window_wide_kernel: four rows of a key head; those of whole units are already written.
+template <int D, bool F16, int RG>
+__global__ __launch_bounds__(join_threads(1)) void window_wide_join_kernel(Window a) {
+  const int lane = threadIdx.x & 63, li = lane & 15, wave = uniform(static_cast<int>(threadIdx.x >> 6));
+  int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + wave;
+  const int quads = (a.max_tokens * a.group + 3) >> 2;
+  const int first = static_cast<int>(u % quads) * 4;
+  u /= quads;
+  const int kh = static_cast<int>(u % a.kv_heads), b = static_cast<int>(u / a.kv_heads);
+  if (b >= a.requests) return;
+  const Ragged rq = ragged(a, b);
+  const int rows = rq.tokens * a.group;
+  if (first >= rows) return;
+  const Groups g = groups_of<RG>(a, rq);
+  const int64_t total = a.sums[a.requests - 1];
+  const int n = shares_of(a, total), rg = first / RG;
+  const int64_t begin = (b ? a.sums[b - 1] : 0) + kh * g.template upto<RG>(g.n) + g.template upto<RG>(rg);
+  const int64_t cost = g.template upto<RG>(rg + 1) - g.template upto<RG>(rg);
+  const Span span = span_of<7>(a, rq.first + rg * RG / a.group, rq.first + (min(rg * RG + RG, rows) - 1) / a.group);
+  // the share that position `at` is in
+  auto share = [&](int64_t at) {
+    int k = static_cast<int>(min<int64_t>(at / max<int64_t>(total / n, 1), n - 1));
+    while (share_begin(total, k, n) > at) --k;
+    while (k + 1 < n && share_begin(total, k + 1, n) <= at) ++k;
+    return k;
+  };
+  const int g0 = share(begin), g1 = share(begin + cost - 1);
+  if (g0 == g1 || span.tiles == 0) return;
+  // (shares at either end may have none of the tiles)
+  auto has = [&](int k) {
+    return tile_at(share_begin(total, k, n) - begin, cost, span.tiles) <
+           tile_at(share_begin(total, k + 1, n) - begin, cost, span.tiles);
+  };
+  int s0 = g0, s1 = g1;
+  while (s0 < s1 && !has(s0)) ++s0;
+  while (s1 > s0 && !has(s1)) --s1;
+  if (s0 == s1) return;
+  const int row = min(first + (lane >> 4), rows - 1), t = row / a.group, head = kh * a.group + row - t * a.group;
+  uint16_t* p = a.out + (rq.row0 + t) * a.out_row + head * a.out_head + D / 16 * li;
+  join_rows<D, F16, 1, 4>(a.part, a.stat, s1 - s0 + 1, lane, wave, first + (lane >> 4) < rows ? p : nullptr,
+                          a.lse ? a.lse + static_cast<int64_t>(rq.row0 + t) * a.q_heads + head : nullptr,
+                          [&](int i) { return static_cast<int64_t>(2 * (s0 + i) + (s0 + i == g0)) * RG + row - rg * RG; });
+}
+
 // The launch shape, a function of sizes the host knows (never of what the device
 // arrays hold, so that a captured call replays with other lengths).
 struct Plan {
-  int r, wr;  // row tiles per wave, waves per key slice (4-bit: one tile per wave, r times the waves)
+  int wide;   // rows of a group that share tiles through LDS, or 0
+  int r, wr;  // else row tiles per wave, waves per key slice (4-bit: one tile per wave, r times the waves)
   int groups, splits, min_steps;
 };
 Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t max_tokens, int64_t max_context, int64_t window,
-          int64_t sinks) {
+          int64_t sinks, bool fp4) {
   const int64_t rows = max_tokens * (q_heads / kv_heads);
   Plan p{};
+  p.splits = 1;
+  p.wide = rows <= 64 || fp4 ? 0 : rows <= 128 ? 128 : 256;
+  if (p.wide) return p;
   p.r = rows <= 16 ? 1 : 2;
   p.wr = rows <= 32 ? 1 : 2;
   p.groups = static_cast<int>((rows + 63) / 64);
@@ -516,15 +909,16 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t max_token
   const int64_t seen = window + std::min(sinks, max_context) + tokens >= max_context ? max_context : window + sinks + tokens;
   const int64_t steps = (seen + 31) / 32 * p.wr;
   p.min_steps = units * (steps / kCoarseSteps) <= 128 ? kFineSteps : kCoarseSteps;
-  p.splits = 1;
   if (steps >= kWholeSteps)
     p.splits = static_cast<int>(
         std::max<int64_t>(1, std::min<int64_t>({(1024 + units - 1) / units, steps / p.min_steps, 256})));
   return p;
 }
-int64_t slots_of(const Plan& p, int64_t rows, int64_t q_heads) { return p.splits == 1 ? 0 : rows * q_heads * p.splits; }
-size_t workspace_bytes(const Plan& p, int64_t rows, int64_t q_heads, int64_t head_dim) {
-  return static_cast<size_t>(slots_of(p, rows, q_heads)) * (head_dim + 4) * 4;
+int64_t slots_of(const Plan& p, int64_t rows, int64_t q_heads) {
+  return p.wide ? int64_t{2} * kShares * p.wide : p.splits == 1 ? 0 : rows * q_heads * p.splits;
+}
+size_t workspace_bytes(const Plan& p, int64_t rows, int64_t requests, int64_t q_heads, int64_t head_dim) {
+  return static_cast<size_t>(slots_of(p, rows, q_heads)) * (head_dim + 4) * 4 + (p.wide ? 8 * requests : 0);
 }
 
 bool sizes_ok(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_tokens,
@@ -538,8 +932,20 @@ bool sizes_ok(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads,
   return most <= 0x3fffffff && requests * (most + 64 * kv_heads) <= int64_t{0x3fffffff};  // (grids are 32-bit)
 }
 
+template <int D, int R, int NW, bool F16>
+int launch_wide(const Window& a, hipStream_t st) {
+  constexpr int RG = 16 * R * NW;
+  hipLaunchKernelGGL((window_wide_kernel<D, R, NW, F16>), dim3(kShares), dim3(64 * NW), 0, st, a);
+  if (int rc = check_launch("window attention kernel")) return rc;
+  const int64_t quads = static_cast<int64_t>(a.requests) * a.kv_heads * ((a.max_tokens * a.group + 3) / 4);
+  hipLaunchKernelGGL((window_wide_join_kernel<D, F16, RG>), dim3(static_cast<unsigned>((quads + 3) / 4)), dim3(256), 0, st, a);
+  return check_launch("window attention join kernel");
+}
+
 template <int D, bool F16, bool FP4>
 int launch(const Window& a, const Plan& p, hipStream_t st) {
+  if constexpr (!FP4)
+    if (p.wide) return p.wide == 128 ? launch_wide<D, 1, 8, F16>(a, st) : launch_wide<D, 2, 8, F16>(a, st);
   const dim3 g(static_cast<unsigned>(static_cast<int64_t>(a.requests) * a.kv_heads * p.groups * p.splits));
   constexpr int R = FP4 ? 1 : 2;
   if (p.r == 1) hipLaunchKernelGGL((window_kernel<D, 1, 1, 4, F16, FP4>), g, dim3(256), 0, st, a);
@@ -570,12 +976,12 @@ using namespace pgs;
 
 extern "C" size_t pgs_window_attention_workspace_bytes(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads,
                                                        int64_t head_dim, int64_t max_tokens, int64_t max_context,
-                                                       int64_t window, int64_t sinks) {
+                                                       int64_t window, int64_t sinks, int four_bits) {
   if (!sizes_ok(rows, requests, q_heads, kv_heads, head_dim, max_tokens, max_context, window, sinks) || rows == 0 ||
       requests == 0)
     return 0;
-  const Plan p = plan(requests, q_heads, kv_heads, std::min(max_tokens, rows), max_context, window, sinks);
-  return workspace_bytes(p, rows, q_heads, head_dim);
+  const Plan p = plan(requests, q_heads, kv_heads, std::min(max_tokens, rows), max_context, window, sinks, four_bits);
+  return workspace_bytes(p, rows, requests, q_heads, head_dim);
 }
 
 extern "C" int pgs_window_attention(const pgs_window_attention_args* args, void* workspace, size_t workspace_bytes_given,
@@ -602,8 +1008,8 @@ extern "C" int pgs_window_attention(const pgs_window_attention_args* args, void*
   if (!aligned(g.q, 16) || !aligned(g.out, 16) || !aligned(g.lse, 4) || !aligned(g.lens, 4) || !aligned(g.offsets, 4))
     return fail(PGS_ERR_MISALIGNED, "%s: misaligned", fn);
   const int64_t most = std::min(g.max_tokens, g.rows);  // (no request has more rows than the batch)
-  const Plan p = plan(g.requests, g.q_heads, a.kv_heads, most, g.max_context, g.window, g.sinks);
-  const size_t need = workspace_bytes(p, g.rows, g.q_heads, dim);
+  const Plan p = plan(g.requests, g.q_heads, a.kv_heads, most, g.max_context, g.window, g.sinks, !g.cache);
+  const size_t need = workspace_bytes(p, g.rows, g.requests, g.q_heads, dim);
   if (need > 0 && (!workspace || workspace_bytes_given < need || !aligned(workspace, 256)))
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -621,6 +1027,7 @@ extern "C" int pgs_window_attention(const pgs_window_attention_args* args, void*
   a.c = g.scale * 1.44269504088896340736f;
   a.part = static_cast<float*>(workspace);
   a.stat = a.part + slots_of(p, g.rows, g.q_heads) * dim;
+  a.sums = reinterpret_cast<int64_t*>(a.stat + slots_of(p, g.rows, g.q_heads) * 4);
   auto go = [&](auto d, auto f16) {
     constexpr int D = decltype(d)::value;
     constexpr bool F = decltype(f16)::value;

@@ -135,12 +135,15 @@ def test_nothing_to_do(native_lib):
 
 
 def test_workspaces(native_lib):
-    need = native_lib.pgs_window_attention_workspace_bytes
+    def need(*sizes, four=0):
+        return native_lib.pgs_window_attention_workspace_bytes(*sizes, four)
+
     assert need(1, 1, 16, 2, 128, 1, 64, 64, 0) == 0
     assert need(1, 1, 16, 2, 128, 1, 100000, 1 << 30, 0) > 0
     # a window bounds the split whatever the context, and no request has more rows than the batch
     assert need(1, 1, 16, 2, 128, 1, 100000, 100, 4) == 0
     assert need(1, 1, 16, 2, 128, 1, 100000, 1 << 30, 0) == need(1, 1, 16, 2, 128, 500, 100000, 1 << 30, 0)
+    assert need(900, 1, 16, 2, 128, 900, 100000, 1 << 30, 0) > 0
     assert need(-1, 1, 16, 2, 128, 1, 64, 64, 0) == 0 and need(1, 1, 15, 2, 128, 1, 64, 64, 0) == 0
     assert native_lib.pgs_evict_tokens_workspace_bytes(3, 100) == 3 * 101 * 4
     assert native_lib.pgs_evict_tokens_workspace_bytes(0, 100) == 0
