@@ -41,6 +41,11 @@ __device__ __forceinline__ u32x2 read_transposed(uint32_t address) {
 __device__ __forceinline__ void load_lds(const uint16_t* p, uint32_t address) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(address), "v"(p) : "m0", "memory");
 }
+// The same from `base` (wave-uniform) + the lane's `offset` bytes.
+__device__ __forceinline__ void load_lds(const void* base, uint32_t offset, uint32_t address) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(address), "v"(offset), "s"(base)
+               : "m0", "memory");
+}
 template <int N>
 __device__ __forceinline__ void arrived() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");

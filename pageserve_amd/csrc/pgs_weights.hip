@@ -37,7 +37,7 @@ __global__ __launch_bounds__(64 * kWaves) void weigh_kernel(Weigh g) {
     const int key0 = static_cast<int>(tile) * kTile + 32 * wave;
     // the rows that see some of them
     int t0 = max(0, key0 - rq.first), t1 = rq.tokens;
-    if (key0 >= a.sinks) t1 = static_cast<int>(min<int64_t>(t1, static_cast<int64_t>(key0) + 31 + a.window - rq.first));
+    if (key0 >= a.sinks) t1 = static_cast<int>(least(t1, static_cast<int64_t>(key0) + 31 + a.window - rq.first));
     if (t0 >= t1 && key0 + 32 <= fresh) continue;
     bool bad[2];
     int64_t blk[2];
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(Evict a) {
   const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6;
   const int b = blockIdx.x;
   const int64_t room = static_cast<int64_t>(a.cols) * a.bs;
-  const int len = static_cast<int>(min<int64_t>(max(a.lens[b], 0), room));
+  const int len = static_cast<int>(least(max(a.lens[b], 0), room));
   const int most = max(a.budget[b], 0);
   const int32_t* table = a.tables + b * a.tstride;
   if (len <= most || len > a.most) {

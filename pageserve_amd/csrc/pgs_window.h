@@ -25,6 +25,16 @@
 namespace pgs {
 namespace {
 
+// (the device's own min and max of two 64-bit integers go by way of doubles)
+__device__ __forceinline__ int64_t least(int64_t a, int64_t b) { return a < b ? a : b; }
+__device__ __forceinline__ int64_t largest(int64_t a, int64_t b) { return a > b ? a : b; }
+
+// A unit of work whose first part a share computed and the rest others; b < 0: none.
+struct Begun {
+  int32_t b, kh, rg, slot;  // slot: which of the share's two holds its sums
+  int64_t begin, cost, total;
+};
+
 struct Window {
   const uint16_t* q;
   uint16_t* out;
@@ -44,10 +54,11 @@ struct Window {
   int32_t rows, requests, q_heads, kv_heads, group;  // group: q_heads / kv_heads
   int32_t max_tokens, window, sinks;
   int32_t groups, splits, min_steps;  // row groups of a request; parts of the keys
-  float c;      // scale * log2(e)
+  float c;      // |scale| * log2(e) (accumulate_weights: signed)
+  uint32_t flip;  // the sign bits of a negative scale, for the rows
   float* part;  // sums of the parts of rows: [slots][D]
   float* stat;  // [slots][4]: reference, sum, sum of the weights before their rounding, -
-  int64_t* sums;  // (wide) [requests]: counts of work up to and with each request
+  Begun* begun;   // (wide) [shares]
 };
 
 // The request of a unit and its sizes, each brought into range: whatever the device
@@ -63,7 +74,7 @@ __device__ __forceinline__ Ragged ragged(const Args& a, int b) {
   r.row0 = lo;
   r.tokens = min(hi - lo, a.max_tokens);
   const int64_t most = static_cast<int64_t>(a.cols) * a.bs;
-  r.len = static_cast<int>(min<int64_t>(max(a.lens[b], 0), most));
+  r.len = static_cast<int>(least(max(a.lens[b], 0), most));
   r.first = r.len - (hi - lo);
   return r;
 }

@@ -10,11 +10,28 @@
 // tokens x query heads of one key head as columns, so that a row's scores, maximum, sums and
 // output stay in the lanes l%16 = row.
 #include <algorithm>
+#include <cmath>
 
 #include "pgs_window.h"
 
 namespace pgs {
 namespace {
+
+// The order of a block that has M matrix products, T exponentials and V more vector
+// instructions: the others spread between the products.
+template <int M, int T, int V>
+__device__ __forceinline__ void interleave() {
+  auto part = [](int i, int n) { return (i + 1) * n / M - i * n / M; };
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      if (n < part(i, V)) __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
+      if (n < part(i, T)) __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+    }
+  }
+}
 
 // 16 R rows of a wave and their running sums.  The output MFMA d covers the dims
 // (4 lg + i) D/16 + d of its lanes (SPREAD: values straight from 16-bit rows), or 16 d + 4 lg + i.
@@ -25,7 +42,7 @@ struct Rows {
   u32x4 q[R][DC];
   f32x4 o[R][DV], l[R];  // (l: every element the same)
   float exact[R], mx[R];  // the lane's own part of the weights' sum before they are rounded; the reference
-  int pos[R], low[R];     // where the row stands; pos - window
+  int pos[R];  // where the row stands
   bool far;               // some row's reference is beyond kFar (the same in all lanes)
 
   __device__ __forceinline__ void load(const Window& a, const Ragged& rq, int kh, int row0, int nrows, int li, int lg) {
@@ -34,9 +51,8 @@ struct Rows {
       const int row = min(row0 + 16 * r + li, nrows - 1), t = row / a.group;  // (rows past the last repeat it)
       const uint16_t* p = a.q + (rq.row0 + t) * a.q_row + (kh * a.group + row - t * a.group) * a.q_head + 8 * lg;
 #pragma unroll
-      for (int d = 0; d < DC; ++d) q[r][d] = ld16(p + 32 * d);
+      for (int d = 0; d < DC; ++d) q[r][d] = ld16(p + 32 * d) ^ a.flip;
       pos[r] = rq.first + t;
-      low[r] = low_of(pos[r], a.window);
     }
     // (they have arrived here: a wait for them inside the loop over the keys would be
     // a wait for the keys on their way too)
@@ -55,68 +71,82 @@ struct Rows {
     }
   }
 
-  // Weights of a step: s[r][h] the scores of keys key0 + 16 h + 4 lg + i, x[r][4 h + i] the
-  // weights' exponents against the rows' references, which are raised first where a score
-  // needs it.  masked: some row may not see some key, or a half's block is absent (bad).
-  __device__ __forceinline__ void weights(const Window& a, const f32x4 (&s)[R][2], float (&x)[R][8], uint32_t (&ok)[R],
-                                          int key0, bool masked, bool bad0, bool bad1, int lg) {
+  // New references, the largest score of each row so far, if a score x[r][e] (of those in
+  // ok[r]) passes its row's by too much.
+  __device__ __forceinline__ void raise(const Window& a, const float (&x)[R][8], const uint32_t (&ok)[R]) {
+    float top[R];
     bool over = false;
-    if (masked || far) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        ok[r] = 0;
+    for (int r = 0; r < R; ++r) {
+      top[r] = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int key = key0 + 16 * (e >> 2) + 4 * lg + (e & 3);
-          const bool in = visible(key, pos[r], low[r], a.sinks) && !(e >> 2 ? bad1 : bad0);
-          ok[r] |= in ? 1u << e : 0;
-          x[r][e] = in ? exponent(s[r][e >> 2][e & 3], a.c, mx[r], far) : -INFINITY;
-          over = over || x[r][e] > kSlack + E::kHead;
-        }
-      }
-    } else {
+      for (int e = 0; e < 8; ++e) top[r] = fmaxf(top[r], ok[r] >> e & 1 ? x[r][e] * a.c : -INFINITY);
+      over = over || top[r] - mx[r] > kSlack + E::kHead;
+    }
+    if (!__ballot(over)) return;
+    bool beyond = false;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        ok[r] = 0xff;
-        float top = -INFINITY;
+    for (int r = 0; r < R; ++r) {
+      const float t = quad_max(top[r]);
+      const float ref = fmaxf(fabsf(t) > kFar ? t : t - E::kHead, mx[r]), f = __builtin_amdgcn_exp2f(mx[r] - ref);
+      mx[r] = ref;
+      beyond = beyond || fabsf(ref) > kFar;
+      exact[r] *= f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[r][e] = fmaf(s[r][e >> 2][e & 3], a.c, -mx[r]);
-          top = fmaxf(top, x[r][e]);
-        }
-        over = over || top > kSlack + E::kHead;
+      for (int i = 0; i < 4; ++i) l[r][i] *= f;
+#pragma unroll
+      for (int d = 0; d < DV; ++d) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[r][d][i] *= f;
       }
     }
-    if (__ballot(over)) {
-      // new references: the largest score of each row so far
-      bool beyond = false;
+    far = __ballot(beyond);
+  }
+  // which of the step's eight keys of this lane its row r sees
+  __device__ __forceinline__ uint32_t seen(const Window& a, int r, int key0, bool bad0, bool bad1, int lg) const {
+    const int low = low_of(pos[r], a.window);
+    uint32_t ok = 0;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float t = -INFINITY;
+    for (int e = 0; e < 8; ++e) {
+      const int key = key0 + 16 * (e >> 2) + 4 * lg + (e & 3);
+      ok |= visible(key, pos[r], low, a.sinks) && !(e >> 2 ? bad1 : bad0) ? 1u << e : 0;
+    }
+    return ok;
+  }
+  // Weights of a step: s[r][h] the scores of keys key0 + 16 h + 4 lg + i, x[r][4 h + i] the
+  // weights against the rows' references, which are raised first where a score needs it.
+  // masked: some row may not see some key, or a half's block is absent (bad).
+  __device__ __forceinline__ void weights(const Window& a, const f32x4 (&s)[R][2], float (&x)[R][8], int key0, bool masked,
+                                          bool bad0, bool bad1, int lg) {
+    bool over = masked || far;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t = fmaxf(t, ok[r] >> e & 1 ? s[r][e >> 2][e & 3] * a.c : -INFINITY);
-        t = quad_max(t);
-        const float ref = fmaxf(fabsf(t) > kFar ? t : t - E::kHead, mx[r]), f = __builtin_amdgcn_exp2f(mx[r] - ref);
-        mx[r] = ref;
-        beyond = beyond || fabsf(ref) > kFar;
-        exact[r] *= f;
+    for (int r = 0; r < R; ++r) {
+      float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) l[r][i] *= f;
-#pragma unroll
-        for (int d = 0; d < DV; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[r][d][i] *= f;
+      for (int e = 0; e < 8; ++e) {
+        x[r][e] = s[r][e >> 2][e & 3];
+        top = fmaxf(top, x[r][e]);
       }
-      far = __ballot(beyond);
+      over = over || fmaf(top, a.c, -mx[r]) > kSlack + E::kHead;
+    }
+    uint32_t ok[R];
+    if (__ballot(over)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) ok[r] = masked ? seen(a, r, key0, bad0, bad1, lg) : 0xff;
+      raise(a, x, ok);
+    }
+    if (masked || far) {
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[r][e] = ok[r] >> e & 1 ? exponent(s[r][e >> 2][e & 3], a.c, mx[r], far) : -INFINITY;
+        for (int e = 0; e < 8; ++e)
+          x[r][e] = ok[r] >> e & 1 ? __builtin_amdgcn_exp2f(exponent(x[r][e], a.c, mx[r], far)) : 0.f;
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[r][e] = __builtin_amdgcn_exp2f(fmaf(x[r][e], a.c, -mx[r]));
     }
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[r][e] = __builtin_amdgcn_exp2f(x[r][e]);
   }
 
   // The step's part of the sums and outputs, the weights rounded to the rows' type; the row
@@ -144,6 +174,10 @@ struct Rows {
 #pragma unroll
       for (int r = 0; r < R; ++r) o[r][d] = E::mfma(v, p[r], o[r][d]);
     }
+    if (odd) add_odd(a, p, key0, odd, li, lg, value);
+  }
+  template <typename Value>
+  __device__ __forceinline__ void add_odd(const Window& a, const u32x4 (&p)[R], int key0, uint32_t odd, int li, int lg, Value value) {
     for (uint32_t w = odd; w; w &= w - 1) {
       const int j = __builtin_ctz(w);
       const auto row = value(j);
@@ -151,11 +185,15 @@ struct Rows {
       for (int r = 0; r < R; ++r) {
         const uint32_t lo = j & 2 ? p[r][1] : p[r][0], hi = j & 2 ? p[r][3] : p[r][2];
         const float pj = E::low(__shfl(j & 16 ? hi : lo, 16 * (j >> 2 & 3) + li) >> (16 * (j & 1)));
-        if (!visible(key0 + j, pos[r], low[r], a.sinks)) continue;
+        const bool in = visible(key0 + j, pos[r], low_of(pos[r], a.window), a.sinks);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int d = 0; d < DV; ++d) {
 #pragma unroll
-          for (int d = 0; d < DV; ++d) o[r][d][i] += pj * row(SPREAD ? (4 * lg + i) * DV + d : 16 * d + 4 * lg + i);
+          for (int i = 0; i < 4; ++i) {
+            const float y = o[r][d][i] + pj * row(SPREAD ? (4 * lg + i) * DV + d : 16 * d + 4 * lg + i);
+            o[r][d][i] = in ? y : o[r][d][i];
+          }
+        }
       }
     }
   }
@@ -165,8 +203,13 @@ struct Rows {
   // leave fp16's range; the codes are exact in both), in two terms where they are fp16, whose
   // finer rounding the output shall have.  A token that is not seen has weight 0 whatever its
   // scale holds.
-  __device__ __forceinline__ void add4(const float (&x)[R][8], const uint32_t (&ok)[R], const Values4<D>& n, bool masked) {
+  __device__ __forceinline__ void add4(const Window& a, const float (&x)[R][8], const Values4<D>& n, int key0, bool masked,
+                                       bool bad0, bool bad1, int lg) {
     static_assert(!SPREAD, "the codes' order");
+    uint32_t ok[R] = {};
+    if (masked)
+#pragma unroll
+      for (int r = 0; r < R; ++r) ok[r] = seen(a, r, key0, bad0, bad1, lg);
 #pragma unroll
     for (int r = 0; r < R; ++r)
       exact[r] += ((x[r][0] + x[r][1]) + (x[r][2] + x[r][3])) + ((x[r][4] + x[r][5]) + (x[r][6] + x[r][7]));
@@ -343,7 +386,6 @@ __global__ __launch_bounds__(64 * NW, 2) void window_kernel(Window a) {
     const bool masked = bad[0] || bad[1] || !all_visible(a, key0, key0 + 31, pmin, pmax);
     f32x4 s[R][2];
     float x[R][8];
-    uint32_t ok[R];
     if constexpr (FP4) {
       Keys4<D> k;
       Values4<D> v;
@@ -358,8 +400,8 @@ __global__ __launch_bounds__(64 * NW, 2) void window_kernel(Window a) {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int r = 0; r < R; ++r) s[r][h] = scores<D, F16>(k, h, w.q[r]);
-      w.weights(a, s, x, ok, key0, masked, bad[0], bad[1], lg);
-      w.add4(x, ok, v, masked);
+      w.weights(a, s, x, key0, masked, bad[0], bad[1], lg);
+      w.add4(a, x, v, key0, masked, bad[0], bad[1], lg);
     } else {
       Keys16<D> k;
       Values16<D> v;
@@ -398,7 +440,7 @@ __global__ __launch_bounds__(64 * NW, 2) void window_kernel(Window a) {
           }
         }
       }
-      w.weights(a, s, x, ok, key0, masked, bad[0], bad[1], lg);
+      w.weights(a, s, x, key0, masked, bad[0], bad[1], lg);
       auto values = [&](int d) {
         u32x4 vt;
 #pragma unroll
@@ -508,9 +550,9 @@ __global__ __launch_bounds__(join_threads(WAVES)) void window_join_kernel(Window
 // request costs min(base + RG (g + 1), cap) + unit (unit alone while that is below 0).  A share takes of each unit the part of
 // its tiles that its part of the counts covers; of a unit that is not whole it leaves sums
 // in slot 2 share (the unit began in an earlier share) or 2 share + 1.
-constexpr int kTile = 128;    // keys of a tile
+constexpr int kTileBits = 6, kTile = 1 << kTileBits;  // keys of a tile
 constexpr int kShares = 256;  // workgroups: one per CU
-constexpr int kUnit = 2 * kTile;  // what a unit costs besides its tiles, in keys
+constexpr int kUnit = 256;    // what a unit costs besides its tiles, in keys
 
 struct Groups {
   int n;            // of a request
@@ -529,16 +571,16 @@ __device__ __forceinline__ Groups groups_of(const Window& a, const Ragged& rq) {
   g.n = (rq.tokens * a.group + RG - 1) / RG;
   g.base = static_cast<int64_t>(rq.first) * a.group;
   // (the most that a group sees: its windows and the sinks)
-  g.cap = min<int64_t>(static_cast<int64_t>(a.window) + min(a.sinks, rq.len), rq.len) * a.group + RG;
-  g.none = static_cast<int>(min<int64_t>(max<int64_t>(-g.base, 0) / RG, g.n));
-  g.rising = static_cast<int>(min<int64_t>(max<int64_t>((g.cap - g.base) / RG, g.none), g.n));
+  g.cap = least(static_cast<int64_t>(a.window) + min(a.sinks, rq.len), rq.len) * a.group + RG;
+  g.none = static_cast<int>(least(largest(-g.base, 0) / RG, g.n));
+  g.rising = static_cast<int>(least(largest((g.cap - g.base) / RG, g.none), g.n));
   g.unit = static_cast<int64_t>(kUnit) * a.group;
   return g;
 }
 // A unit of T tiles costs at most T (3 kTile + 1) group + 2 RG counts, so that a share inside of it
 // has one of its tiles at least.
 __device__ __forceinline__ int shares_of(const Window& a, int64_t total) {
-  return static_cast<int>(min<int64_t>(kShares, max<int64_t>(1, total / (4 * (kTile * a.group + 128)))));
+  return static_cast<int>(least(kShares, largest(1, total / (4 * (kTile * a.group + 128)))));
 }
 __device__ __forceinline__ int64_t share_begin(int64_t total, int g, int n) {
   // (total * g may pass 64 bits only where total passes 2^54)
@@ -580,13 +622,11 @@ struct Work {
     pre[thread] = v;
     __syncthreads();
   }
-  // the total; with `keep` the sums of all requests are left there for the join
-  __device__ __forceinline__ void start(int64_t* keep) {
-    const int thread = here(threadIdx.x);
+  // the total
+  __device__ __forceinline__ void start() {
     total = 0;
     for (int f = 0; f < a.requests; f += NT) {
       fill(f, total);
-      if (keep && f + thread < a.requests) keep[f + thread] = pre[thread];
       total = uniform64(pre[NT - 1]);
     }
     if (base) fill(0, 0);
@@ -616,130 +656,314 @@ struct Work {
       else end = mid - 1;
     }
     u.rg = uniform(at);
-    u.begin = head + g.template upto<RG>(u.rg);
-    u.cost = g.template upto<RG>(u.rg + 1) - g.template upto<RG>(u.rg);
+    u.begin = uniform64(head + g.template upto<RG>(u.rg));
+    u.cost = uniform64(g.template upto<RG>(u.rg + 1) - g.template upto<RG>(u.rg));
     return u;
   }
 };
+// a < b, both wave-uniform: 64-bit numbers are compared in vector registers, where none shall
+// be kept for it
+__device__ __forceinline__ bool below(int64_t a, int64_t b) {
+  asm volatile("" : "+s"(b));
+  return a < b;
+}
 // the first of a unit's `tiles` that lies behind `counts` of its cost
 __device__ __forceinline__ int tile_at(int64_t counts, int64_t cost, int tiles) {
   return counts <= 0 ? 0 : counts >= cost ? tiles : static_cast<int>(counts * tiles / cost);
 }
 
-// NW waves of 16 R rows share tiles of 128 keys through LDS.  A tile goes from memory to LDS
-// past the registers, into the buffer that is not computed: one barrier per tile, and a load
-// has a tile's arithmetic to arrive.
-//
-// LDS rows are D/8 pieces of 16 bytes.  A wave reads keys as A operands, 16 keys x one
-// piece per access: piece p of key r lies at p ^ (r D / 128), so that the sixteen lanes
-// of an access meet all banks.  Values are read transposed, 4 keys x 16 dims per 16 lanes
-// (ds_read_b64_tr_b16: lane n gets dim n of the four keys), a pair of pieces of 16 keys per
-// access: they are exchanged in pairs, p ^ 2 (r D / 128).
-template <int D, int R, int NW, bool F16>
-__global__ __launch_bounds__(64 * NW, 1) void window_wide_kernel(Window a0) {
-  using W = Rows<D, R, F16, false>;
+// 32 rows of a wave and their running sums, for v_mfma_f32_32x32x16: lane l holds row l%32 and
+// of a step's 32 keys or of 32 dims those 8 b + 4 (l/32) + i (b, i < 4).  S^T = K Q^T: A = K
+// (lane: key l%32, 8 dims from 8 (l/32) of each sixteen), B = Q^T.  O^T = V^T P^T: B = P^T as
+// it lies there, two products of sixteen keys, A = V^T in the same order.
+template <int D, bool F16>
+struct Rows32 {
   using E = Elem<F16>;
-  constexpr int TK = kTile, RG = 16 * R * NW;
-  constexpr int P = D / 8;            // pieces per row
-  constexpr int KI = 64 / P;          // keys of one wave-wide load
-  constexpr int KW = TK / NW;         // keys of a wave's loads
-  constexpr int J = KW / KI;          // loads per wave, tile and matrix
-  constexpr int H = KW / 16;          // halves of steps in them, each in one block
-  static_assert(KW % 16 == 0 && 16 % KI == 0);
-  __shared__ __attribute__((aligned(256))) uint16_t lkv[2][2][TK * D];  // (whole rows aligned: k_at)
-  __shared__ uint32_t lbad[2][TK / 16], lodd[2][TK / 16];  // of sixteen keys: absent; those whose values are not finite
+  static constexpr int DC = D / 16, DV = D / 32;
+  u32x4 q[DC];
+  f32x16 o[DV];
+  float mx, sum;  // the reference; the lane's own part of the weights' sum
+  int pos;        // where the row stands
+  bool far;       // some row's reference is beyond kFar (the same in all lanes)
+
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    typedef typename E::x8 x8;
+    if constexpr (F16)
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float both(float v, bool max) {
+    const uint32_t x = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max ? fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])) : __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  }
+
+  __device__ __forceinline__ void load(const Window& a, const Ragged& rq, int kh, int row0, int nrows, int lane) {
+    const int row = min(row0 + (lane & 31), nrows - 1), t = row / a.group;  // (rows past the last repeat it)
+    const uint16_t* p = a.q + (rq.row0 + t) * a.q_row + (kh * a.group + row - t * a.group) * a.q_head + 8 * (lane >> 5);
+#pragma unroll
+    for (int d = 0; d < DC; ++d) q[d] = ld16(p + 16 * d) ^ a.flip;
+    pos = rq.first + t;
+    // (they have arrived here: a wait for them inside the loop over the keys would be
+    // a wait for the keys on their way too)
+#pragma unroll
+    for (int d = 0; d < DC; ++d) asm volatile("" : "+v"(q[d]));
+    far = false;
+    mx = kLow;
+    sum = 0.f;
+#pragma unroll
+    for (int d = 0; d < DV; ++d) o[d] = f32x16{};
+  }
+
+  static __device__ __forceinline__ int key_of(int e, int lane) { return 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
+  // which of the step's sixteen keys of this lane its row sees
+  __device__ __forceinline__ uint32_t seen(const Window& a, int key0, bool bad0, bool bad1, int lane) const {
+    const int low = low_of(pos, a.window);
+    uint32_t ok = 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      ok |= visible(key0 + key_of(e, lane), pos, low, a.sinks) && !(e >> 3 ? bad1 : bad0) ? 1u << e : 0;
+    return ok;
+  }
+  // as in Rows
+  __device__ __forceinline__ void raise(const Window& a, const f32x16& x, uint32_t ok) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = fmaxf(top, ok >> e & 1 ? x[e] * a.c : -INFINITY);
+    if (!__ballot(top - mx > kSlack + E::kHead)) return;
+    const float t = both(top, true);
+    const float ref = fmaxf(fabsf(t) > kFar ? t : t - E::kHead, mx), f = __builtin_amdgcn_exp2f(mx - ref);
+    mx = ref;
+    far = __ballot(fabsf(ref) > kFar);
+    sum *= f;
+#pragma unroll
+    for (int d = 0; d < DV; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] *= f;
+  }
+  // Weights of a step's half h, rounded in p; their sum.
+  static __device__ __forceinline__ float take(const float (&y)[8], u32x4& p) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) p[e] = E::pack(y[2 * e], y[2 * e + 1]);
+    return ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+  }
+  __device__ __forceinline__ float weights(const Window& a, const f32x16& x, int h, u32x4& p) const {
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(fmaf(x[8 * h + e], a.c, -mx));
+    return take(y, p);
+  }
+  // The same where there are masks, or references that the exponent's rounding matters for.
+  __device__ __forceinline__ float unusual(const Window& a, const f32x16& x, uint32_t ok, u32x4& p0, u32x4& p1) const {
+    float sum = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        y[e] = ok >> (8 * h + e) & 1 ? __builtin_amdgcn_exp2f(exponent(x[8 * h + e], a.c, mx, far)) : 0.f;
+      sum += take(y, h ? p1 : p0);
+    }
+    return sum;
+  }
+  // values that are not finite (bit of odd; the products had zeros for them), for the rows that see them
+  template <typename Value>
+  __device__ __forceinline__ void add_odd(const Window& a, const u32x4& p0, const u32x4& p1, int key0, uint32_t odd, int lane,
+                                          Value value) {
+    for (uint32_t w = odd; w; w &= w - 1) {
+      const int j = __builtin_ctz(w), e = 4 * (j >> 3) + (j & 3);
+      const auto row = value(j);
+      uint32_t y = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y = e >> 1 == i ? (i >> 2 ? p1 : p0)[i & 3] : y;
+      const float pj = E::low(__shfl(y, (lane & 31) + 32 * (j >> 2 & 1)) >> (16 * (e & 1)));
+      if (!visible(key0 + j, pos, low_of(pos, a.window), a.sinks)) continue;
+#pragma unroll
+      for (int d = 0; d < DV; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] += pj * row(32 * d + key_of(i, lane));
+    }
+  }
+  // The row's output, or (whole false: other keys of its are elsewhere) its sums at `slot0` + row.
+  __device__ __forceinline__ void store(const Window& a, const Ragged& rq, int kh, int row0, int nrows, int lane, bool whole,
+                                        int64_t slot0) {
+    const int row = row0 + (lane & 31), at = 4 * (lane >> 5);
+    const float total = both(sum, false);
+    if (row >= nrows) return;
+    const int t = row / a.group, head = kh * a.group + row - t * a.group;
+    const int64_t token = rq.row0 + t;
+    if (whole) {
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      uint16_t* p = a.out + token * a.out_row + head * a.out_head + at;
+#pragma unroll
+      for (int d = 0; d < DV; ++d)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          *reinterpret_cast<u32x2*>(p + 32 * d + 8 * b) = u32x2{E::pack(o[d][4 * b] * inv, o[d][4 * b + 1] * inv),
+                                                                E::pack(o[d][4 * b + 2] * inv, o[d][4 * b + 3] * inv)};
+      if (a.lse && lane < 32) a.lse[token * a.q_heads + head] = log_sum(mx, total);
+    } else {
+      float* p = a.part + (slot0 + row) * D + at;
+#pragma unroll
+      for (int d = 0; d < DV; ++d)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          *reinterpret_cast<f32x4*>(p + 32 * d + 8 * b) = f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
+      if (lane < 32) *reinterpret_cast<f32x4*>(a.stat + 4 * (slot0 + row)) = f32x4{mx, total, total, 0.f};
+    }
+  }
+};
+
+// Eight waves of 32 rows share tiles of 64 keys through LDS.  A tile goes from memory to LDS past
+// the registers, three ahead of the one that is computed: one barrier per tile, behind which
+// the next one is whole and the last one's buffer is free.
+//
+// LDS rows are D/8 pieces of 16 bytes.  A wave reads keys as A operands, piece 2 c + l/32 of
+// key l%32: piece p of key r lies at p ^ (r D / 128), so that the sixteen lanes of an access
+// meet all banks.  Values are read transposed, 4 keys x 16 dims per 16 lanes (ds_read_b64_tr_b16:
+// lane n gets dim n of the four keys), a pair of pieces of four keys per access: pairs are
+// exchanged by twos, so that four keys x two pairs meet all banks.
+//
+// Bound by the matrix units and LDS alike (a step of 32 keys and 256 rows takes 1024 cycles of
+// either).  Between products of 32 x 32 there is room for six other instructions each, between
+// those of 16 x 16, half as long, for one or two: they cover the softmax (three and an exponential
+// a product), given that there is one to issue.  So a wave's products and softmax overlap a step
+// apart: the products of the next step's scores run beside this step's weights, those of this
+// step's output beside the next step's largest scores.
+template <int D, bool F16>
+__global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
+  using W = Rows32<D, F16>;
+  using E = Elem<F16>;
+  constexpr int DC = W::DC, DV = W::DV, NW = 8, TK = kTile, RG = 32 * NW;
+  constexpr int P = D / 8;       // pieces per row
+  constexpr int KI = 64 / P;     // keys of one wave-wide load
+  constexpr int KW = TK / NW;    // keys of a wave's loads: of one block
+  constexpr int J = KW / KI;     // loads per wave, tile and matrix
+  constexpr int kBuffers = 4;
+  static_assert(16 % KW == 0 && TK == 64);
+  __shared__ __attribute__((aligned(256))) uint16_t lkv[kBuffers][2][TK * D];  // (whole rows aligned: k_at)
+  __shared__ uint32_t lflags[kBuffers][NW];  // of a wave's keys: those whose values are not finite; absent (bit 16)
+  __shared__ __attribute__((aligned(16))) uint32_t lfrom[64 * NW][2 * J];
+  __shared__ uint32_t lany;  // some block of the unit's has been absent
   __shared__ int64_t lpre[64 * NW], lsum[NW];
   const int lane = threadIdx.x & 63;
   const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
-  // LDS byte addresses of this lane's pieces of the first step: key li, piece lg; and
-  // dims 4 (li % 4) .. +3 of key 4 lg + li / 4
-  const int li = lane & 15, lg = lane >> 4, vkey = 4 * lg + (li >> 2);
-  const uint32_t k_at = lds_address(lkv) + li * (2 * D) + 16 * (lg ^ (li * P / 16 & (P - 1)));
+  // the exchanges of row r
+  auto turn_k = [](int r) { return r * P / 16 & (P - 1); };
+  auto turn_v = [](int r) { return P == 16 ? 4 * (r & 3) : 4 * (r >> 1 & 1); };
+  // LDS byte addresses of this lane's pieces of the first step: key l%32, piece l/32; and of
+  // dims 16 (l/16 % 2) + 4 (l%4) .. +3 of key 4 (l/32) + l/4 % 4
+  const int vkey = 4 * (lane >> 5) + (lane >> 2 & 3);
+  const uint32_t k_at = lds_address(lkv) + (lane & 31) * (2 * D) + 16 * ((lane >> 5) ^ turn_k(lane & 31));
   const uint32_t v_at = lds_address(lkv) + TK * D * 2 + vkey * (2 * D) +
-                        16 * ((li >> 1 & 1) ^ (2 * (vkey * P / 16) & (P - 1))) + 8 * (li & 1);
+                        16 * ((2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ turn_v(vkey)) + 8 * (lane & 1);
   Work<RG, 64 * NW> work{again<Window>(), lpre, lsum, 0, 0, 0};
-  work.start(blockIdx.x == 0 ? work.a.sums : nullptr);
+  work.start();
   const int shares = shares_of(work.a, work.total), share = xcd_remap(blockIdx.x, gridDim.x);
+  if (threadIdx.x == 0) a0.begun[share].b = -1;
   if (share >= shares) return;
   const int64_t begin = uniform64(share_begin(work.total, share, shares));
   const int64_t end = uniform64(share_begin(work.total, share + 1, shares));
 
-  for (int64_t pos = begin; pos < end;) {
+  for (int64_t pos = begin; below(pos, end);) {
     work.a = again<Window>();
     const auto un = work.find(pos);
     const Window& a = a0;
     const Ragged& rq = un.rq;
-    const int nrows = rq.tokens * a.group, first_row = un.rg * RG;
+    const int kh = un.kh, nrows = rq.tokens * a.group, first_row = un.rg * RG;
     const int pmin = rq.first + first_row / a.group, pmax = rq.first + (min(first_row + RG, nrows) - 1) / a.group;
-    const Span span = span_of<7>(a, pmin, pmax);
+    const Span span = span_of<kTileBits>(a, pmin, pmax);
     // this share's tiles of the unit
     const int t0 = uniform(tile_at(pos - un.begin, un.cost, span.tiles));
     const int t1 = uniform(tile_at(end - un.begin, un.cost, span.tiles));
     pos = un.begin + un.cost;  // the next unit's
     const bool whole = t0 == 0 && t1 == span.tiles;
-    if (t0 >= t1 && !(span.tiles == 0 && un.begin >= begin)) continue;
-    const int row0 = first_row + wave * (16 * R);  // of this wave
-    const bool active = row0 < nrows;
-    const int kh = un.kh;
-    // what this wave's rows are at
-    const int wmin = rq.first + min(row0, nrows - 1) / a.group, wmax = rq.first + (min(row0 + 16 * R, nrows) - 1) / a.group;
+    if (t0 == 0 && t1 > 0 && !whole && threadIdx.x == 0) {
+      int64_t total = work.total;
+      asm volatile("" : "+s"(total));
+      a0.begun[share] = Begun{un.b, kh, un.rg, !below(un.begin, begin), un.begin, un.cost, total};
+    }
+    if (t0 >= t1 && !(span.tiles == 0 && !below(un.begin, begin))) continue;
+    const int row0 = first_row + wave * 32;  // of this wave (that has none: it computes the last row)
+    // where this wave's rows stand
+    const int wmin = rq.first + min(row0, nrows - 1) / a.group, wmax = rq.first + (min(row0 + 32, nrows) - 1) / a.group;
 
     const int32_t* table = a.tables + un.b * a.tstride;
     const uint16_t *kc = static_cast<const uint16_t*>(a.kc) + kh * a.kc_head;
     const uint16_t *vc = static_cast<const uint16_t*>(a.vc) + kh * a.vc_head;
-    // Lane i: the blocks of this wave's keys of tile number id0 + i.  (Waited for where they are
-    // loaded: a wait for them further on would be one for the keys on their way too.)
-    int id_lane[H], id0 = -64;
-    // this share's i-th tile into buffer `to`; bit h: its half h of this wave's is absent
-    auto load = [&](int i, int to) {
-      const int ln = here(lane), kin = ln / P, piece = ln % P;
-      const uint32_t at_k = lds_address(lkv) + to * (4 * TK * D) + wave * (KW * 2 * D), at_v = at_k + 2 * TK * D;
-      const int t = span.tile(i);
-      if (t >= id0 + 64 || t < id0) {
+    // the share's tiles of whose keys every row sees all (of the windows' part): plain0 .. plain0 + plains - 1
+    const int plain0 = max(max(low_of(pmax, a.window) + TK, 0) / TK - span.from, 0) + span.sinks;
+    const int plains = max((pmin + 1) / TK - span.from + span.sinks - plain0, 0);
+    auto plain = [&](int i) { return static_cast<uint32_t>(i - plain0) < static_cast<uint32_t>(plains); };
+    // Lane i: the block of this wave's keys of tile number id0 + i.  (Waited for where it is
+    // loaded: a wait for it further on would be one for the keys on their way too.)
+    int id_lane = 0, id0 = -(1 << 30);
+    uint32_t absent = 0;  // bit i % 4: this wave's keys of the share's i-th tile are of an absent block
+    uint32_t flagged = ~0u;  // bit i % 4: the wave's flags of that buffer may not be 0
+    // The lane's pieces of its wave's rows (it fills piece l % P of its key's row in LDS: the
+    // exchange picks what it reads), kept in LDS.
+    {
+      uint32_t from[2 * J];
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int ln = here(lane), piece = ln % P, at = j * KI + ln / P, r = wave * KW + at;
+        from[2 * j] = 2 * (at * a.kc_slot + 8 * (piece ^ turn_k(r)));
+        from[2 * j + 1] = 2 * (at * a.vc_slot + 8 * (piece ^ turn_v(r)));
+      }
+#pragma unroll
+      for (int j = 0; j < 2 * J; ++j) lfrom[here(threadIdx.x)][j] = from[j];
+    }
+    // This share's i-th tile into its buffer, in three pieces that stand between the products of
+    // another one (behind the last tile: that one again, where nothing reads it).
+    int load_slot = 0, load_block = 0;
+    auto load_id = [&](int i) {
+      const int t = span.tile(min(i, t1 - 1));
+      // (keys of a sixteen past the last one are those of the sixteen with the last one instead, and masked)
+      const int last = (pmax & ~15) + wave * KW % 16;
+      if (__builtin_expect(static_cast<uint32_t>(t - id0) >= 64u, 0)) {
         id0 = t;
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-          int slot;
-          const int64_t key = min<int64_t>(static_cast<int64_t>(t + ln) * TK + wave * KW + 16 * h, pmax & ~15);
-          id_lane[h] = table[block_of(a, static_cast<int>(key), slot)];
-        }
-#pragma unroll
-        for (int h = 0; h < H; ++h) asm volatile("" : "+v"(id_lane[h]));
-      }
-      uint32_t bad = 0;
-#pragma unroll
-      for (int h = 0; h < H; ++h) {
-        // (sixteen keys past the last one are the sixteen with the last one instead, and masked)
-        const int id = __builtin_amdgcn_readlane(id_lane[h], t - id0);
-        if (id < 0 || id >= a.blocks) bad |= 1u << h;
-        const int64_t blk = id < 0 || id >= a.blocks ? 0 : id;
         int slot;
-        block_of(a, min(t * TK + wave * KW + 16 * h, pmax & ~15), slot);
-        const int64_t at0 = slot;
-        const uint16_t *kb = kc + blk * a.kc_block + at0 * a.kc_slot, *vb = vc + blk * a.vc_block + at0 * a.vc_slot;
-        // (lane l fills piece l % P of its key's row in LDS: the exchange picks what it reads)
-#pragma unroll
-        for (int j = 0; j < 16 / KI; ++j) {
-          const uint32_t at = j * KI + kin;
-          const int turn = (wave * KW + 16 * h + j * KI + kin) * P / 16;
-          load_lds(kb + at * a.kc_slot + 8 * (piece ^ (turn & (P - 1))), at_k + 1024 * (h * (16 / KI) + j));
-          load_lds(vb + at * a.vc_slot + 8 * (piece ^ (2 * turn & (P - 1))), at_v + 1024 * (h * (16 / KI) + j));
-        }
+        const int64_t key = least(static_cast<int64_t>(t + here(lane)) * TK + wave * KW, last);
+        id_lane = table[block_of(a, static_cast<int>(key), slot)];
+        asm volatile("" : "+v"(id_lane));
       }
-      return bad;
+      const int id = __builtin_amdgcn_readlane(id_lane, t - id0);
+      block_of(a, min(t * TK + wave * KW, last), load_slot);
+      const bool bad = static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.blocks);
+      absent = (absent & ~(1u << i % kBuffers)) | static_cast<uint32_t>(bad) << i % kBuffers;
+      load_block = bad ? 0 : id;
     };
-    // This wave's part of the i-th tile has arrived in buffer `in`: as in window_kernel, no
-    // infinity or NaN may meet a weight of 0.
-    auto settle = [&](int i, int in, uint32_t bad) {
-      const int ln = here(lane), kin = ln / P;
+    auto load_part = [&](int i, int m) {  // m: keys, values
+      const uint32_t to = lds_address(lkv) + (i % kBuffers) * (4 * TK * D) + m * (2 * TK * D) + wave * (KW * 2 * D);
+      const uint16_t* base = m ? vc + (static_cast<int64_t>(load_block) * a.vc_block + static_cast<int64_t>(load_slot) * a.vc_slot)
+                               : kc + (static_cast<int64_t>(load_block) * a.kc_block + static_cast<int64_t>(load_slot) * a.kc_slot);
+      uint32_t from[J];
+#pragma unroll
+      for (int j = 0; j < J; ++j) from[j] = lfrom[here(threadIdx.x)][2 * j + m];
+#pragma unroll
+      for (int j = 0; j < J; ++j) load_lds(base, from[j], to + 1024 * j);
+    };
+    auto load = [&](int i) {
+      load_id(i);
+      load_part(i, 0);
+      load_part(i, 1);
+    };
+    // This wave's part of the i-th tile has arrived: as in window_kernel, no infinity or NaN
+    // may meet a weight of 0.
+    auto to_settle = [&](int i) { return i < t1 && !(plain(i) && !((absent | flagged) >> i % kBuffers & 1)); };
+    auto settle = [&](int i) {
+      const int in = i % kBuffers;
       const int key0 = span.tile(i) * TK + wave * KW;
-      uint32_t odd[H] = {};
-      if (bad || !all_visible(a, key0, key0 + KW - 1, pmin, pmax)) {
+      const bool bad = absent >> in & 1, seen = !bad && all_visible(a, key0, key0 + KW - 1, pmin, pmax);
+      uint32_t flags = bad ? 1u << 16 : 0;
+      flagged = (flagged & ~(1u << in)) | static_cast<uint32_t>(!seen) << in;
+      if (!seen) {
+        const int ln = here(lane), kin = ln / P;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-          const int h = j * KI / 16;
           u32x4* const at = reinterpret_cast<u32x4*>(&lkv[in][1][(wave * J + j) * 512 + 8 * ln]);
-          const bool gone = (bad >> h & 1) || key0 + j * KI + kin > pmax;
+          const bool gone = bad || key0 + j * KI + kin > pmax;
           const u32x4 v = *at;
           bool wild = false;
 #pragma unroll
@@ -748,142 +972,191 @@ __global__ __launch_bounds__(64 * NW, 1) void window_wide_kernel(Window a0) {
           const unsigned long long m = __ballot(wild && !gone), one = P == 16 ? 0xffffull : 0xffull;
 #pragma unroll
           for (int k = 0; k < KI; ++k)
-            if (m >> (P * k) & one) odd[h] |= 1u << (j * KI % 16 + k);
-          if (gone || (m >> (P * kin) & one)) *at = u32x4{0, 0, 0, 0};
+            if (m >> (P * k) & one) flags |= 1u << (j * KI + k);
+          const uint32_t zero = here(0);  // (no register keeps it meanwhile)
+          if (gone || (m >> (P * kin) & one)) *at = u32x4{zero, zero, zero, zero};
         }
       }
-      if (ln == 0) {
-#pragma unroll
-        for (int h = 0; h < H; ++h) lbad[in][wave * H + h] = bad >> h & 1, lodd[in][wave * H + h] = odd[h];
+      if (here(lane) == 0) {
+        lflags[in][wave] = flags;
+        if (bad) lany = 1;
       }
     };
+    // bit h: sixteen h of the share's i-th tile is absent, from its flags
+    auto absent_of = [&](uint32_t flags) {
+      const uint32_t m = static_cast<uint32_t>(__ballot(here(lane) < NW && flags >> 16));
+      uint32_t b = 0;
+#pragma unroll
+      for (int h = 0; h < 4; ++h) b |= (m >> (h * (16 / KW)) & 1) << h;
+      return b;
+    };
 
-    // One barrier per tile.  Behind it, tile i is whole in its buffer and the one that held
-    // tile i - 1 is free: tile i + 1 is sent for, i is computed, and each wave waits for its
-    // part of i + 1.
-    uint32_t bad = t0 < t1 ? load(t0, 0) : 0;
     W w;
-    if (active) {
-      const int ln = here(lane);
-      w.load(again<Window>(), rq, kh, row0, nrows, ln & 15, ln >> 4);
-    }
-    const bool want = a.lse != nullptr;
-    arrived<0>();
-    if (t0 < t1) settle(t0, 0, bad);
+    typedef f32x16 Scores[2];  // of a tile's two steps
+    // keys of a quarter n of tile i's (step n / 2, half of the dims n % 2) as A operands: a piece's
+    // exchange is an exclusive or of its row's address with 16 bytes times the piece, steps are
+    // whole sixteens apart
+    auto read_keys = [&](int i, int n, u32x4 (&k)[DC / 2]) {
+      const uint32_t at = k_at + (i % kBuffers) * (4 * TK * D) + 32 * (n >> 1) * (2 * D);
+#pragma unroll
+      for (int d = 0; d < DC / 2; ++d) k[d] = *lds<const u32x4>(at ^ (32 * (d + (n & 1) * (DC / 2))));
+    };
+    auto multiply_keys = [&](int n, const u32x4 (&k)[DC / 2], Scores& s) {
+      if ((n & 1) == 0) s[n >> 1] = f32x16{};
+#pragma unroll
+      for (int d = 0; d < DC / 2; ++d) s[n >> 1] = W::mfma(k[d], w.q[d + (n & 1) * (DC / 2)], s[n >> 1]);
+    };
+    // values of a quarter's sixteen keys, transposed
+    auto read_values = [&](int i, int n, u32x4 (&v)[DV]) {
+      const uint32_t at0 = v_at + (i % kBuffers) * (4 * TK * D) + 16 * n * (2 * D);
+#pragma unroll
+      for (int d = 0; d < DV; ++d) {
+        const uint32_t at = at0 ^ (64 * d);
+        const u32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * (2 * D));
+        v[d] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+      }
+    };
+    // which of a tile's keys the lane's row sees, where some row does not see all
+    auto seen = [&](int i, bool masked, uint32_t bm, int j) {
+      return masked ? w.seen(a, span.tile(i) * TK + 32 * j, bm >> (2 * j) & 1, bm >> (2 * j + 1) & 1, here(lane)) : 0xffff;
+    };
+    // tile i's scores in s: whether it has masks, its absent sixteens; the references raised
+    auto take = [&](int i, const Scores& s, bool over, uint32_t any, uint32_t& bm) {
+      bool masked = !plain(i);
+      bm = 0;
+      if (__builtin_expect(masked || any, 0)) {
+        bm = absent_of(lflags[i % kBuffers][here(lane) & (NW - 1)]);
+        const int key0 = span.tile(i) * TK;
+        masked = bm || !all_visible(a, key0, key0 + TK - 1, wmin, wmax);
+      }
+      if (__builtin_expect(masked || over || w.far, 0)) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) w.raise(a, s[j], seen(i, masked, bm, j));
+      }
+      return masked;
+    };
+
+    constexpr int L = 2 * J;  // loads of a wave per tile
+    if (threadIdx.x == 0) lany = 0;
     __syncthreads();
-    int buf = 0;
-    for (int i = t0; i < t1; ++i) {
-      if (i + 1 < t1) bad = load(i + 1, buf ^ 1);
-      if (active) {
-        const int tile0 = span.tile(i) * TK;
-        const int ln = here(lane);
-        const uint32_t bm = static_cast<uint32_t>(__ballot(ln < TK / 16 && lbad[buf][ln % (TK / 16)]));
+    if (t0 < t1)
 #pragma unroll 1
-        for (int h = 0; h < TK / 32; ++h) {
-          const int key0 = tile0 + 32 * h;
-          // (no row of this wave sees any of them)
-          if (key0 > wmax) break;
-          if (key0 + 31 <= low_of(wmin, a.window) && key0 >= a.sinks) continue;
-          const bool bad0 = bm >> (2 * h) & 1, bad1 = bm >> (2 * h + 1) & 1;
-          const bool masked = bad0 || bad1 || !all_visible(a, key0, key0 + 31, wmin, wmax);
-          // a piece's exchange is an exclusive or of its row's address with 16 bytes times
-          // the piece, halves of a step and steps are 16 and 32 whole rows apart
-          const uint32_t kat = k_at + buf * (4 * TK * D) + 32 * h * (2 * D);
-          const uint32_t vat = v_at + buf * (4 * TK * D) + 32 * h * (2 * D);
-          const int lg_ = here(lane) >> 4;
-          Keys16<D> k;
-#pragma unroll
-          for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d) k.k[g][d] = *lds<const u32x4>((kat ^ (64 * d)) + 16 * g * (2 * D));
-          f32x4 s[R][2];
-          float x[R][8];
-          uint32_t ok[R];
-#pragma unroll
-          for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int r = 0; r < R; ++r) s[r][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-              for (int r = 0; r < R; ++r) s[r][g] = E::mfma(k.k[g][d], w.q[r][d], s[r][g]);
-          w.weights(a, s, x, ok, key0, masked, bad0, bad1, lg_);
-          auto values = [&](int d) {
-            const u32x2 y = read_transposed((vat ^ (32 * d))), z = read_transposed((vat ^ (32 * d)) + 16 * (2 * D));
-            return u32x4{y[0], y[1], z[0], z[1]};
-          };
-          uint32_t odd = 0;
-          if (masked) odd = lodd[buf][2 * h] | lodd[buf][2 * h + 1] << 16;
-          const int ln = here(lane);
-          w.add(a, x, values, key0, uniform(static_cast<int>(odd)), want, ln & 15, ln >> 4, [&](int j) {
-            int slot;
-            const int id = table[block_of(a, key0 + j, slot)];
-            const uint16_t* p = vc + static_cast<int64_t>(id) * a.vc_block + static_cast<int64_t>(slot) * a.vc_slot;
-            return [p](int e) { return E::low(p[e]); };
-          });
-        }
-      }
-      if (i + 1 < t1) {
-        arrived<0>();
-        settle(i + 1, buf ^ 1, bad);
-      }
-      buf ^= 1;
+      for (int i = t0; i < t0 + 3; ++i) load(i);
+    w.load(again<Window>(), rq, kh, min(row0, nrows - 1), nrows, here(lane));
+    if (t0 < t1) {
+      Scores s0, s1;
+      arrived<0>();
+      settle(t0);
       __syncthreads();
-    }
-    if (active) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) w.exact[r] = quad_sum(w.exact[r]);
-      const int64_t slot0 = static_cast<int64_t>(2 * share + (un.begin >= begin)) * RG - first_row;
-      const int ln = here(lane);
-      w.store(again<Window>(), rq, kh, row0, nrows, ln & 15, ln >> 4, whole, [&](int row, int64_t, int) { return slot0 + row; });
+      for (int n = 0; n < 4; ++n) {
+        u32x4 k[DC / 2];
+        read_keys(t0, n, k);
+        multiply_keys(n, k, s0);
+      }
+      uint32_t bm;
+      bool masked = take(t0, s0, true, lany, bm), settles = to_settle(t0 + 1);
+
+      // Tile i, its scores in x; the next one's go to s.
+      auto tile = [&](int i, const Scores& x, Scores& s) {
+        // One barrier per tile: behind it the next one is whole, and the buffer of the one
+        // before free.
+        arrived<L>();  // (all but the tile after the next)
+        if (__builtin_expect(settles, 0)) settle(i + 1);
+        __syncthreads();
+        const uint32_t any_v = lany;
+        u32x4 k[2][DC / 2], v[2][DV], p[4];
+        float sum = 0.f;
+        read_keys(i + 1, 0, k[0]);
+        // this tile's weights beside the next one's scores (behind the last: of what lies there)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (n < 3) read_keys(i + 1, n + 1, k[~n & 1]);
+          else read_values(i, 0, v[0]);
+          __builtin_amdgcn_sched_barrier(0);
+          multiply_keys(n, k[n & 1], s);
+          sum += w.weights(a, x[n >> 1], n & 1, p[n]);
+          asm volatile("" : "+v"(p[n]), "+v"(sum));  // (here, not where they are used)
+          interleave<DC / 2, 8, 16 + (F16 ? 12 : 4)>();
+          __builtin_amdgcn_sched_barrier(0);
+          if (n == 0) load_id(i + 3);
+          if (n == 1 || n == 2) load_part(i + 3, n - 1);
+          if (n == 3) settles = to_settle(i + 2);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (__builtin_expect(masked || w.far, 0)) {
+          sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) sum += w.unusual(a, x[j], seen(i, masked, bm, j), p[2 * j], p[2 * j + 1]);
+        }
+        w.sum += sum;
+        // its output beside the next one's largest scores
+        float top = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (n < 3) read_values(i, n + 1, v[~n & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int d = 0; d < DV; ++d) w.o[d] = W::mfma(v[n & 1][d], p[n], w.o[d]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, s[n >> 1][8 * (n & 1) + e]);
+          interleave<DV, 0, 4>();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (__builtin_expect(masked, 0)) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t odd = 0;
+#pragma unroll
+            for (int n = 0; n < 32 / KW; ++n) odd |= (lflags[i % kBuffers][j * (32 / KW) + n] & 0xffff) << (n * KW);
+            odd = uniform(static_cast<int>(odd));
+            const int key0 = span.tile(i) * TK + 32 * j;
+            if (odd) w.add_odd(a, p[2 * j], p[2 * j + 1], key0, odd, here(lane), [&](int n) {
+              int slot;
+              const int id = table[block_of(a, key0 + n, slot)];
+              const uint16_t* at = vc + static_cast<int64_t>(id) * a.vc_block + static_cast<int64_t>(slot) * a.vc_slot;
+              return [at](int e) { return E::low(at[e]); };
+            });
+          }
+        }
+        if (i + 1 < t1) masked = take(i + 1, s, __ballot(fmaf(top, a.c, -w.mx) > kSlack + E::kHead), uniform(static_cast<int>(any_v)), bm);
+      };
+      for (int i = t0; i < t1; i += 2) {
+        tile(i, s0, s1);
+        if (i + 1 < t1) tile(i + 1, s1, s0);
+      }
+      __syncthreads();  // (the next unit's tiles go where these were)
     }
+    w.store(again<Window>(), rq, kh, row0, nrows, here(lane), whole,
+            static_cast<int64_t>(2 * share + (!below(un.begin, begin))) * RG - first_row);
   }
 }
 
-// Behind window_wide_kernel: four rows of a key head; those of whole units are already written.
+// Behind window_wide_kernel: the units that a share began and left to others, four rows a wave.
 template <int D, bool F16, int RG>
 __global__ __launch_bounds__(join_threads(1)) void window_wide_join_kernel(Window a) {
   const int lane = threadIdx.x & 63, li = lane & 15, wave = uniform(static_cast<int>(threadIdx.x >> 6));
-  int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-  const int quads = (a.max_tokens * a.group + 3) >> 2;
-  const int first = static_cast<int>(u % quads) * 4;
-  u /= quads;
-  const int kh = static_cast<int>(u % a.kv_heads), b = static_cast<int>(u / a.kv_heads);
-  if (b >= a.requests) return;
-  const Ragged rq = ragged(a, b);
-  const int rows = rq.tokens * a.group;
-  if (first >= rows) return;
-  const Groups g = groups_of<RG>(a, rq);
-  const int64_t total = a.sums[a.requests - 1];
-  const int n = shares_of(a, total), rg = first / RG;
-  const int64_t begin = (b ? a.sums[b - 1] : 0) + kh * g.template upto<RG>(g.n) + g.template upto<RG>(rg);
-  const int64_t cost = g.template upto<RG>(rg + 1) - g.template upto<RG>(rg);
-  const Span span = span_of<7>(a, rq.first + rg * RG / a.group, rq.first + (min(rg * RG + RG, rows) - 1) / a.group);
-  // the share that position `at` is in
-  auto share = [&](int64_t at) {
-    int k = static_cast<int>(min<int64_t>(at / max<int64_t>(total / n, 1), n - 1));
-    while (share_begin(total, k, n) > at) --k;
-    while (k + 1 < n && share_begin(total, k + 1, n) <= at) ++k;
-    return k;
-  };
-  const int g0 = share(begin), g1 = share(begin + cost - 1);
-  if (g0 == g1 || span.tiles == 0) return;
-  // (shares at either end may have none of the tiles)
-  auto has = [&](int k) {
-    return tile_at(share_begin(total, k, n) - begin, cost, span.tiles) <
-           tile_at(share_begin(total, k + 1, n) - begin, cost, span.tiles);
-  };
-  int s0 = g0, s1 = g1;
-  while (s0 < s1 && !has(s0)) ++s0;
-  while (s1 > s0 && !has(s1)) --s1;
-  if (s0 == s1) return;
-  const int row = min(first + (lane >> 4), rows - 1), t = row / a.group, head = kh * a.group + row - t * a.group;
+  const int s0 = blockIdx.x / (RG / 16), first = (blockIdx.x % (RG / 16)) * 16 + 4 * wave;
+  const Begun u = a.begun[s0];
+  if (u.b < 0) return;
+  const Ragged rq = ragged(a, u.b);
+  const int rows = rq.tokens * a.group, first_row = u.rg * RG;
+  if (first_row + first >= rows) return;
+  const Span span = span_of<kTileBits>(a, rq.first + first_row / a.group,
+                                       rq.first + (min(first_row + RG, rows) - 1) / a.group);
+  // the last share that has some of its tiles
+  const int64_t total = u.total;
+  const int n = shares_of(a, total);
+  int s1 = static_cast<int>(least((u.begin + u.cost) / largest(total / n, 1), n - 1));
+  while (s1 > s0 && tile_at(share_begin(total, s1, n) - u.begin, u.cost, span.tiles) >= span.tiles) --s1;
+  const int row = min(first_row + first + (lane >> 4), rows - 1), t = row / a.group, head = u.kh * a.group + row - t * a.group;
   uint16_t* p = a.out + (rq.row0 + t) * a.out_row + head * a.out_head + D / 16 * li;
-  join_rows<D, F16, 1, 4>(a.part, a.stat, s1 - s0 + 1, lane, wave, first + (lane >> 4) < rows ? p : nullptr,
-                          a.lse ? a.lse + static_cast<int64_t>(rq.row0 + t) * a.q_heads + head : nullptr,
-                          [&](int i) { return static_cast<int64_t>(2 * (s0 + i) + (s0 + i == g0)) * RG + row - rg * RG; });
+  join_rows<D, F16, 1, 4>(a.part, a.stat, s1 - s0 + 1, lane, wave, first_row + first + (lane >> 4) < rows ? p : nullptr,
+                          a.lse ? a.lse + static_cast<int64_t>(rq.row0 + t) * a.q_heads + head : nullptr, [&](int i) {
+                            return static_cast<int64_t>(2 * (s0 + i) + (i == 0 ? u.slot : 0)) * RG + row - first_row;
+                          });
 }
 
 // The launch shape, a function of sizes the host knows (never of what the device
@@ -898,7 +1171,7 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t max_token
   const int64_t rows = max_tokens * (q_heads / kv_heads);
   Plan p{};
   p.splits = 1;
-  p.wide = rows <= 64 || fp4 ? 0 : rows <= 128 ? 128 : 256;
+  p.wide = rows <= 64 || fp4 ? 0 : 256;
   if (p.wide) return p;
   p.r = rows <= 16 ? 1 : 2;
   p.wr = rows <= 32 ? 1 : 2;
@@ -917,8 +1190,8 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t max_token
 int64_t slots_of(const Plan& p, int64_t rows, int64_t q_heads) {
   return p.wide ? int64_t{2} * kShares * p.wide : p.splits == 1 ? 0 : rows * q_heads * p.splits;
 }
-size_t workspace_bytes(const Plan& p, int64_t rows, int64_t requests, int64_t q_heads, int64_t head_dim) {
-  return static_cast<size_t>(slots_of(p, rows, q_heads)) * (head_dim + 4) * 4 + (p.wide ? 8 * requests : 0);
+size_t workspace_bytes(const Plan& p, int64_t rows, int64_t q_heads, int64_t head_dim) {
+  return static_cast<size_t>(slots_of(p, rows, q_heads)) * (head_dim + 4) * 4 + (p.wide ? kShares * sizeof(Begun) : 0);
 }
 
 bool sizes_ok(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_tokens,
@@ -932,20 +1205,18 @@ bool sizes_ok(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads,
   return most <= 0x3fffffff && requests * (most + 64 * kv_heads) <= int64_t{0x3fffffff};  // (grids are 32-bit)
 }
 
-template <int D, int R, int NW, bool F16>
+template <int D, bool F16>
 int launch_wide(const Window& a, hipStream_t st) {
-  constexpr int RG = 16 * R * NW;
-  hipLaunchKernelGGL((window_wide_kernel<D, R, NW, F16>), dim3(kShares), dim3(64 * NW), 0, st, a);
+  hipLaunchKernelGGL((window_wide_kernel<D, F16>), dim3(kShares), dim3(512), 0, st, a);
   if (int rc = check_launch("window attention kernel")) return rc;
-  const int64_t quads = static_cast<int64_t>(a.requests) * a.kv_heads * ((a.max_tokens * a.group + 3) / 4);
-  hipLaunchKernelGGL((window_wide_join_kernel<D, F16, RG>), dim3(static_cast<unsigned>((quads + 3) / 4)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((window_wide_join_kernel<D, F16, 256>), dim3(kShares * 16), dim3(256), 0, st, a);
   return check_launch("window attention join kernel");
 }
 
 template <int D, bool F16, bool FP4>
 int launch(const Window& a, const Plan& p, hipStream_t st) {
   if constexpr (!FP4)
-    if (p.wide) return p.wide == 128 ? launch_wide<D, 1, 8, F16>(a, st) : launch_wide<D, 2, 8, F16>(a, st);
+    if (p.wide) return launch_wide<D, F16>(a, st);
   const dim3 g(static_cast<unsigned>(static_cast<int64_t>(a.requests) * a.kv_heads * p.groups * p.splits));
   constexpr int R = FP4 ? 1 : 2;
   if (p.r == 1) hipLaunchKernelGGL((window_kernel<D, 1, 1, 4, F16, FP4>), g, dim3(256), 0, st, a);
@@ -981,7 +1252,7 @@ extern "C" size_t pgs_window_attention_workspace_bytes(int64_t rows, int64_t req
       requests == 0)
     return 0;
   const Plan p = plan(requests, q_heads, kv_heads, std::min(max_tokens, rows), max_context, window, sinks, four_bits);
-  return workspace_bytes(p, rows, requests, q_heads, head_dim);
+  return workspace_bytes(p, rows, q_heads, head_dim);
 }
 
 extern "C" int pgs_window_attention(const pgs_window_attention_args* args, void* workspace, size_t workspace_bytes_given,
@@ -1009,7 +1280,7 @@ extern "C" int pgs_window_attention(const pgs_window_attention_args* args, void*
     return fail(PGS_ERR_MISALIGNED, "%s: misaligned", fn);
   const int64_t most = std::min(g.max_tokens, g.rows);  // (no request has more rows than the batch)
   const Plan p = plan(g.requests, g.q_heads, a.kv_heads, most, g.max_context, g.window, g.sinks, !g.cache);
-  const size_t need = workspace_bytes(p, g.rows, g.requests, g.q_heads, dim);
+  const size_t need = workspace_bytes(p, g.rows, g.q_heads, dim);
   if (need > 0 && (!workspace || workspace_bytes_given < need || !aligned(workspace, 256)))
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -1024,10 +1295,12 @@ extern "C" int pgs_window_attention(const pgs_window_attention_args* args, void*
   a.max_tokens = static_cast<int32_t>(most);
   a.window = static_cast<int32_t>(g.window), a.sinks = static_cast<int32_t>(g.sinks);
   a.groups = p.groups, a.splits = p.splits, a.min_steps = p.min_steps;
-  a.c = g.scale * 1.44269504088896340736f;
+  // (a negative scale changes the rows' signs: the largest score is then always the largest weight's)
+  a.c = std::fabs(g.scale) * 1.44269504088896340736f;
+  a.flip = std::signbit(g.scale) ? 0x80008000u : 0;
   a.part = static_cast<float*>(workspace);
   a.stat = a.part + slots_of(p, g.rows, g.q_heads) * dim;
-  a.sums = reinterpret_cast<int64_t*>(a.stat + slots_of(p, g.rows, g.q_heads) * 4);
+  a.begun = reinterpret_cast<Begun*>(a.stat + slots_of(p, g.rows, g.q_heads) * 4);
   auto go = [&](auto d, auto f16) {
     constexpr int D = decltype(d)::value;
     constexpr bool F = decltype(f16)::value;
