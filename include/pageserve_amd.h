@@ -697,12 +697,9 @@ typedef struct pgs_window_attention_args {
 int pgs_window_attention(const pgs_window_attention_args* args, void* workspace,
                          size_t workspace_bytes, void* stream);
 
-/* Workspace bytes of pgs_window_attention (0: none needed), over a cache in 16
- * bits or in 4. */
-size_t pgs_window_attention_workspace_bytes(int64_t rows, int64_t requests, int64_t q_heads,
-                                            int64_t kv_heads, int64_t head_dim,
-                                            int64_t max_tokens, int64_t max_context,
-                                            int64_t window, int64_t sinks, int four_bits);
+/* Workspace bytes of a call with these arguments (0: none needed); its pointers, but
+ * for the cache's sizes, are not looked at. */
+size_t pgs_window_attention_workspace_bytes(const pgs_window_attention_args* args);
 
 /* The arguments of pgs_accumulate_weights; those with a name of
  * pgs_window_attention_args mean the same. */

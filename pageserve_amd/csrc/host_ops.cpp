@@ -675,7 +675,6 @@ std::vector<at::Tensor> window_attention(const at::Tensor& q, const std::vector<
     a.cache = &c;
   }
   const int64_t dim = four ? c4.head_dim : c.head_dim, size = four ? c4.block_size : c.block_size;
-  const int64_t kv_heads = four ? c4.kv_heads : c.kv_heads;
   const at::Device dev = cache[0].device();
   at::hip::HIPGuardMasqueradingAsCUDA guard(dev);
   const at::Tensor qr = rows_of(q, -1, -1, dim, dev, what, "q");
@@ -711,8 +710,7 @@ std::vector<at::Tensor> window_attention(const at::Tensor& q, const std::vector<
   a.window = window.has_value() ? *window : kEverything;
   a.sinks = sinks;
   a.scale = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(dim)));
-  const size_t need = pgs_window_attention_workspace_bytes(a.rows, a.requests, a.q_heads, kv_heads, dim, a.max_tokens,
-                                                           a.max_context, a.window, a.sinks, four);
+  const size_t need = pgs_window_attention_workspace_bytes(&a);
   at::Tensor ws;  // (per call, as in tree_attention)
   if (need) ws = at::empty({static_cast<int64_t>(need)}, qr.options().dtype(at::kByte));
   void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();

@@ -1159,20 +1159,75 @@ __global__ __launch_bounds__(join_threads(1)) void window_wide_join_kernel(Windo
                           });
 }
 
+// Many rows over a 4-bit cache: every request's tokens are widened once into 16-bit blocks of
+// sixteen, [request][columns][head][16][D], exactly, with a table of their own, and the wide
+// kernel reads those.  Each value is read by hundreds of rows, which this costs one write and one
+// read of 16 bits; widened in the wide kernel it would be a third more instructions beside its
+// products.  One workgroup per block: a thread has eight dims of a token.
+struct Widen {
+  Window w;
+  uint16_t *k, *v;
+  int32_t* tables;  // [requests][columns]
+  int32_t columns;
+};
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void widen_kernel(Widen g) {
+  const Window& a = g.w;
+  constexpr int C = D / 32, P = D / 8;
+  const int b = blockIdx.x / g.columns, col = blockIdx.x % g.columns;
+  const Ragged rq = ragged(a, b);
+  if (col * 16 >= rq.len) return;
+  // (what no row of the request sees, if it has any, is left out)
+  if (rq.tokens == 0 || (col * 16 + 15 <= low_of(rq.first, a.window) && col * 16 >= a.sinks)) return;
+  int slot;
+  const int id = a.tables[b * a.tstride + block_of(a, col * 16, slot)];
+  const bool bad = id < 0 || id >= a.blocks;
+  if (threadIdx.x == 0) g.tables[blockIdx.x] = bad ? -1 : static_cast<int32_t>(blockIdx.x);
+  if (bad) return;
+  for (int u = threadIdx.x; u < a.kv_heads * 16 * P; u += 256) {
+    const int i = u % P, token = u / P % 16, h = u / (16 * P), c = i / 4;
+    const int64_t row = row_of(a, id, slot, h), at = row + token;
+    const uint32_t key = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.kc) + at * (D / 2))[C * (i % 4) + c];
+    const uint8_t* p = static_cast<const uint8_t*>(a.vc) + row * (D / 2) + ((16 * (token >> 2) + 8 * (i & 1)) * 4 + (token & 3)) * C + c;
+    uint32_t value = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) value |= (p[e * 4 * C] >> (i & 2 ? 4 : 0) & 15u) << (4 * e);
+    const float ks = low_bf16(a.ks[at * C + c]), vs = low_bf16(a.vs[at * C + c]);
+    const int64_t to = (static_cast<int64_t>(blockIdx.x) * a.kv_heads * 16 + (h * 16 + token)) * D + 8 * i;
+    float f[8];
+    fp4x8_to_f32(key, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= ks;
+    store_dequant16<F16 ? PGS_DTYPE_F16 : PGS_DTYPE_BF16>(g.k, to, f);
+    fp4x8_to_f32(value, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= vs;
+    store_dequant16<F16 ? PGS_DTYPE_F16 : PGS_DTYPE_BF16>(g.v, to, f);
+  }
+}
+
 // The launch shape, a function of sizes the host knows (never of what the device
 // arrays hold, so that a captured call replays with other lengths).
 struct Plan {
   int wide;   // rows of a group that share tiles through LDS, or 0
   int r, wr;  // else row tiles per wave, waves per key slice (4-bit: one tile per wave, r times the waves)
   int groups, splits, min_steps;
+  int64_t columns, chunk;  // (wide, 4-bit) blocks of sixteen a request, requests widened at a time
 };
-Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t max_tokens, int64_t max_context, int64_t window,
-          int64_t sinks, bool fp4) {
+constexpr int64_t kWidened = int64_t{1} << 29;  // bytes of 16-bit keys and values at a time, if one request's are no more
+Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_tokens, int64_t max_context,
+          int64_t window, int64_t sinks, bool fp4, int64_t columns, int64_t block_size) {
   const int64_t rows = max_tokens * (q_heads / kv_heads);
   Plan p{};
   p.splits = 1;
-  p.wide = rows <= 64 || fp4 ? 0 : 256;
-  if (p.wide) return p;
+  p.wide = rows <= 64 ? 0 : 256;
+  if (p.wide) {
+    if (fp4) {
+      p.columns = (columns * block_size + 15) / 16;
+      p.chunk = std::max<int64_t>(1, std::min<int64_t>(requests, kWidened / std::max<int64_t>(1, p.columns * kv_heads * 64 * head_dim)));
+    }
+    return p;
+  }
   p.r = rows <= 16 ? 1 : 2;
   p.wr = rows <= 32 ? 1 : 2;
   p.groups = static_cast<int>((rows + 63) / 64);
@@ -1190,8 +1245,13 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t max_token
 int64_t slots_of(const Plan& p, int64_t rows, int64_t q_heads) {
   return p.wide ? int64_t{2} * kShares * p.wide : p.splits == 1 ? 0 : rows * q_heads * p.splits;
 }
-size_t workspace_bytes(const Plan& p, int64_t rows, int64_t q_heads, int64_t head_dim) {
-  return static_cast<size_t>(slots_of(p, rows, q_heads)) * (head_dim + 4) * 4 + (p.wide ? kShares * sizeof(Begun) : 0);
+// the sums of parts, then (wide) the units begun, then (4-bit) keys, values and tables
+size_t parts_bytes(const Plan& p, int64_t rows, int64_t q_heads, int64_t head_dim) {
+  return (static_cast<size_t>(slots_of(p, rows, q_heads)) * (head_dim + 4) * 4 + (p.wide ? kShares * sizeof(Begun) : 0) + 255) /
+         256 * 256;
+}
+size_t workspace_bytes(const Plan& p, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
+  return parts_bytes(p, rows, q_heads, head_dim) + static_cast<size_t>(p.chunk * p.columns) * (kv_heads * 64 * head_dim + 4);
 }
 
 bool sizes_ok(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_tokens,
@@ -1213,10 +1273,34 @@ int launch_wide(const Window& a, hipStream_t st) {
   return check_launch("window attention join kernel");
 }
 
+template <int D, bool F16>
+int launch_wide4(const Window& a, const Plan& p, char* widened, hipStream_t st) {
+  const int64_t block = static_cast<int64_t>(a.kv_heads) * 16 * D;
+  for (int64_t b = 0; b < a.requests; b += p.chunk) {
+    Widen g{a, reinterpret_cast<uint16_t*>(widened), nullptr, nullptr, static_cast<int32_t>(p.columns)};
+    g.v = g.k + p.chunk * p.columns * block;
+    g.tables = reinterpret_cast<int32_t*>(g.v + p.chunk * p.columns * block);
+    Window& w = g.w;
+    w.requests = static_cast<int32_t>(std::min<int64_t>(p.chunk, a.requests - b));
+    w.lens += b, w.offsets += b, w.tables += b * a.tstride;
+    hipLaunchKernelGGL((widen_kernel<D, F16>), dim3(static_cast<unsigned>(w.requests * p.columns)), dim3(256), 0, st, g);
+    if (int rc = check_launch("widen kernel")) return rc;
+    w.kc = g.k, w.vc = g.v;
+    w.kc_block = w.vc_block = block, w.kc_head = w.vc_head = 16 * D, w.kc_slot = w.vc_slot = D;
+    w.blocks = static_cast<int32_t>(w.requests * p.columns), w.bs = 16, w.bs_inv = 1u << 28;
+    // (lengths are cut to what the caller's tables hold, a multiple of sixteen too)
+    w.tables = g.tables, w.tstride = p.columns, w.cols = static_cast<int32_t>(p.columns);
+    if (int rc = launch_wide<D, F16>(w, st)) return rc;
+  }
+  return PGS_OK;
+}
+
 template <int D, bool F16, bool FP4>
-int launch(const Window& a, const Plan& p, hipStream_t st) {
-  if constexpr (!FP4)
-    if (p.wide) return launch_wide<D, F16>(a, st);
+int launch(const Window& a, const Plan& p, char* widened, hipStream_t st) {
+  if (p.wide) {
+    if constexpr (FP4) return p.columns == 0 ? launch_wide<D, F16>(a, st) : launch_wide4<D, F16>(a, p, widened, st);
+    else return launch_wide<D, F16>(a, st);
+  }
   const dim3 g(static_cast<unsigned>(static_cast<int64_t>(a.requests) * a.kv_heads * p.groups * p.splits));
   constexpr int R = FP4 ? 1 : 2;
   if (p.r == 1) hipLaunchKernelGGL((window_kernel<D, 1, 1, 4, F16, FP4>), g, dim3(256), 0, st, a);
@@ -1245,14 +1329,17 @@ int launch(const Window& a, const Plan& p, hipStream_t st) {
 
 using namespace pgs;
 
-extern "C" size_t pgs_window_attention_workspace_bytes(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads,
-                                                       int64_t head_dim, int64_t max_tokens, int64_t max_context,
-                                                       int64_t window, int64_t sinks, int four_bits) {
-  if (!sizes_ok(rows, requests, q_heads, kv_heads, head_dim, max_tokens, max_context, window, sinks) || rows == 0 ||
-      requests == 0)
+extern "C" size_t pgs_window_attention_workspace_bytes(const pgs_window_attention_args* args) {
+  if (!args || !args->cache == !args->cache4) return 0;
+  const pgs_window_attention_args& g = *args;
+  const int64_t kv = g.cache ? g.cache->kv_heads : g.cache4->kv_heads, dim = g.cache ? g.cache->head_dim : g.cache4->head_dim;
+  const int64_t size = g.cache ? g.cache->block_size : g.cache4->block_size;
+  if (!sizes_ok(g.rows, g.requests, g.q_heads, kv, dim, g.max_tokens, g.max_context, g.window, g.sinks) || g.rows == 0 ||
+      g.requests == 0 || size < 16 || size > 0x10000 || g.columns < 0 || g.columns > 0x7fff0000 / size)
     return 0;
-  const Plan p = plan(requests, q_heads, kv_heads, std::min(max_tokens, rows), max_context, window, sinks, four_bits);
-  return workspace_bytes(p, rows, q_heads, head_dim);
+  const Plan p = plan(g.requests, g.q_heads, kv, dim, std::min(g.max_tokens, g.rows), g.max_context, g.window, g.sinks,
+                      !g.cache, g.columns, size);
+  return workspace_bytes(p, g.rows, g.q_heads, kv, dim);
 }
 
 extern "C" int pgs_window_attention(const pgs_window_attention_args* args, void* workspace, size_t workspace_bytes_given,
@@ -1279,8 +1366,9 @@ extern "C" int pgs_window_attention(const pgs_window_attention_args* args, void*
   if (!aligned(g.q, 16) || !aligned(g.out, 16) || !aligned(g.lse, 4) || !aligned(g.lens, 4) || !aligned(g.offsets, 4))
     return fail(PGS_ERR_MISALIGNED, "%s: misaligned", fn);
   const int64_t most = std::min(g.max_tokens, g.rows);  // (no request has more rows than the batch)
-  const Plan p = plan(g.requests, g.q_heads, a.kv_heads, most, g.max_context, g.window, g.sinks, !g.cache);
-  const size_t need = workspace_bytes(p, g.rows, g.q_heads, dim);
+  const Plan p = plan(g.requests, g.q_heads, a.kv_heads, dim, most, g.max_context, g.window, g.sinks, !g.cache, g.columns, a.bs);
+  const size_t need = workspace_bytes(p, g.rows, g.q_heads, a.kv_heads, dim);
+  if (p.chunk * p.columns > 0x7fffffff) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: too large", fn);
   if (need > 0 && (!workspace || workspace_bytes_given < need || !aligned(workspace, 256)))
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -1301,10 +1389,11 @@ extern "C" int pgs_window_attention(const pgs_window_attention_args* args, void*
   a.part = static_cast<float*>(workspace);
   a.stat = a.part + slots_of(p, g.rows, g.q_heads) * dim;
   a.begun = reinterpret_cast<Begun*>(a.stat + slots_of(p, g.rows, g.q_heads) * 4);
+  char* widened = static_cast<char*>(workspace) + parts_bytes(p, g.rows, g.q_heads, dim);
   auto go = [&](auto d, auto f16) {
     constexpr int D = decltype(d)::value;
     constexpr bool F = decltype(f16)::value;
-    return g.cache ? launch<D, F, false>(a, p, st) : launch<D, F, true>(a, p, st);
+    return g.cache ? launch<D, F, false>(a, p, widened, st) : launch<D, F, true>(a, p, widened, st);
   };
   if (dim == 64) return g.dtype == PGS_DTYPE_F16 ? go(Int<64>{}, Int<1>{}) : go(Int<64>{}, Int<0>{});
   return g.dtype == PGS_DTYPE_F16 ? go(Int<128>{}, Int<1>{}) : go(Int<128>{}, Int<0>{});

@@ -135,15 +135,26 @@ def test_nothing_to_do(native_lib):
 
 
 def test_workspaces(native_lib):
-    def need(*sizes, four=0):
-        return native_lib.pgs_window_attention_workspace_bytes(*sizes, four)
+    def need(four=False, columns=6250, **change):
+        c, c4 = _cache(), _cache4()
+        a = _native.WindowAttentionArgs(rows=1, requests=1, q_heads=16, max_tokens=1, max_context=64, window=1 << 30,
+                                        columns=columns, table_stride=columns)
+        if four:
+            a.cache4 = ctypes.pointer(c4)
+        else:
+            a.cache = ctypes.pointer(c)
+        return native_lib.pgs_window_attention_workspace_bytes(ctypes.byref(_set(a, change)))
 
-    assert need(1, 1, 16, 2, 128, 1, 64, 64, 0) == 0
-    assert need(1, 1, 16, 2, 128, 1, 100000, 1 << 30, 0) > 0
+    assert need() == need(four=True) == 0
+    assert need(max_context=100000) > 0
     # a window bounds the split whatever the context, and no request has more rows than the batch
-    assert need(1, 1, 16, 2, 128, 1, 100000, 100, 4) == 0
-    assert need(1, 1, 16, 2, 128, 1, 100000, 1 << 30, 0) == need(1, 1, 16, 2, 128, 500, 100000, 1 << 30, 0)
-    assert need(900, 1, 16, 2, 128, 900, 100000, 1 << 30, 0) > 0
-    assert need(-1, 1, 16, 2, 128, 1, 64, 64, 0) == 0 and need(1, 1, 15, 2, 128, 1, 64, 64, 0) == 0
+    assert need(max_context=100000, window=100, sinks=4) == 0
+    assert need(max_context=100000) == need(max_context=100000, max_tokens=500)
+    many = {"rows": 900, "max_tokens": 900, "max_context": 100000}
+    assert need(**many) > 0
+    # (many rows over a 4-bit cache: one request's tokens in 16 bits, and the table of them)
+    assert need(four=True, **many) - need(**many) == 6250 * (2 * 64 * 128 + 4)
+    assert need(rows=-1) == need(q_heads=15) == need(columns=-1) == 0
+    assert native_lib.pgs_window_attention_workspace_bytes(None) == 0
     assert native_lib.pgs_evict_tokens_workspace_bytes(3, 100) == 3 * 101 * 4
     assert native_lib.pgs_evict_tokens_workspace_bytes(0, 100) == 0
