@@ -55,7 +55,7 @@ struct Window {
   int32_t max_tokens, window, sinks;
   int32_t groups, splits, min_steps;  // row groups of a request; parts of the keys
   float c;      // |scale| * log2(e) (accumulate_weights: signed)
-  uint32_t flip;  // the sign bits of a negative scale, for the rows
+  uint32_t flip, keep;  // for the rows: the sign bits of a negative scale; no bits where it is 0
   float* part;  // sums of the parts of rows: [slots][D]
   float* stat;  // [slots][4]: reference, sum, sum of the weights before their rounding, -
   Begun* begun;   // (wide) [shares]
@@ -99,6 +99,12 @@ __device__ __forceinline__ Span span_of(const Args& a, int pmin, int pmax) {
 
 // whether a row at p sees token j; low: p - window
 __device__ __forceinline__ bool visible(int j, int p, int low, int sinks) { return j <= p && (j > low || j < sinks); }
+// bits 0 .. n - 1 (none below 0, all from 32 on)
+__device__ __forceinline__ uint32_t bits(int n) { return n >= 32 ? ~0u : (1u << max(n, 0)) - 1; }
+// which of the keys key0 .. key0 + 31 it sees
+__device__ __forceinline__ uint32_t visible32(int key0, int p, int low, int sinks) {
+  return bits(p - key0 + 1) & (~bits(low < key0 ? 0 : low - key0 + 1) | bits(sinks - key0));
+}
 // (p - window for any p: where there is none p is below 0 and sees nothing anyhow)
 __device__ __forceinline__ int low_of(int p, int window) { return max(p, -1) - window; }
 // whether all rows at pmin .. pmax see all of the keys key0 .. last

@@ -51,7 +51,7 @@ struct Rows {
       const int row = min(row0 + 16 * r + li, nrows - 1), t = row / a.group;  // (rows past the last repeat it)
       const uint16_t* p = a.q + (rq.row0 + t) * a.q_row + (kh * a.group + row - t * a.group) * a.q_head + 8 * lg;
 #pragma unroll
-      for (int d = 0; d < DC; ++d) q[r][d] = ld16(p + 32 * d) ^ a.flip;
+      for (int d = 0; d < DC; ++d) q[r][d] = (ld16(p + 32 * d) ^ a.flip) & a.keep;
       pos[r] = rq.first + t;
     }
     // (they have arrived here: a wait for them inside the loop over the keys would be
@@ -104,14 +104,9 @@ struct Rows {
   }
   // which of the step's eight keys of this lane its row r sees
   __device__ __forceinline__ uint32_t seen(const Window& a, int r, int key0, bool bad0, bool bad1, int lg) const {
-    const int low = low_of(pos[r], a.window);
-    uint32_t ok = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int key = key0 + 16 * (e >> 2) + 4 * lg + (e & 3);
-      ok |= visible(key, pos[r], low, a.sinks) && !(e >> 2 ? bad1 : bad0) ? 1u << e : 0;
-    }
-    return ok;
+    const uint32_t m = visible32(key0, pos[r], low_of(pos[r], a.window), a.sinks) & ((bad0 ? 0 : 0xffffu) | (bad1 ? 0 : 0xffff0000u));
+    const uint32_t t = m >> (4 * lg);
+    return (t & 0xf) | (t >> 12 & 0xf0);
   }
   // Weights of a step: s[r][h] the scores of keys key0 + 16 h + 4 lg + i, x[r][4 h + i] the
   // weights against the rows' references, which are raised first where a score needs it.
@@ -558,6 +553,11 @@ struct Groups {
   int n;            // of a request
   int none, rising;  // those before `none` see nothing; those before `rising` cost less than cap
   int64_t base, cap, unit;
+  // counts of group m
+  template <int RG>
+  __device__ __forceinline__ int64_t cost(int m) const {
+    return unit + (m < none ? 0 : m < rising ? base + RG * static_cast<int64_t>(m + 1) : cap);
+  }
   // counts of the first m groups
   template <int RG>
   __device__ __forceinline__ int64_t upto(int m) const {
@@ -599,6 +599,15 @@ struct Work {
     int b, kh, rg;
     int64_t begin, cost;  // where its counts begin, how many they are
   };
+  // the unit behind u; whether it is one of its request and head
+  __device__ __forceinline__ bool step(Unit& u) const {
+    const Groups g = groups_of<RG>(a, u.rq);
+    if (u.rg + 1 >= g.n) return false;
+    ++u.rg;
+    u.begin += u.cost;
+    u.cost = uniform64(g.template cost<RG>(u.rg));
+    return true;
+  }
   // pre for the requests from `first` on; every thread must call it
   __device__ __forceinline__ void fill(int first, int64_t before) {
     const int thread = here(threadIdx.x), lane = thread & 63, wave = thread >> 6;
@@ -646,7 +655,9 @@ struct Work {
     u.rq = Ragged{uniform(rq.row0), uniform(rq.tokens), uniform(rq.len), uniform(rq.first)};
     const Groups g = groups_of<RG>(a, u.rq);
     const int64_t first = uniform64(lo ? pre[lo - 1] : carry), per = g.template upto<RG>(g.n);
-    u.kh = uniform(static_cast<int>((pos - first) / per));
+    int kh = 0;  // (few: no division)
+    while (kh + 1 < a.kv_heads && first + (kh + 1) * per <= pos) ++kh;
+    u.kh = uniform(kh);
     const int64_t head = first + u.kh * per;
     // the last group that begins by pos
     int at = 0, end = g.n - 1;
@@ -657,7 +668,7 @@ struct Work {
     }
     u.rg = uniform(at);
     u.begin = uniform64(head + g.template upto<RG>(u.rg));
-    u.cost = uniform64(g.template upto<RG>(u.rg + 1) - g.template upto<RG>(u.rg));
+    u.cost = uniform64(g.template cost<RG>(u.rg));
     return u;
   }
 };
@@ -667,9 +678,14 @@ __device__ __forceinline__ bool below(int64_t a, int64_t b) {
   asm volatile("" : "+s"(b));
   return a < b;
 }
-// the first of a unit's `tiles` that lies behind `counts` of its cost
+// The first of a unit's `tiles` that lies behind `counts` of its cost.  (In floats: any rule does
+// that never falls as counts grow and that both shares of a border follow; a 64-bit division takes
+// a hundred instructions.)
 __device__ __forceinline__ int tile_at(int64_t counts, int64_t cost, int tiles) {
-  return counts <= 0 ? 0 : counts >= cost ? tiles : static_cast<int>(counts * tiles / cost);
+  if (counts <= 0) return 0;
+  if (counts >= cost) return tiles;
+  const float per = static_cast<float>(tiles) * __builtin_amdgcn_rcpf(static_cast<float>(cost));
+  return min(static_cast<int>(static_cast<float>(counts) * per), tiles);
 }
 
 // 32 rows of a wave and their running sums, for v_mfma_f32_32x32x16: lane l holds row l%32 and
@@ -703,7 +719,7 @@ struct Rows32 {
     const int row = min(row0 + (lane & 31), nrows - 1), t = row / a.group;  // (rows past the last repeat it)
     const uint16_t* p = a.q + (rq.row0 + t) * a.q_row + (kh * a.group + row - t * a.group) * a.q_head + 8 * (lane >> 5);
 #pragma unroll
-    for (int d = 0; d < DC; ++d) q[d] = ld16(p + 16 * d) ^ a.flip;
+    for (int d = 0; d < DC; ++d) q[d] = (ld16(p + 16 * d) ^ a.flip) & a.keep;
     pos = rq.first + t;
     // (they have arrived here: a wait for them inside the loop over the keys would be
     // a wait for the keys on their way too)
@@ -717,20 +733,20 @@ struct Rows32 {
   }
 
   static __device__ __forceinline__ int key_of(int e, int lane) { return 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
-  // which of the step's sixteen keys of this lane its row sees
-  __device__ __forceinline__ uint32_t seen(const Window& a, int key0, bool bad0, bool bad1, int lane) const {
-    const int low = low_of(pos, a.window);
-    uint32_t ok = 0;
+  // the scores of a step at key0, -infinity where the lane's row does not see the key; bad: its absent sixteens
+  __device__ __forceinline__ void hide(const Window& a, f32x16& x, int key0, uint32_t bad, int lane) const {
+    const uint32_t m = visible32(key0, pos, low_of(pos, a.window), a.sinks) & ((bad & 1 ? 0 : 0xffffu) | (bad & 2 ? 0 : 0xffff0000u));
+    const uint32_t t = m >> (4 * (lane >> 5));
+    const uint32_t ok = (t & 0xf) | (t >> 4 & 0xf0) | (t >> 8 & 0xf00) | (t >> 12 & 0xf000);
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      ok |= visible(key0 + key_of(e, lane), pos, low, a.sinks) && !(e >> 3 ? bad1 : bad0) ? 1u << e : 0;
-    return ok;
+    for (int e = 0; e < 16; ++e) x[e] = ok >> e & 1 ? x[e] : -INFINITY;
   }
-  // as in Rows
-  __device__ __forceinline__ void raise(const Window& a, const f32x16& x, uint32_t ok) {
+  // as in Rows, for two steps
+  __device__ __forceinline__ void raise(const Window& a, const f32x16 (&x)[2]) {
     float top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) top = fmaxf(top, ok >> e & 1 ? x[e] * a.c : -INFINITY);
+    for (int e = 0; e < 16; ++e) top = fmaxf(fmaxf(top, x[0][e]), x[1][e]);
+    top *= a.c;
     if (!__ballot(top - mx > kSlack + E::kHead)) return;
     const float t = both(top, true);
     const float ref = fmaxf(fabsf(t) > kFar ? t : t - E::kHead, mx), f = __builtin_amdgcn_exp2f(mx - ref);
@@ -754,18 +770,12 @@ struct Rows32 {
     for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(fmaf(x[8 * h + e], a.c, -mx));
     return take(y, p);
   }
-  // The same where there are masks, or references that the exponent's rounding matters for.
-  __device__ __forceinline__ float unusual(const Window& a, const f32x16& x, uint32_t ok, u32x4& p0, u32x4& p1) const {
-    float sum = 0.f;
+  // The same for references that the exponent's rounding matters for.
+  __device__ __forceinline__ float weights_far(const Window& a, const f32x16& x, int h, u32x4& p) const {
+    float y[8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float y[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        y[e] = ok >> (8 * h + e) & 1 ? __builtin_amdgcn_exp2f(exponent(x[8 * h + e], a.c, mx, far)) : 0.f;
-      sum += take(y, h ? p1 : p0);
-    }
-    return sum;
+    for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(exponent(x[8 * h + e], a.c, mx, true));
+    return take(y, p);
   }
   // values that are not finite (bit of odd; the products had zeros for them), for the rows that see them
   template <typename Value>
@@ -866,9 +876,13 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
   const int64_t begin = uniform64(share_begin(work.total, share, shares));
   const int64_t end = uniform64(share_begin(work.total, share + 1, shares));
 
+  typename Work<RG, 64 * NW>::Unit un;
+  bool known = false;
   for (int64_t pos = begin; below(pos, end);) {
     work.a = again<Window>();
-    const auto un = work.find(pos);
+    if (known) known = work.step(un);
+    if (!known) un = work.find(pos);
+    known = true;
     const Window& a = a0;
     const Ragged& rq = un.rq;
     const int kh = un.kh, nrows = rq.tokens * a.group, first_row = un.rg * RG;
@@ -917,15 +931,19 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
     // This share's i-th tile into its buffer, in three pieces that stand between the products of
     // another one (behind the last tile: that one again, where nothing reads it).
     int load_slot = 0, load_block = 0;
+    auto fetch_ids = [&](int t) {
+      const int last = (pmax & ~15) + wave * KW % 16;
+      id0 = t;
+      int slot;
+      const int64_t key = least(static_cast<int64_t>(t + here(lane)) * TK + wave * KW, last);
+      id_lane = table[block_of(a, static_cast<int>(key), slot)];
+    };
     auto load_id = [&](int i) {
       const int t = span.tile(min(i, t1 - 1));
       // (keys of a sixteen past the last one are those of the sixteen with the last one instead, and masked)
       const int last = (pmax & ~15) + wave * KW % 16;
       if (__builtin_expect(static_cast<uint32_t>(t - id0) >= 64u, 0)) {
-        id0 = t;
-        int slot;
-        const int64_t key = least(static_cast<int64_t>(t + here(lane)) * TK + wave * KW, last);
-        id_lane = table[block_of(a, static_cast<int>(key), slot)];
+        fetch_ids(t);
         asm volatile("" : "+v"(id_lane));
       }
       const int id = __builtin_amdgcn_readlane(id_lane, t - id0);
@@ -1016,36 +1034,34 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
         v[d] = u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
     };
-    // which of a tile's keys the lane's row sees, where some row does not see all
-    auto seen = [&](int i, bool masked, uint32_t bm, int j) {
-      return masked ? w.seen(a, span.tile(i) * TK + 32 * j, bm >> (2 * j) & 1, bm >> (2 * j + 1) & 1, here(lane)) : 0xffff;
-    };
-    // tile i's scores in s: whether it has masks, its absent sixteens; the references raised
-    auto take = [&](int i, const Scores& s, bool over, uint32_t any, uint32_t& bm) {
+    // tile i's scores in s, whether one of them may need a higher reference: what its rows do not
+    // see is hidden, references are raised; whether it has masks
+    auto take = [&](int i, Scores& s, bool over, uint32_t any) {
       bool masked = !plain(i);
-      bm = 0;
+      uint32_t bm = 0;
       if (__builtin_expect(masked || any, 0)) {
         bm = absent_of(lflags[i % kBuffers][here(lane) & (NW - 1)]);
         const int key0 = span.tile(i) * TK;
         masked = bm || !all_visible(a, key0, key0 + TK - 1, wmin, wmax);
+        if (masked) {
+          w.hide(a, s[0], key0, bm, here(lane));
+          w.hide(a, s[1], key0 + 32, bm >> 2, here(lane));
+        }
       }
-      if (__builtin_expect(masked || over || w.far, 0)) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) w.raise(a, s[j], seen(i, masked, bm, j));
-      }
+      if (__builtin_expect(masked || over || w.far, 0)) w.raise(a, s);
       return masked;
     };
 
     constexpr int L = 2 * J;  // loads of a wave per tile
     if (threadIdx.x == 0) lany = 0;
+    if (t0 < t1) fetch_ids(span.tile(t0));
+    w.load(again<Window>(), rq, kh, min(row0, nrows - 1), nrows, here(lane));
     __syncthreads();
-    if (t0 < t1)
+    if (t0 < t1) {
 #pragma unroll 1
       for (int i = t0; i < t0 + 3; ++i) load(i);
-    w.load(again<Window>(), rq, kh, min(row0, nrows - 1), nrows, here(lane));
-    if (t0 < t1) {
       Scores s0, s1;
-      arrived<0>();
+      arrived<2 * L>();
       settle(t0);
       __syncthreads();
 #pragma unroll
@@ -1054,8 +1070,7 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
         read_keys(t0, n, k);
         multiply_keys(n, k, s0);
       }
-      uint32_t bm;
-      bool masked = take(t0, s0, true, lany, bm), settles = to_settle(t0 + 1);
+      bool masked = take(t0, s0, true, lany), settles = to_settle(t0 + 1);
 
       // Tile i, its scores in x; the next one's go to s.
       auto tile = [&](int i, const Scores& x, Scores& s) {
@@ -1085,10 +1100,10 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
           if (n == 3) settles = to_settle(i + 2);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (__builtin_expect(masked || w.far, 0)) {
+        if (__builtin_expect(w.far, 0)) {
           sum = 0.f;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) sum += w.unusual(a, x[j], seen(i, masked, bm, j), p[2 * j], p[2 * j + 1]);
+          for (int n = 0; n < 4; ++n) sum += w.weights_far(a, x[n >> 1], n & 1, p[n]);
         }
         w.sum += sum;
         // its output beside the next one's largest scores
@@ -1121,7 +1136,7 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
             });
           }
         }
-        if (i + 1 < t1) masked = take(i + 1, s, __ballot(fmaf(top, a.c, -w.mx) > kSlack + E::kHead), uniform(static_cast<int>(any_v)), bm);
+        if (i + 1 < t1) masked = take(i + 1, s, __ballot(fmaf(top, a.c, -w.mx) > kSlack + E::kHead), uniform(static_cast<int>(any_v)));
       };
       for (int i = t0; i < t1; i += 2) {
         tile(i, s0, s1);
@@ -1168,21 +1183,17 @@ struct Widen {
   Window w;
   uint16_t *k, *v;
   int32_t* tables;  // [requests][columns]
-  int32_t columns;
+  int32_t columns, grid;  // grid: workgroups of a request
 };
 template <int D, bool F16>
-__global__ __launch_bounds__(256) void widen_kernel(Widen g) {
+__device__ __forceinline__ void widen_block(const Widen& g, int b, int col) {
   const Window& a = g.w;
   constexpr int C = D / 32, P = D / 8;
-  const int b = blockIdx.x / g.columns, col = blockIdx.x % g.columns;
-  const Ragged rq = ragged(a, b);
-  if (col * 16 >= rq.len) return;
-  // (what no row of the request sees, if it has any, is left out)
-  if (rq.tokens == 0 || (col * 16 + 15 <= low_of(rq.first, a.window) && col * 16 >= a.sinks)) return;
   int slot;
   const int id = a.tables[b * a.tstride + block_of(a, col * 16, slot)];
   const bool bad = id < 0 || id >= a.blocks;
-  if (threadIdx.x == 0) g.tables[blockIdx.x] = bad ? -1 : static_cast<int32_t>(blockIdx.x);
+  const int at0 = b * g.columns + col;
+  if (threadIdx.x == 0) g.tables[at0] = bad ? -1 : at0;
   if (bad) return;
   for (int u = threadIdx.x; u < a.kv_heads * 16 * P; u += 256) {
     const int i = u % P, token = u / P % 16, h = u / (16 * P), c = i / 4;
@@ -1193,7 +1204,7 @@ __global__ __launch_bounds__(256) void widen_kernel(Widen g) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) value |= (p[e * 4 * C] >> (i & 2 ? 4 : 0) & 15u) << (4 * e);
     const float ks = low_bf16(a.ks[at * C + c]), vs = low_bf16(a.vs[at * C + c]);
-    const int64_t to = (static_cast<int64_t>(blockIdx.x) * a.kv_heads * 16 + (h * 16 + token)) * D + 8 * i;
+    const int64_t to = (static_cast<int64_t>(at0) * a.kv_heads * 16 + (h * 16 + token)) * D + 8 * i;
     float f[8];
     fp4x8_to_f32(key, f);
 #pragma unroll
@@ -1206,13 +1217,26 @@ __global__ __launch_bounds__(256) void widen_kernel(Widen g) {
   }
 }
 
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void widen_kernel(Widen g) {
+  const Window& a = g.w;
+  const int b = blockIdx.x / g.grid;
+  const Ragged rq = ragged(a, b);
+  if (rq.tokens == 0) return;
+  for (int64_t col = blockIdx.x % g.grid; col * 16 < rq.len; col += g.grid) {
+    // (what no row of the request sees is left out)
+    if (col * 16 + 15 <= low_of(rq.first, a.window) && col * 16 >= a.sinks) continue;
+    widen_block<D, F16>(g, b, static_cast<int>(col));
+  }
+}
+
 // The launch shape, a function of sizes the host knows (never of what the device
 // arrays hold, so that a captured call replays with other lengths).
 struct Plan {
   int wide;   // rows of a group that share tiles through LDS, or 0
   int r, wr;  // else row tiles per wave, waves per key slice (4-bit: one tile per wave, r times the waves)
   int groups, splits, min_steps;
-  int64_t columns, chunk;  // (wide, 4-bit) blocks of sixteen a request, requests widened at a time
+  int64_t columns, chunk, widen;  // (wide, 4-bit) blocks of sixteen a request, requests widened at a time, workgroups each
 };
 constexpr int64_t kWidened = int64_t{1} << 29;  // bytes of 16-bit keys and values at a time, if one request's are no more
 Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_tokens, int64_t max_context,
@@ -1224,6 +1248,7 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
   if (p.wide) {
     if (fp4) {
       p.columns = (columns * block_size + 15) / 16;
+      p.widen = std::max<int64_t>(1, std::min(p.columns, (max_context + 15) / 16));
       p.chunk = std::max<int64_t>(1, std::min<int64_t>(requests, kWidened / std::max<int64_t>(1, p.columns * kv_heads * 64 * head_dim)));
     }
     return p;
@@ -1277,13 +1302,13 @@ template <int D, bool F16>
 int launch_wide4(const Window& a, const Plan& p, char* widened, hipStream_t st) {
   const int64_t block = static_cast<int64_t>(a.kv_heads) * 16 * D;
   for (int64_t b = 0; b < a.requests; b += p.chunk) {
-    Widen g{a, reinterpret_cast<uint16_t*>(widened), nullptr, nullptr, static_cast<int32_t>(p.columns)};
+    Widen g{a, reinterpret_cast<uint16_t*>(widened), nullptr, nullptr, static_cast<int32_t>(p.columns), static_cast<int32_t>(p.widen)};
     g.v = g.k + p.chunk * p.columns * block;
     g.tables = reinterpret_cast<int32_t*>(g.v + p.chunk * p.columns * block);
     Window& w = g.w;
     w.requests = static_cast<int32_t>(std::min<int64_t>(p.chunk, a.requests - b));
     w.lens += b, w.offsets += b, w.tables += b * a.tstride;
-    hipLaunchKernelGGL((widen_kernel<D, F16>), dim3(static_cast<unsigned>(w.requests * p.columns)), dim3(256), 0, st, g);
+    hipLaunchKernelGGL((widen_kernel<D, F16>), dim3(static_cast<unsigned>(w.requests * p.widen)), dim3(256), 0, st, g);
     if (int rc = check_launch("widen kernel")) return rc;
     w.kc = g.k, w.vc = g.v;
     w.kc_block = w.vc_block = block, w.kc_head = w.vc_head = 16 * D, w.kc_slot = w.vc_slot = D;
@@ -1385,7 +1410,9 @@ extern "C" int pgs_window_attention(const pgs_window_attention_args* args, void*
   a.groups = p.groups, a.splits = p.splits, a.min_steps = p.min_steps;
   // (a negative scale changes the rows' signs: the largest score is then always the largest weight's)
   a.c = std::fabs(g.scale) * 1.44269504088896340736f;
-  a.flip = std::signbit(g.scale) ? 0x80008000u : 0;
+  // (and a scale of 0 the rows to zeros: -infinity times it would be no score)
+  a.flip = std::signbit(g.scale) ? 0x80008000u : 0, a.keep = g.scale == 0.f ? 0 : ~0u;
+  if (g.scale == 0.f) a.c = 1.f;
   a.part = static_cast<float*>(workspace);
   a.stat = a.part + slots_of(p, g.rows, g.q_heads) * dim;
   a.begun = reinterpret_cast<Begun*>(a.stat + slots_of(p, g.rows, g.q_heads) * 4);
