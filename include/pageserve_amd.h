@@ -725,7 +725,12 @@ typedef struct pgs_accumulate_weights_args {
  * heads that see j: sum of e^(scale q . k_j - lse).  Sums are fp32, in a fixed
  * order.  Tokens in a block outside the cache are left out.
  */
-int pgs_accumulate_weights(const pgs_accumulate_weights_args* args, void* stream);
+int pgs_accumulate_weights(const pgs_accumulate_weights_args* args, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of a call with these arguments (0: none needed), 4-byte aligned, no
+ * fill needed. */
+size_t pgs_accumulate_weights_workspace_bytes(const pgs_accumulate_weights_args* args);
 
 /*
  * Cuts each request of more than budget[b] tokens to budget[b] (below 0: 0): the

@@ -185,7 +185,8 @@ SIGNATURES = {
     "pgs_read_kv4": (_INT, [ctypes.POINTER(KVCache4), _VP, _I64, _VP, _VP, _INT, _VP]),
     "pgs_window_attention": (_INT, [ctypes.POINTER(WindowAttentionArgs), _VP, _SZ, _VP]),
     "pgs_window_attention_workspace_bytes": (_SZ, [ctypes.POINTER(WindowAttentionArgs)]),
-    "pgs_accumulate_weights": (_INT, [ctypes.POINTER(AccumulateWeightsArgs), _VP]),
+    "pgs_accumulate_weights": (_INT, [ctypes.POINTER(AccumulateWeightsArgs), _VP, _SZ, _VP]),
+    "pgs_accumulate_weights_workspace_bytes": (_SZ, [ctypes.POINTER(AccumulateWeightsArgs)]),
     "pgs_evict_tokens": (_INT, [_VP] * 4 + [_I64] * 8 + [ctypes.POINTER(KVCache), _I64, ctypes.POINTER(KVCache4), _I64,
                                                          _VP, _VP, _SZ, _VP]),
     "pgs_evict_tokens_workspace_bytes": (_SZ, [_I64, _I64]),

@@ -780,7 +780,10 @@ void accumulate_weights(const at::Tensor& q, const std::vector<at::Tensor>& cach
   a.sinks = sinks;
   a.scale = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(dim)));
   void* st = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
-  check_rc(pgs_accumulate_weights(&a, st), what);
+  const size_t need = pgs_accumulate_weights_workspace_bytes(&a);
+  at::Tensor ws;  // (per call, as in tree_attention)
+  if (need) ws = at::empty({static_cast<int64_t>(need)}, qr.options().dtype(at::kByte));
+  check_rc(pgs_accumulate_weights(&a, need ? ws.data_ptr() : nullptr, need, st), what);
 }
 
 at::Tensor evict_tokens(const at::Tensor& weights, const at::Tensor& lens, const at::Tensor& budget,

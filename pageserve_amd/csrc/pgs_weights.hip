@@ -13,89 +13,176 @@ namespace {
 
 struct Weigh {
   Window w;
-  float* weights;      // [blocks][block_size]
+  float* weights;        // [blocks][block_size]
   const int32_t* fresh;  // [requests], or null: the last tokens whose sums start from 0
-  int tiles;           // of kTile tokens: workgroups per request
+  int tiles, parts;      // of kTile tokens: workgroups per request; parts of the rows
+  float* sums;           // (parts > 1) [requests][columns * block_size][parts]
 };
-constexpr int kTile = 128, kWaves = kTile / 32;
+constexpr int kWaves = 4, kTile = 32 * kWaves;
 
-// A wave's 32 tokens stay in registers as A operands, one key head after the other; the rows
-// pass by as B operands, sixteen (token, query head) at a time, and lane l adds up the
-// weights of tokens 4 (l/16) + i for row l%16.  Every sum is one wave's: the order of the
-// additions is fixed.
+// One workgroup per request, tile of 128 tokens and part of the rows (of all key heads, 32 (token,
+// query head) at a time).  A wave's 32 tokens stay in registers as A operands of
+// v_mfma_f32_32x32x16, 4-bit ones widened exactly; the rows pass by through LDS as B operands,
+// shared by the waves, and lane l adds up the weights of tokens 8 b + 4 (l/32) + i for row l%32.
+// Every sum is one wave's, those of the parts are added in order: the order of all additions is
+// fixed.  Bound by the vector units (a fused multiply-add, an exponential and an addition a
+// score, next to a product of 128 dims), for single rows by reading the keys.
 template <int D, bool F16, bool FP4>
-__global__ __launch_bounds__(64 * kWaves) void weigh_kernel(Weigh g) {
+__global__ __launch_bounds__(64 * kWaves, 4) void weigh_kernel(Weigh g) {
   const Window& a = g.w;
-  constexpr int DC = D / 32;
-  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  typedef typename Elem<F16>::x8 x8;
+  constexpr int DC = D / 16, P = D / 8, KI = 64 / P, J = 32 / kWaves / KI;
+  static_assert(J >= 1);
+  __shared__ __attribute__((aligned(256))) uint16_t lq[2][32 * D];
+  const int lane = threadIdx.x & 63, li = lane & 31, h = lane >> 5;
   const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
-  const int b = blockIdx.x / g.tiles;
+  // piece p of row r lies at p ^ turn: sixteen rows' pieces meet all banks
+  auto turn = [](int r) { return r * P / 16 & (P - 1); };
+  const uint32_t q_at = lds_address(lq) + li * (2 * D) + 16 * (h ^ turn(li));
+  const int part = blockIdx.x % g.parts, unit = blockIdx.x / g.parts, b = unit / g.tiles;
   const Ragged rq = ragged(a, b);
   const int32_t* table = a.tables + b * a.tstride;
   const int fresh = rq.len - (g.fresh ? min(max(g.fresh[b], 0), rq.len) : 0);  // the first of them
-  for (int64_t tile = blockIdx.x % g.tiles; tile * kTile + 32 * wave < rq.len; tile += g.tiles) {
-    const int key0 = static_cast<int>(tile) * kTile + 32 * wave;
-    // the rows that see some of them
-    int t0 = max(0, key0 - rq.first), t1 = rq.tokens;
-    if (key0 >= a.sinks) t1 = static_cast<int>(least(t1, static_cast<int64_t>(key0) + 31 + a.window - rq.first));
-    if (t0 >= t1 && key0 + 32 <= fresh) continue;
-    bool bad[2];
-    int64_t blk[2];
-    int slot[2];
+  for (int64_t tile = unit % g.tiles; tile * kTile < rq.len; tile += g.tiles) {
+    const int tile0 = static_cast<int>(tile) * kTile, key0 = tile0 + 32 * wave;
+    // the tokens whose rows see some of them
+    const int ta = max(0, tile0 - rq.first);
+    int tb = rq.tokens;
+    if (tile0 >= a.sinks) tb = static_cast<int>(least(tb, largest(static_cast<int64_t>(tile0) + kTile - 1 + a.window - rq.first, ta)));
+    if (ta >= tb && tile0 + kTile <= fresh) continue;
+    // the lane's key (one past the last is the last, and masked)
+    int slot;
+    const int id = table[block_of(a, min(key0 + li, rq.len - 1), slot)];
+    const bool bad = id < 0 || id >= a.blocks;
+    const int64_t blk = bad ? 0 : id;
+    // the sum that this lane holds in the end: token `in`'s, and what it stood at
+    const int e = li & 15, in = 8 * (e >> 2) + 4 * h + (e & 3), j = key0 + in;
+    const bool bad_j = __shfl(static_cast<int>(bad), in);
+    float* p = g.weights + static_cast<int64_t>(__shfl(static_cast<int>(blk), in)) * a.bs + __shfl(slot, in);
+    const float old = g.parts == 1 && li < 16 && j < fresh && !bad_j ? *p : 0.f;
+    const int rows = max(tb - ta, 0) * a.group, count = (rows + 31) / 32;  // of a key head: rows, tiles of them
+    const int64_t all = static_cast<int64_t>(count) * a.kv_heads;
+    const int n0 = static_cast<int>(all * part / g.parts), n1 = static_cast<int>(all * (part + 1) / g.parts);
+    float sum[16] = {};
+    u32x4 k[DC];
+    // row tile n into a buffer; the lane's row of it: its lse and where it stands
+    auto send = [&](int n, int to) {
+      const int kh = n / count, row0 = (n - kh * count) * 32;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      // (a half behind the last token reads the other one's block, and is masked)
-      const int id = uniform(table[block_of(a, key0 + (key0 + 16 * h < rq.len ? 16 * h : 0), slot[h])]);
-      bad[h] = id < 0 || id >= a.blocks;
-      blk[h] = bad[h] ? 0 : id;
-    }
-    float sum[2][4] = {};
-    for (int kh = 0; t0 < t1 && kh < a.kv_heads; ++kh) {
-      std::conditional_t<FP4, Keys4<D>, Keys16<D>> k;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if constexpr (FP4) load_keys4<D>(a, row_of(a, blk[h], slot[h], kh), li, lg, k.k[h], k.s[h]);
-        else load_keys<D>(a, blk[h], slot[h], kh, li, lg, k.k[h]);
+      for (int j = 0; j < J; ++j) {
+        const int ln = here(lane), r = (wave * J + j) * KI + ln / P, row = min(row0 + r, rows - 1), t = row / a.group;
+        const uint16_t* p = a.q + static_cast<int64_t>(rq.row0 + ta + t) * a.q_row + (kh * a.group + row - t * a.group) * a.q_head +
+                            8 * (ln % P ^ turn(r));
+        load_lds(p, lds_address(lq) + to * (64 * D) + (wave * J + j) * 1024);
       }
-      for (int row0 = t0 * a.group; row0 < t1 * a.group; row0 += 16) {
-        const int row = min(row0 + li, t1 * a.group - 1), t = row / a.group, head = kh * a.group + row - t * a.group;
-        const uint16_t* p = a.q + (rq.row0 + t) * a.q_row + head * a.q_head + 8 * lg;
-        u32x4 q[DC];
+    };
+    float lse1 = 0.f;
+    int pos1 = 0;
+    auto row_of_lane = [&](int n) {
+      const int kh = n / count, row0 = (n - kh * count) * 32, row = min(row0 + li, rows - 1), t = row / a.group;
+      lse1 = a.lse[static_cast<int64_t>(rq.row0 + ta + t) * a.q_heads + kh * a.group + row - t * a.group];
+      pos1 = row0 + li < rows ? rq.first + ta + t : -1;  // (past the last one: sees nothing)
+    };
+    if (n0 < n1) {
+      send(n0, 0);
+      row_of_lane(n0);
+    }
+    int head = -1;
+    for (int n = n0; n < n1; ++n) {
+      const int kh = n / count, row0 = (n - kh * count) * 32, buf = (n - n0) & 1;
+      if (kh != head) {
+        head = kh;
+        if constexpr (FP4) {
+          const int64_t at = row_of(a, blk, slot, kh);
+          const uint8_t* p = static_cast<const uint8_t*>(a.kc) + at * (D / 2) + h * (D / 8);
+          uint32_t w[2][D / 32], s[D / 64];
+          load_words(p, w[0]);
+          load_words(p + D / 4, w[1]);
+          if constexpr (D == 128) load_words(a.ks + at * 4, s);
+          else s[0] = *reinterpret_cast<const uint32_t*>(a.ks + at * 2);
 #pragma unroll
-        for (int d = 0; d < DC; ++d) q[d] = ld16(p + 32 * d);
-        const float lse = a.lse[static_cast<int64_t>(rq.row0 + t) * a.q_heads + head] * 1.44269504088896340736f;
-        const int pos = rq.first + t, low = low_of(pos, a.window);
-        const int first = rq.first + row0 / a.group, last = rq.first + (min(row0 + 16, t1 * a.group) - 1) / a.group;
-        const bool masked = row0 + 16 > t1 * a.group || !all_visible(a, key0, key0 + 31, first, last);
+          for (int d = 0; d < DC; ++d) {
+            const float sc = d >> 1 & 1 ? high_bf16(s[d >> 2]) : low_bf16(s[d >> 2]);
+            float f[8];
+            fp4x8_to_f32(w[d & 1][d >> 1], f);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const f32x4 s = scores<D, F16>(k, h, q);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float e = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse));
-            const bool in = !masked || (row0 + li < t1 * a.group && visible(key0 + 16 * h + 4 * lg + i, pos, low, a.sinks));
-            sum[h][i] += in ? e : 0.f;
+            for (int e = 0; e < 4; ++e) k[d][e] = Elem<F16>::pack(f[2 * e] * sc, f[2 * e + 1] * sc);
           }
+        } else {
+          const uint16_t* p = static_cast<const uint16_t*>(a.kc) + blk * a.kc_block + static_cast<int64_t>(slot) * a.kc_slot +
+                              kh * a.kc_head + 8 * h;
+#pragma unroll
+          for (int d = 0; d < DC; ++d) k[d] = ld16(p + 16 * d);
         }
       }
-    }
-    // over the rows of the lanes: lane 16 lg then has tokens 4 lg + i
+      const float lse = lse1 * 1.44269504088896340736f;
+      const int pos = pos1;
+      arrived<0>();
+      __syncthreads();  // (the rows are whole; the other buffer's have been read)
+      if (n + 1 < n1) {
+        send(n + 1, buf ^ 1);
+        row_of_lane(n + 1);
+      }
+      f32x16 s{};
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int d = 0; d < DC; ++d) {
+        const x8 q = __builtin_bit_cast(x8, *lds<const u32x4>((q_at ^ (32 * d)) + buf * (64 * D))), kd = __builtin_bit_cast(x8, k[d]);
+        if constexpr (F16) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kd, q, s, 0, 0, 0);
+        else s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kd, q, s, 0, 0, 0);
+      }
+      const int first = rq.first + ta + row0 / a.group, last = rq.first + ta + (min(row0 + 32, rows) - 1) / a.group;
+      if (row0 + 32 <= rows && all_visible(a, key0, key0 + 31, first, last)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int e = 0; e < 16; ++e) sum[e] += __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -lse));
+      } else {
+        const uint32_t t = pos < 0 ? 0 : visible32(key0, pos, low_of(pos, a.window), a.sinks) >> (4 * h);
+        const uint32_t ok = (t & 0xf) | (t >> 4 & 0xf0) | (t >> 8 & 0xf00) | (t >> 12 & 0xf000);
 #pragma unroll
-        for (int x = 1; x < 16; x <<= 1) sum[h][i] += __shfl_xor(sum[h][i], x);
-    if (li < 8) {
-      const int h = li >> 2, i = li & 3, j = key0 + 16 * h + 4 * lg + i;
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s = li == e ? sum[e >> 2][e & 3] : s;
-      if (j < rq.len && !(h ? bad[1] : bad[0])) {
-        float* p = g.weights + (h ? blk[1] : blk[0]) * a.bs + (h ? slot[1] : slot[0]) + 4 * lg + i;
-        *p = (j >= fresh ? 0.f : *p) + s;
+        for (int e = 0; e < 16; ++e) sum[e] += ok >> e & 1 ? __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -lse)) : 0.f;
       }
     }
+    __syncthreads();  // (the next tile's rows go where these were)
+    // Over the rows of the lanes, halving the lanes and the tokens of each: lane l then has that of
+    // element l%16 (b = l%16 / 4, i = l%4).
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum[e] += __shfl_xor(sum[e], 16);
+#pragma unroll
+    for (int x = 8; x >= 1; x >>= 1)
+#pragma unroll
+      for (int e = 0; e < x; ++e) {
+        const float mine = li & x ? sum[e + x] : sum[e], other = li & x ? sum[e] : sum[e + x];
+        sum[e] = mine + __shfl_xor(other, x);
+      }
+    if (li < 16 && j < rq.len) {
+      if (g.parts > 1) {
+        g.sums[(static_cast<int64_t>(b) * a.cols * a.bs + j) * g.parts + part] = sum[0];
+      } else if (!bad_j) {
+        *p = old + sum[0];
+      }
+    }
+  }
+}
+
+// (parts > 1) Behind it: the parts' sums, in order.
+__global__ __launch_bounds__(256) void weigh_join_kernel(Weigh g) {
+  const Window& a = g.w;
+  const int per = (g.tiles * kTile + 255) / 256, b = blockIdx.x / per;
+  const Ragged rq = ragged(a, b);
+  const int fresh = rq.len - (g.fresh ? min(max(g.fresh[b], 0), rq.len) : 0);
+  for (int64_t j = static_cast<int64_t>(blockIdx.x % per) * 256 + threadIdx.x; j < rq.len; j += static_cast<int64_t>(per) * 256) {
+    const int tile0 = static_cast<int>(j) / kTile * kTile;
+    const int ta = max(0, tile0 - rq.first);
+    int tb = rq.tokens;
+    if (tile0 >= a.sinks) tb = static_cast<int>(least(tb, largest(static_cast<int64_t>(tile0) + kTile - 1 + a.window - rq.first, ta)));
+    if (ta >= tb && tile0 + kTile <= fresh) continue;  // (as above: nothing was left there)
+    int slot;
+    const int id = a.tables[b * a.tstride + block_of(a, static_cast<int>(j), slot)];
+    if (id < 0 || id >= a.blocks) continue;
+    const float* p = g.sums + (static_cast<int64_t>(b) * a.cols * a.bs + j) * g.parts;
+    float s = 0.f;
+    for (int i = 0; i < g.parts; ++i) s += p[i];
+    float* w = g.weights + static_cast<int64_t>(id) * a.bs + slot;
+    *w = (j >= fresh ? 0.f : *w) + s;
   }
 }
 
@@ -340,7 +427,49 @@ __global__ __launch_bounds__(kMoveThreads) void move4_kernel(Move m) {
 
 using namespace pgs;
 
-extern "C" int pgs_accumulate_weights(const pgs_accumulate_weights_args* args, void* stream) {
+namespace pgs {
+namespace {
+// Workgroups per request, and the parts that the rows are cut into while there are too few
+// workgroups for all CUs: of 128 rows at least in a request of the batch's average.  (Not by
+// max_tokens: the order of the additions, and so the last bits, are the same for any that is
+// large enough.)
+struct WeighPlan {
+  int64_t tiles, parts;
+};
+WeighPlan weigh_plan(const pgs_accumulate_weights_args& g, int64_t block_size) {
+  const int64_t context = std::min(g.max_context, g.columns * block_size);
+  WeighPlan p;
+  // (a request that is longer than max_context takes further turns; grids are 32-bit)
+  p.tiles = std::max<int64_t>(1, std::min((context + kTile - 1) / kTile, 0x3fffffff / std::max<int64_t>(g.requests, 1)));
+  const int64_t rows = g.rows * g.q_heads / std::max<int64_t>(g.requests, 1);
+  p.parts = std::max<int64_t>(1, std::min({1024 / (p.tiles * std::max<int64_t>(g.requests, 1)), rows / 128, int64_t{64}}));
+  return p;
+}
+bool weigh_sizes_ok(const pgs_accumulate_weights_args& g, int64_t kv_heads) {
+  return g.rows >= 0 && g.rows <= 0x7fffffff / 64 && g.requests >= 0 && g.requests <= 0x100000 && g.q_heads >= kv_heads &&
+         kv_heads >= 1 && g.q_heads % kv_heads == 0 && g.q_heads <= 4096 && g.max_tokens >= 1 &&
+         g.max_tokens <= 0x7fffffff / 64 && g.max_context >= 0 && g.max_context <= 0x7fffffff && g.window >= 1 &&
+         g.window <= 0x7fffffff && g.sinks >= 0 && g.sinks <= 0x7fffffff &&
+         std::min(g.max_tokens, std::max<int64_t>(g.rows, 1)) * g.q_heads <= 0x3fffffff;
+}
+size_t weigh_bytes(const pgs_accumulate_weights_args& g, const WeighPlan& p, int64_t block_size) {
+  return p.parts == 1 ? 0 : static_cast<size_t>(g.requests * g.columns * block_size * p.parts) * 4;
+}
+}  // namespace
+}  // namespace pgs
+
+extern "C" size_t pgs_accumulate_weights_workspace_bytes(const pgs_accumulate_weights_args* args) {
+  if (!args || !args->cache == !args->cache4) return 0;
+  const pgs_accumulate_weights_args& g = *args;
+  const int64_t size = g.cache ? g.cache->block_size : g.cache4->block_size;
+  if (!weigh_sizes_ok(g, g.cache ? g.cache->kv_heads : g.cache4->kv_heads) || size < 16 || size > 0x10000 || g.columns < 0 ||
+      g.columns > 0x7fff0000 / size || g.requests == 0)
+    return 0;
+  return weigh_bytes(g, weigh_plan(g, size), size);
+}
+
+extern "C" int pgs_accumulate_weights(const pgs_accumulate_weights_args* args, void* workspace, size_t workspace_bytes,
+                                      void* stream) {
   const char* fn = "pgs_accumulate_weights";
   if (!args) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: null arguments", fn);
   const pgs_accumulate_weights_args& g = *args;
@@ -350,10 +479,7 @@ extern "C" int pgs_accumulate_weights(const pgs_accumulate_weights_args* args, v
   Window& a = w.w;
   if (int rc = take_cache(fn, a, g.cache, g.cache4, false, g.block_tables, g.table_stride, g.columns)) return rc;
   const int64_t dim = g.cache ? g.cache->head_dim : g.cache4->head_dim;
-  if (g.rows < 0 || g.rows > 0x7fffffff / 64 || g.requests < 0 || g.requests > 0x100000 || g.q_heads < a.kv_heads ||
-      g.q_heads % a.kv_heads != 0 || g.q_heads > 4096 || g.max_tokens < 1 || g.max_tokens > 0x7fffffff / 64 ||
-      g.max_context < 0 || g.max_context > 0x7fffffff || g.window < 1 || g.window > 0x7fffffff || g.sinks < 0 ||
-      g.sinks > 0x7fffffff || std::min(g.max_tokens, std::max<int64_t>(g.rows, 1)) * g.q_heads > 0x3fffffff)
+  if (!weigh_sizes_ok(g, a.kv_heads))
     return fail(PGS_ERR_INVALID_ARGUMENT,
                 "%s: rows=%lld requests=%lld q_heads=%lld kv_heads=%d max_tokens=%lld window=%lld sinks=%lld: q_heads is a "
                 "multiple of kv_heads, max_tokens and window 1 at least, sinks 0 at least",
@@ -368,6 +494,10 @@ extern "C" int pgs_accumulate_weights(const pgs_accumulate_weights_args* args, v
   if (!aligned(g.q, 16) || !aligned(g.lse, 4) || !aligned(g.weights, 4) || !aligned(g.lens, 4) || !aligned(g.offsets, 4) ||
       !aligned(g.new_lens, 4))
     return fail(PGS_ERR_MISALIGNED, "%s: misaligned", fn);
+  const WeighPlan p = weigh_plan(g, a.bs);
+  const size_t need = weigh_bytes(g, p, a.bs);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 4)))
+    return fail(PGS_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %zu bytes", fn, need);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (int rc = require_device(fn, st)) return rc;
   a.q = static_cast<const uint16_t*>(g.q);
@@ -380,10 +510,9 @@ extern "C" int pgs_accumulate_weights(const pgs_accumulate_weights_args* args, v
   a.window = static_cast<int32_t>(g.window), a.sinks = static_cast<int32_t>(g.sinks);
   a.c = g.scale * 1.44269504088896340736f;
   w.weights = g.weights, w.fresh = g.new_lens;
-  // (a request that is longer than max_context takes further turns; grids are 32-bit)
-  const int64_t context = std::min(g.max_context, g.columns * a.bs);
-  w.tiles = static_cast<int>(std::max<int64_t>(1, std::min((context + kTile - 1) / kTile, 0x3fffffff / g.requests)));
-  const dim3 grid(static_cast<unsigned>(g.requests * w.tiles)), block(64 * kWaves);
+  w.tiles = static_cast<int>(p.tiles), w.parts = static_cast<int>(p.parts);
+  w.sums = static_cast<float*>(workspace);
+  const dim3 grid(static_cast<unsigned>(g.requests * p.tiles * p.parts)), block(64 * kWaves);
   auto go = [&](auto d, auto f16) {
     constexpr int D = decltype(d)::value;
     constexpr bool F = decltype(f16)::value;
@@ -393,7 +522,11 @@ extern "C" int pgs_accumulate_weights(const pgs_accumulate_weights_args* args, v
   const bool f16 = g.dtype == PGS_DTYPE_F16;
   if (dim == 64) f16 ? go(Int<64>{}, Int<1>{}) : go(Int<64>{}, Int<0>{});
   else f16 ? go(Int<128>{}, Int<1>{}) : go(Int<128>{}, Int<0>{});
-  return check_launch("accumulate_weights kernel");
+  if (int rc = check_launch("accumulate_weights kernel")) return rc;
+  if (p.parts == 1) return PGS_OK;
+  const int64_t per = (p.tiles * kTile + 255) / 256;
+  hipLaunchKernelGGL(weigh_join_kernel, dim3(static_cast<unsigned>(g.requests * per)), dim3(256), 0, st, w);
+  return check_launch("accumulate_weights join kernel");
 }
 
 extern "C" size_t pgs_evict_tokens_workspace_bytes(int64_t requests, int64_t max_context) {

@@ -1093,7 +1093,7 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
           multiply_keys(n, k[n & 1], s);
           sum += w.weights(a, x[n >> 1], n & 1, p[n]);
           asm volatile("" : "+v"(p[n]), "+v"(sum));  // (here, not where they are used)
-          interleave<DC / 2, 8, 16 + (F16 ? 12 : 4)>();
+          interleave<DC / 2, 8, 16 + 4>();
           __builtin_amdgcn_sched_barrier(0);
           if (n == 0) load_id(i + 3);
           if (n == 1 || n == 2) load_part(i + 3, n - 1);

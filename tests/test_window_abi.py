@@ -46,11 +46,11 @@ def _attend(lib, cache={}, cache4=None, workspace=P, given=BIG, **change):  # no
     return lib.pgs_window_attention(ctypes.byref(_paged(a, cache, cache4, change)), workspace, given, None)
 
 
-def _weigh(lib, cache={}, cache4=None, **change):  # noqa: B006
+def _weigh(lib, cache={}, cache4=None, workspace=P, given=BIG, **change):  # noqa: B006
     a = _native.AccumulateWeightsArgs(q=256, q_row=2048, q_head=128, block_tables=256, table_stride=4, columns=4, lens=256,
                                       offsets=256, lse=256, new_lens=256, weights=256, rows=5, requests=2, q_heads=16,
                                       max_tokens=5, max_context=64, window=8, sinks=4, scale=0.1, dtype=1)
-    return lib.pgs_accumulate_weights(ctypes.byref(_paged(a, cache, cache4, change)), None)
+    return lib.pgs_accumulate_weights(ctypes.byref(_paged(a, cache, cache4, change)), workspace, given, None)
 
 
 def _write(lib, k=P, v=P, k_row=256, v_head=128, dtype=1, cache4={}, slots=P, rows=3):  # noqa: B006
@@ -90,6 +90,8 @@ CASES = (
         {"workspace": None, "window": 1 << 20}, {"given": 8, "window": 1 << 20},
         {"workspace": ctypes.c_void_p(128), "window": 1 << 20})]
     + [(_weigh, c) for c in ({"lse": None}, {"lse": 258}, {"weights": None}, {"weights": 258}, {"new_lens": 257})]
+    + [(_weigh, {"rows": 200, "max_tokens": 200, **c}) for c in ({"workspace": None}, {"given": 8},
+                                                                 {"workspace": ctypes.c_void_p(258)})]
     + [(_write, c) for c in ({"k": None}, {"v": None}, {"slots": None}, {"k": ODD}, {"v": ctypes.c_void_p(264)}, {"slots": ODD},
                              {"k_row": 4}, {"v_head": -8}, {"dtype": 0}, {"dtype": 7}, {"rows": -1}, {"rows": BIG},
                              {"cache4": None})]
@@ -115,7 +117,7 @@ def test_bad_arguments(native_lib, call, change):
 
 def test_null_arguments(native_lib):
     assert native_lib.pgs_window_attention(None, P, BIG, None) in (1, 2)
-    assert native_lib.pgs_accumulate_weights(None, None) in (1, 2)
+    assert native_lib.pgs_accumulate_weights(None, P, BIG, None) in (1, 2)
 
 
 @pytest.mark.parametrize("call", [_attend, _weigh, _write, _read, _evict])
