@@ -203,6 +203,7 @@ struct Evict {
 
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 constexpr int kDigit = 11, kBins = 1 << kDigit;  // three digits: 11 + 11 + 10 bits
+constexpr int kHeld = 32768;                      // a request's first tokens whose weights lie in LDS
 
 // a token's slot; below 0 where its block is absent
 __device__ __forceinline__ int64_t slot_of(const Evict& a, const int32_t* table, int token) {
@@ -210,22 +211,33 @@ __device__ __forceinline__ int64_t slot_of(const Evict& a, const int32_t* table,
   const int id = table[block_of(a, token, at)];
   return id < 0 || id >= a.blocks ? -1 : static_cast<int64_t>(id) * a.bs + at;
 }
-// A weight's place in the order: larger numbers stay first, a NaN before all, zeros alike, an
-// absent token last.
-__device__ __forceinline__ uint32_t order_of(const Evict& a, const int32_t* table, int token) {
+// A token's weight as bits, kAbsent where its block is absent (a NaN of just these bits takes
+// another's).
+constexpr uint32_t kAbsent = 0xffffffffu;
+__device__ __forceinline__ uint32_t weight_of(const Evict& a, const int32_t* table, int token) {
   const int64_t s = slot_of(a, table, token);
-  if (s < 0) return 0;
-  const float x = a.weights[s] + 0.f;
+  if (s < 0) return kAbsent;
+  return min(__float_as_uint(a.weights[s]), kAbsent - 1);
+}
+// Its place in the order: larger numbers stay first, a NaN before all, zeros alike, an absent
+// token last.
+__device__ __forceinline__ uint32_t order_of(uint32_t weight) {
+  if (weight == kAbsent) return 0;
+  const float x = __uint_as_float(weight) + 0.f;
   if (x != x) return 0xffffffffu;
   const uint32_t u = __float_as_uint(x);
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// One workgroup per request.  Of the tokens that may go, the place in the order of the last
-// one that stays: its digits from the highest on, from counts of the tokens that agree with
-// the digits so far.  Then the places of all that stay, in order, and their weights.
+// One workgroup per request.  Its weights go into LDS (those of tokens from kHeld on are read
+// again).  Of the tokens that may go, the place in the order of the last one that stays: its
+// digits from the highest on, from counts of the tokens that agree with the digits so far, until
+// all of them stay.  Then the places of all that stay, in order, and their weights.  Bound by
+// latency: the blocks, the weights, and some ten waits of the workgroup.
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(Evict a) {
-  __shared__ int32_t bins[kBins], found[2], lowest;
+  __shared__ uint32_t held[kHeld];
+  __shared__ int32_t ids[kHeld / 16];
+  __shared__ int32_t bins[kBins], found[3], lowest;
   __shared__ int32_t count[2][kSelectWaves];
   const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6;
   const int b = blockIdx.x;
@@ -237,6 +249,31 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(Evict a) {
     if (thread == 0) a.kept[b] = len, a.begin[b] = len;
     return;
   }
+  const int mine = min(len, kHeld);
+  for (int i = thread; i * a.bs < mine; i += kSelectThreads) ids[i] = table[i];
+  __syncthreads();
+  for (int j0 = thread; j0 < mine; j0 += 8 * kSelectThreads) {
+    uint32_t x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = weight_of(a, ids, min(j0 + u * kSelectThreads, mine - 1));
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (j0 + u * kSelectThreads < mine) held[j0 + u * kSelectThreads] = x[u];
+  }
+  // four tokens' weights, `step` apart from j on (behind the end: the last one's)
+  auto weights4 = [&](int j, int step, int stop, uint32_t (&x)[4]) {
+    if (stop <= kHeld) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] = held[min(j + u * step, stop - 1)];
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int t = min(j + u * step, stop - 1);
+        x[u] = t < kHeld ? held[t] : weight_of(a, table, t);
+      }
+    }
+  };
+  __syncthreads();
   const int sinks = min(a.sinks, most), recent = min(a.recent, most - sinks);
   const int first = sinks, end = len - recent;  // those that may go
   int need = most - sinks - recent;             // of them stay
@@ -246,89 +283,111 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(Evict a) {
       const int digits = shift == 0 ? kDigit - 1 : kDigit;
       for (int i = thread; i < kBins; i += kSelectThreads) bins[i] = 0;
       __syncthreads();
-      for (int j = first + thread; j < end; j += kSelectThreads) {
-        const uint32_t o = order_of(a, table, j);
-        if ((o & mask) == at) atomicAdd(&bins[o >> shift & ((1u << digits) - 1)], 1);
+      for (int j = first + thread; j < end; j += 4 * kSelectThreads) {
+        uint32_t x[4];
+        weights4(j, kSelectThreads, end, x);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t o = order_of(x[u]);
+          if (j + u * kSelectThreads < end && (o & mask) == at) atomicAdd(&bins[o >> shift & ((1u << digits) - 1)], 1);
+        }
       }
       __syncthreads();
-      // the bin, from the highest on, in which the need is met
-      if (wave == 0) {
-        const int per = (1 << digits) / 64;
-        int mine = 0;
-        for (int i = 0; i < per; ++i) mine += bins[(63 - lane) * per + i];
-        int upto = mine;
+      // the bin, from the highest on, in which the need is met: two for each thread
+      const int top = kBins - 1 - 2 * thread, n0 = bins[top], n1 = bins[top - 1];
+      int upto = n0 + n1;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const int o = __shfl_up(upto, d);
-          if (lane >= d) upto += o;
-        }
-        if (upto >= need && upto - mine < need) {
-          int left = need - (upto - mine), i = per - 1;
-          while (bins[(63 - lane) * per + i] < left) left -= bins[(63 - lane) * per + i--];
-          found[0] = (63 - lane) * per + i;
-          found[1] = left;
-        }
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+      }
+      if (lane == 63) count[0][wave] = upto;
+      __syncthreads();
+      for (int w = 0; w < wave; ++w) upto += count[0][w];
+      if (upto >= need && upto - n0 - n1 < need) {
+        const int left = need - (upto - n0 - n1);
+        const bool one = left <= n0;
+        found[0] = one ? top : top - 1;
+        found[1] = one ? left : left - n0;
+        found[2] = one ? n0 : n1;
       }
       __syncthreads();
       at |= static_cast<uint32_t>(found[0]) << shift;
       mask |= ((1u << digits) - 1) << shift;
       need = found[1];
+      if (need == found[2]) break;
     }
   }
   // `need` of the tokens at `at` stay, the first ones, and all that lie above.  A wave counts
   // those of its part of the tokens, then knows where its first one goes.
   const int part = (len + kSelectThreads - 1) / kSelectThreads * 64, lo = min(wave * part, len), hi = min(lo + part, len);
-  auto flags = [&](int j, bool& above, bool& equal) {
+  auto flags = [&](int j, uint32_t weight, bool& above, bool& equal) {
     above = equal = false;
     if (j >= hi) return;
     if (j < first || j >= end) {
       above = true;
     } else if (mask) {
-      const uint32_t o = order_of(a, table, j);
+      const uint32_t o = order_of(weight) & mask;
       above = o > at;
       equal = o == at;
     }
   };
   int above_n = 0, equal_n = 0;
-  for (int j0 = lo; j0 < hi; j0 += 64) {
-    bool above, equal;
-    flags(j0 + lane, above, equal);
-    above_n += __popcll(__ballot(above));
-    equal_n += __popcll(__ballot(equal));
+  for (int j0 = lo; j0 < hi; j0 += 256) {
+    uint32_t x[4];
+    weights4(j0 + lane, 64, hi, x);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      bool above, equal;
+      flags(j0 + 64 * u + lane, x[u], above, equal);
+      above_n += __popcll(__ballot(above));
+      equal_n += __popcll(__ballot(equal));
+    }
   }
+  __syncthreads();  // (the counts of the last digit have been read)
   if (lane == 0) count[0][wave] = above_n, count[1][wave] = equal_n;
   if (thread == 0) lowest = most;
   __syncthreads();
-  int above_at = 0, equal_at = 0;  // of the waves before
+  int above_at = 0, equal_at = 0, low = most;  // of the waves before
   for (int w = 0; w < wave; ++w) above_at += count[0][w], equal_at += count[1][w];
   int32_t* from = a.from + static_cast<int64_t>(b) * a.most;
-  for (int j0 = lo; j0 < hi; j0 += 64) {
-    bool above, equal;
-    flags(j0 + lane, above, equal);
-    const unsigned long long am = __ballot(above), em = __ballot(equal), before = (1ull << lane) - 1;
-    const int e = equal_at + __popcll(em & before), n = above_at + __popcll(am & before) + min(e, need);
-    if (above || (equal && e < need)) {
-      from[n] = j0 + lane;
-      if (n != j0 + lane) atomicMin(&lowest, n);
+  for (int j0 = lo; j0 < hi; j0 += 256) {
+    uint32_t x[4];
+    weights4(j0 + lane, 64, hi, x);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = j0 + 64 * u + lane;
+      bool above, equal;
+      flags(j, x[u], above, equal);
+      const unsigned long long am = __ballot(above), em = __ballot(equal), before = (1ull << lane) - 1;
+      const int e = equal_at + __popcll(em & before), n = above_at + __popcll(am & before) + min(e, need);
+      if (above || (equal && e < need)) {
+        from[n] = j;
+        if (n != j) {
+          low = min(low, n);
+          if (n < kHeld && x[u] != kAbsent) {  // (its own weight lies in LDS: nobody reads it any more)
+            const int64_t to = slot_of(a, ids, n);
+            if (to >= 0) a.weights[to] = __uint_as_float(x[u]);
+          }
+        }
+      }
+      above_at += __popcll(am);
+      equal_at += __popcll(em);
     }
-    above_at += __popcll(am);
-    equal_at += __popcll(em);
   }
+  if (low < most) atomicMin(&lowest, low);
   __threadfence_block();
   __syncthreads();
   const int begin = lowest;
   if (thread == 0) a.kept[b] = most, a.begin[b] = begin;
-  // the weights: a place takes that of a token further on, and is read before that
-  for (int i0 = begin; i0 < most; i0 += kSelectThreads) {
+  // the other places' weights: each takes that of a token further on, and is read before that
+  for (int i0 = max(begin, kHeld); i0 < most; i0 += kSelectThreads) {
     const int i = i0 + thread;
-    float x = 0.f;
-    int64_t to = -1;
-    if (i < most) {
-      const int64_t s = slot_of(a, table, from[i]);
-      if (s >= 0) to = slot_of(a, table, i), x = a.weights[s];
-    }
+    uint32_t x = kAbsent;
+    if (i < most) x = weight_of(a, table, from[i]);
+    const int64_t to = x == kAbsent ? -1 : slot_of(a, table, i);
     __syncthreads();
-    if (to >= 0) a.weights[to] = x;
+    if (to >= 0) a.weights[to] = __uint_as_float(x);
     // (the next turn reads places that no earlier one writes)
   }
 }
@@ -346,7 +405,8 @@ struct Move {
 
 // What stays of a request, moved together: one workgroup per (request, cache, keys or values,
 // head, slice of the token's pieces).  A place takes a token from further on, so a turn's
-// tokens are read before any of its places is written, and the next turn's lie behind them.
+// tokens are read before any of its places is written, and while the turn before is written:
+// that writes nothing that later turns read.
 // P pieces of type T of a token; piece(base of the block, slot, p): where one is.
 template <typename T, int U, typename Where>
 __device__ __forceinline__ void move_pieces(const Evict& e, int b, int p0, int pieces, Where where) {
@@ -354,22 +414,59 @@ __device__ __forceinline__ void move_pieces(const Evict& e, int b, int p0, int p
   const int32_t* from = e.from + static_cast<int64_t>(b) * e.most;
   const int begin = e.begin[b], kept = e.kept[b];
   const int64_t all = static_cast<int64_t>(kept - begin) * pieces;
-  for (int64_t n0 = 0; n0 < all; n0 += U * kMoveThreads) {
-    T x[U];
-    T* to[U];
+  T x[U], next[U];
+  T *to[U], *next_to[U];
+  // the places of a turn two turns ahead, their tokens' blocks one ahead
+  int token[U], src[U], dst[U], s[U], d[U];
+  const int64_t mine = threadIdx.x;
+  auto place = [&](int64_t n0, int u) {
+    const int64_t n = n0 + u * kMoveThreads + mine;
+    return n < all ? begin + static_cast<int>(n / pieces) : -1;
+  };
+  auto find = [&](int64_t n0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t n = n0 + u * kMoveThreads + threadIdx.x;
-      to[u] = nullptr;
-      if (n >= all) continue;
-      const int i = begin + static_cast<int>(n / pieces), p = p0 + static_cast<int>(n % pieces);
-      int s, d;
-      const int j = from[i], src = table[block_of(e, j, s)], dst = table[block_of(e, i, d)];
-      if (j == i || src < 0 || src >= e.blocks || dst < 0 || dst >= e.blocks) continue;
-      x[u] = *where(src, s, p);
-      to[u] = where(dst, d, p);
+      const int i = place(n0, u);
+      token[u] = i < 0 ? -1 : from[i];
+    }
+  };
+  auto blocks = [&](int64_t n0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = place(n0, u);
+      src[u] = -1;
+      if (i < 0 || token[u] == i) continue;
+      src[u] = table[block_of(e, token[u], s[u])];
+      dst[u] = table[block_of(e, i, d[u])];
+    }
+  };
+  auto load = [&](int64_t n0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      next_to[u] = nullptr;
+      if (src[u] < 0 || src[u] >= e.blocks || dst[u] < 0 || dst[u] >= e.blocks) continue;
+      const int p = p0 + static_cast<int>((n0 + u * kMoveThreads + mine) % pieces);
+      next[u] = *where(src[u], s[u], p);
+      next_to[u] = where(dst[u], d[u], p);
+    }
+  };
+  constexpr int64_t N = U * kMoveThreads;
+  find(0);
+  blocks(0);
+  find(N);
+  load(0);
+  blocks(N);
+  find(2 * N);
+  for (int64_t n0 = 0; n0 < all; n0 += N) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      x[u] = next[u], to[u] = next_to[u];
+      asm volatile("" : "+v"(x[u]));  // (here: they have arrived before the barrier)
     }
     __syncthreads();
+    load(n0 + N);
+    blocks(n0 + 2 * N);
+    find(n0 + 3 * N);
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (to[u]) *to[u] = x[u];
@@ -602,9 +699,12 @@ extern "C" int pgs_evict_tokens(float* weights, const int32_t* lens, const int32
       const pgs_kv_cache& c = caches[i0 + i];
       m.c[i] = MoveCache{c.k, c.v, nullptr, nullptr, c.k_block, c.k_slot, c.k_head, c.v_block, c.v_slot, c.v_head};
     }
-    m.slices = 1;
+    // (a slice has whole lines of 128 bytes: of 64 the move of 8 requests of 8192 tokens in 4
+    // layers of 2 x 128 dims takes 134 us)
+    m.slices = std::max(1, static_cast<int>(pieces * (vec ? 16 : 2)) / 128);
+    while (pieces % m.slices) --m.slices;
     const int64_t units = requests * m.caches * 2 * m.heads;
-    while (m.slices < 4 && units * m.slices < 512 && pieces % (2 * m.slices) == 0) m.slices *= 2;
+    while (units * m.slices < 128 && pieces % (2 * m.slices) == 0 && pieces / m.slices > 2) m.slices *= 2;
     const dim3 grid(static_cast<unsigned>(units * m.slices));
     if (vec) hipLaunchKernelGGL(move_kernel<u32x4>, grid, dim3(kMoveThreads), 0, st, m, pieces);
     else hipLaunchKernelGGL(move_kernel<uint16_t>, grid, dim3(kMoveThreads), 0, st, m, pieces);

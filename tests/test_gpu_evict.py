@@ -169,7 +169,7 @@ def test_wrong_lengths_and_block_numbers_stay_inside(gpu):
 def test_a_cache_in_other_strides_and_many_layers(gpu):
     lens, budget = [150, 80], [64, 64]
     w, tables, caches, args = evict_case(gpu, lens, budget, 4, layers=19)
-    # heads in front of slots, halves of one tensor, rows that are not 16 bytes apart
+    # heads in front of slots, halves of one tensor
     moved = []
     for n, (k, v) in enumerate(caches):
         both = torch.stack((k, v), 1 if n % 3 else 4)
@@ -180,6 +180,36 @@ def test_a_cache_in_other_strides_and_many_layers(gpu):
     kept = W.evict(w.copy(), tables, lens, budget, before, 1, 2)
     assert evict_tokens(*args[:4], moved, sinks=1, recent=2).tolist() == kept
     for x, y in zip(contents(moved, *w.shape, gpu), before):
+        assert np.array_equal(x, y)
+
+
+@pytest.mark.parametrize("lens,budget", [([33000, 70000], [32900, 40000]), ([32768, 32769, 5], [32767, 32768, 1]),
+                                         ([65000], [20])])
+@pytest.mark.parametrize("bs", [16, 96])
+def test_more_tokens_than_are_held_on_the_chip(gpu, lens, budget, bs):
+    w, tables, caches, args = evict_case(gpu, lens, budget, 6, 64, 1, bs, layers=1)
+    before = contents(caches, *w.shape, gpu)
+    want_w = w.copy()
+    kept = W.evict(want_w, tables, lens, budget, before, 7, 400)
+    assert evict_tokens(*args, sinks=7, recent=400).tolist() == kept
+    assert np.array_equal(args[0].cpu().numpy(), want_w)
+    for x, y in zip(contents(caches, *w.shape, gpu), before):
+        assert np.array_equal(x, y)
+
+
+@pytest.mark.parametrize("heads,dim", [(3, 64), (1, 20), (2, 128)])
+def test_a_cache_whose_rows_lie_at_odd_addresses(gpu, heads, dim):
+    """Any size of rows at any address of two bytes."""
+    lens, budget = [600, 80], [300, 64]
+    w, tables, _, args = evict_case(gpu, lens, budget, 5, dim, heads, layers=0)
+    rng, pair = np.random.default_rng(7), []
+    for _ in range(2):
+        flat = torch.from_numpy(rng.standard_normal(w.size * heads * dim + 1)).to(torch.float16).to(gpu)
+        pair.append(flat[1:].view(*w.shape, heads, dim))
+    before = contents([pair], *w.shape, gpu)
+    kept = W.evict(w.copy(), tables, lens, budget, before, 2, 30)
+    assert evict_tokens(*args[:4], [tuple(pair)], sinks=2, recent=30).tolist() == kept
+    for x, y in zip(contents([pair], *w.shape, gpu), before):
         assert np.array_equal(x, y)
 
 
