@@ -243,6 +243,27 @@ __device__ __forceinline__ f32x4 scores(const Keys4<D>& n, int h, const u32x4 (&
   return s;
 }
 
+// The same where columns r and r + 8 are row r, with its q of even chunks in one and of odd ones in
+// the other (zeros elsewhere): one accumulator has two chunks' sums, each lane its own's scale
+// (sel: the half of a word of two that it takes), and the two halves are added.
+__device__ __forceinline__ uint32_t pair_half(int li) { return li < 8 ? 0x01000c0cu : 0x03020c0cu; }
+__device__ __forceinline__ float half_of(uint32_t w, uint32_t sel) { return __uint_as_float(__builtin_amdgcn_perm(w, w, sel)); }
+template <int D, bool F16>
+__device__ __forceinline__ f32x4 pair_scores(const Keys4<D>& n, int h, const u32x4 (&q)[D / 32], uint32_t sel) {
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int d = 0; d < D / 64; ++d) {
+    f32x4 t = Elem<F16>::mfma(widen8<F16>(n.k[h][2 * d]), q[2 * d], f32x4{0.f, 0.f, 0.f, 0.f});
+    t = Elem<F16>::mfma(widen8<F16>(n.k[h][2 * d + 1]), q[2 * d + 1], t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = fmaf(t[i], half_of(n.s[h][i * (D / 64) + d], sel), s[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    s[i] += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(s[i]), 0x128, 0xf, 0xf, true));  // (lanes 8 on in the row)
+  return s;
+}
+
 // Host: the cache and the tables of a call, checked, into its arguments.  One of c and c4
 // is given; values: whether the call reads them.
 inline int take_cache(const char* fn, Window& a, const pgs_kv_cache* c, const pgs_kv_cache4* c4, bool values,

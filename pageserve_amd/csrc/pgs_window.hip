@@ -35,8 +35,13 @@ __device__ __forceinline__ void interleave() {
 
 // 16 R rows of a wave and their running sums.  The output MFMA d covers the dims
 // (4 lg + i) D/16 + d of its lanes (SPREAD: values straight from 16-bit rows), or 16 d + 4 lg + i.
-template <int D, int R, bool F16, bool SPREAD>
+// PAIR (4-bit): columns l%16 and l%16 + 8 are one of eight rows, the first with its q and output
+// of the even chunks of 32 dims, the second of the odd ones, so that a lane multiplies by half
+// the scales.
+template <int D, int R, bool F16, bool SPREAD, bool PAIR>
 struct Rows {
+  static_assert(!PAIR || (R == 1 && !SPREAD));
+  static constexpr int kRows = PAIR ? 8 : 16;  // of a tile
   using E = Elem<F16>;
   static constexpr int DC = D / 32, DV = D / 16;
   u32x4 q[R][DC];
@@ -48,10 +53,13 @@ struct Rows {
   __device__ __forceinline__ void load(const Window& a, const Ragged& rq, int kh, int row0, int nrows, int li, int lg) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int row = min(row0 + 16 * r + li, nrows - 1), t = row / a.group;  // (rows past the last repeat it)
+      const int row = min(row0 + 16 * r + li % kRows, nrows - 1), t = row / a.group;  // (rows past the last repeat it)
       const uint16_t* p = a.q + (rq.row0 + t) * a.q_row + (kh * a.group + row - t * a.group) * a.q_head + 8 * lg;
 #pragma unroll
-      for (int d = 0; d < DC; ++d) q[r][d] = (ld16(p + 32 * d) ^ a.flip) & a.keep;
+      for (int d = 0; d < DC; ++d) {
+        q[r][d] = (ld16(p + 32 * d) ^ a.flip) & a.keep;
+        if (PAIR && (li >> 3) != (d & 1)) q[r][d] = u32x4{};
+      }
       pos[r] = rq.first + t;
     }
     // (they have arrived here: a wait for them inside the loop over the keys would be
@@ -194,61 +202,75 @@ struct Rows {
   }
 
   // The same from 4-bit values, whose scales multiply the weights in front of the rounding:
-  // one operand per 32 dims.  It is bf16 whatever the rows are (a weight times a scale may
-  // leave fp16's range; the codes are exact in both), in two terms where they are fp16, whose
-  // finer rounding the output shall have.  A token that is not seen has weight 0 whatever its
-  // scale holds.
-  __device__ __forceinline__ void add4(const Window& a, const float (&x)[R][8], const Values4<D>& n, int key0, bool masked,
-                                       bool bad0, bool bad1, int lg) {
-    static_assert(!SPREAD, "the codes' order");
-    uint32_t ok[R] = {};
-    if (masked)
+  // one operand per 32 dims (PAIR: per 64, the lanes of even columns with the first's scales).  It
+  // is bf16 whatever the rows are (a weight times a scale may leave fp16's range; the codes are
+  // exact in both), in two terms where they are fp16, whose finer rounding the output shall have.
+  // A token that is not seen has weight 0 whatever its scale holds.
+  __device__ __forceinline__ void add4(const Window& a, const float (&x)[R][8], Values4<D>& n, int key0, bool masked,
+                                       bool bad0, bool bad1, int li, int lg) {
+    static_assert(!SPREAD && R == 1, "the codes' order, one row's mask");
+    if (masked) {
+      const uint32_t ok = seen(a, 0, key0, bad0, bad1, lg);
 #pragma unroll
-      for (int r = 0; r < R; ++r) ok[r] = seen(a, r, key0, bad0, bad1, lg);
+      for (int e = 0; e < 8; ++e)
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      exact[r] += ((x[r][0] + x[r][1]) + (x[r][2] + x[r][3])) + ((x[r][4] + x[r][5]) + (x[r][6] + x[r][7]));
-    group4<0>(x, ok, n, masked);
-    group4<1>(x, ok, n, masked);
-    if constexpr (DC == 4) {
-      group4<2>(x, ok, n, masked);
-      group4<3>(x, ok, n, masked);
+        for (int c = 0; c < DC / 2; ++c) {
+          uint32_t& w = n.s[e >> 2][(e & 3) * (DC / 2) + c];
+          w = ok >> e & 1 ? w : 0;
+        }
     }
-  }
-  template <int G>
-  __device__ __forceinline__ void group4(const float (&x)[R][8], const uint32_t (&ok)[R], const Values4<D>& n, bool masked) {
-    // codes of dims 32 G + li and 16 further, pairs of keys
-    u32x4 v[2];
+    exact[0] += ((x[0][0] + x[0][1]) + (x[0][2] + x[0][3])) + ((x[0][4] + x[0][5]) + (x[0][6] + x[0][7]));
+    // codes of two keys side by side: dims 32 c + l%16 (byte c of `low`) and 16 further
+    uint32_t low[4], high[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t k0, k1;
-        if constexpr (DC == 4) k0 = widen2<G>(n.v[h][2 * i]), k1 = widen2<G>(n.v[h][2 * i + 1]);
-        else k0 = widen2<G>(n.v[h][i]), k1 = widen2<G + 2>(n.v[h][i]);
-        v[0][2 * h + i] = __builtin_amdgcn_perm(k1, k0, 0x05040100u);
-        v[1][2 * h + i] = __builtin_amdgcn_perm(k1, k0, 0x07060302u);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t* v = n.v[i >> 1];
+      if constexpr (DC == 4) {
+        const uint32_t v0 = v[2 * (i & 1)], v1 = v[2 * (i & 1) + 1];
+        low[i] = (v0 & 0x0f0f0f0fu) | (v1 << 4 & 0xf0f0f0f0u);
+        high[i] = (v0 >> 4 & 0x0f0f0f0fu) | (v1 & 0xf0f0f0f0u);
+      } else {
+        const uint32_t w = v[i & 1];
+        low[i] = (w & 0x0f0fu) | (w >> 12 & 0xf0f0u);
+        high[i] = (w >> 4 & 0x0f0fu) | (w >> 16 & 0xf0f0u);
       }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
+    }
+    const uint32_t sel = pair_half(li);
+    auto group = [&](auto first) {
+      constexpr int G = decltype(first)::value;
       u32x4 p, rest;
+      __builtin_amdgcn_sched_barrier(0);  // (one after the other: registers)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float y[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int e = 2 * i + j;
-          y[j] = x[r][e] * n.scale(e >> 2, e & 3, G);
-          if (masked) y[j] = ok[r] >> e & 1 ? y[j] : 0.f;
+          y[j] = x[0][e] * (PAIR ? half_of(n.s[e >> 2][(e & 3) * (DC / 2) + G / 2], sel) : n.scale(e >> 2, e & 3, G));
         }
         p[i] = pack_bf16x2(y[0], y[1]);
         if constexpr (F16) rest[i] = pack_bf16x2(y[0] - low_bf16(p[i]), y[1] - high_bf16(p[i]));
       }
+      auto product = [&](auto chunk) {
+        constexpr int C = decltype(chunk)::value;
 #pragma unroll
-      for (int d = 0; d < 2; ++d) {
-        o[r][2 * G + d] = Elem<false>::mfma(v[d], p, o[r][2 * G + d]);
-        if constexpr (F16) o[r][2 * G + d] = Elem<false>::mfma(v[d], rest, o[r][2 * G + d]);
-      }
+        for (int d = 0; d < 2; ++d) {
+          u32x4 v;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = widen2<C>(d ? high[i] : low[i]);
+          o[0][2 * C + d] = Elem<false>::mfma(v, p, o[0][2 * C + d]);
+          if constexpr (F16) o[0][2 * C + d] = Elem<false>::mfma(v, rest, o[0][2 * C + d]);
+        }
+      };
+      product(first);
+      if constexpr (PAIR) product(Int<G + 1>{});
+    };
+    group(Int<0>{});
+    if constexpr (PAIR) {
+      if constexpr (DC == 4) group(Int<2>{});
+    } else {
+      group(Int<1>{});
+      if constexpr (DC == 4) group(Int<2>{}), group(Int<3>{});
     }
   }
 
@@ -259,10 +281,17 @@ struct Rows {
                                         bool whole, Slot slot) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int row = row0 + 16 * r + li;
+      const int row = row0 + 16 * r + li % kRows;
       if (row >= nrows) continue;
       const int t = row / a.group, head = kh * a.group + row - t * a.group;
       const int64_t token = rq.row0 + t;
+      if constexpr (PAIR) {  // (the lane's chunks into the places of the even ones)
+#pragma unroll
+        for (int e = 0; e < DV; ++e)
+          if (!(e & 2)) o[r][e] = li < 8 ? o[r][e] : o[r][e + 2];
+      }
+      const bool first = lg == 0 && li < kRows;
+      const int shift = PAIR && li >= 8 ? 32 : 0;
       if (whole) {
         const float inv = l[r][0] == 0.f ? 0.f : 1.f / l[r][0];
         uint16_t* d = a.out + token * a.out_row + head * a.out_head + 4 * lg * (SPREAD ? DV : 1);
@@ -278,10 +307,11 @@ struct Rows {
         } else {
 #pragma unroll
           for (int e = 0; e < DV; ++e)
-            *reinterpret_cast<u32x2*>(d + 16 * e) = u32x2{E::pack(o[r][e][0] * inv, o[r][e][1] * inv),
-                                                          E::pack(o[r][e][2] * inv, o[r][e][3] * inv)};
+            if (!PAIR || !(e & 2))
+              *reinterpret_cast<u32x2*>(d + shift + 16 * e) = u32x2{E::pack(o[r][e][0] * inv, o[r][e][1] * inv),
+                                                                    E::pack(o[r][e][2] * inv, o[r][e][3] * inv)};
         }
-        if (a.lse && lg == 0) a.lse[token * a.q_heads + head] = log_sum(mx[r], exact[r]);
+        if (a.lse && first) a.lse[token * a.q_heads + head] = log_sum(mx[r], exact[r]);
       } else {
         const int64_t at = slot(row, token, head);
         float* d = a.part + at * D + 4 * lg * (SPREAD ? DV : 1);
@@ -294,9 +324,10 @@ struct Rows {
                   f32x4{o[r][e][i], o[r][e + 1][i], o[r][e + 2][i], o[r][e + 3][i]};
         } else {
 #pragma unroll
-          for (int e = 0; e < DV; ++e) *reinterpret_cast<f32x4*>(d + 16 * e) = o[r][e];
+          for (int e = 0; e < DV; ++e)
+            if (!PAIR || !(e & 2)) *reinterpret_cast<f32x4*>(d + shift + 16 * e) = o[r][e];
         }
-        if (lg == 0) *reinterpret_cast<f32x4*>(a.stat + 4 * at) = f32x4{mx[r], l[r][0], exact[r], 0.f};
+        if (first) *reinterpret_cast<f32x4*>(a.stat + 4 * at) = f32x4{mx[r], l[r][0], exact[r], 0.f};
       }
     }
   }
@@ -318,9 +349,10 @@ __device__ __forceinline__ Span group_span(const Window& a, const Ragged& rq, in
 
 // Rows straight from memory: a workgroup's NW waves are WR row tiles of 16 R x NW/WR key
 // slices; each wave loads the keys and values of its steps into registers.
-template <int D, int R, int WR, int NW, bool F16, bool FP4>
+template <int D, int R, int WR, int NW, bool F16, bool FP4, bool PAIR>
 __global__ __launch_bounds__(64 * NW, 2) void window_kernel(Window a) {
-  using W = Rows<D, R, F16, !FP4>;
+  static_assert(!PAIR || WR == 1);
+  using W = Rows<D, R, F16, !FP4, PAIR>;
   using E = Elem<F16>;
   constexpr int DC = W::DC, DV = W::DV;
   constexpr int WK = NW / WR;      // key slices
@@ -394,9 +426,12 @@ __global__ __launch_bounds__(64 * NW, 2) void window_kernel(Window a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int r = 0; r < R; ++r) s[r][h] = scores<D, F16>(k, h, w.q[r]);
+        for (int r = 0; r < R; ++r) {
+          if constexpr (PAIR) s[r][h] = pair_scores<D, F16>(k, h, w.q[r], pair_half(li));
+          else s[r][h] = scores<D, F16>(k, h, w.q[r]);
+        }
       w.weights(a, s, x, key0, masked, bad[0], bad[1], lg);
-      w.add4(a, x, v, key0, masked, bad[0], bad[1], lg);
+      w.add4(a, x, v, key0, masked, bad[0], bad[1], li, lg);
     } else {
       Keys16<D> k;
       Values16<D> v;
@@ -1235,6 +1270,7 @@ __global__ __launch_bounds__(256) void widen_kernel(Widen g) {
 struct Plan {
   int wide;   // rows of a group that share tiles through LDS, or 0
   int r, wr;  // else row tiles per wave, waves per key slice (4-bit: one tile per wave, r times the waves)
+  bool pair;  // (4-bit) eight rows at most, in pairs of columns
   int groups, splits, min_steps;
   int64_t columns, chunk, widen;  // (wide, 4-bit) blocks of sixteen a request, requests widened at a time, workgroups each
 };
@@ -1254,6 +1290,7 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
     return p;
   }
   p.r = rows <= 16 ? 1 : 2;
+  p.pair = fp4 && rows <= 8;
   p.wr = rows <= 32 ? 1 : 2;
   p.groups = static_cast<int>((rows + 63) / 64);
   const int64_t units = requests * kv_heads * p.groups;
@@ -1262,9 +1299,11 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
   const int64_t seen = window + std::min(sinks, max_context) + tokens >= max_context ? max_context : window + sinks + tokens;
   const int64_t steps = (seen + 31) / 32 * p.wr;
   p.min_steps = units * (steps / kCoarseSteps) <= 128 ? kFineSteps : kCoarseSteps;
+  // (as many workgroups as run at a time: 4-bit rows leave registers for three per CU, where a
+  // fourth would wait: 32 requests of 16000 tokens in 25.6 instead of 29.0 us)
   if (steps >= kWholeSteps)
     p.splits = static_cast<int>(
-        std::max<int64_t>(1, std::min<int64_t>({(1024 + units - 1) / units, steps / p.min_steps, 256})));
+        std::max<int64_t>(1, std::min<int64_t>({((fp4 ? 768 : 1024) + units - 1) / units, steps / p.min_steps, 256})));
   return p;
 }
 int64_t slots_of(const Plan& p, int64_t rows, int64_t q_heads) {
@@ -1328,9 +1367,10 @@ int launch(const Window& a, const Plan& p, char* widened, hipStream_t st) {
   }
   const dim3 g(static_cast<unsigned>(static_cast<int64_t>(a.requests) * a.kv_heads * p.groups * p.splits));
   constexpr int R = FP4 ? 1 : 2;
-  if (p.r == 1) hipLaunchKernelGGL((window_kernel<D, 1, 1, 4, F16, FP4>), g, dim3(256), 0, st, a);
-  else if (p.wr == 1) hipLaunchKernelGGL((window_kernel<D, R, 2 / R, 4, F16, FP4>), g, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((window_kernel<D, R, 4 / R, 4, F16, FP4>), g, dim3(256), 0, st, a);
+  if (FP4 && p.pair) hipLaunchKernelGGL((window_kernel<D, 1, 1, 4, F16, FP4, FP4>), g, dim3(256), 0, st, a);
+  else if (p.r == 1) hipLaunchKernelGGL((window_kernel<D, 1, 1, 4, F16, FP4, false>), g, dim3(256), 0, st, a);
+  else if (p.wr == 1) hipLaunchKernelGGL((window_kernel<D, R, 2 / R, 4, F16, FP4, false>), g, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((window_kernel<D, R, 4 / R, 4, F16, FP4, false>), g, dim3(256), 0, st, a);
   if (int rc = check_launch("window attention kernel")) return rc;
   if (p.splits == 1) return PGS_OK;
   const int64_t quads = static_cast<int64_t>(a.requests) * a.kv_heads * ((a.max_tokens * a.group + 3) / 4);
