@@ -533,13 +533,16 @@ namespace {
 struct WeighPlan {
   int64_t tiles, parts;
 };
+constexpr int64_t kSums = int64_t{1} << 26;
 WeighPlan weigh_plan(const pgs_accumulate_weights_args& g, int64_t block_size) {
   const int64_t context = std::min(g.max_context, g.columns * block_size);
   WeighPlan p;
   // (a request that is longer than max_context takes further turns; grids are 32-bit)
   p.tiles = std::max<int64_t>(1, std::min((context + kTile - 1) / kTile, 0x3fffffff / std::max<int64_t>(g.requests, 1)));
   const int64_t rows = g.rows * g.q_heads / std::max<int64_t>(g.requests, 1);
-  p.parts = std::max<int64_t>(1, std::min({1024 / (p.tiles * std::max<int64_t>(g.requests, 1)), rows / 128, int64_t{64}}));
+  // (and their sums, one for each token that the tables have room for, take kSums bytes at most)
+  const int64_t each = std::max<int64_t>(1, g.requests * g.columns * block_size * 4);
+  p.parts = std::max<int64_t>(1, std::min({1024 / (p.tiles * std::max<int64_t>(g.requests, 1)), rows / 128, kSums / each, int64_t{64}}));
   return p;
 }
 bool weigh_sizes_ok(const pgs_accumulate_weights_args& g, int64_t kv_heads) {
@@ -574,7 +577,8 @@ extern "C" int pgs_accumulate_weights(const pgs_accumulate_weights_args* args, v
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: dtype %d must be bf16 or fp16", fn, g.dtype);
   Weigh w{};
   Window& a = w.w;
-  if (int rc = take_cache(fn, a, g.cache, g.cache4, false, g.block_tables, g.table_stride, g.columns)) return rc;
+  if (int rc = take_cache(fn, a, g.cache, g.cache4, false, g.block_tables, g.table_stride, g.columns, g.requests))
+    return rc;
   const int64_t dim = g.cache ? g.cache->head_dim : g.cache4->head_dim;
   if (!weigh_sizes_ok(g, a.kv_heads))
     return fail(PGS_ERR_INVALID_ARGUMENT,

@@ -267,7 +267,7 @@ __device__ __forceinline__ f32x4 pair_scores(const Keys4<D>& n, int h, const u32
 // Host: the cache and the tables of a call, checked, into its arguments.  One of c and c4
 // is given; values: whether the call reads them.
 inline int take_cache(const char* fn, Window& a, const pgs_kv_cache* c, const pgs_kv_cache4* c4, bool values,
-                      const int32_t* tables, int64_t table_stride, int64_t columns) {
+                      const int32_t* tables, int64_t table_stride, int64_t columns, int64_t requests) {
   if (!c == !c4) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: one cache, of 16 or of 4 bits", fn);
   const int64_t blocks = c ? c->blocks : c4->blocks, size = c ? c->block_size : c4->block_size;
   const int64_t heads = c ? c->kv_heads : c4->kv_heads, dim = c ? c->head_dim : c4->head_dim;
@@ -279,7 +279,7 @@ inline int take_cache(const char* fn, Window& a, const pgs_kv_cache* c, const pg
   // (a tile behind the last token still has a 32-bit number)
   if (columns < 0 || table_stride < columns || columns > 0x7fff0000 / size)
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: bad block table", fn);
-  if (columns > 0 && !tables) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
+  if (columns > 0 && requests > 0 && !tables) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
   if (!aligned(tables, 4)) return fail(PGS_ERR_MISALIGNED, "%s: misaligned", fn);
   if (c) {
     if (!c->k || (values && !c->v)) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: null cache", fn);

@@ -1415,7 +1415,8 @@ extern "C" int pgs_window_attention(const pgs_window_attention_args* args, void*
   if (g.dtype != PGS_DTYPE_BF16 && g.dtype != PGS_DTYPE_F16)
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: dtype %d must be bf16 or fp16", fn, g.dtype);
   Window a{};
-  if (int rc = take_cache(fn, a, g.cache, g.cache4, true, g.block_tables, g.table_stride, g.columns)) return rc;
+  if (int rc = take_cache(fn, a, g.cache, g.cache4, true, g.block_tables, g.table_stride, g.columns, g.requests))
+    return rc;
   const int64_t dim = g.cache ? g.cache->head_dim : g.cache4->head_dim;
   if (!sizes_ok(g.rows, g.requests, g.q_heads, a.kv_heads, dim, g.max_tokens, g.max_context, g.window, g.sinks))
     return fail(PGS_ERR_INVALID_ARGUMENT,
