@@ -150,17 +150,18 @@ __device__ __forceinline__ Args again() {
 }
 
 // Four rows' outputs from n parts' sums each: brought to one reference, added in order and
-// divided by the joined sum.  Sixteen lanes per row, each with D/16 neighbouring dims;
-// slot(i): where part i of the lane's row is; p: the lane's dims of the output, or null.
+// divided by the joined sum.  Sixteen lanes per row, each with DIMS/16 neighbouring dims of the
+// DIMS that `parts` points to; slot(i): where part i of the lane's row is; p: the lane's dims of
+// the output, or null.
 // STATS: numbers of a part, 2 (reference, sum) or 4 (and the sum of the weights before they
 // were rounded, whose logarithm goes to lse; the fourth is unused).  WAVES: of the workgroup,
 // each taking that share of the parts (all must call it), joined in LDS; or 1.  Bound by
-// memory and, few rows of many parts, by its latency: up to eight parts' loads are on their
-// way together (four of four numbers).
-template <int D, bool F16, int WAVES, int STATS, typename Slot>
+// memory and, few rows of many parts, by its latency: BATCH parts' loads are on their way
+// together.
+template <int D, bool F16, int WAVES, int STATS, int DIMS = D, int BATCH = STATS == 2 ? 8 : 4, typename Slot>
 __device__ __forceinline__ void join_rows(const float* parts, const float* stats, int n, int lane, int wave, uint16_t* p,
                                           float* lse, Slot slot) {
-  constexpr int W = D / 16;
+  constexpr int W = DIMS / 16;
   const int li = lane & 15;
   typedef float Stat __attribute__((ext_vector_type(STATS)));
   float ref = kLow, sum = 0.f, exact = 0.f, o[W];
@@ -198,11 +199,11 @@ __device__ __forceinline__ void join_rows(const float* parts, const float* stats
     }
   };
   int i = WAVES == 1 ? 0 : n * wave / WAVES;
-  if constexpr (STATS == 2) {
+  if constexpr (BATCH == 8) {
     for (; end - i > 4; i += 8) batch(i, Int<8>{});
     if (end - i > 2) batch(i, Int<4>{});
     else if (end > i) batch(i, Int<2>{});
-  } else {  // (eight parts of four numbers do not fit the registers that sixteen waves have)
+  } else {
     for (; end - i > 2; i += 4) batch(i, Int<4>{});
     if (end > i) batch(i, Int<2>{});
   }
@@ -220,7 +221,7 @@ __device__ __forceinline__ void join_rows(const float* parts, const float* stats
     sum = exact = 0.f;
 #pragma unroll
     for (int d = 0; d < W; ++d) o[d] = 0.f;
-    constexpr int kUnroll = STATS == 4 ? 4 : WAVES;  // (registers again)
+    constexpr int kUnroll = BATCH == 4 ? 4 : WAVES;  // (registers)
 #pragma unroll kUnroll
     for (int w = 0; w < WAVES; ++w) {
       const float g = __builtin_amdgcn_exp2f(lref[w][lane] - ref);
