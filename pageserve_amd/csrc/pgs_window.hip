@@ -1287,7 +1287,19 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
   const int64_t rows = max_tokens * (q_heads / kv_heads);
   Plan p{};
   p.splits = 1;
-  p.wide = rows <= 64 ? 0 : 256;
+  const int64_t tokens = std::min<int64_t>(max_tokens, 64);  // of a row group
+  // (the most tokens that a row group sees)
+  const int64_t seen = window + std::min(sinks, max_context) + tokens >= max_context ? max_context : window + sinks + tokens;
+  p.groups = static_cast<int>((rows + 63) / 64);
+  const int64_t units = requests * kv_heads * p.groups;
+  // Rows that share tiles through LDS run at three times the rate, but their equal shares cost 30
+  // us before that.  By units x steps of 32 keys, us straight from memory and shared (128 dims,
+  // 16 bits): 256 (64 rows over 500 tokens) 21 / 38, 2048 (four of 64 over 1000) 22 / 44, 4032
+  // (256 over 2000) 31 / 48, 8192 (1024 over as many) 45 / 47, 16000 (512 over 4000) 67 / 57.  Of
+  // 64 dims, and of 4 bits, which are not widened first then, they meet at twice as many: 14000
+  // (512 over 4000) 42 / 44, 16000 63 / 62, 28000 (2048 over as many, 64 dims) 48 / 46.
+  const int64_t few = fp4 || head_dim == 64 ? 16384 : 8192;
+  p.wide = rows <= 64 || units * std::max<int64_t>(1, (seen + 31) / 32) <= few ? 0 : 256;
   if (p.wide) {
     if (fp4) {
       p.columns = (columns * block_size + 15) / 16;
@@ -1299,11 +1311,6 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
   p.r = rows <= 16 ? 1 : 2;
   p.pair = fp4 && rows <= 8;
   p.wr = rows <= 32 ? 1 : 2;
-  p.groups = static_cast<int>((rows + 63) / 64);
-  const int64_t units = requests * kv_heads * p.groups;
-  const int64_t tokens = std::min<int64_t>(max_tokens, 64);  // of a row group
-  // (the most tokens that a row group sees)
-  const int64_t seen = window + std::min(sinks, max_context) + tokens >= max_context ? max_context : window + sinks + tokens;
   const int64_t steps = (seen + 31) / 32 * p.wr;
   p.min_steps = units * (steps / kCoarseSteps) <= 128 ? kFineSteps : kCoarseSteps;
   // (as many workgroups as run at a time: 4-bit rows leave registers for three per CU, where a
