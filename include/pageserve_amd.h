@@ -723,7 +723,8 @@ typedef struct pgs_accumulate_weights_args {
 /*
  * Adds to weights[slot of token j] the attention weights of the rows and query
  * heads that see j: sum of e^(scale q . k_j - lse).  Sums are fp32, in a fixed
- * order.  Tokens in a block outside the cache are left out.
+ * order.  Tokens in a block outside the cache are left out; no block may be in two
+ * requests' tables, or twice in one (an addition may be lost).
  */
 int pgs_accumulate_weights(const pgs_accumulate_weights_args* args, void* workspace,
                            size_t workspace_bytes, void* stream);

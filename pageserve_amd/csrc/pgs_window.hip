@@ -348,7 +348,10 @@ __device__ __forceinline__ Span group_span(const Window& a, const Ragged& rq, in
 }
 
 // Rows straight from memory: a workgroup's NW waves are WR row tiles of 16 R x NW/WR key
-// slices; each wave loads the keys and values of its steps into registers.
+// slices; each wave loads the keys and values of its steps into registers.  16 bits: bound by
+// memory, 48 requests of one row and 4100 tokens each 35 us, 5.7 TB/s (a part from caches).  4
+// bits: by what a step's vector instructions take next to its loads (of 32 keys and eight rows
+// some 260; 500 without pairs of columns), 32 requests of 16000 tokens 25.6 us, 4.3 TB/s.
 template <int D, int R, int WR, int NW, bool F16, bool FP4, bool PAIR>
 __global__ __launch_bounds__(64 * NW, 2) void window_kernel(Window a) {
   static_assert(!PAIR || WR == 1);
@@ -877,12 +880,15 @@ struct Rows32 {
 // lane n gets dim n of the four keys), a pair of pieces of four keys per access: pairs are
 // exchanged by twos, so that four keys x two pairs meet all banks.
 //
-// Bound by the matrix units and LDS alike (a step of 32 keys and 256 rows takes 1024 cycles of
-// either).  Between products of 32 x 32 there is room for six other instructions each, between
-// those of 16 x 16, half as long, for one or two: they cover the softmax (three and an exponential
-// a product), given that there is one to issue.  So a wave's products and softmax overlap a step
-// apart: the products of the next step's scores run beside this step's weights, those of this
-// step's output beside the next step's largest scores.
+// Bound by issue: the products of a step of 32 keys and 256 rows take 1024 cycles of a SIMD and
+// hide what is issued beside them, LDS is busy a fifth of the time.  Between products of 32 x 32
+// there is room for six other instructions each, between those of 16 x 16, half as long, for one
+// or two: they cover the softmax (three and an exponential a product), given that there is one to
+// issue.  So a wave's products and softmax overlap a step apart: the products of the next step's
+// scores run beside this step's weights, those of this step's output beside the next step's
+// largest scores.  Four requests of 2048 rows over 4160 of 8000 tokens (204 GFLOP): 258 us in
+// fp16, 790 TFLOP/s, the join 15; matrix units busy 36 % (two row tiles per wave of 16 x 16 took 317
+// to 400, halves of the workgroup half a tile apart 333).
 template <int D, bool F16>
 __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
   using W = Rows32<D, F16>;
@@ -1192,6 +1198,7 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
 }
 
 // Behind window_wide_kernel: the units that a share began and left to others, four rows a wave.
+// Bound by memory: two parts a share at most, 69 MB in 14.5 us.
 template <int D, bool F16, int RG>
 __global__ __launch_bounds__(join_threads(1)) void window_wide_join_kernel(Window a) {
   const int lane = threadIdx.x & 63, li = lane & 15, wave = uniform(static_cast<int>(threadIdx.x >> 6));
@@ -1220,7 +1227,8 @@ __global__ __launch_bounds__(join_threads(1)) void window_wide_join_kernel(Windo
 // sixteen, [request][columns][head][16][D], exactly, with a table of their own, and the wide
 // kernel reads those.  Each value is read by hundreds of rows, which this costs one write and one
 // read of 16 bits; widened in the wide kernel it would be a third more instructions beside its
-// products.  One workgroup per block: a thread has eight dims of a token.
+// products.  One workgroup per block: a thread has eight dims of a token.  Bound by memory: 2 x
+// 16000 tokens of 2 x 128 dims (19 MB to 33 MB) 9.5 us.
 struct Widen {
   Window w;
   uint16_t *k, *v;

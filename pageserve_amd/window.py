@@ -63,12 +63,12 @@ def window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     q . k, head_dim ** -0.5 by default.
 
     Returns (rows, q_heads, head_dim), or writes to ``out`` (contiguous; it may be q
-    itself); with ``return_lse`` also the natural logarithm of each row's sum of e^score, fp32 (rows,
-    q_heads).  A row that sees no token gets zeros and -inf.  Rows that belong to no
+    itself); with ``return_lse`` also the natural logarithm of each row's sum of
+    e^score, fp32 (rows, q_heads).  A row that sees no token gets zeros and -inf.  Rows that belong to no
     request are not written: in a new tensor they hold anything, in ``out`` what they
     held.  Softmax and sums are fp32; the weights are rounded to the tensors' dtype
-    before they multiply v, and divided by the sum of the rounded ones.  A key or
-    value that is not finite reaches only the rows that see it."""
+    before they multiply v.  A key or value that is not finite reaches only the rows
+    that see it."""
     r = _native.load_host().window_attention(q, [k_cache, v_cache], block_tables, lens, offsets, window, sinks, max_tokens,
                                              max_context, scale, return_lse, out)
     return (r[0], r[1]) if return_lse else r[0]
@@ -99,7 +99,9 @@ def accumulate_weights(q: torch.Tensor, k_cache: torch.Tensor | KVCache4, block_
     arguments are those of that call; ``k_cache`` may be a :class:`KVCache4`.  With
     ``new_lens`` (int32 [requests], as :func:`append_blocks` took it) that many last
     tokens of a request start from nothing: their slots hold what an earlier owner
-    left there.  One ``weights`` for each layer, or one for all of them.
+    left there.  One ``weights`` for each layer, or one for all of them.  No block may
+    be in two requests' tables, or twice in one: of the additions to a slot that two
+    reach, one may be lost.
 
     Sums are fp32 in a fixed order: the same call gives the same bits."""
     cache = k_cache.parts if isinstance(k_cache, KVCache4) else [k_cache]

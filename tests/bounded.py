@@ -9,10 +9,10 @@ exponent lies in reach; v_exp_f32 and the rescaling by a few more units); its ro
 the type t by u = half a step of t.  fp32 additions in each of keys / 32 steps and in the
 joins: (keys / 32 + 64) 2^-23.
 
-16 bits: out = sum p v / sum p with the same rounded p above and below: off by (u + e)
-sum w (|v| + |out|).  A p that fp16 rounds to a multiple of 2^-24 may be off by 2^-25
-instead, times at most `keys` against a sum of at least 1.  The wide kernel of the 4-bit
-cache is the same (its values are exact in both types).
+16 bits: out = sum p v / sum p, p rounded above, and below either the same or unrounded:
+off by (u + e) sum w (|v| + |out|).  A p that fp16 rounds to a multiple of 2^-24 may be
+off by 2^-25 instead, times at most `keys` against a sum of at least 1.  Many rows over the
+4-bit cache are the same (its values are exact in both types).
 4 bits, single rows: the numerator's p * scale is rounded to bf16 (for fp16 rows in two
 terms, off by 2^-17), the sum is of the weights before that: u sum w |v| and e as above.
 Both: then the output's own rounding.
