@@ -1195,6 +1195,7 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
     w.store(again<Window>(), rq, kh, row0, nrows, here(lane), whole,
             static_cast<int64_t>(2 * share + (!below(un.begin, begin))) * RG - first_row);
   }
+  arrived<0>();  // (no load into LDS outlives the workgroup)
 }
 
 // Behind window_wide_kernel: the units that a share began and left to others, four rows a wave.
@@ -1459,7 +1460,12 @@ extern "C" int pgs_window_attention(const pgs_window_attention_args* args, void*
   const int64_t most = std::min(g.max_tokens, g.rows);  // (no request has more rows than the batch)
   const Plan p = plan(g.requests, g.q_heads, a.kv_heads, dim, most, g.max_context, g.window, g.sinks, !g.cache, g.columns, a.bs);
   const size_t need = workspace_bytes(p, g.rows, g.q_heads, a.kv_heads, dim);
-  if (p.chunk * p.columns > 0x7fffffff) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: too large", fn);
+  // (what all units cost has to fit 64 bits)
+  const double group = static_cast<double>(g.q_heads / a.kv_heads);
+  const double counts = (static_cast<double>(g.rows) * group / 256 + static_cast<double>(g.requests)) * a.kv_heads *
+                        (static_cast<double>(g.columns) * a.bs + 2 * kUnit) * group;
+  if (p.chunk * p.columns > 0x7fffffff || (p.wide && counts > 4e18))
+    return fail(PGS_ERR_INVALID_ARGUMENT, "%s: too large", fn);
   if (need > 0 && (!workspace || workspace_bytes_given < need || !aligned(workspace, 256)))
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

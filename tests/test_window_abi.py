@@ -89,6 +89,8 @@ CASES = (
     + [(_attend, {"rows": 2, "requests": 1, "max_context": 1 << 20, **c}) for c in (
         {"workspace": None, "window": 1 << 20}, {"given": 8, "window": 1 << 20},
         {"workspace": ctypes.c_void_p(128), "window": 1 << 20})]
+    + [(_attend, {"rows": 262143, "max_tokens": 262143, "requests": 1, "q_heads": 4096, "cache": {"kv_heads": 1},
+                  "columns": 0x7FFF0000 // 16, "table_stride": 0x7FFF0000 // 16, "max_context": 0x7FFFFFFF})]
     + [(_weigh, c) for c in ({"lse": None}, {"lse": 258}, {"weights": None}, {"weights": 258}, {"new_lens": 257})]
     + [(_weigh, {"rows": 200, "max_tokens": 200, **c}) for c in ({"workspace": None}, {"given": 8},
                                                                  {"workspace": ctypes.c_void_p(258)})]
