@@ -786,41 +786,51 @@ struct Rows32 {
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[e] = ok >> e & 1 ? x[e] : -INFINITY;
   }
-  // as in Rows, for two steps
-  __device__ __forceinline__ void raise(const Window& a, const f32x16 (&x)[2]) {
+  // The reference for two more steps' scores: another one, the largest so far, if one of them passes
+  // the row's by too much; what was summed so far is brought to it later (settle).
+  __device__ __forceinline__ bool lift(const Window& a, const f32x16 (&x)[2], float& next) {
     float top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; ++e) top = fmaxf(fmaxf(top, x[0][e]), x[1][e]);
     top *= a.c;
-    if (!__ballot(top - mx > kSlack + E::kHead)) return;
+    if (!__ballot(top - mx > kSlack + E::kHead)) return false;
     const float t = both(top, true);
-    const float ref = fmaxf(fabsf(t) > kFar ? t : t - E::kHead, mx), f = __builtin_amdgcn_exp2f(mx - ref);
-    mx = ref;
-    far = __ballot(fabsf(ref) > kFar);
+    next = fmaxf(fabsf(t) > kFar ? t : t - E::kHead, mx);
+    far = __ballot(fabsf(next) > kFar);
+    return true;
+  }
+  __device__ __forceinline__ void settle(float next) {
+    const float f = __builtin_amdgcn_exp2f(mx - next);
+    mx = next;
     sum *= f;
 #pragma unroll
     for (int d = 0; d < DV; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] *= f;
   }
-  // Weights of a step's half h, rounded in p; their sum.
-  static __device__ __forceinline__ float take(const float (&y)[8], u32x4& p) {
+  // Weights of a quarter n of a step against reference ref, rounded in p; their sum.
+  static __device__ __forceinline__ float weights(const Window& a, const f32x16& x, int n, float ref, u32x4 (&p)[2]) {
+    float y[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) p[e] = E::pack(y[2 * e], y[2 * e + 1]);
-    return ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+    for (int e = 0; e < 4; ++e) y[e] = __builtin_amdgcn_exp2f(fmaf(x[4 * n + e], a.c, -ref));
+    return take(y, n, p);
   }
-  __device__ __forceinline__ float weights(const Window& a, const f32x16& x, int h, u32x4& p) const {
-    float y[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(fmaf(x[8 * h + e], a.c, -mx));
-    return take(y, p);
+  static __device__ __forceinline__ float take(const float (&y)[4], int n, u32x4 (&p)[2]) {
+    p[n >> 1][2 * (n & 1)] = E::pack(y[0], y[1]);
+    p[n >> 1][2 * (n & 1) + 1] = E::pack(y[2], y[3]);
+    return (y[0] + y[1]) + (y[2] + y[3]);
   }
-  // The same for references that the exponent's rounding matters for.
-  __device__ __forceinline__ float weights_far(const Window& a, const f32x16& x, int h, u32x4& p) const {
-    float y[8];
+  // The same of a whole step, for references that the exponent's rounding matters for.
+  static __device__ __forceinline__ float weights_far(const Window& a, const f32x16& x, float ref, u32x4 (&p)[2]) {
+    float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(exponent(x[8 * h + e], a.c, mx, true));
-    return take(y, p);
+    for (int n = 0; n < 4; ++n) {
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = __builtin_amdgcn_exp2f(exponent(x[4 * n + e], a.c, ref, true));
+      sum += take(y, n, p);
+    }
+    return sum;
   }
   // values that are not finite (bit of odd; the products had zeros for them), for the rows that see them
   template <typename Value>
@@ -1082,9 +1092,9 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
         v[d] = u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
     };
-    // tile i's scores in s, whether one of them may need a higher reference: what its rows do not
-    // see is hidden, references are raised; whether it has masks
-    auto take = [&](int i, Scores& s, bool over, uint32_t any) {
+    // Tile i's scores in s, whether one of them may need a higher reference: what its rows do not
+    // see is hidden; the reference that they go by.  masked: whether it has masks.
+    auto take = [&](int i, Scores& s, bool over, uint32_t any, float& ref, bool& lifted) {
       bool masked = !plain(i);
       uint32_t bm = 0;
       if (__builtin_expect(masked || any, 0)) {
@@ -1096,7 +1106,7 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
           w.hide(a, s[1], key0 + 32, bm >> 2, here(lane));
         }
       }
-      if (__builtin_expect(masked || over || w.far, 0)) w.raise(a, s);
+      if (__builtin_expect(masked || over || w.far, 0)) lifted = w.lift(a, s, ref);
       return masked;
     };
 
@@ -1118,9 +1128,16 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
         read_keys(t0, n, k);
         multiply_keys(n, k, s0);
       }
-      bool masked = take(t0, s0, true, lany), settles = to_settle(t0 + 1);
+      float ref = w.mx;
+      bool lifted = false, masked = take(t0, s0, true, lany, ref, lifted), settles = to_settle(t0 + 1);
+      if (lifted) w.settle(ref);
+      u32x4 first[2];  // the weights of a tile's first step
+#pragma unroll
+      for (int n = 0; n < 4; ++n) w.sum += W::weights(a, s0[0], n, w.mx, first);
+      if (w.far) w.sum = W::weights_far(a, s0[0], w.mx, first);
 
-      // Tile i, its scores in x; the next one's go to s.
+      // Tile i, its scores in x, its first step's weights in `first`; the next one's go to s and
+      // `first`.
       auto tile = [&](int i, const Scores& x, Scores& s) {
         // One barrier per tile: behind it the next one is whole, and the buffer of the one
         // before free.
@@ -1128,10 +1145,10 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
         if (__builtin_expect(settles, 0)) settle(i + 1);
         __syncthreads();
         const uint32_t any_v = lany;
-        u32x4 k[2][DC / 2], v[2][DV], p[4];
-        float sum = 0.f;
+        u32x4 k[2][DC / 2], v[2][DV], second[2];
+        float sum = 0.f, top = -INFINITY;
         read_keys(i + 1, 0, k[0]);
-        // this tile's weights beside the next one's scores (behind the last: of what lies there)
+        // the next one's scores beside the second step's weights (behind the last: of what lies there)
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           __builtin_amdgcn_sched_barrier(0);
@@ -1139,33 +1156,40 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
           else read_values(i, 0, v[0]);
           __builtin_amdgcn_sched_barrier(0);
           multiply_keys(n, k[n & 1], s);
-          sum += w.weights(a, x[n >> 1], n & 1, p[n]);
-          asm volatile("" : "+v"(p[n]), "+v"(sum));  // (here, not where they are used)
-          interleave<DC / 2, 8, 16 + 4>();
+          sum += W::weights(a, x[1], n, w.mx, second);
+          if (n >= 2)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, s[0][8 * (n & 1) + e]);
+          asm volatile("" : "+v"(second[n >> 1]), "+v"(sum));  // (here, not where they are used)
+          interleave<DC / 2, 4, 10>();
           __builtin_amdgcn_sched_barrier(0);
           if (n == 0) load_id(i + 3);
           if (n == 1 || n == 2) load_part(i + 3, n - 1);
           if (n == 3) settles = to_settle(i + 2);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (__builtin_expect(w.far, 0)) {
-          sum = 0.f;
-#pragma unroll
-          for (int n = 0; n < 4; ++n) sum += w.weights_far(a, x[n >> 1], n & 1, p[n]);
-        }
+        if (__builtin_expect(w.far, 0)) sum = W::weights_far(a, x[1], w.mx, second);
         w.sum += sum;
-        // its output beside the next one's largest scores
-        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[1][e]);
+        float ref = w.mx;
+        bool lifted = false, masks = false;
+        if (i + 1 < t1)
+          masks = take(i + 1, s, __ballot(fmaf(top, a.c, -w.mx) > kSlack + E::kHead), uniform(static_cast<int>(any_v)), ref, lifted);
+        // this one's output beside the next one's weights of its first step
+        u32x4 next[2];
+        sum = 0.f;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           __builtin_amdgcn_sched_barrier(0);
           if (n < 3) read_values(i, n + 1, v[~n & 1]);
           __builtin_amdgcn_sched_barrier(0);
+          const u32x4 p = n < 2 ? first[n] : second[n - 2];
 #pragma unroll
-          for (int d = 0; d < DV; ++d) w.o[d] = W::mfma(v[n & 1][d], p[n], w.o[d]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, s[n >> 1][8 * (n & 1) + e]);
-          interleave<DV, 0, 4>();
+          for (int d = 0; d < DV; ++d) w.o[d] = W::mfma(v[n & 1][d], p, w.o[d]);
+          sum += W::weights(a, s[0], n, ref, next);
+          asm volatile("" : "+v"(next[n >> 1]), "+v"(sum));
+          interleave<DV, 4, 10>();
         }
         __builtin_amdgcn_sched_barrier(0);
         if (__builtin_expect(masked, 0)) {
@@ -1176,7 +1200,7 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
             for (int n = 0; n < 32 / KW; ++n) odd |= (lflags[i % kBuffers][j * (32 / KW) + n] & 0xffff) << (n * KW);
             odd = uniform(static_cast<int>(odd));
             const int key0 = span.tile(i) * TK + 32 * j;
-            if (odd) w.add_odd(a, p[2 * j], p[2 * j + 1], key0, odd, here(lane), [&](int n) {
+            if (odd) w.add_odd(a, j ? second[0] : first[0], j ? second[1] : first[1], key0, odd, here(lane), [&](int n) {
               int slot;
               const int id = table[block_of(a, key0 + n, slot)];
               const uint16_t* at = vc + static_cast<int64_t>(id) * a.vc_block + static_cast<int64_t>(slot) * a.vc_slot;
@@ -1184,7 +1208,11 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
             });
           }
         }
-        if (i + 1 < t1) masked = take(i + 1, s, __ballot(fmaf(top, a.c, -w.mx) > kSlack + E::kHead), uniform(static_cast<int>(any_v)));
+        if (__builtin_expect(w.far, 0)) sum = W::weights_far(a, s[0], ref, next);
+        if (__builtin_expect(lifted, 0)) w.settle(ref);
+        if (i + 1 < t1) w.sum += sum;
+        first[0] = next[0], first[1] = next[1];
+        masked = masks;
       };
       for (int i = t0; i < t1; i += 2) {
         tile(i, s0, s1);
