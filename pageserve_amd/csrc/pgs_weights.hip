@@ -23,7 +23,8 @@ constexpr int kWaves = 4, kTile = 32 * kWaves;
 
 // One workgroup per request, tile of 128 tokens and part of the rows (of all key heads, 32 (token,
 // query head) at a time).  A wave's 32 tokens stay in registers as A operands of
-// v_mfma_f32_32x32x16, 4-bit ones widened exactly; the rows pass by through LDS as B operands,
+// v_mfma_f32_32x32x16, 4-bit ones widened exactly (fp16: below 2^-16 to a multiple of
+// 2^-24, which moves a score by 2^-25 sum |q| at most); the rows pass by through LDS as B operands,
 // SUB tiles between two barriers (one: a key head has no more), shared by the waves, and lane l
 // adds up the weights of tokens 8 b + 4 (l/32) + i for row l%32.  Every sum is one wave's, those
 // of the parts are added in order: the order of all additions is fixed.

@@ -890,15 +890,16 @@ struct Rows32 {
 // lane n gets dim n of the four keys), a pair of pieces of four keys per access: pairs are
 // exchanged by twos, so that four keys x two pairs meet all banks.
 //
-// Bound by issue: the products of a step of 32 keys and 256 rows take 1024 cycles of a SIMD and
-// hide what is issued beside them, LDS is busy a fifth of the time.  Between products of 32 x 32
-// there is room for six other instructions each, between those of 16 x 16, half as long, for one
-// or two: they cover the softmax (three and an exponential a product), given that there is one to
-// issue.  So a wave's products and softmax overlap a step apart: the products of the next step's
-// scores run beside this step's weights, those of this step's output beside the next step's
-// largest scores.  Four requests of 2048 rows over 4160 of 8000 tokens (204 GFLOP): 258 us in
-// fp16, 790 TFLOP/s, the join 15; matrix units busy 36 % (two row tiles per wave of 16 x 16 took 317
-// to 400, halves of the workgroup half a tile apart 333).
+// Bound by issue: the products of a step of 32 keys and 256 rows take 1024 cycles of a SIMD, its
+// softmax nearly as many of the vector unit (an exponential takes four times an addition).  Between
+// products of 32 x 32 there is room for six other instructions each, between those of 16 x 16,
+// half as long, for one or two.  So a wave's products and softmax overlap: the products of the next
+// tile's scores run beside the weights of this one's second step, those of this one's output
+// beside the weights of the next one's first step, once its references are known.  Four requests of
+// 2048 rows over 4160 of 8000 tokens (204 GFLOP): 251 us in fp16, 810 TFLOP/s, the join 15; matrix
+// units busy 46 %, LDS 20 % (all of a tile's weights beside the scores, its maxima beside the
+// output: 258; two row tiles per wave of 16 x 16: 317 to 400; halves of the workgroup half a tile
+// apart: 333).
 template <int D, bool F16>
 __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
   using W = Rows32<D, F16>;
@@ -1253,8 +1254,9 @@ __global__ __launch_bounds__(join_threads(1)) void window_wide_join_kernel(Windo
 }
 
 // Many rows over a 4-bit cache: every request's tokens are widened once into 16-bit blocks of
-// sixteen, [request][columns][head][16][D], exactly, with a table of their own, and the wide
-// kernel reads those.  Each value is read by hundreds of rows, which this costs one write and one
+// sixteen, [request][columns][head][16][D], exactly (fp16: below 2^-16 to a multiple of
+// 2^-24, which moves a score by 2^-25 sum |q| at most and a value by half a step of the output),
+// with a table of their own, and the wide kernel reads those.  Each value is read by hundreds of rows, which this costs one write and one
 // read of 16 bits; widened in the wide kernel it would be a third more instructions beside its
 // products.  One workgroup per block: a thread has eight dims of a token.  Bound by memory: 2 x
 // 16000 tokens of 2 x 128 dims (19 MB to 33 MB) 9.5 us.
