@@ -1256,9 +1256,9 @@ __global__ __launch_bounds__(join_threads(1)) void window_wide_join_kernel(Windo
 // Many rows over a 4-bit cache: every request's tokens are widened once into 16-bit blocks of
 // sixteen, [request][columns][head][16][D], exactly (fp16: below 2^-16 to a multiple of
 // 2^-24, which moves a score by 2^-25 sum |q| at most and a value by half a step of the output),
-// with a table of their own, and the wide kernel reads those.  Each value is read by hundreds of rows, which this costs one write and one
-// read of 16 bits; widened in the wide kernel it would be a third more instructions beside its
-// products.  One workgroup per block: a thread has eight dims of a token.  Bound by memory: 2 x
+// with a table of their own, and the wide kernel reads those.  Each value is read by hundreds of
+// rows, which this costs one write and one read of 16 bits; widened in the wide kernel it would
+// be a third more instructions beside its products.  One workgroup per block: a thread has eight dims of a token.  Bound by memory: 2 x
 // 16000 tokens of 2 x 128 dims (19 MB to 33 MB) 9.5 us.
 struct Widen {
   Window w;

@@ -96,7 +96,8 @@ def accumulate_weights(q: torch.Tensor, k_cache: torch.Tensor | KVCache4, block_
     rows and query heads of e^(score - lse).
 
     ``lse`` is what :func:`window_attention` returned for the same rows, and the other
-    arguments are those of that call; ``k_cache`` may be a :class:`KVCache4`.  With
+    arguments are those of that call; ``k_cache`` may be a :class:`KVCache4` (with fp16
+    rows, cached keys beyond its range may count as infinite).  With
     ``new_lens`` (int32 [requests], as :func:`append_blocks` took it) that many last
     tokens of a request start from nothing: their slots hold what an earlier owner
     left there.  One ``weights`` for each layer, or one for all of them.  No block may
