@@ -19,31 +19,35 @@ struct Weigh {
   int tiles, parts;      // of kTile tokens: workgroups per request; parts of the rows
   float* sums;           // (parts > 1) [requests][columns * block_size][parts]
 };
-constexpr int kWaves = 4, kTile = 32 * kWaves;
+constexpr int kWaves = 4, kTile = 32 * kWaves, kFewRows = 16;
 
 // One workgroup per request, tile of 128 tokens and part of the rows (of all key heads, 32 (token,
 // query head) at a time).  A wave's 32 tokens stay in registers as A operands of
 // v_mfma_f32_32x32x16, 4-bit ones widened exactly (fp16: below 2^-16 to a multiple of
 // 2^-24, which moves a score by 2^-25 sum |q| at most); the rows pass by through LDS as B operands,
-// SUB tiles between two barriers (one: a key head has no more), shared by the waves, and lane l
-// adds up the weights of tokens 8 b + 4 (l/32) + i for row l%32.  Every sum is one wave's, those
+// SUB tiles between two barriers (one: a key head has sixteen rows at most), shared by the waves,
+// and lane l adds up the weights of tokens 8 b + 4 (l/32) + i for row l%32.  Every sum is one wave's, those
 // of the parts are added in order: the order of all additions is fixed.
 // Prompts are bound by the vector units (a fused multiply-add, an exponential, which takes four
 // times as long, and an addition a score, next to a product of 128 dims): 2 x 512 rows over 8192
-// tokens in 4 bits 39 us, 3.4 T scores a second.  Single rows wait for their keys: 16 requests
-// of 8000 tokens 15 us, 2.2 TB/s.
+// tokens in 4 bits 39 us, 3.4 T scores a second.  Single rows are bound by reading the keys: 16-bit
+// ones go through LDS too, in whole lines and a head ahead of the products, 16 requests of 8000
+// tokens in 13.5 us, 4.9 TB/s (straight into registers, a head after the other, 16).
 template <int D, bool F16, bool FP4, int SUB>
 __global__ __launch_bounds__(64 * kWaves, 4) void weigh_kernel(Weigh g) {
   const Window& a = g.w;
   typedef typename Elem<F16>::x8 x8;
-  constexpr int DC = D / 16, P = D / 8, KI = 64 / P, J = 32 / kWaves / KI;
-  static_assert(J >= 1);
-  __shared__ __attribute__((aligned(256))) uint16_t lq[2][SUB][32 * D];
+  constexpr int DC = D / 16, P = D / 8, KI = 64 / P;
+  constexpr int QR = SUB == 1 ? kFewRows : 32;             // rows of a tile
+  constexpr int J = QR < kWaves * KI ? 1 : QR / kWaves / KI;  // loads of a wave for it (of too many waves some have none)
+  constexpr bool STAGED = SUB == 1 && !FP4;                // the keys too go through LDS, a head ahead
+  __shared__ __attribute__((aligned(256))) uint16_t lq[2][SUB][QR * D];
+  __shared__ __attribute__((aligned(256))) uint16_t lk[STAGED ? kWaves : 1][STAGED ? 32 * D : 8];
   const int lane = threadIdx.x & 63, li = lane & 31, h = lane >> 5;
   const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
   // piece p of row r lies at p ^ turn: sixteen rows' pieces meet all banks
   auto turn = [](int r) { return r * P / 16 & (P - 1); };
-  const uint32_t q_at = lds_address(lq) + li * (2 * D) + 16 * (h ^ turn(li));
+  const uint32_t q_at = lds_address(lq) + li % QR * (2 * D) + 16 * (h ^ turn(li % QR));
   const int part = blockIdx.x % g.parts, unit = blockIdx.x / g.parts, b = unit / g.tiles;
   const Ragged rq = ragged(a, b);
   const int32_t* table = a.tables + b * a.tstride;
@@ -115,7 +119,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void weigh_kernel(Weigh g) {
             const int ln = here(lane), r = (wave * J + j) * KI + ln / P, t = min(x.t, tokens - 1);
             const uint16_t* p = a.q + static_cast<int64_t>(rq.row0 + ta + t) * a.q_row + (kh * a.group + x.r) * a.q_head +
                                 8 * (ln % P ^ turn(r));
-            load_lds(p, lds_address(lq) + (to * SUB + u) * (64 * D) + (wave * J + j) * 1024);
+            if (QR >= kWaves * KI || wave < QR / KI)
+              load_lds(p, lds_address(lq) + (to * SUB + u) * (QR * 2 * D) + (wave * J + j) * 1024);
           }
           if (SUB > 1) on(sent);
           lse1[u] = a.lse[static_cast<int64_t>(rq.row0 + ta + min(own.t, tokens - 1)) * a.q_heads + kh * a.group + own.r];
@@ -124,7 +129,21 @@ __global__ __launch_bounds__(64 * kWaves, 4) void weigh_kernel(Weigh g) {
         }
       }
     };
+    // The wave's keys of head kh into its part of lk: both sixteens whole (one behind the last token
+    // is that with the last one again, and masked), piece p of a row at p ^ turn.
+    auto fetch = [&] {
+#pragma unroll
+      for (int n = 0; n < 32 / KI; ++n) {
+        const int ln = here(lane), r = n * KI + ln / P, from = n * KI & 16;
+        const int64_t block = __builtin_amdgcn_readlane(static_cast<int>(blk), from);
+        const int first = __builtin_amdgcn_readlane(slot, from) & ~15;
+        const uint16_t* p = static_cast<const uint16_t*>(a.kc) + block * a.kc_block + static_cast<int64_t>(first) * a.kc_slot +
+                            kh * a.kc_head + (r & 15) * a.kc_slot + 8 * (ln % P ^ turn(r));
+        load_lds(p, lds_address(lk) + wave * (64 * D) + n * 1024);
+      }
+    };
     if (n0 < n1) {
+      if constexpr (STAGED) fetch();
       start();
       send(0);
     }
@@ -149,7 +168,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void weigh_kernel(Weigh g) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) k[d][e] = Elem<F16>::pack(f[2 * e] * sc, f[2 * e + 1] * sc);
           }
-        } else {
+        } else if constexpr (!STAGED) {
           const uint16_t* p = static_cast<const uint16_t*>(a.kc) + blk * a.kc_block + static_cast<int64_t>(slot) * a.kc_slot +
                               kh * a.kc_head + 8 * h;
 #pragma unroll
@@ -162,12 +181,21 @@ __global__ __launch_bounds__(64 * kWaves, 4) void weigh_kernel(Weigh g) {
       for (int u = 0; u < SUB; ++u) lse[u] = lse1[u] * 1.44269504088896340736f, pos[u] = pos1[u];
       arrived<0>();
       __syncthreads();  // (the rows are whole; the other buffer's have been read)
+      if constexpr (STAGED) {
+#pragma unroll
+        for (int d = 0; d < DC; ++d)
+          k[d] = *lds<const u32x4>((lds_address(lk) + wave * (64 * D) + li * (2 * D) + 16 * (h ^ turn(li))) ^ (32 * d));
+#pragma unroll
+        for (int d = 0; d < DC; ++d) asm volatile("" : "+v"(k[d]));  // (here: the next head's go there)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
       if (n + 1 < n1) {
         row0 += 32 * SUB;
         if (row0 >= rows) {
           row0 = 0, ++kh;
           if (SUB > 1) start();
         }
+        if constexpr (STAGED) fetch();
         send(buf ^ 1);
       }
 #pragma unroll 1  // (a step's kernel waits for its instructions too)
@@ -179,7 +207,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void weigh_kernel(Weigh g) {
         f32x16 s{};
 #pragma unroll
         for (int d = 0; d < DC; ++d) {
-          const x8 q = __builtin_bit_cast(x8, *lds<const u32x4>((q_at ^ (32 * d)) + (buf * SUB + u) * (64 * D)));
+          const x8 q = __builtin_bit_cast(x8, *lds<const u32x4>((q_at ^ (32 * d)) + (buf * SUB + u) * (QR * 2 * D)));
           const x8 kd = __builtin_bit_cast(x8, k[d]);
           if constexpr (F16) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kd, q, s, 0, 0, 0);
           else s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kd, q, s, 0, 0, 0);
@@ -675,7 +703,7 @@ extern "C" int pgs_accumulate_weights(const pgs_accumulate_weights_args* args, v
   auto go = [&](auto d, auto f16) {
     constexpr int D = decltype(d)::value;
     constexpr bool F = decltype(f16)::value;
-    const bool one = static_cast<int64_t>(a.max_tokens) * a.group <= 32;
+    const bool one = static_cast<int64_t>(a.max_tokens) * a.group <= kFewRows;
     if (g.cache) {
       if (one) hipLaunchKernelGGL((weigh_kernel<D, F, false, 1>), grid, block, 0, st, w);
       else hipLaunchKernelGGL((weigh_kernel<D, F, false, 2>), grid, block, 0, st, w);
