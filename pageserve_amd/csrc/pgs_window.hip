@@ -1094,7 +1094,7 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
       }
     };
     // Tile i's scores in s, whether one of them may need a higher reference: what its rows do not
-    // see is hidden; the reference that they go by.  masked: whether it has masks.
+    // see is hidden; the reference that they go by.
     auto take = [&](int i, Scores& s, bool over, uint32_t any, float& ref, bool& lifted) {
       bool masked = !plain(i);
       uint32_t bm = 0;
@@ -1108,7 +1108,6 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
         }
       }
       if (__builtin_expect(masked || over || w.far, 0)) lifted = w.lift(a, s, ref);
-      return masked;
     };
 
     constexpr int L = 2 * J;  // loads of a wave per tile
@@ -1130,7 +1129,8 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
         multiply_keys(n, k, s0);
       }
       float ref = w.mx;
-      bool lifted = false, masked = take(t0, s0, true, lany, ref, lifted), settles = to_settle(t0 + 1);
+      bool lifted = false, settles = to_settle(t0 + 1);
+      take(t0, s0, true, lany, ref, lifted);
       if (lifted) w.settle(ref);
       u32x4 first[2];  // the weights of a tile's first step
 #pragma unroll
@@ -1174,9 +1174,9 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, s[1][e]);
         float ref = w.mx;
-        bool lifted = false, masks = false;
+        bool lifted = false;
         if (i + 1 < t1)
-          masks = take(i + 1, s, __ballot(fmaf(top, a.c, -w.mx) > kSlack + E::kHead), uniform(static_cast<int>(any_v)), ref, lifted);
+          take(i + 1, s, __ballot(fmaf(top, a.c, -w.mx) > kSlack + E::kHead), uniform(static_cast<int>(any_v)), ref, lifted);
         // this one's output beside the next one's weights of its first step
         u32x4 next[2];
         sum = 0.f;
@@ -1193,7 +1193,9 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
           interleave<DV, 4, 10>();
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (__builtin_expect(masked, 0)) {
+        // (settle took values out of a tile for all rows where one of the workgroup's does not see it
+        // whole, so this wave's may see it whole and still be owed them)
+        if (__builtin_expect(!plain(i), 0)) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             uint32_t odd = 0;
@@ -1213,7 +1215,6 @@ __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
         if (__builtin_expect(lifted, 0)) w.settle(ref);
         if (i + 1 < t1) w.sum += sum;
         first[0] = next[0], first[1] = next[1];
-        masked = masks;
       };
       for (int i = t0; i < t1; i += 2) {
         tile(i, s0, s1);
