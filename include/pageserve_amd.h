@@ -747,6 +747,7 @@ size_t pgs_accumulate_weights_workspace_bytes(const pgs_accumulate_weights_args*
  * request of more than max_context tokens is left as it is.  No block may be in
  * two requests' tables, no two caches may share an element, and no array that is
  * written may share memory with another.
+ * requests at most 65536, requests * kv_heads at most 2^24.
  * workspace: pgs_evict_tokens_workspace_bytes() bytes, no fill needed.
  */
 int pgs_evict_tokens(float* weights, const int32_t* lens, const int32_t* budget,

@@ -477,13 +477,14 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(Evict a) {
 }
 
 constexpr int kMoveThreads = 1024, kMaxCaches = 16;
+constexpr int64_t kMoveGroups = 0xffffffff / kMoveThreads;  // of a launch: its threads are fewer than 2^32
 struct MoveCache {
   void *k, *v, *ks, *vs;
   int64_t k_block, k_slot, k_head, v_block, v_slot, v_head;
 };
 struct Move {
   Evict e;
-  int32_t heads, slices, caches;
+  int32_t heads, slices, caches, first;  // first: request
   MoveCache c[kMaxCaches];
 };
 
@@ -568,7 +569,7 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(Move m, int pieces) 
   const bool values = u & 1;
   u >>= 1;
   const MoveCache& c = m.c[u % m.caches];
-  const int b = u / m.caches;
+  const int b = m.first + u / m.caches;
   uint16_t* base = static_cast<uint16_t*>(values ? c.v : c.k) + h * (values ? c.v_head : c.k_head);
   const int64_t block = values ? c.v_block : c.k_block, step = values ? c.v_slot : c.k_slot;
   const int p0 = pieces * slice / m.slices, p1 = pieces * (slice + 1) / m.slices;
@@ -587,7 +588,7 @@ __global__ __launch_bounds__(kMoveThreads) void move4_kernel(Move m) {
   const int part = u & 3;
   u >>= 2;
   const MoveCache& c = m.c[u % m.caches];
-  const int b = u / m.caches;
+  const int b = m.first + u / m.caches;
   auto row = [&](int blk, int slot) { return (static_cast<int64_t>(blk) * m.heads + h) * m.e.bs + slot; };
   if (part == 0) {
     typedef std::conditional_t<C == 4, u32x4, u32x2> T;
@@ -764,8 +765,9 @@ extern "C" int pgs_evict_tokens(float* weights, const int32_t* lens, const int32
     if (!aligned(c.k, 16) || !aligned(c.v, 16) || !aligned(c.k_scale, 16) || !aligned(c.v_scale, 16))
       return fail(PGS_ERR_MISALIGNED, "%s: misaligned", fn);
   }
-  for (int64_t heads : {count ? caches[0].kv_heads : 1, count4 ? caches4[0].kv_heads : 1})  // (grids are 32-bit)
-    if (requests * heads > 0x7fffffff / (kMaxCaches * 8)) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: too many requests", fn);
+  for (int64_t heads : {count ? caches[0].kv_heads : 1, count4 ? caches4[0].kv_heads : 1})
+    if (requests * heads > 0x1000000)
+      return fail(PGS_ERR_INVALID_ARGUMENT, "%s: requests=%lld x kv_heads=%lld is above 2^24", fn, (long long)requests, (long long)heads);
   if (requests == 0) return PGS_OK;
   if ((blocks > 0 && !weights) || !lens || !budget || !kept || (columns > 0 && !block_tables))
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
@@ -787,11 +789,23 @@ extern "C" int pgs_evict_tokens(float* weights, const int32_t* lens, const int32
   e.begin = static_cast<int32_t*>(workspace), e.from = e.begin + requests;
   hipLaunchKernelGGL(select_kernel, dim3(static_cast<unsigned>(requests)), dim3(kSelectThreads), 0, st, e);
   if (int rc = check_launch("evict_tokens kernel")) return rc;
-  for (int64_t i0 = 0; i0 < count; i0 += kMaxCaches) {
-    m.caches = static_cast<int32_t>(std::min<int64_t>(count - i0, kMaxCaches));
+  // Caches and requests of a launch, `units` workgroups each.
+  auto launches = [&](int64_t caches_left, int64_t units, auto launch) {
+    m.caches = static_cast<int32_t>(std::min({caches_left, int64_t{kMaxCaches}, kMoveGroups / units}));
+    const int64_t most_requests = kMoveGroups / (units * m.caches);
+    int rc = PGS_OK;
+    for (int64_t r = 0; r < requests && rc == PGS_OK; r += most_requests) {
+      m.first = static_cast<int32_t>(r);
+      launch(dim3(static_cast<unsigned>(std::min(requests - r, most_requests) * m.caches * units)));
+      rc = check_launch("move kernel");
+    }
+    return rc;
+  };
+  for (int64_t i0 = 0; i0 < count; i0 += m.caches) {
     m.heads = static_cast<int32_t>(caches[0].kv_heads);
     const int pieces = static_cast<int>(vec ? caches[0].head_dim / 8 : caches[0].head_dim);
-    for (int i = 0; i < m.caches; ++i) {
+    const int64_t left = std::min<int64_t>(count - i0, kMaxCaches);
+    for (int64_t i = 0; i < left; ++i) {
       const pgs_kv_cache& c = caches[i0 + i];
       m.c[i] = MoveCache{c.k, c.v, nullptr, nullptr, c.k_block, c.k_slot, c.k_head, c.v_block, c.v_slot, c.v_head};
     }
@@ -799,24 +813,26 @@ extern "C" int pgs_evict_tokens(float* weights, const int32_t* lens, const int32
     // layers of 2 x 128 dims takes 134 us)
     m.slices = std::max(1, static_cast<int>(pieces * (vec ? 16 : 2)) / 128);
     while (pieces % m.slices) --m.slices;
-    const int64_t units = requests * m.caches * 2 * m.heads;
-    while (units * m.slices < 128 && pieces % (2 * m.slices) == 0 && pieces / m.slices > 2) m.slices *= 2;
-    const dim3 grid(static_cast<unsigned>(units * m.slices));
-    if (vec) hipLaunchKernelGGL(move_kernel<u32x4>, grid, dim3(kMoveThreads), 0, st, m, pieces);
-    else hipLaunchKernelGGL(move_kernel<uint16_t>, grid, dim3(kMoveThreads), 0, st, m, pieces);
-    if (int rc = check_launch("move kernel")) return rc;
+    while (requests * left * 2 * m.heads * m.slices < 128 && pieces % (2 * m.slices) == 0 && pieces / m.slices > 2) m.slices *= 2;
+    // (2 x 4096 heads x 256 slices at most: one cache of one request always fits)
+    if (int rc = launches(left, int64_t{2} * m.heads * m.slices, [&](dim3 grid) {
+          if (vec) hipLaunchKernelGGL(move_kernel<u32x4>, grid, dim3(kMoveThreads), 0, st, m, pieces);
+          else hipLaunchKernelGGL(move_kernel<uint16_t>, grid, dim3(kMoveThreads), 0, st, m, pieces);
+        }))
+      return rc;
   }
-  for (int64_t i0 = 0; i0 < count4; i0 += kMaxCaches) {
-    m.caches = static_cast<int32_t>(std::min<int64_t>(count4 - i0, kMaxCaches));
+  for (int64_t i0 = 0; i0 < count4; i0 += m.caches) {
     m.heads = static_cast<int32_t>(caches4[0].kv_heads);
-    for (int i = 0; i < m.caches; ++i) {
+    const int64_t left = std::min<int64_t>(count4 - i0, kMaxCaches);
+    for (int64_t i = 0; i < left; ++i) {
       const pgs_kv_cache4& c = caches4[i0 + i];
       m.c[i] = MoveCache{c.k, c.v, c.k_scale, c.v_scale, 0, 0, 0, 0, 0, 0};
     }
-    const dim3 grid(static_cast<unsigned>(requests * m.caches * 4 * m.heads));
-    if (caches4[0].head_dim == 64) hipLaunchKernelGGL(move4_kernel<64>, grid, dim3(kMoveThreads), 0, st, m);
-    else hipLaunchKernelGGL(move4_kernel<128>, grid, dim3(kMoveThreads), 0, st, m);
-    if (int rc = check_launch("move kernel")) return rc;
+    if (int rc = launches(left, int64_t{4} * m.heads, [&](dim3 grid) {
+          if (caches4[0].head_dim == 64) hipLaunchKernelGGL(move4_kernel<64>, grid, dim3(kMoveThreads), 0, st, m);
+          else hipLaunchKernelGGL(move4_kernel<128>, grid, dim3(kMoveThreads), 0, st, m);
+        }))
+      return rc;
   }
   return PGS_OK;
 }
