@@ -623,8 +623,9 @@ constexpr int64_t kSums = int64_t{1} << 26;
 WeighPlan weigh_plan(const pgs_accumulate_weights_args& g, int64_t block_size) {
   const int64_t context = std::min(g.max_context, g.columns * block_size);
   WeighPlan p;
-  // (a request that is longer than max_context takes further turns; grids are 32-bit)
-  p.tiles = std::max<int64_t>(1, std::min((context + kTile - 1) / kTile, 0x3fffffff / std::max<int64_t>(g.requests, 1)));
+  // (a request that is longer than its tiles takes further turns; a launch has fewer than 2^32 threads)
+  constexpr int64_t most = 0xffffffff / (64 * kWaves);
+  p.tiles = std::max<int64_t>(1, std::min((context + kTile - 1) / kTile, most / std::max<int64_t>(g.requests, 1)));
   const int64_t rows = g.rows * g.q_heads / std::max<int64_t>(g.requests, 1);
   // (and their sums, one for each token that the tables have room for, take kSums bytes at most)
   const int64_t each = std::max<int64_t>(1, g.requests * g.columns * block_size * 4);

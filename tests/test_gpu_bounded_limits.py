@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from pageserve_amd import KVCache4, evict_tokens
+from pageserve_amd import KVCache4, accumulate_weights, evict_tokens, window_attention, window_attention4
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,33 @@ def test_eviction_of_many_requests_in_many_layers(gpu, bits, heads, dim):
     assert torch.equal(weights, want_weights)
     for x, y in zip(parts(caches), parts(want)):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_sums_of_many_requests_over_wide_tables(gpu, tokens, bits):
+    """1024 requests of tables for 2^21 tokens: 2^24 workgroups of 256 threads.  Some have tokens; the call
+    gives what the same call for shorter texts gives."""
+    requests, bs, columns, live, lens = 1024, 65536, 32, [0, 7, 1000, 1023], [300, 41, 129, 40]
+    blocks = len(live) + 1
+    tables = torch.full((requests, columns), -1, dtype=torch.int32)
+    all_lens, counts = torch.zeros(requests, dtype=torch.int32), torch.zeros(requests, dtype=torch.int32)
+    for i, (b, n) in enumerate(zip(live, lens)):
+        tables[b, 0], all_lens[b], counts[b] = blocks - 1 - i, n, tokens
+    offsets = torch.nn.functional.pad(counts.cumsum(0), (1, 0)).to(torch.int32)
+    q = numbers(gpu, int(offsets[-1]), 4, 64)
+    if bits == 16:
+        cache = tuple(numbers(gpu, blocks, bs, 1, 64, seed=i + 1) for i in range(2))
+    else:
+        c = KVCache4(blocks, bs, 1, 64, gpu)
+        c.k.random_(), c.v.random_(), c.k_scale.fill_(0.25), c.v_scale.fill_(0.5)
+        cache = (c,)
+    rest = [x.to(gpu) for x in (tables, all_lens, offsets)]
+    attend = window_attention if bits == 16 else window_attention4
+    _, lse = attend(q, *cache, *rest, max_tokens=tokens, max_context=1000, return_lse=True)
+    sums, want = torch.zeros(blocks, bs, device=gpu), torch.zeros(blocks, bs, device=gpu)
+    accumulate_weights(q, cache[0], *rest, lse, sums, max_tokens=tokens)
+    accumulate_weights(q, cache[0], *rest, lse, want, max_tokens=tokens, max_context=1000)
+    assert torch.equal(sums, want)
+    rows = lse.numel()  # (each row's weights add up to 1, each within 2^-17 of its own)
+    assert abs(float(sums.double().sum()) - rows) <= rows * 2.0 ** -15
