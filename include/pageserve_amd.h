@@ -649,7 +649,7 @@ typedef struct pgs_kv_cache4 {
  * row and head given) in 4 bits into slot slots[i] of the cache; a slot outside
  * the cache is left out.  The slots of the rows must differ (of two rows with one
  * slot, pieces of either may stay).  head_dim 64 or 128, block_size a multiple
- * of 16, the cache 16-byte aligned.
+ * of 16, the cache 16-byte aligned; rows * kv_heads * head_dim at most 2^34 - 1024.
  */
 int pgs_write_kv4(const void* k, int64_t k_row, int64_t k_head, const void* v,
                   int64_t v_row, int64_t v_head, int dtype,
@@ -657,7 +657,8 @@ int pgs_write_kv4(const void* k, int64_t k_row, int64_t k_head, const void* v,
                   void* stream);
 
 /* The rows at slots[i] back: k, v [rows, kv_heads, head_dim] (bf16, fp16 or
- * fp32, contiguous, 16-byte aligned); zeros for a slot outside the cache. */
+ * fp32, contiguous, 16-byte aligned); zeros for a slot outside the cache.  As many
+ * rows as above. */
 int pgs_read_kv4(const pgs_kv_cache4* cache, const int64_t* slots, int64_t rows,
                  void* k, void* v, int dtype, void* stream);
 

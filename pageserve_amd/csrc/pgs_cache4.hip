@@ -192,7 +192,9 @@ int check_cache4(const char* fn, const pgs_kv_cache4* cache, int64_t rows) {
       c.kv_heads < 1 || c.kv_heads > 4096)
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: the cache needs blocks of a multiple of 16 tokens (block_size=%lld)", fn,
                 (long long)c.block_size);
-  if (rows < 0 || rows > (int64_t{1} << 36) / (c.kv_heads * c.head_dim)) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: rows=%lld", fn, (long long)rows);
+  // (a launch has fewer than 2^32 threads, each of four numbers at least, in whole workgroups)
+  if (rows < 0 || rows > ((int64_t{1} << 34) - 4 * kRowThreads) / (c.kv_heads * c.head_dim))
+    return fail(PGS_ERR_INVALID_ARGUMENT, "%s: rows=%lld: rows x kv_heads x head_dim must be at most 2^34 - 1024", fn, (long long)rows);
   if (rows > 0 && c.blocks > 0 && (!c.k || !c.k_scale || !c.v || !c.v_scale))
     return fail(PGS_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
   if (!aligned(c.k, 16) || !aligned(c.k_scale, 16) || !aligned(c.v, 16) || !aligned(c.v_scale, 16))
