@@ -1343,7 +1343,8 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
   if (p.wide) {
     if (fp4) {
       p.columns = (columns * block_size + 15) / 16;
-      p.widen = std::max<int64_t>(1, std::min(p.columns, (max_context + 15) / 16));
+      // (a launch has fewer than 2^32 threads: of several requests' chunk it always has)
+      p.widen = std::max<int64_t>(1, std::min({p.columns, (max_context + 15) / 16, int64_t{0xffffffff / 256}}));
       p.chunk = std::max<int64_t>(1, std::min<int64_t>(requests, kWidened / std::max<int64_t>(1, p.columns * kv_heads * 64 * head_dim)));
     }
     return p;

@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from bounded import Batch
 from pageserve_amd import KVCache4, accumulate_weights, evict_tokens, window_attention, window_attention4
 
 pytestmark = pytest.mark.gpu
@@ -87,3 +88,15 @@ def test_sums_of_many_requests_over_wide_tables(gpu, tokens, bits):
     assert torch.equal(sums, want)
     rows = lse.numel()  # (each row's weights add up to 1, each within 2^-17 of its own)
     assert abs(float(sums.double().sum()) - rows) <= rows * 2.0 ** -15
+
+
+def test_many_rows_over_a_table_for_a_very_long_text_in_4_bits(gpu):
+    """2^28 tokens and more: as many sixteens to widen as make 2^24 workgroups of 256 threads, 69 GB of room"""
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GB of free memory")
+    b = Batch(5, [70000], [80], 2, 1, 64, 65536, torch.bfloat16, 4, columns=4097)
+    args = b.args(gpu)
+    b.check(window_attention4(*args, window=300, sinks=9, return_lse=True), b.oracle(window=300, sinks=9))
+    torch.cuda.empty_cache()
+    b.check(window_attention4(*args, return_lse=True), b.oracle())
+    torch.cuda.empty_cache()
