@@ -8,6 +8,8 @@
 //   upto_b = sum of the needs of requests 0 .. b (those whose table has the columns)
 // It is served if need = 0 or upto_b <= the free count, so the served needs are a
 // prefix; entry e = (upto_b - need) + j of them takes free[count - 1 - e].
+#include <algorithm>
+
 #include "pgs_linear.h"
 
 namespace pgs {
@@ -307,7 +309,8 @@ extern "C" int pgs_append_blocks(int32_t* lens, const int32_t* new_lens, int32_t
   if (int rc = check_tables(fn, lens, new_lens, block_tables, table_stride, columns, free_blocks, free_capacity,
                             free_count, block_size, requests))
     return rc;
-  if (rows < 0 || rows > (int64_t{1} << 31) * kRowThreads / 2) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: rows=%lld", fn, (long long)rows);
+  if (rows < 0 || rows > 0xffffffff - kRowThreads)  // (threads of a launch)
+    return fail(PGS_ERR_INVALID_ARGUMENT, "%s: rows=%lld", fn, (long long)rows);
   if (!offsets || (requests > 0 && !status) || (rows > 0 && !slots)) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
   if (!aligned(offsets, 4) || !aligned(index, 4) || !aligned(slots, 8) || !aligned(status, 4))
     return fail(PGS_ERR_MISALIGNED, "%s: misaligned", fn);
@@ -371,12 +374,19 @@ extern "C" int pgs_write_kv(const void* k, int64_t k_row, int64_t k_head, const 
   if (rows > (int64_t{1} << 38) / per) return fail(PGS_ERR_INVALID_ARGUMENT, "%s: too large", fn);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (int rc = require_device(fn, st)) return rc;
-  const WriteArgs a{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), k_row, k_head, v_row, v_head,
-                    static_cast<uint16_t*>(c.k), static_cast<uint16_t*>(c.v), c.k_block, c.k_slot, c.k_head, c.v_block,
-                    c.v_slot, c.v_head, c.blocks * c.block_size, static_cast<int>(c.block_size),
-                    static_cast<int>(c.kv_heads), pieces, slots, rows * per};
-  const dim3 grid(static_cast<unsigned>((a.units + kRowThreads - 1) / kRowThreads)), block(kRowThreads);
-  if (vec) hipLaunchKernelGGL(write_kv_kernel<true>, grid, block, 0, st, a);
-  else hipLaunchKernelGGL(write_kv_kernel<false>, grid, block, 0, st, a);
-  return check_launch("write_kv kernel");
+  WriteArgs a{nullptr, nullptr, k_row, k_head, v_row, v_head,
+              static_cast<uint16_t*>(c.k), static_cast<uint16_t*>(c.v), c.k_block, c.k_slot, c.k_head, c.v_block,
+              c.v_slot, c.v_head, c.blocks * c.block_size, static_cast<int>(c.block_size),
+              static_cast<int>(c.kv_heads), pieces, nullptr, 0};
+  // (a launch has fewer than 2^32 threads, and larger counts are cut without an error)
+  const int64_t most = (0xffffffff - kRowThreads) / per;  // of 2^28 units a row at most
+  for (int64_t row = 0; row < rows; row += most) {
+    a.k = static_cast<const uint16_t*>(k) + row * k_row, a.v = static_cast<const uint16_t*>(v) + row * v_row, a.slots = slots + row;
+    a.units = std::min(rows - row, most) * per;
+    const dim3 grid(static_cast<unsigned>((a.units + kRowThreads - 1) / kRowThreads)), block(kRowThreads);
+    if (vec) hipLaunchKernelGGL(write_kv_kernel<true>, grid, block, 0, st, a);
+    else hipLaunchKernelGGL(write_kv_kernel<false>, grid, block, 0, st, a);
+    if (int rc = check_launch("write_kv kernel")) return rc;
+  }
+  return PGS_OK;
 }

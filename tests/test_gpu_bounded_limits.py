@@ -1,4 +1,5 @@
-"""Calls of the operators of long texts whose grids pass what one launch may have: 2^32 threads."""
+"""Calls of the paged cache and of the operators of long texts whose grids pass what one launch may have:
+2^32 threads."""
 
 from __future__ import annotations
 
@@ -6,7 +7,7 @@ import pytest
 import torch
 
 from bounded import Batch
-from pageserve_amd import KVCache4, accumulate_weights, evict_tokens, window_attention, window_attention4
+from pageserve_amd import KVCache4, accumulate_weights, evict_tokens, window_attention, window_attention4, write_kv
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +101,19 @@ def test_many_rows_over_a_table_for_a_very_long_text_in_4_bits(gpu):
     torch.cuda.empty_cache()
     b.check(window_attention4(*args, return_lse=True), b.oracle())
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("aligned", [False, True])
+def test_rows_beyond_one_launch_of_write_kv(gpu, aligned):
+    """2^32 pieces and more (of one number where something is not aligned, else of eight): the last rows too"""
+    dim, bs, rows = (256, 16, (1 << 24) + 300) if not aligned else (1024, 16, (1 << 25) + 300)
+    buffer = numbers(gpu, 2, dim + 8)
+    k, v = (x[8 if aligned else 1:][:dim].expand(rows, 1, dim) for x in buffer)
+    cache = [torch.zeros(4, bs, 1, dim, dtype=torch.bfloat16, device=gpu) for _ in range(2)]
+    slots = torch.full((rows,), -1, dtype=torch.int64, device=gpu)
+    slots[0], slots[(1 << 24) - 1], slots[-1] = 3, 20, 37
+    write_kv(k, v, *cache, slots)
+    for part, x in zip(cache, (k, v)):
+        want = torch.zeros_like(part)
+        want.view(-1, dim)[[3, 20, 37]] = x[0, 0]
+        assert torch.equal(part, want)
