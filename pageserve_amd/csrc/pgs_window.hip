@@ -1381,7 +1381,9 @@ bool sizes_ok(int64_t rows, int64_t requests, int64_t q_heads, int64_t kv_heads,
         window <= 0x7fffffff && sinks >= 0 && sinks <= 0x7fffffff))
     return false;
   const int64_t most = std::min(max_tokens, std::max<int64_t>(rows, 1)) * q_heads;  // rows x heads of a request
-  return most <= 0x3fffffff && requests * (most + 64 * kv_heads) <= int64_t{0x3fffffff};  // (grids are 32-bit)
+  // (Rows straight from memory: workgroups of 256 threads for requests x key heads, or few, and fewer
+  // than 2^32 threads.  Shared tiles have one grid whatever there is.)
+  return most <= 0x3fffffff && requests * kv_heads <= 0xffffff && requests * most <= int64_t{1} << 40;
 }
 
 template <int D, bool F16>

@@ -117,3 +117,14 @@ def test_rows_beyond_one_launch_of_write_kv(gpu, aligned):
         want = torch.zeros_like(part)
         want.view(-1, dim)[[3, 20, 37]] = x[0, 0]
         assert torch.equal(part, want)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_step_of_many_requests_that_says_nothing_of_its_rows(gpu, bits):
+    """8192 requests of one row: by default planned as if each could have all 8192"""
+    lens = [1 + 7 * b % 40 for b in range(8192)]
+    b = Batch(8, lens, [1] * 8192, 16, 1, 64, 16, torch.bfloat16, bits, garbage=float("nan"))
+    args, want = b.args(gpu), b.oracle(window=20, sinks=2)
+    attend = window_attention if bits == 16 else window_attention4
+    for most in (None, 1):
+        b.check(attend(*args, window=20, sinks=2, max_tokens=most, return_lse=True), want, f"max_tokens={most}")
