@@ -1,0 +1,101 @@
+"""Sums of weights on other streams, and eviction of rows far into a large cache: what is written,
+number by number (tests/test_gpu_evict.py: the bound of sums)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from bounded import Batch
+from oracle import window_oracle as W
+from pageserve_amd import KVCache4, accumulate_weights, evict_tokens, read_kv4, window_attention, window_attention4
+from test_gpu_evict import check_weights
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("tokens", [2, 70, 600])
+def test_sums_on_other_streams(gpu, tokens, bits):
+    """Two streams at once, each step's attention and sums behind the other: every step's sums"""
+    b = Batch(tokens, [tokens + 100, 200, 40, tokens], [tokens, 1, 0, tokens], 16, 2, 128, 16, torch.bfloat16, bits)
+    args, seen = b.args(gpu), {"window": 90, "sinks": 4}
+    start = torch.rand(b.blocks, b.bs, device=gpu)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for s in streams * 3:
+        with torch.cuda.stream(s):
+            _, lse = (window_attention4 if bits == 4 else window_attention)(*args, return_lse=True, **seen)
+            sums = start.clone()
+            accumulate_weights(args[0], args[1], *args[-3:], lse, sums, **seen)
+            got.append((lse, sums))
+    for s in streams:
+        s.synchronize()
+    for lse, sums in got:
+        want, far = W.accumulate(start.cpu().numpy(), b.q.double().numpy(), b.dense()[0], b.tables, b.lens, b.offsets,
+                                 lse.double().cpu().numpy(), b.dim ** -0.5, None, **seen)
+        check_weights(b, sums, want, far)
+        assert torch.equal(sums, got[0][1])
+
+
+@pytest.mark.parametrize("bits,dim", [(16, 128), (16, 64), (4, 128), (4, 64)])
+def test_eviction_moves_rows_beyond_32_bits(gpu, bits, dim):
+    """Blocks whose bytes and elements lie beyond 2^32 and 2^31, and others at the front"""
+    bs, kv, lens, budget = 64, 2, [300, 77], [60, 70]
+    high = (1 << 32) // (bs * kv * (2 * dim if bits == 16 else dim // 2)) + 100
+    blocks = high + 9
+    tables = torch.tensor([[high + 4, 2, high + 8, high, 1], [high + 1, high + 6, -1, -1, -1]], dtype=torch.int32, device=gpu)
+    mine = tables[tables >= 0].long()
+    gen = torch.Generator(device=gpu).manual_seed(3)
+
+    def fill(part):
+        x = torch.randint(-30000, 30000, (len(mine), *part.shape[1:]), generator=gen, device=gpu).to(torch.int16)
+        part.view(torch.uint8 if part.dtype == torch.uint8 else torch.int16)[mine] = x.to(torch.uint8) if bits == 4 and (
+            part.dtype == torch.uint8) else x & 0x3FFF  # (finite numbers)
+        return part
+
+    if bits == 16:
+        cache = tuple(fill(torch.empty(blocks, bs, kv, dim, dtype=torch.bfloat16, device=gpu)) for _ in range(2))
+    else:
+        cache = KVCache4(blocks, bs, kv, dim, gpu)
+        for part in cache.parts:
+            fill(part)
+
+    def rows(r, n):
+        """The first n tokens of request r: (k, v)"""
+        slots = (tables[r].long()[:, None] * bs + torch.arange(bs, device=gpu)).flatten()[:n]
+        if bits == 4:
+            return read_kv4(cache, slots, torch.float32)
+        return [c[slots // bs, slots % bs] for c in cache]
+
+    weights = torch.rand(blocks, bs, generator=gen, device=gpu)
+    lens_, budget_ = [torch.tensor(x, dtype=torch.int32, device=gpu) for x in (lens, budget)]
+    want = []
+    for r in range(2):
+        w = weights[tables[r].clamp(min=0).long()].flatten()[:lens[r]].tolist()
+        stay = torch.tensor(W.stays(w, lens[r], budget[r], 5, 10), device=gpu)
+        want.append(([x[stay] for x in rows(r, lens[r])], torch.tensor(w, device=gpu)[stay]))
+    kept = evict_tokens(weights, lens_, budget_, tables, [cache], sinks=5, recent=10)
+    assert kept.tolist() == budget
+    for r in range(2):
+        for x, y in zip(rows(r, budget[r]), want[r][0]):
+            assert torch.equal(x, y)
+        assert torch.equal(weights[tables[r].clamp(min=0).long()].flatten()[:budget[r]], want[r][1])
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("tokens", [1, 5, 90])
+def test_sums_by_the_lse_of_rows_that_see_nothing(gpu, tokens, bits):
+    """window_attention's lse as it is, -inf for rows all of whose tokens are absent"""
+    b = Batch(tokens, [tokens + 40, tokens, 33, 3], [tokens, tokens, 1, 3 + tokens], 8, 2, 64, 16, torch.bfloat16, bits)
+    b.tables[0, -2:], b.tables[1], b.tables[2, 1:] = -1, -1, 1 << 20
+    args = b.args(gpu)
+    for seen in ({"window": 12, "sinks": 0}, {"window": 30, "sinks": 2}, {"window": None, "sinks": 0}):
+        _, lse = (window_attention4 if bits == 4 else window_attention)(*args, return_lse=True, **seen)
+        given = lse.double().cpu().numpy()
+        assert (given == -float("inf")).any()
+        sums = torch.zeros(b.blocks, b.bs, device=gpu)
+        accumulate_weights(args[0], args[1], *args[-3:], lse, sums, **seen)
+        want, far = W.accumulate(sums.cpu().numpy() * 0, b.q.double().numpy(), b.dense()[0], b.tables, b.lens, b.offsets,
+                                 given, b.dim ** -0.5, None, **seen)
+        check_weights(b, sums, want, far)
