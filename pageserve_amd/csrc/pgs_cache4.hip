@@ -61,7 +61,7 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
 // Eight lanes per row and head of k, and eight of v.  Of k a lane has D/8 neighbouring dims
 // (its codes are whole dwords), of v dims 2 i and 2 i + 1 of every sixteen (whole bytes of
 // two neighbouring dims' codes).  Bound by the launch: 64 rows of 2 x 64 dims 3.5 us; 8192 rows of
-// 2 x 128 dims 6.7, two of them for what memory needs, the rest for the words of values that go out
+// 2 x 128 dims 6.5, two of them for what memory needs, the rest for the words of values that go out
 // by four bytes.
 template <int D, bool F16>
 __global__ __launch_bounds__(kRowThreads) void write_kv4_kernel(Write4 a) {
@@ -147,7 +147,7 @@ struct Read4 {
 };
 
 // One thread per eight dims of a row.  Bound by the launch and one load behind another (slots, then
-// codes and scales): the same sizes 3.4 and 5.7 us.
+// codes and scales): the same sizes 3.4 and 5.2 us.
 template <int D, int OUT>
 __global__ __launch_bounds__(kRowThreads) void read_kv4_kernel(Read4 a) {
   constexpr int C = D / 32, P = D / 8;

@@ -28,11 +28,13 @@ constexpr int kWaves = 4, kTile = 32 * kWaves, kFewRows = 16;
 // SUB tiles between two barriers (one: a key head has sixteen rows at most), shared by the waves,
 // and lane l adds up the weights of tokens 8 b + 4 (l/32) + i for row l%32.  Every sum is one wave's, those
 // of the parts are added in order: the order of all additions is fixed.
-// Prompts are bound by the vector units (a fused multiply-add, an exponential, which takes four
-// times as long, and an addition a score, next to a product of 128 dims): 2 x 512 rows over 8192
-// tokens in 4 bits 39 us, 3.4 T scores a second.  Single rows are bound by reading the keys: 16-bit
-// ones go through LDS too, in whole lines and a head ahead of the products, 16 requests of 8000
-// tokens in 13.5 us, 4.9 TB/s (straight into registers, a head after the other, 16).
+// Prompts are bound by issue: 512 rows over 4096 tokens and 256 over 8192 in 4 bits (64.5 M scores of
+// 128 dims) 38 us, 1.7 T scores a second.  The products of all scores take 13 at a large product's
+// rate, the exponentials, at a quarter of the vector units' rate, 8, a multiply-add and an addition a
+// score 4; in a wave they follow one another, and only other waves' run beside them.  Single rows
+// are bound by reading the keys, behind lengths and block numbers: 16-bit ones go through LDS too, in whole
+// lines and a head ahead of the products, 16 requests of 4000 to 8000 tokens (49 MB) in 13.3 us, 3.7
+// TB/s (straight into registers, a head after the other, 16).
 template <int D, bool F16, bool FP4, int SUB>
 __global__ __launch_bounds__(64 * kWaves, 4) void weigh_kernel(Weigh g) {
   const Window& a = g.w;
@@ -316,8 +318,8 @@ __device__ __forceinline__ uint32_t order_of(uint32_t weight) {
 // again).  Of the tokens that may go, the place in the order of the last one that stays: its
 // digits from the highest on, from counts of the tokens that agree with the digits so far, until
 // all of them stay.  Then the places of all that stay, in order, and their weights.  Bound by
-// latency (the blocks, the weights, and some ten waits of the workgroup): 8 requests of 8192
-// tokens 22 us, 4 of 1100 12.  With the weights read again for each digit they took 50 and 15.
+// latency (the blocks, the weights, and some ten waits of the workgroup): 8 requests of 6144 to 8192
+// tokens 22 us, 4 of 825 to 1100 12.  With the weights read again for each digit they took 50 and 15.
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(Evict a) {
   __shared__ uint32_t held[kHeld];
   __shared__ int32_t ids[kHeld / 16];
@@ -491,8 +493,10 @@ struct Move {
 // What stays of a request, moved together: one workgroup per (request, cache, keys or values,
 // head, slice of the token's pieces).  A place takes a token from further on, so a turn's
 // tokens are read before any of its places is written, and while the turn before is written:
-// that writes nothing that later turns read.  Bound by memory: 8 requests of 8192 tokens, half of
-// them to go, in 4 layers of 2 x 128 dims (256 MB) 70 us, 3.8 TB/s.
+// that writes nothing that later turns read.  Bound by memory where there are many workgroups: 8
+// requests of 6144 to 8192 tokens cut to 4096, in 4 layers of 2 x 128 dims (267 MB read and written), 70
+// us, 3.8 TB/s.  By the turns' latency where there are few: one request of 32000 tokens cut to half, in one
+// layer, has 32 (selection and move 107 us; in 4 bits, where a head's codes or scales have one each, 240).
 // P pieces of type T of a token; piece(base of the block, slot, p): where one is.
 template <typename T, int U, typename Where>
 __device__ __forceinline__ void move_pieces(const Evict& e, int b, int p0, int pieces, Where where) {
@@ -615,7 +619,8 @@ namespace {
 // Workgroups per request, and the parts that the rows are cut into while there are too few
 // workgroups for all CUs: of 128 rows at least in a request of the batch's average.  (Not by
 // max_tokens: the order of the additions, and so the last bits, are the same for any that is
-// large enough.)
+// large enough.  A long prompt among single tokens gets no parts: 2048 rows beside 31 single ones, of 8000
+// tokens each, take 819 us, in calls of their own 112 and 24.)
 struct WeighPlan {
   int64_t tiles, parts;
 };
@@ -810,8 +815,7 @@ extern "C" int pgs_evict_tokens(float* weights, const int32_t* lens, const int32
       const pgs_kv_cache& c = caches[i0 + i];
       m.c[i] = MoveCache{c.k, c.v, nullptr, nullptr, c.k_block, c.k_slot, c.k_head, c.v_block, c.v_slot, c.v_head};
     }
-    // (a slice has whole lines of 128 bytes: of 64 the move of 8 requests of 8192 tokens in 4
-    // layers of 2 x 128 dims takes 134 us)
+    // (a slice has whole lines of 128 bytes: of 64 the move of 8 requests above, 70 us, takes 134)
     m.slices = std::max(1, static_cast<int>(pieces * (vec ? 16 : 2)) / 128);
     while (pieces % m.slices) --m.slices;
     while (requests * left * 2 * m.heads * m.slices < 128 && pieces % (2 * m.slices) == 0 && pieces / m.slices > 2) m.slices *= 2;

@@ -351,7 +351,7 @@ __device__ __forceinline__ Span group_span(const Window& a, const Ragged& rq, in
 // slices; each wave loads the keys and values of its steps into registers.  16 bits: bound by
 // memory, 48 requests of one row and 4100 tokens each 35 us, 5.7 TB/s (a part from caches).  4
 // bits: by what a step's vector instructions take next to its loads (of 32 keys and eight rows
-// some 260; 500 without pairs of columns), 32 requests of 16000 tokens 25.6 us, 4.3 TB/s.
+// some 260; 500 without pairs of columns), 32 requests of 8000 to 16000 tokens (111 MB) 25.4 us, 4.4 TB/s.
 template <int D, int R, int WR, int NW, bool F16, bool FP4, bool PAIR>
 __global__ __launch_bounds__(64 * NW, 2) void window_kernel(Window a) {
   static_assert(!PAIR || WR == 1);
@@ -587,9 +587,9 @@ __global__ __launch_bounds__(join_threads(WAVES)) void window_join_kernel(Window
 // that order, cut into equal shares for the workgroups, whatever the requests' rows and lengths
 // are.  What a group costs is counted in keys times `group`, so that it grows by RG from one
 // to the next until the window holds it, and sums over groups need no loop: group g of a
-// request costs min(base + RG (g + 1), cap) + unit (unit alone while that is below 0).  A share takes of each unit the part of
-// its tiles that its part of the counts covers; of a unit that is not whole it leaves sums
-// in slot 2 share (the unit began in an earlier share) or 2 share + 1.
+// request costs min(base + RG (g + 1), cap) + unit (unit alone while that is below 0).  A share takes of
+// each unit the part of its tiles that its part of the counts covers; of a unit that is not whole it
+// leaves sums in slot 2 share (the unit began in an earlier share) or 2 share + 1.
 constexpr int kTileBits = 6, kTile = 1 << kTileBits;  // keys of a tile
 constexpr int kShares = 256;  // workgroups: one per CU
 constexpr int kUnit = 256;    // what a unit costs besides its tiles, in keys
@@ -622,8 +622,9 @@ __device__ __forceinline__ Groups groups_of(const Window& a, const Ragged& rq) {
   g.unit = static_cast<int64_t>(kUnit) * a.group;
   return g;
 }
-// A unit of T tiles costs at most T (3 kTile + 1) group + 2 RG counts, so that a share inside of it
-// has one of its tiles at least.
+// A unit of T tiles costs at most (kUnit + T kTile) group + RG counts: from two tiles on less than a
+// share for each of them, so that a share inside of the unit has one of its tiles at least.  A unit of one
+// tile may be longer than a share: the share that holds its end takes it whole, the others leave nothing.
 __device__ __forceinline__ int shares_of(const Window& a, int64_t total) {
   return static_cast<int>(least(kShares, largest(1, total / (4 * (kTile * a.group + 128)))));
 }
@@ -896,10 +897,10 @@ struct Rows32 {
 // half as long, for one or two.  So a wave's products and softmax overlap: the products of the next
 // tile's scores run beside the weights of this one's second step, those of this one's output
 // beside the weights of the next one's first step, once its references are known.  Four requests of
-// 2048 rows over 4160 of 8000 tokens (204 GFLOP): 251 us in fp16, 810 TFLOP/s, the join 15; matrix
-// units busy 46 %, LDS 20 % (all of a tile's weights beside the scores, its maxima beside the
-// output: 258; two row tiles per wave of 16 x 16: 317 to 400; halves of the workgroup half a tile
-// apart: 333).
+// 1024 to 2048 rows over 4160 of their 4000 to 8000 tokens (201 GFLOP) in fp16: 251 us under a trace, 800
+// TFLOP/s, the join 15, and as much without a trace for both; matrix units busy 46 %, LDS 20 % (all of a
+// tile's weights beside the scores, its maxima beside the output: 258; two row tiles per wave of
+// 16 x 16: 317 to 400; halves of the workgroup half a tile apart: 333).
 template <int D, bool F16>
 __global__ __launch_bounds__(64 * 8, 2) void window_wide_kernel(Window a0) {
   using W = Rows32<D, F16>;
@@ -1259,8 +1260,9 @@ __global__ __launch_bounds__(join_threads(1)) void window_wide_join_kernel(Windo
 // 2^-24, which moves a score by 2^-25 sum |q| at most and a value by half a step of the output),
 // with a table of their own, and the wide kernel reads those.  Each value is read by hundreds of
 // rows, which this costs one write and one read of 16 bits; widened in the wide kernel it would
-// be a third more instructions beside its products.  One workgroup per block: a thread has eight dims of a token.  Bound by memory: 2 x
-// 16000 tokens of 2 x 128 dims (19 MB to 33 MB) 9.5 us.
+// be a third more instructions beside its products.  One workgroup per block: a thread has eight dims
+// of a token.  8000 and 16000 tokens of 2 x 128 dims (6.9 MB to 24.6 MB) 9.5 us, 3.3 TB/s of the 5.1 of a
+// copy: a workgroup's loads wait for its block's number, and it has one turn of them.
 struct Widen {
   Window w;
   uint16_t *k, *v;
@@ -1335,9 +1337,11 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
   // Rows that share tiles through LDS run at three times the rate, but their equal shares cost 30
   // us before that.  By units x steps of 32 keys, us straight from memory and shared (128 dims,
   // 16 bits): 256 (64 rows over 500 tokens) 21 / 38, 2048 (four of 64 over 1000) 22 / 44, 4032
-  // (256 over 2000) 31 / 48, 8192 (1024 over as many) 45 / 47, 16000 (512 over 4000) 67 / 57.  Of
+  // (256 over 2000) 31 / 48, 8192 (1024 over 1024) 45 / 47, 16000 (512 over 4000) 67 / 57.  Of
   // 64 dims, and of 4 bits, which are not widened first then, they meet at twice as many: 14000
-  // (512 over 4000) 42 / 44, 16000 63 / 62, 28000 (2048 over as many, 64 dims) 48 / 46.
+  // (512 over 4000, 64 dims) 42 / 44, 16000 (512 over 4000, 4 bits) 63 / 62, 28000 (2048 over 2048, 64
+  // dims) 48 / 46.  (For the batch as a whole, by its longest request: one prompt among single tokens
+  // takes them into shared tiles too, where each of them is a row group of its own.)
   const int64_t few = fp4 || head_dim == 64 ? 16384 : 8192;
   p.wide = rows <= 64 || units * std::max<int64_t>(1, (seen + 31) / 32) <= few ? 0 : 256;
   if (p.wide) {
@@ -1355,7 +1359,7 @@ Plan plan(int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
   const int64_t steps = (seen + 31) / 32 * p.wr;
   p.min_steps = units * (steps / kCoarseSteps) <= 128 ? kFineSteps : kCoarseSteps;
   // (as many workgroups as run at a time: 4-bit rows leave registers for three per CU, where a
-  // fourth would wait: 32 requests of 16000 tokens in 25.6 instead of 29.0 us)
+  // fourth would wait: 32 requests of 8000 to 16000 tokens in 25.6 instead of 29.0 us)
   if (steps >= kWholeSteps)
     p.splits = static_cast<int>(
         std::max<int64_t>(1, std::min<int64_t>({((fp4 ? 768 : 1024) + units - 1) / units, steps / p.min_steps, 256})));

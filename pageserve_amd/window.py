@@ -19,6 +19,12 @@ request has outgrown its budget, ``evict_tokens`` for all layers and
 ``truncate_blocks``.  Lengths, tables and budgets are read on the device: nothing
 waits for the host, and a step can be one captured HIP graph.
 
+Prompts and single tokens may be in one call, but the kernels are chosen for the
+whole batch by its bounds: a long prompt among single tokens makes them cost several
+times what they cost alone.  Two calls over slices of ``lens``, ``block_tables`` and
+``offsets`` (``offsets[b0 : b1 + 1]``, the rows where they are), into one ``out``, give
+each kind its own.
+
 The rows ``offsets[b] .. offsets[b + 1] - 1`` are request ``b``'s newest tokens, in
 order, and ``lens[b]`` counts them: their keys and values are in the cache when the
 call runs.  Row ``t`` of ``n`` stands at ``p = lens[b] - n + t`` and sees token
@@ -59,8 +65,8 @@ def window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     ``max_tokens`` bounds the rows of a request (default: the rows there are; a
     request's rows beyond it are not computed) and ``max_context`` its tokens
     (default: what the tables can hold).  The kernels and the split of long contexts
-    are chosen by them; max_context never changes what is computed.  ``scale``: of
-    q . k, head_dim ** -0.5 by default.
+    are chosen by them, so a step of single tokens says ``max_tokens=1``; max_context
+    never changes what is computed.  ``scale``: of q . k, head_dim ** -0.5 by default.
 
     Returns (rows, q_heads, head_dim), or writes to ``out`` (contiguous; it may be q
     itself); with ``return_lse`` also the natural logarithm of each row's sum of
@@ -80,7 +86,8 @@ def window_attention4(q: torch.Tensor, cache: KVCache4, block_tables: torch.Tens
                       out: torch.Tensor | None = None) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """:func:`window_attention` over a cache in 4 bits; q and the result are bf16 or
     fp16, whatever rows the cache was written from (with fp16, cached values beyond
-    its range may count as infinite)."""
+    its range may count as infinite).  Of a value that is not finite, all dims of its
+    group of 32 are not finite in the rows that see it: it is the group's scale."""
     r = _native.load_host().window_attention(q, cache.parts, block_tables, lens, offsets, window, sinks, max_tokens,
                                              max_context, scale, return_lse, out)
     return (r[0], r[1]) if return_lse else r[0]

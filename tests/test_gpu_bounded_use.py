@@ -99,3 +99,27 @@ def test_sums_by_the_lse_of_rows_that_see_nothing(gpu, tokens, bits):
         want, far = W.accumulate(sums.cpu().numpy() * 0, b.q.double().numpy(), b.dense()[0], b.tables, b.lens, b.offsets,
                                  given, b.dim ** -0.5, None, **seen)
         check_weights(b, sums, want, far)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_prompts_and_single_tokens_in_calls_of_their_own(gpu, bits):
+    """Two calls over slices of one batch's requests, into one output and one tensor of sums"""
+    tokens = [300, 70] + [1] * 9
+    lens = [400, 70] + [1 + 37 * i for i in range(9)]
+    b = Batch(2, lens, tokens, 16, 2, 128, 16, torch.bfloat16, bits, pad=3)
+    q, *cache, tables, lens_, offsets = b.args(gpu)
+    seen = {"window": 150, "sinks": 3}
+    attend = window_attention4 if bits == 4 else window_attention
+    out, whole = torch.full_like(q, 9.0), torch.full(q.shape[:2], float("nan"), device=gpu)
+    sums = torch.zeros(b.blocks, b.bs, device=gpu)
+    for part, most in ((slice(0, 2), 300), (slice(2, 11), 1)):
+        some = (tables[part], lens_[part], offsets[part.start:part.stop + 1])
+        _, lse = attend(q, *cache, *some, max_tokens=most, max_context=400, return_lse=True, out=out, **seen)
+        rows = slice(b.offsets[part.start], b.offsets[part.stop])
+        whole[rows] = lse[rows]
+        accumulate_weights(q, cache[0], *some, lse, sums, max_tokens=most, max_context=400, **seen)
+    assert (out[-3:] == 9.0).all()
+    b.check((out, whole), b.oracle(**seen))
+    want, far = W.accumulate(sums.cpu().numpy() * 0, b.q.double().numpy(), b.dense()[0], b.tables, b.lens, b.offsets,
+                             torch.nan_to_num(whole).double().cpu().numpy(), b.dim ** -0.5, None, **seen)
+    check_weights(b, sums, want, far)
