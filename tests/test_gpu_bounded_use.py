@@ -3,6 +3,7 @@ number by number (tests/test_gpu_evict.py: the bound of sums)."""
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -123,3 +124,78 @@ def test_prompts_and_single_tokens_in_calls_of_their_own(gpu, bits):
     want, far = W.accumulate(sums.cpu().numpy() * 0, b.q.double().numpy(), b.dense()[0], b.tables, b.lens, b.offsets,
                              torch.nan_to_num(whole).double().cpu().numpy(), b.dim ** -0.5, None, **seen)
     check_weights(b, sums, want, far)
+
+
+def sums_of(b, args, lse, start, cache=None, **kw):
+    """accumulate_weights on a copy of start, and the check of it against the oracle"""
+    sums = start.clone()
+    accumulate_weights(args[0], cache if cache is not None else args[1], *args[-3:], lse, sums, **kw)
+    given = lse.double().cpu().numpy()
+    if kw.get("max_tokens") is not None:
+        for r in range(len(b.lens)):  # (rows beyond it: e^-10000)
+            given[b.offsets[r] + kw["max_tokens"]:b.offsets[r + 1]] = 1e4
+    scale = kw.get("scale")
+    want, far = W.accumulate(start.cpu().numpy(), b.q[:len(given)].double().numpy(), b.dense()[0], b.tables, b.lens, b.offsets,
+                             given, b.dim ** -0.5 if scale is None else scale, None, kw.get("window"), kw.get("sinks", 0))
+    # check_weights' bound, and beside it 2^-126 for each of the weights that are added: fp32 has no normal
+    # number below, and an exponential that is smaller may come as 0
+    rows = b.offsets[-1] * b.heads
+    e = (b.dim + 12) * 2.0 ** -23 * far + 2.0 ** -20 + (rows + 16) * 2.0 ** -24
+    assert (np.abs(sums.double().cpu().numpy() - want) <= e * np.abs(want) + rows * 2.0 ** -126).all(), f"{kw}"
+    return sums
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("tokens", [1, 40])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0, 20.0])
+def test_sums_of_other_scales(gpu, scale, tokens, bits):
+    b = Batch(tokens, [tokens + 90, 33, 70], [tokens, 1, min(tokens, 20)], 4, 2, 64, 16, torch.float16, bits)
+    args, kw = b.args(gpu), {"window": 50, "sinks": 3, "scale": scale}
+    _, lse = (window_attention4 if bits == 4 else window_attention)(*args, return_lse=True, **kw)
+    sums_of(b, args, lse, torch.zeros(b.blocks, b.bs, device=gpu), **kw)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("bs", [32, 48, 80, 256])
+@pytest.mark.parametrize("tokens", [1, 2, 30, 300])
+@pytest.mark.parametrize("heads,kv,dim", [(16, 2, 128), (14, 2, 64)])
+def test_sums_over_blocks_of_other_sizes_and_rows_beyond_max_tokens(gpu, heads, kv, dim, tokens, bs, bits):
+    b = Batch(bs, [tokens + 500, 257, 40], [tokens, 1, min(tokens, 40)], heads, kv, dim, bs, torch.bfloat16, bits,
+              garbage=float("nan"))
+    args, start = b.args(gpu), torch.rand(b.blocks, bs, device=gpu)
+    _, lse = (window_attention4 if bits == 4 else window_attention)(*args, return_lse=True, window=200, sinks=10)
+    whole = sums_of(b, args, lse, start, window=200, sinks=10)
+    assert torch.equal(whole, sums_of(b, args, lse, start, window=200, sinks=10, max_tokens=tokens))
+    if tokens > 1:
+        sums_of(b, args, lse, start, window=200, sinks=10, max_tokens=max(1, tokens - 3))
+
+
+@pytest.mark.parametrize("tokens", [1, 60])
+def test_sums_from_rows_and_keys_of_other_strides(gpu, tokens):
+    b = Batch(6, [tokens + 300, 100], [tokens, min(tokens, 9)], 8, 2, 128, 16, torch.bfloat16)
+    q, k, v, *rest = args = b.args(gpu)
+    _, lse = window_attention(*args, return_lse=True)
+    start = torch.zeros(b.blocks, b.bs, device=gpu)
+    want = sums_of(b, args, lse, start)
+    fused = torch.full((q.shape[0], 12, 128), float("nan"), dtype=q.dtype, device=gpu)
+    fused[:, 2:10] = q
+    turned = k.transpose(1, 2).contiguous().transpose(1, 2)
+    both = torch.stack((v, k), 3)[:, :, :, 1]
+    far = torch.full((b.blocks, 3, b.bs, 2, 128), float("nan"), dtype=k.dtype, device=gpu)[:, 1]
+    far.copy_(k)
+    for rows in (q, fused[:, 2:10], q.transpose(0, 1).contiguous().transpose(0, 1), q.transpose(1, 2).contiguous().transpose(1, 2)):
+        for keys in (k, turned, both, far):
+            assert torch.equal(sums_of(b, [rows, keys, *rest], lse, start), want)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("bs", [32, 48, 80, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_rows_over_blocks_of_other_sizes(gpu, dtype, bs, bits):
+    b = Batch(bs, [700, 257, 40, 128], [300, 1, 40, 0], 16, 2, 128, bs, dtype, bits, garbage=float("inf"))
+    args = b.args(gpu)
+    q = torch.nn.functional.pad(args[0], (0, 0, 0, 0, 0, 40000))  # (as many rows as make it one of many)
+    attend, n = window_attention4 if bits == 4 else window_attention, b.offsets[-1]
+    for window, sinks in ((None, 0), (130, 20), (64, 200), (1, 1)):
+        out, lse = attend(q, *args[1:], window=window, sinks=sinks, return_lse=True)
+        b.check((out[:n], lse[:n]), b.oracle(window=window, sinks=sinks), f"{window} {sinks}")
